@@ -365,6 +365,42 @@ int uh_mx_moe_forward_noalloc(const uint16_t* x, const float* logits, int T, int
                               const uint8_t* const* tab, float limit, uint16_t* out, int32_t* sel, float* wt,
                               void* stream);
 
+/* ---- the 8-bit paged key / value cache and its attention (include/unholy/kernels/kv_cache.hpp has the layout and the
+ * full contracts; no reference counterpart). One layer: kc e4m3 [pages, Hkv, page, D], vc e4m3 [pages, Hkv, D, page], ks / vs
+ * e8m0 [pages, Hkv]; page 16, 32, 64 or 128 tokens, D 64, 128 or 256. table int32 [B, max_blocks] (page numbers, -1: none),
+ * lens int32 [B] (tokens of a sequence, the step's new ones included), cu int32 [B + 1] (the step's rows of each sequence),
+ * all on the device; rows: of the row arrays; max_new: at least any sequence's rows. ---- */
+/* The new rows' keys / values k, v bf16 [rows, Hkv, D] (row strides ldk, ldv) quantized into their slots, a power-of-two
+ * scale for each block and head that only grows while the block fills. */
+int uh_kv_append(const uint16_t* k, int ldk, const uint16_t* v, int ldv, const int32_t* cu, int rows, int max_new,
+                 const int32_t* lens, const int32_t* table, int max_blocks, int B, uint8_t* kc, uint8_t* vc, uint8_t* ks,
+                 uint8_t* vs, int pages, int page, int Hkv, int D, void* stream);
+/* Causal attention of the rows q bf16 [rows, Hq, D] over the cached tokens into out (the same shape): every token up to
+ * the row's own, with window > 0 the last `window` of them and the first `sinks` tokens of the sequence. lse (may be NULL)
+ * fp32 [rows, Hq]. ws: uh_kv_attend_workspace_size bytes, 16-byte aligned. */
+size_t uh_kv_attend_workspace_size(int rows, int max_new, int B, int Hq, int Hkv, int D);
+int uh_kv_attend(const uint16_t* q, int ldq, const int32_t* cu, int rows, int max_new, const int32_t* lens,
+                 const int32_t* table, int max_blocks, int B, const uint8_t* kc, const uint8_t* vc, const uint8_t* ks,
+                 const uint8_t* vs, int pages, int page, int Hq, int Hkv, int D, float scale, int window, int sinks,
+                 uint16_t* out, int ldo, float* lse, void* ws, size_t ws_bytes, void* stream);
+/* Pages, on the device: refs int32 [pages] counts the table entries that name a page (0: free); the caches here are all
+ * layers' [layers, pages, ...]. reserve: pages for the next grow[b] tokens, lens[b] += grow[b], a shared last page that is
+ * not full copied first; ok[b] 0: untouched, no pages left. fork: empty slot b becomes a fork of sequence from[b] (-1:
+ * none), done[b] 1 where it did. free: sequence b keeps its first keep[b] tokens. compact: the used pages moved to the
+ * lowest numbers, *live of them (device, may be NULL); table_out / refs_out may be table / refs. ws:
+ * uh_kv_pages_workspace_size bytes, 16-byte aligned. */
+size_t uh_kv_pages_workspace_size(int B, int pages);
+int uh_kv_reserve(int32_t* table, int max_blocks, int32_t* lens, const int32_t* grow, int B, int32_t* refs, uint8_t* kc,
+                  uint8_t* vc, uint8_t* ks, uint8_t* vs, int layers, int pages, int page, int Hkv, int D, int32_t* ok,
+                  void* ws, size_t ws_bytes, void* stream);
+int uh_kv_fork(int32_t* table, int max_blocks, int32_t* lens, const int32_t* from, int B, int32_t* refs, int pages,
+               int page, int32_t* done, void* stream);
+int uh_kv_free(int32_t* table, int max_blocks, int32_t* lens, const int32_t* keep, int B, int32_t* refs, int pages,
+               int page, void* stream);
+int uh_kv_compact(const int32_t* table, int32_t* table_out, int max_blocks, int B, const int32_t* refs,
+                  int32_t* refs_out, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, int layers, int pages, int page,
+                  int Hkv, int D, int32_t* live, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,7 @@
 #include "unholy/model/expert_pack.hpp"
 #include "unholy/kernels/gemm_wmma.hpp"
 #include "unholy/kernels/gemv.hpp"
+#include "unholy/kernels/kv_cache.hpp"
 #include "unholy/kernels/moe_dispatch.hpp"
 #include "unholy/kernels/mx_moe.hpp"
 #include "unholy/kernels/ref.hpp"
@@ -940,6 +941,54 @@ int uh_mx_moe_forward_noalloc(const uint16_t* x, const float* logits, int T, int
   });
   if (rc) return rc;
   return uh_mx_moe_forward_ev(x, logits, T, K, E, D, I, tab, limit, ws, kScratchBytes, out, sel, wt, stream, nullptr);
+}
+
+int uh_kv_append(const uint16_t* kx, int ldk, const uint16_t* vx, int ldv, const int32_t* cu, int rows, int max_new,
+                 const int32_t* lens, const int32_t* table, int max_blocks, int B, uint8_t* kc, uint8_t* vc, uint8_t* ks,
+                 uint8_t* vs, int pages, int page, int Hkv, int D, void* st) {
+  return guard([&] {
+    k::kv_append(kx, ldk, vx, ldv, {cu, lens, table, B, max_blocks, rows, max_new}, {kc, vc, ks, vs, pages, page, Hkv, D},
+                 S(st));
+  });
+}
+size_t uh_kv_attend_workspace_size(int rows, int max_new, int B, int Hq, int Hkv, int D) {
+  return k::kv_attend_workspace(rows, max_new, B, Hq, Hkv, D);
+}
+int uh_kv_attend(const uint16_t* q, int ldq, const int32_t* cu, int rows, int max_new, const int32_t* lens,
+                 const int32_t* table, int max_blocks, int B, const uint8_t* kc, const uint8_t* vc, const uint8_t* ks,
+                 const uint8_t* vs, int pages, int page, int Hq, int Hkv, int D, float scale, int window, int sinks,
+                 uint16_t* out, int ldo, float* lse, void* ws, size_t ws_bytes, void* st) {
+  return guard([&] {
+    const auto rw = [](const uint8_t* p) { return const_cast<uint8_t*>(p); };  // read only by kv_attend
+    k::kv_attend(q, ldq, {cu, lens, table, B, max_blocks, rows, max_new},
+                 {rw(kc), rw(vc), rw(ks), rw(vs), pages, page, Hkv, D}, Hq, scale, window, sinks, out, ldo, lse, ws,
+                 ws_bytes, S(st));
+  });
+}
+size_t uh_kv_pages_workspace_size(int B, int pages) { return k::kv_pages_workspace(B, pages); }
+int uh_kv_reserve(int32_t* table, int max_blocks, int32_t* lens, const int32_t* grow, int B, int32_t* refs, uint8_t* kc,
+                  uint8_t* vc, uint8_t* ks, uint8_t* vs, int layers, int pages, int page, int Hkv, int D, int32_t* ok,
+                  void* ws, size_t ws_bytes, void* st) {
+  return guard([&] {
+    k::kv_reserve({table, lens, B, max_blocks}, grow, refs, {kc, vc, ks, vs, pages, page, Hkv, D}, layers, ok, ws,
+                  ws_bytes, S(st));
+  });
+}
+int uh_kv_fork(int32_t* table, int max_blocks, int32_t* lens, const int32_t* from, int B, int32_t* refs, int pages,
+               int page, int32_t* done, void* st) {
+  return guard([&] { k::kv_fork({table, lens, B, max_blocks}, from, refs, pages, page, done, S(st)); });
+}
+int uh_kv_free(int32_t* table, int max_blocks, int32_t* lens, const int32_t* keep, int B, int32_t* refs, int pages,
+               int page, void* st) {
+  return guard([&] { k::kv_free({table, lens, B, max_blocks}, keep, refs, pages, page, S(st)); });
+}
+int uh_kv_compact(const int32_t* table, int32_t* table_out, int max_blocks, int B, const int32_t* refs,
+                  int32_t* refs_out, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs, int layers, int pages, int page,
+                  int Hkv, int D, int32_t* live, void* ws, size_t ws_bytes, void* st) {
+  return guard([&] {
+    k::kv_compact(table, table_out, max_blocks, B, refs, refs_out, {kc, vc, ks, vs, pages, page, Hkv, D}, layers, live,
+                  ws, ws_bytes, S(st));
+  });
 }
 
 }  // extern "C"
