@@ -256,7 +256,7 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(KvCache c, int layers, Pag
     const uint4* src = reinterpret_cast<const uint4*>(data + (base + pair.x) * bytes + size_t(part) * CP_BYTES);
     uint4* dst = reinterpret_cast<uint4*>(data + (base + pair.y) * bytes + size_t(part) * CP_BYTES);
     const int vecs = int(min(bytes - size_t(part) * CP_BYTES, size_t(CP_BYTES)) / 16);
-    uint4 v[CP_BYTES / 16 / 256];
+    uint4 v[CP_BYTES / 16 / 256] = {};
 #pragma unroll
     for (int i = 0; i < CP_BYTES / 16 / 256; ++i)
       if (int(threadIdx.x) + i * 256 < vecs) v[i] = src[threadIdx.x + i * 256];
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(64) void kv_free_kernel(KvSeqs s, const int32_t* __
 void check_seqs(const char* who, const KvSeqs& s, const int32_t* more, const int32_t* refs, int pages, int page) {
   const auto fail = [&](const char* what) { throw std::runtime_error(std::string(who) + ": " + what); };
   if (s.B < 0 || s.max_blocks < 0) fail("negative size");
-  if (s.max_blocks > (1 << 24)) fail("max_blocks > 2^24");
+  if (s.max_blocks > (1 << 23)) fail("max_blocks > 2^23");
   if (page != 16 && page != 32 && page != 64 && page != 128) fail("page must be 16, 32, 64 or 128");
   check_pages(who, pages);
   if ((!s.table && s.max_blocks) || !s.lens || !more || !refs) fail("null operand");
@@ -440,7 +440,7 @@ void kv_compact(const int32_t* table, int32_t* table_out, int max_blocks, int B,
                 const KvCache& c, int layers, int32_t* live, void* ws, size_t ws_bytes, hipStream_t st) {
   check_cache("kv_compact", c);
   if (B < 0 || max_blocks < 0) throw std::runtime_error("kv_compact: negative size");
-  if (max_blocks > (1 << 24)) throw std::runtime_error("kv_compact: max_blocks > 2^24");
+  if (max_blocks > (1 << 23)) throw std::runtime_error("kv_compact: max_blocks > 2^23");
   const size_t entries = size_t(B) * max_blocks;
   if (layers < 1) throw std::runtime_error("kv_compact: layers < 1");
   if (!refs || !refs_out || (entries && (!table || !table_out))) throw std::runtime_error("kv_compact: null operand");

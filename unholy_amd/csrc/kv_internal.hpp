@@ -47,7 +47,7 @@ inline void check_cache(const char* who, const KvCache& c) {
 inline void check_step(const char* who, const KvStep& s) {
   const auto fail = [&](const char* what) { throw std::runtime_error(std::string(who) + ": " + what); };
   if (s.B < 0 || s.rows < 0 || s.max_blocks < 0 || s.max_new < 0) fail("negative size");
-  if (s.max_blocks > (1 << 24)) fail("max_blocks > 2^24");  // positions stay in 31 bits
+  if (s.max_blocks > (1 << 23)) fail("max_blocks > 2^23");  // positions stay in 30 bits
   if (!s.cu || !s.lens || (!s.table && s.max_blocks)) fail("null operand");
 }
 
