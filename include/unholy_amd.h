@@ -377,7 +377,8 @@ int uh_kv_append(const uint16_t* k, int ldk, const uint16_t* v, int ldv, const i
                  uint8_t* vs, int pages, int page, int Hkv, int D, void* stream);
 /* Causal attention of the rows q bf16 [rows, Hq, D] over the cached tokens into out (the same shape): every token up to
  * the row's own, with window > 0 the last `window` of them and the first `sinks` tokens of the sequence. lse (may be NULL)
- * fp32 [rows, Hq]. ws: uh_kv_attend_workspace_size bytes, 16-byte aligned. */
+ * fp32 [rows, Hq]. ws: uh_kv_attend_workspace_size bytes, 16-byte aligned, zeroed before its first call
+ * (calls that may overlap need one each). */
 size_t uh_kv_attend_workspace_size(int rows, int max_new, int B, int Hq, int Hkv, int D);
 int uh_kv_attend(const uint16_t* q, int ldq, const int32_t* cu, int rows, int max_new, const int32_t* lens,
                  const int32_t* table, int max_blocks, int B, const uint8_t* kc, const uint8_t* vc, const uint8_t* ks,

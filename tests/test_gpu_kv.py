@@ -45,7 +45,7 @@ def attend(c, q, Hq, scale, window=0, sinks=0, pad=0, max_new=None, stream=None,
     dl = dev(np.full((rows, Hq), np.nan, np.float32))
     most = max(s.n + [0]) if max_new is None else max_new
     need = call("uh_kv_attend_workspace_size", rows, most, s.B, Hq, s.Hkv, s.D)
-    ws = dev(np.full(need + 64, GUARD, np.uint8))
+    ws = dev(np.concatenate([np.zeros(need, np.uint8), np.full(64, GUARD, np.uint8)]))
     call("uh_kv_attend", dq, ld, c.cu, rows, most, c.lens, c.table, s.max_blocks, s.B, *c.arrays(), s.pages, s.page, Hq,
          s.Hkv, s.D, scale, window, sinks, out, ld, dl if lse else None, ws, need, stream)
     synchronize()
@@ -512,7 +512,7 @@ def test_captured_step_replays_with_new_lengths():
     c = Cache(s)
     wa = call("uh_kv_attend_workspace_size", 4, 2, 3, Hq, 2, 128)
     wp = call("uh_kv_pages_workspace_size", 3, s.pages)
-    ws_a, ws_p = DeviceBuffer(wa), DeviceBuffer(wp)
+    ws_a, ws_p = dev(np.zeros(wa, np.uint8)), DeviceBuffer(wp)
 
     def work():
         h = st.handle

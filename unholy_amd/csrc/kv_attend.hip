@@ -18,9 +18,28 @@ constexpr int AT_NT = 256;        // threads of a workgroup
 constexpr int AT_WAVES = AT_NT / 64;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
-__device__ __forceinline__ bool visible(int p, int t, int window, int sinks) {
-  return t <= p && (window <= 0 || p - t < window || t < sinks);
+// Bits of the first n of up to 16 tokens.
+__device__ __forceinline__ uint32_t first_bits(int n) { return (1u << min(max(n, 0), 16)) - 1; }
+// Which of the 16 tokens from t on a row at position p sees.
+__device__ __forceinline__ uint32_t seen_bits(int p, int t, int window, int sinks) {
+  uint32_t see = first_bits(p - t + 1);
+  if (window > 0) see &= ~first_bits(int(min(int64_t(p) - window - t + 1, int64_t(16)))) | first_bits(sinks - t);
+  return see;
 }
+// Inclusive sum over the wave's lanes (all active): DPP shifts within rows of 16, then the rows' last lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  const auto step = [](uint32_t x, auto ctrl, auto rows) {
+    return x + uint32_t(__builtin_amdgcn_update_dpp(0, int(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  v = step(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr:1
+  v = step(v, integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  v = step(v, integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  v = step(v, integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  v = step(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15 into rows 1 and 3
+  return step(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return uint32_t(__builtin_amdgcn_readlane(int(v), lane)); }
 
 // What every workgroup knows of the call.
 struct Attend {
@@ -31,8 +50,10 @@ struct Attend {
   KvCache c;
   int ldq, ldo, group, page_shift, window, sinks;
   float scale2;  // scale * log2(e): the kernels take powers of two
-  float* po;     // partial results: values [slot][16 RT][D], then maximum and sum [slot][16 RT][2]
-  float* pml;
+  int target;    // workgroups that the chip holds at a time
+  int rounds;    // of them, where segments are many
+  uint32_t* counters;  // of finished pieces, [slot]; zero between launches
+  float *po, *pml;     // partial sums: values [slot][ROWS][D]; maximum and weight sum [slot][ROWS][2]
 };
 
 // The 64-token tiles that some row of a sequence sees: with a window the sinks' tiles [0, sink_tiles) and those from
@@ -55,39 +76,73 @@ __device__ __forceinline__ Tiles tiles_of(const Attend& a, const Seq& q) {
 }
 __device__ __forceinline__ int row_groups(int rows, int per) { return (rows + per - 1) / per; }
 
-// Sums over the workgroup's threads before this one, and over all (wsum: AT_WAVES of LDS).
-__device__ __forceinline__ int64_t scan64(int64_t v, int64_t* wsum, int64_t& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int64_t x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) wsum[w] = x;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < AT_WAVES; ++i) {
-    before += i < w ? wsum[i] : 0;
-    total += wsum[i];
-  }
-  return before + x - v;
+// The split of a launch's work, worked out by every workgroup from the lengths, which only the device knows: a segment is
+// a (sequence, key / value head, row group) and its tiles; each is cut into pieces of at most `share` tiles, as equal as
+// they can be, a workgroup each. share makes about `target` pieces, so that long and short sequences load the chip evenly.
+// A segment of several pieces leaves partial sums in slots slot0 .. slot0 + pieces - 1: with u the tiles before it in the
+// launch and f = u / share, slots from 2 f on, of which there are 2 (f' - f) >= 2 floor(tiles / share) >= pieces before the
+// next segment's.
+struct Piece {
+  int b, h, rg, index, pieces, i0, i1, slot0;
+};
+__device__ __forceinline__ uint32_t pieces_of(uint32_t tiles, uint32_t share) {
+  return max((tiles + share - 1) / share, 1u);  // (no tiles: a piece that writes zeros)
 }
-
-// The split of a launch's work, the same in every workgroup and in the launch that joins them. The units are the tiles of
-// every (sequence, key / value head, row group), in this order; workgroup w takes units [w share, (w + 1) share), so that
-// long and short sequences load the chip evenly whatever their lengths, which only the device knows.
-template <int ROWS>
-__device__ __forceinline__ int64_t units_of(const Attend& a, int b, int& rg) {
-  const Seq q = seq_of(a.st, b);
-  rg = row_groups((q.r1 - q.r0) * a.group, ROWS);
-  return rg ? int64_t(tiles_of(a, q).count) * rg * a.c.heads : 0;
-}
-__device__ __forceinline__ int64_t share_of(int64_t units, int wgs) {
-  return max((units + wgs - 1) / wgs, int64_t(AT_WAVES));  // a tile for each wave at least
+// Every wave for itself, a sequence a lane: no barriers, and for up to 64 sequences one pass over registers.
+template <int ROWS, int LEAST>
+__device__ __forceinline__ bool find_piece(const Attend& a, Piece& p, Seq& q, Tiles& t) {
+  const int lane = threadIdx.x & 63;
+  Tiles mt{0, 0, 0};
+  uint32_t segs = 0;  // of this lane's sequence
+  const auto look = [&](int b) {
+    segs = 0;
+    mt = Tiles{0, 0, 0};
+    if (b < a.st.B) {
+      q = seq_of(a.st, b);
+      segs = uint32_t(row_groups((q.r1 - q.r0) * a.group, ROWS)) * a.c.heads;
+      if (segs) mt = tiles_of(a, q);
+    }
+  };
+  float tiles = 0.0f;
+  uint32_t all = 0;
+  for (int b0 = 0; b0 < a.st.B; b0 += 64) {
+    look(b0 + lane);
+    tiles += wave_sum(float(mt.count) * float(segs));
+    all += lane_of(wave_scan(segs), 63);
+  }
+  // about `target` pieces where the segments are few, one round of the chip; else more and smaller ones than it holds, which
+  // even out as they come and go
+  const float want = float(all <= uint32_t(a.target) / 2 ? a.target - int(all) : a.target * a.rounds);
+  // (past 2^31 tiles the prefix below would wrap: no segment is cut then)
+  const uint32_t share = tiles < 2.0e9f ? max(uint32_t(ceilf(tiles * 1.0001f / want)), uint32_t(LEAST)) : 1u << 30;
+  uint32_t wg0 = 0, u0 = 0;
+  for (int b0 = 0; b0 < a.st.B; b0 += 64) {
+    if (a.st.B > 64) look(b0 + lane);
+    const uint32_t n = segs * pieces_of(uint32_t(mt.count), share), u = segs * uint32_t(mt.count);
+    const uint32_t wg_end = wg0 + wave_scan(n), u_end = u0 + wave_scan(u);
+    const uint64_t hit = __ballot(blockIdx.x < wg_end);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;  // (a lane of no segments ends where the one before it does)
+      p.b = b0 + l;
+      q = Seq{int(lane_of(q.r0, l)), int(lane_of(q.r1, l)), int(lane_of(q.len, l)), int(lane_of(q.first, l))};
+      t = Tiles{int(lane_of(mt.sink_tiles, l)), int(lane_of(mt.skip, l)), int(lane_of(mt.count, l))};
+      const uint32_t sg = lane_of(segs, l), first = lane_of(wg_end - n, l), ut = lane_of(u_end - u, l);
+      const uint32_t rgs = sg / uint32_t(a.c.heads), pieces = pieces_of(uint32_t(t.count), share);
+      const uint32_t in = blockIdx.x - first, seg = in / pieces, i = in % pieces;
+      const uint32_t each = uint32_t(t.count) / pieces, more = uint32_t(t.count) % pieces;
+      p.index = int(i);
+      p.pieces = int(pieces);
+      p.h = int(seg / rgs);
+      p.rg = int(seg % rgs);
+      p.i0 = int(i * each + min(i, more));
+      p.i1 = p.i0 + int(each + (i < more ? 1 : 0));
+      p.slot0 = int((ut + seg * uint32_t(t.count)) / share * 2);
+      return true;
+    }
+    wg0 = lane_of(wg_end, 63);
+    u0 = lane_of(u_end, 63);
+  }
+  return false;
 }
 
 __device__ __forceinline__ bf16x8 bf16x8_of(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
@@ -97,438 +152,362 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {  // the high bit of 
 }
 
 // ---- few rows a sequence: decode and verify steps ---------------------------------------------------------------------
-// Bound by reading the cache once. A wave takes 16 RT rows (the (token, query head) pairs that share a key / value head) and
-// 64 tokens at a time straight from the cache into registers, no LDS: with S^T = K Q^T the 16x16 product leaves lane
+// Bound by reading the cache once. A wave takes 16 rows ((token, query head) pairs that share a key / value head) and
+// 16 J tokens at a time straight from the cache into registers, no LDS: with S^T = K Q^T the 16x16 product leaves lane
 // (row c, group g) the scores of tokens 4g .. 4g + 3 of a 16-token tile, and the tiles' rows are taken in such an order of
-// tokens (tile j, row r: token 16 (r / 4) + 4j + r % 4) that over four tiles these are tokens 16g .. 16g + 15: the
-// very tokens whose values one 16-byte load of the transposed cache gives it for O^T = V^T P^T. The weights go from one
-// product to the other in place, and a row's running maximum and sum are its lane's own.
+// tokens (tile j, row r: token 4J (r / 4) + 4j + r % 4) that over the J tiles these are tokens 4J g .. 4J g + 4J - 1: the
+// very tokens whose values one load of the transposed cache gives it for O^T = V^T P^T. The weights go from one product
+// to the other in place, and a row's running maximum and sum are its lane's own.
 // The codes become bf16 exactly (v_cvt_scalef32, the block's scale with them), the products sum in fp32; the weights are
 // rounded to bf16 for the second product (2^-8 of each at most, as much as the output's own rounding), their sum is taken in
 // fp32 before that.
-// The waves of a workgroup take every fourth tile and are joined in LDS; workgroups that share rows leave partial sums
-// and kv_join_kernel adds them, in the order of the tiles.
-constexpr int wgs_per_cu(int dim, int rt) { return rt * dim <= 128 ? 2 : 1; }  // by their registers
-template <int D, int RT>
+// The four waves are RW sets of 16 rows (they read the same tokens, which L1 serves) times 4 / RW that take every
+// (4 / RW)-th tile and are joined in LDS. The workgroup that finishes last of those that share rows adds their partial
+// sums, in the order of the tiles whichever it is: the result does not depend on timing.
+template <int D, int RW>
 struct Split {
-  static constexpr int ROWS = 16 * RT;
+  static constexpr int J = D == 256 ? 2 : 4;  // (four tiles of 256 channels do not leave room for two waves)
+  static constexpr int TOK = 16 * J;
+  static constexpr int TW = AT_WAVES / RW;  // waves that share rows
+  static constexpr int ROWS = 16 * RW;
   static constexpr int KL = D / 64;  // 16-byte loads of a key row's quarter
   static constexpr int DT = D / 16;  // 16-channel tiles
   struct Lds {
-    float o[2][ROWS * D];
-    float ml[AT_WAVES][ROWS][2];
+    float o[TW > 1 ? AT_WAVES / 2 : 1][16 * D];
+    float ml[AT_WAVES][16][2];
   };
 };
+constexpr int kTarget = 512;  // two workgroups on each CU
+constexpr int kMostSlots = 4 * kTarget;
+constexpr size_t kCounterBytes = kMostSlots * sizeof(uint32_t);
+constexpr int rounds_of(int rw) { return rw == 4 ? 1 : 2; }
+constexpr int slots_of(int rw) { return 2 * kTarget * rounds_of(rw); }  // two a share of the tiles
 
-template <int D, int RT>
-__global__ __launch_bounds__(AT_NT, wgs_per_cu(D, RT)) void kv_split_kernel(Attend a) {
-  using S = Split<D, RT>;
-  __shared__ __align__(16) char lds_raw[sizeof(typename S::Lds)];
-  auto& lds = *reinterpret_cast<typename S::Lds*>(lds_raw);
-  __shared__ int64_t wsum[AT_WAVES];
-  __shared__ int64_t found_at;
-  __shared__ int found_b;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-
-  // the whole, and where this workgroup's share begins
-  int64_t total = 0, sum, mine = 0, before = 0;
-  int rg;
-  for (int b0 = 0; b0 < a.st.B; b0 += AT_NT) {
-    mine = b0 + tid < a.st.B ? units_of<S::ROWS>(a, b0 + tid, rg) : 0;
-    before = total + scan64(mine, wsum, sum);
-    total += sum;
-  }
-  const int64_t share = share_of(total, gridDim.x), u0 = share * blockIdx.x, u1 = min(u0 + share, total);
-  if (u0 >= total) return;
-  if (a.st.B <= AT_NT) {
-    if (u0 >= before && u0 < before + mine) found_b = tid, found_at = before;
-  } else {
-    int64_t at = 0;
-    for (int b0 = 0; b0 < a.st.B && at <= u0; b0 += AT_NT) {
-      mine = b0 + tid < a.st.B ? units_of<S::ROWS>(a, b0 + tid, rg) : 0;
-      before = at + scan64(mine, wsum, sum);
-      if (u0 >= before && u0 < before + mine) found_b = b0 + tid, found_at = before;
-      at += sum;
-    }
-  }
-  __syncthreads();
-  int b = found_b;
-  int64_t base = found_at;
-
-  for (int64_t u = u0; u < u1; ++b) {
-    const int64_t in_b = units_of<S::ROWS>(a, b, rg);
-    const Seq q = seq_of(a.st, b);
-    const Tiles tiles = tiles_of(a, q);
-    const int nrows = (q.r1 - q.r0) * a.group;
-    for (; u < min(u1, base + in_b);) {
-      const int seg = int((u - base) / tiles.count), h = seg / rg, row0 = seg % rg * S::ROWS;
-      const int64_t seg_at = base + int64_t(seg) * tiles.count;
-      const int i0 = int(u - seg_at), i1 = int(min(int64_t(tiles.count), u1 - seg_at));
-      u = seg_at + i1;
-
-      // this lane's rows: their positions and queries
-      int pos[RT];
-      bf16x8 qf[RT][2 * S::KL];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const int ri = min(row0 + 16 * r + c, nrows - 1), tok = ri / a.group, hq = h * a.group + ri % a.group;
-        pos[r] = q.first + tok;
-        const bf16* x = a.q + size_t(q.r0 + tok) * a.ldq + size_t(hq) * D + 16 * g;
-#pragma unroll
-        for (int m = 0; m < S::KL; ++m) {
-          qf[r][2 * m] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m));
-          qf[r][2 * m + 1] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m + 8));
-        }
-      }
-      const int pos_lo = q.first + row0 / a.group;  // of all rows here
-      const int pos_hi = q.first + min(row0 + S::ROWS - 1, nrows - 1) / a.group;
-
-      v4f o[RT][S::DT];
-      float mx[RT], l[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        mx[r] = -INFINITY;
-        l[r] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) o[r][d] = v4f{0, 0, 0, 0};
-      }
-
-      const int mask = a.c.page - 1, sh = a.page_shift;
-      const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
-        pk = page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (t0 + 16 * (c >> 2)) >> sh);
-        pv = page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (t0 + 16 * g) >> sh);
-      };
-      uint4 kr[4][S::KL], vr[S::DT];
-      int ksb, vsb;
-      const auto load_k = [&](int t0, int pk) {
-        const size_t ph = size_t(max(pk, 0)) * a.c.heads + h;
-        const uint8_t* p = a.c.k + ((ph << sh) + ((t0 + 16 * (c >> 2) + (c & 3)) & mask)) * D + 16 * g;
-        ksb = a.c.ks[ph];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int m = 0; m < S::KL; ++m) kr[j][m] = ld16(p + 4 * j * D + 64 * m);
-      };
-      const auto load_v = [&](int t0, int pv) {
-        const size_t ph = size_t(max(pv, 0)) * a.c.heads + h;
-        const uint8_t* p = a.c.v + ((ph * D + c) << sh) + ((t0 + 16 * g) & mask);
-        vsb = a.c.vs[ph];
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) vr[d] = ld16(p + (size_t(16 * d) << sh));
-      };
-
-      int i = i0 + wave, pk = 0, pv = 0, pk1 = 0, pv1 = 0;
-      if (i < i1) {
-        lookup(tiles.at(i) * TILE, pk, pv);
-        load_k(tiles.at(i) * TILE, pk);
-        load_v(tiles.at(i) * TILE, pv);
-        if (i + AT_WAVES < i1) lookup(tiles.at(i + AT_WAVES) * TILE, pk1, pv1);
-      }
-      for (; i < i1; i += AT_WAVES) {
-        const int t0 = tiles.at(i) * TILE, tn = tiles.at(min(i + AT_WAVES, i1 - 1)) * TILE;
-        const bool more = i + AT_WAVES < i1;
-        const float ks = e8m0_to_f32(uint8_t(ksb)), vs = e8m0_to_f32(uint8_t(vsb));
-        v4f s[RT][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int r = 0; r < RT; ++r) s[r][j] = v4f{0, 0, 0, 0};
-#pragma unroll
-          for (int m = 0; m < S::KL; ++m) {
-            const bf16x8 k0 = fp8x8_to_bf16(kr[j][m].x, kr[j][m].y, ks), k1 = fp8x8_to_bf16(kr[j][m].z, kr[j][m].w, ks);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-              s[r][j] = mfma_bf16(k0, qf[r][2 * m], s[r][j]);
-              s[r][j] = mfma_bf16(k1, qf[r][2 * m + 1], s[r][j]);
-            }
-          }
-        }
-        const int pvt = pv;
-        if (more) {
-          pk = pk1, pv = pv1;
-          load_k(tn, pk);
-          if (i + 2 * AT_WAVES < i1) lookup(tiles.at(i + 2 * AT_WAVES) * TILE, pk1, pv1);
-        }
-        // what a row does not see: only in the tiles at the ends of what the rows see
-        const bool masked = t0 + TILE - 1 > pos_lo || (a.window > 0 && int64_t(t0) + a.window <= pos_hi && t0 + TILE > a.sinks) ||
-                            __any(pvt < 0);
-        uint32_t see[RT];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          see[r] = 0xffff;
-          float top = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s[r][j][e] *= a.scale2;
-              if (masked) {
-                const int t = t0 + 16 * g + 4 * j + e;
-                if (pvt < 0 || !visible(pos[r], t, a.window, a.sinks)) {
-                  s[r][j][e] = -INFINITY;
-                  see[r] &= ~(1u << (4 * j + e));
-                }
-              }
-              top = fmaxf(top, s[r][j][e]);
-            }
-          top = fmaxf(top, __shfl_xor(top, 16, 64));
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float m1 = fmaxf(mx[r], top), ref = m1 == -INFINITY ? 0.0f : m1;
-          const float al = __builtin_amdgcn_exp2f(mx[r] - ref);
-          if (__any(m1 != mx[r])) {
-#pragma unroll
-            for (int d = 0; d < S::DT; ++d) o[r][d] *= al;
-            l[r] *= al;
-          }
-          mx[r] = m1;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s[r][j][e] = __builtin_amdgcn_exp2f(s[r][j][e] - ref);
-              l[r] += s[r][j][e];
-            }
-        }
-        bool nans = false;
-        if (masked) {  // slots past the last token hold anything: zero; NaN among the values that some row sees: below
-          const int n = pvt < 0 ? 0 : min(max(q.len - (t0 + 16 * g), 0), 16);
-          uint32_t keep[4], bad = 0;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) keep[w] = n >= 4 * w + 4 ? ~0u : n <= 4 * w ? 0u : (1u << (8 * (n - 4 * w))) - 1;
-#pragma unroll
-          for (int d = 0; d < S::DT; ++d) {
-            vr[d].x &= keep[0], vr[d].y &= keep[1], vr[d].z &= keep[2], vr[d].w &= keep[3];
-            bad |= nan_bytes(vr[d].x) | nan_bytes(vr[d].y) | nan_bytes(vr[d].z) | nan_bytes(vr[d].w);
-          }
-          nans = __any(bad != 0);
-        }
-        bf16x8 p[RT][2];
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[r][hf][e] = __bf16(s[r][2 * hf + e / 4][e % 4]);
-        if (!nans) {
-#pragma unroll
-          for (int d = 0; d < S::DT; ++d) {
-            const bf16x8 v0 = fp8x8_to_bf16(vr[d].x, vr[d].y, vs), v1 = fp8x8_to_bf16(vr[d].z, vr[d].w, vs);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-              o[r][d] = mfma_bf16(v0, p[r][0], o[r][d]);
-              o[r][d] = mfma_bf16(v1, p[r][1], o[r][d]);
-            }
-          }
-        } else {
-          // 0 x NaN is NaN: the NaN values are taken out, and a product of 0 / 1 operands counts for each row and channel
-          // the NaN that it sees.
-#pragma unroll
-          for (int d = 0; d < S::DT; ++d) {
-            uint32_t x[4] = {vr[d].x, vr[d].y, vr[d].z, vr[d].w};
-            bf16x8 nv[2];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t nb = nan_bytes(x[w]) >> 7;  // 0 / 1 in each byte
-              x[w] &= ~(nb * 0xffu);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) nv[w / 2][w % 2 * 4 + e] = __bf16(float(nb >> (8 * e) & 1));
-            }
-            const bf16x8 v0 = fp8x8_to_bf16(x[0], x[1], vs), v1 = fp8x8_to_bf16(x[2], x[3], vs);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-              bf16x8 sv[2];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) sv[e / 8][e % 8] = __bf16(float(see[r] >> e & 1));
-              v4f n = mfma_bf16(nv[0], sv[0], v4f{0, 0, 0, 0});
-              n = mfma_bf16(nv[1], sv[1], n);
-              o[r][d] = mfma_bf16(v0, p[r][0], o[r][d]);
-              o[r][d] = mfma_bf16(v1, p[r][1], o[r][d]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (n[e] > 0.0f) o[r][d][e] = __builtin_nanf("");
-            }
-          }
-        }
-        if (more) load_v(tn, pv);
-      }
-
-      // join the four waves
-      __syncthreads();  // the last segment's use of the LDS
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        l[r] += __shfl_xor(l[r], 16, 64);
-        l[r] += __shfl_xor(l[r], 32, 64);
-        if (g == 0) lds.ml[wave][16 * r + c][0] = mx[r], lds.ml[wave][16 * r + c][1] = l[r];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < AT_WAVES; ++w) m = fmaxf(m, lds.ml[w][16 * r + c][0]);
-        const float ref = m == -INFINITY ? 0.0f : m, f = __builtin_amdgcn_exp2f(mx[r] - ref);
-        l[r] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < AT_WAVES; ++w)
-          l[r] += lds.ml[w][16 * r + c][1] * __builtin_amdgcn_exp2f(lds.ml[w][16 * r + c][0] - ref);
-        mx[r] = m;
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) o[r][d] *= f;
-      }
-      const auto put = [&](float* to) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int d = 0; d < S::DT; ++d)
-            *reinterpret_cast<v4f*>(to + ((r * S::DT + d) * 64 + lane) * 4) = o[r][d];
-      };
-      const auto add = [&](const float* from) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int d = 0; d < S::DT; ++d)
-            o[r][d] += *reinterpret_cast<const v4f*>(from + ((r * S::DT + d) * 64 + lane) * 4);
-      };
-      if (wave >= 2) put(lds.o[wave - 2]);
-      __syncthreads();
-      if (wave < 2) add(lds.o[wave]);
-      __syncthreads();
-      if (wave == 1) put(lds.o[0]);
-      __syncthreads();
-      if (wave == 0) {
-        add(lds.o[0]);
-        const bool whole = i0 == 0 && i1 == tiles.count;
-        const size_t slot = size_t(blockIdx.x) * 2 + (i0 == 0 ? 1 : 0);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const int ri = row0 + 16 * r + c;
-          if (whole) {
-            if (ri >= nrows) continue;
-            const int row = q.r0 + ri / a.group, hq = h * a.group + ri % a.group;
-            const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
-            bf16* y = a.out + size_t(row) * a.ldo + size_t(hq) * D + 4 * g;
-#pragma unroll
-            for (int d = 0; d < S::DT; ++d) {
-              uint16_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = f32_to_bf16(l[r] == 0.0f ? 0.0f : o[r][d][e] * inv);
-              *reinterpret_cast<uint2*>(y + 16 * d) =
-                  make_uint2(uint32_t(w[0]) | uint32_t(w[1]) << 16, uint32_t(w[2]) | uint32_t(w[3]) << 16);
-            }
-            if (a.lse && g == 0)
-              a.lse[size_t(row) * (a.group * a.c.heads) + hq] = l[r] == 0.0f ? -INFINITY : mx[r] * LN2 + logf(l[r]);
-          } else {
-            float* y = a.po + (slot * S::ROWS + 16 * r + c) * D + 4 * g;
-#pragma unroll
-            for (int d = 0; d < S::DT; ++d) *reinterpret_cast<v4f*>(y + 16 * d) = o[r][d];
-            if (g == 0) {
-              float* ml = a.pml + (slot * S::ROWS + 16 * r + c) * 2;
-              ml[0] = mx[r];
-              ml[1] = l[r];
-            }
-          }
-        }
-      }
-    }
-    base += in_b;
-  }
+// Partial sums pass between workgroups on different XCDs, whose L2 caches do not see each other's lines: stored through
+// to memory and read from there (device-scope accesses), which for these few KiB is far cheaper than the fences that
+// write back and invalidate a whole L2 (a layer of a single-token step over 4097 tokens, 17 pieces a
+// head: 25.0 us with fences, 13.9 with these).
+constexpr int SC1 = 16;  // the cache policy of a device-scope access
+constexpr int JOIN = 8;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t sums_of(float* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00027000);
+}
+__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t p, int at, v4f v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(__attribute__((ext_vector_type(4))) unsigned, v), p, at * 4, 0,
+                                         SC1);
+}
+__device__ __forceinline__ void put2(__amdgpu_buffer_rsrc_t p, int at, float x, float y) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(x), __float_as_uint(y)}, p, at * 4, 0, SC1);
+}
+__device__ __forceinline__ v4f get4(__amdgpu_buffer_rsrc_t p, int at) {
+  return __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(p, at * 4, 0, SC1));
+}
+__device__ __forceinline__ float2 get2(__amdgpu_buffer_rsrc_t p, int at) {
+  const auto v = __builtin_amdgcn_raw_buffer_load_b64(p, at * 4, 0, SC1);
+  return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
 }
 
-// Rows of sequences without a tile: zero. Rows whose tiles went to several workgroups: their partial sums, in the order of the tiles. A workgroup per row and
-// query head; D / 4 lanes hold a partial row, the 1024 / D groups of them take every such partial in turn.
-template <int D, int ROWS>
-__global__ __launch_bounds__(AT_NT) void kv_join_kernel(Attend a, int wgs) {
-  __shared__ int64_t wsum[AT_WAVES];
-  __shared__ int64_t at_b;
-  constexpr int LANES = D / 4, GROUPS = AT_NT / LANES;
-  __shared__ __align__(16) float red[GROUPS][D];
-  __shared__ float redm[AT_WAVES], redl[GROUPS];
-  const int tid = threadIdx.x, row = blockIdx.x, hq = blockIdx.y, h = hq / a.group;
-  int lo = 0, hi = a.st.B;  // the sequence of this row: the first one that ends behind it
-  while (lo < hi) {
-    const int m = (lo + hi) / 2;
-    if (a.st.cu[m + 1] <= row) lo = m + 1; else hi = m;
-  }
-  const int b = lo;
-  if (b >= a.st.B) return;
-  const Seq q = seq_of(a.st, b);
-  if (row < q.r0 || row >= q.r1) return;
-  const int tiles = tiles_of(a, q).count;
-  bf16* y = a.out + size_t(row) * a.ldo + size_t(hq) * D;
-  float* lse = a.lse ? a.lse + size_t(row) * (a.group * a.c.heads) + hq : nullptr;
-  if (tiles == 0) {
-    if (tid < D) y[tid] = 0;
-    if (tid == 0 && lse) *lse = -INFINITY;
-    return;
-  }
-  int64_t total = 0, sum;
-  int rg;
-  for (int b0 = 0; b0 < a.st.B; b0 += AT_NT) {
-    const int64_t mine = b0 + tid < a.st.B ? units_of<ROWS>(a, b0 + tid, rg) : 0;
-    const int64_t before = total + scan64(mine, wsum, sum);
-    if (b0 + tid == b) at_b = before;
-    total += sum;
-  }
-  __syncthreads();
-  const int64_t share = share_of(total, wgs);
-  const int ri = (row - q.r0) * a.group + hq % a.group;
-  rg = row_groups((q.r1 - q.r0) * a.group, ROWS);
-  const int64_t s0 = at_b + (int64_t(h) * rg + ri / ROWS) * tiles, s1 = s0 + tiles;
-  const int w0 = int(s0 / share), w1 = int((s1 - 1) / share), n = w1 - w0 + 1;
-  if (n == 1) return;  // written by the one workgroup that had them all
-  // in the workgroup that begins these rows they are its range's last, in the others the first
-  const auto slot = [&](int i) { return (size_t(w0 + i) * 2 + (i == 0)) * ROWS + ri % ROWS; };
-  float m = -INFINITY;
-  for (int i = tid; i < n; i += AT_NT) m = fmaxf(m, a.pml[slot(i) * 2]);
-  m = wave_max(m);
-  if ((tid & 63) == 0) redm[tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
-  const float ref = m == -INFINITY ? 0.0f : m;
-  const int grp = tid / LANES, d = tid % LANES * 4;
-  v4f acc{0, 0, 0, 0};
-  float l = 0.0f;
-  for (int i = grp; i < n; i += GROUPS) {
-    const size_t sl = slot(i);
-    const float f = __builtin_amdgcn_exp2f(a.pml[sl * 2] - ref);
-    l += f * a.pml[sl * 2 + 1];
-    acc += f * *reinterpret_cast<const v4f*>(a.po + sl * D + d);
-  }
-  *reinterpret_cast<v4f*>(&red[grp][d]) = acc;
-  if (tid % LANES == 0) redl[grp] = l;
-  __syncthreads();
-  if (tid >= LANES) return;
-#pragma unroll
-  for (int i = 1; i < GROUPS; ++i) {
-    acc += *reinterpret_cast<const v4f*>(&red[i][d]);
-    l += redl[i];
-  }
+template <int D>
+__device__ __forceinline__ void store_out(const Attend& a, int row, int hq, int d, v4f o, float l, float m, bool first) {
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t w[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = f32_to_bf16(l == 0.0f ? 0.0f : acc[e] * inv);
-  *reinterpret_cast<uint2*>(y + d) = make_uint2(uint32_t(w[0]) | uint32_t(w[1]) << 16, uint32_t(w[2]) | uint32_t(w[3]) << 16);
-  if (tid == 0 && lse) *lse = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
+  for (int e = 0; e < 4; ++e) w[e] = f32_to_bf16(l == 0.0f ? 0.0f : o[e] * inv);
+  *reinterpret_cast<uint2*>(a.out + size_t(row) * a.ldo + size_t(hq) * D + d) =
+      make_uint2(uint32_t(w[0]) | uint32_t(w[1]) << 16, uint32_t(w[2]) | uint32_t(w[3]) << 16);
+  if (first && a.lse) a.lse[size_t(row) * (a.group * a.c.heads) + hq] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
 }
 
-// The shape of a split launch: row tiles a wave, and as many workgroups as the chip holds at a time.
-struct SplitShape {
-  int rt, wgs;
-  size_t slots() const { return size_t(wgs) * 2 * 16 * rt; }
-};
-SplitShape split_shape(int dim, int rows) {
-  const int rt = rows <= 16 ? 1 : rows <= 32 || dim == 256 ? 2 : 4;
-  return {rt, 256 * wgs_per_cu(dim, rt)};
+template <int D, int RW>
+__global__ __launch_bounds__(AT_NT, 2) void kv_split_kernel(Attend a) {
+  using S = Split<D, RW>;
+  constexpr int J = S::J, TOK = S::TOK, TW = S::TW;
+  __shared__ __align__(16) typename S::Lds lds;
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+  Piece pc;
+  Seq q;
+  Tiles tiles;
+  if (!find_piece<S::ROWS, TW>(a, pc, q, tiles)) return;
+  const int b = pc.b, h = pc.h, nrows = (q.r1 - q.r0) * a.group, row0 = pc.rg * S::ROWS + wave / TW * 16;
+
+  // this lane's row (the last one where there are fewer): its position
+  const int ri = min(row0 + c, nrows - 1), my_row = q.r0 + ri / a.group, my_hq = h * a.group + ri % a.group;
+  const int pos = q.first + ri / a.group;
+  const int pos_lo = q.first + min(row0, nrows - 1) / a.group;  // of the wave's rows
+  const int pos_hi = q.first + min(row0 + 15, nrows - 1) / a.group;
+
+  v4f o[S::DT];
+  float mx = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < S::DT; ++d) o[d] = v4f{0, 0, 0, 0};
+
+  const int mask = a.c.page - 1, sh = a.page_shift;
+  const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
+    pk = page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (t0 + 4 * J * (c >> 2)) >> sh);
+    pv = page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (t0 + 4 * J * g) >> sh);
+  };
+  uint4 kr[J][S::KL];
+  uint32_t vr[S::DT][J];
+  int ksb, vsb;
+  const auto load_k = [&](int t0, int pk) {
+    const size_t ph = size_t(max(pk, 0)) * a.c.heads + h;
+    const uint8_t* p = a.c.k + ((ph << sh) + ((t0 + 4 * J * (c >> 2) + (c & 3)) & mask)) * D + 16 * g;
+    ksb = a.c.ks[ph];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int m = 0; m < S::KL; ++m) kr[j][m] = ld16(p + 4 * j * D + 64 * m);
+  };
+  const auto load_v = [&](int t0, int pv) {
+    const size_t ph = size_t(max(pv, 0)) * a.c.heads + h;
+    const uint8_t* p = a.c.v + ((ph * D + c) << sh) + ((t0 + 4 * J * g) & mask);
+    vsb = a.c.vs[ph];
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+      p += 16 << sh;
+      if constexpr (J == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(w);
+        vr[d][0] = x.x, vr[d][1] = x.y, vr[d][2] = x.z, vr[d][3] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(w);
+        vr[d][0] = x.x, vr[d][1] = x.y;
+      }
+    }
+  };
+  // a 64-token tile is 64 / TOK steps; steps go to the waves in turn
+  constexpr int PER = TILE / TOK;
+  const auto token = [&](int i) { return tiles.at(i / PER) * TILE + i % PER * TOK; };
+  const int i1 = pc.i1 * PER;
+  int i = pc.i0 * PER + wave % TW, pk = 0, pv = 0, pk1 = 0, pv1 = 0;
+  if (row0 >= nrows) i = i1;  // no rows for this wave
+  if (i < i1) lookup(token(i), pk, pv);
+  bf16x8 qf[2 * S::KL];
+  {
+    const bf16* x = a.q + size_t(my_row) * a.ldq + size_t(my_hq) * D + 16 * g;
+#pragma unroll
+    for (int m = 0; m < S::KL; ++m) {
+      qf[2 * m] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m));
+      qf[2 * m + 1] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m + 8));
+    }
+  }
+  if (i < i1) {
+    load_k(token(i), pk);
+    load_v(token(i), pv);
+    if (i + TW < i1) lookup(token(i + TW), pk1, pv1);
+  }
+  for (; i < i1; i += TW) {
+    const int t0 = token(i);
+    const bool more = i + TW < i1;
+    const int tn = token(more ? i + TW : i);
+    const float ks = e8m0_to_f32(uint8_t(ksb));
+    v4f s[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      s[j] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int m = 0; m < S::KL; ++m) {
+        s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].x, kr[j][m].y, ks), qf[2 * m], s[j]);
+        s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].z, kr[j][m].w, ks), qf[2 * m + 1], s[j]);
+      }
+    }
+    const int pvt = pv;
+    if (more) {
+      pk = pk1, pv = pv1;
+      load_k(tn, pk);
+      if (i + 2 * TW < i1) lookup(token(i + 2 * TW), pk1, pv1);
+    }
+    // what a row does not see: only in the tiles at the ends of what the rows see
+    const bool masked = t0 + TOK - 1 > pos_lo || __any(pvt < 0) ||
+                        (a.window > 0 && int64_t(t0) + a.window <= pos_hi && t0 + TOK > a.sinks);
+    uint32_t see = 0xffff;
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] *= a.scale2;
+    if (masked) {
+      see = pvt < 0 ? 0 : seen_bits(pos, t0 + 4 * J * g, a.window, a.sinks);
+#pragma unroll
+      for (int k = 0; k < 4 * J; ++k) s[k / 4][k % 4] = see >> k & 1 ? s[k / 4][k % 4] : -INFINITY;
+    }
+#pragma unroll
+    for (int k = 0; k < 4 * J; ++k) top = fmaxf(top, s[k / 4][k % 4]);
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float m1 = fmaxf(mx, top), ref = m1 == -INFINITY ? 0.0f : m1;
+    if (__any(m1 != mx)) {
+      const float al = __builtin_amdgcn_exp2f(mx - ref);
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) o[d] *= al;
+      l *= al;
+    }
+    mx = m1;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[j][e] = __builtin_amdgcn_exp2f(s[j][e] - ref);
+        l += s[j][e];
+      }
+    const float vs = e8m0_to_f32(uint8_t(vsb));
+    bf16x8 p[J / 2];
+#pragma unroll
+    for (int hf = 0; hf < J / 2; ++hf)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[hf][e] = __bf16(s[2 * hf + e / 4][e % 4]);
+    uint32_t bad = 0;
+    if (masked) {  // slots past the last token hold anything: zero; NaN among the values that some row sees: below
+      const int n = pvt < 0 ? 0 : min(max(q.len - (t0 + 4 * J * g), 0), 4 * J);
+#pragma unroll
+      for (int k = 0; k < J; ++k) {
+        const uint32_t keep = n >= 4 * k + 4 ? ~0u : n <= 4 * k ? 0u : (1u << (8 * (n - 4 * k))) - 1;
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) {
+          vr[d][k] &= keep;
+          bad |= nan_bytes(vr[d][k]);
+        }
+      }
+    }
+    if (__builtin_expect(!__any(bad != 0), 1)) {
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+        for (int hf = 0; hf < J / 2; ++hf)
+          o[d] = mfma_bf16(fp8x8_to_bf16(vr[d][2 * hf], vr[d][2 * hf + 1], vs), p[hf], o[d]);
+    } else {
+      // 0 x NaN is NaN: the NaN values are taken out, and a product of 0 / 1 operands counts for each row and channel the
+      // NaN that it sees.
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) {
+        v4f n{0, 0, 0, 0};
+#pragma unroll
+        for (int hf = 0; hf < J / 2; ++hf) {
+          bf16x8 nv, sv;
+          uint32_t x[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t nb = nan_bytes(vr[d][2 * hf + k]) >> 7;  // 0 / 1 in each byte
+            x[k] = vr[d][2 * hf + k] & ~(nb * 0xffu);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              nv[4 * k + e] = __bf16(float(nb >> (8 * e) & 1));
+              sv[4 * k + e] = __bf16(float(see >> (8 * hf + 4 * k + e) & 1));
+            }
+          }
+          n = mfma_bf16(nv, sv, n);
+          o[d] = mfma_bf16(fp8x8_to_bf16(x[0], x[1], vs), p[hf], o[d]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n[e] > 0.0f) o[d][e] = __builtin_nanf("");
+      }
+    }
+    if (more) load_v(tn, pv);
+  }
+
+  // join the waves that share rows
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if constexpr (TW > 1) {
+    if (g == 0) lds.ml[wave][c][0] = mx, lds.ml[wave][c][1] = l;
+    __syncthreads();
+    const int w0 = wave / TW * TW;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < TW; ++w) m = fmaxf(m, lds.ml[w0 + w][c][0]);
+    const float ref = m == -INFINITY ? 0.0f : m, f = __builtin_amdgcn_exp2f(mx - ref);
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < TW; ++w) l += lds.ml[w0 + w][c][1] * __builtin_amdgcn_exp2f(lds.ml[w0 + w][c][0] - ref);
+    mx = m;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) o[d] *= f;
+    const auto at = [&](int buf, int d) { return reinterpret_cast<v4f*>(&lds.o[buf][(d * 64 + lane) * 4]); };
+#pragma unroll
+    for (int half = TW / 2; half; half /= 2) {  // the upper half of the waves hands its sums to the lower
+      const int k = wave % TW, buf = wave / TW * (TW / 2) + k % half;
+      if (k >= half && k < 2 * half)
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) *at(buf, d) = o[d];
+      __syncthreads();
+      if (k < half)
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) o[d] += *at(buf, d);
+      __syncthreads();
+    }
+  }
+  const bool mine = wave % TW == 0 && row0 + c < nrows;
+  if (pc.pieces == 1) {
+    if (mine)
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) store_out<D>(a, my_row, my_hq, 16 * d + 4 * g, o[d], l, mx, d == 0 && g == 0);
+    return;
+  }
+  if (mine) {
+    const int r = (pc.slot0 + pc.index) * S::ROWS + wave / TW * 16 + c;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) put4(sums_of(a.po), r * D + 4 * g + 16 * d, o[d]);
+    if (g == 0) put2(sums_of(a.pml), r * 2, mx, l);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
+  __syncthreads();
+  if (tid == 0)
+    last = __hip_atomic_fetch_add(&a.counters[pc.slot0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           uint32_t(pc.pieces - 1);
+  __syncthreads();
+  if (!last) return;
+  if (tid == 0)  // as it was found
+    __hip_atomic_store(&a.counters[pc.slot0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // a thread per row and four channels, the loads of eight pieces in flight at a time
+  const int rows = min(S::ROWS, nrows - pc.rg * S::ROWS);
+  const __amdgpu_buffer_rsrc_t po = sums_of(a.po + size_t(pc.slot0) * S::ROWS * D);
+  const __amdgpu_buffer_rsrc_t pml = sums_of(a.pml + size_t(pc.slot0) * S::ROWS * 2);
+  for (int it = tid; it < rows * (D / 4); it += AT_NT) {
+    const int r = it / (D / 4), d = it % (D / 4) * 4;
+    float m = -INFINITY, sum = 0.0f;
+    v4f acc{0, 0, 0, 0};
+    for (int k0 = 0; k0 < pc.pieces; k0 += JOIN) {
+      v4f y[JOIN];
+      float2 x[JOIN];
+#pragma unroll
+      for (int k = 0; k < JOIN; ++k) {
+        const int at = min(k0 + k, pc.pieces - 1) * S::ROWS + r;
+        x[k] = get2(pml, at * 2);
+        y[k] = get4(po, at * D + d);
+      }
+      float m1 = m;
+#pragma unroll
+      for (int k = 0; k < JOIN; ++k) m1 = fmaxf(m1, x[k].x);
+      const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m - ref);
+      m = m1;
+      acc *= al;
+      sum *= al;
+#pragma unroll
+      for (int k = 0; k < JOIN; ++k) {
+        const float f = k0 + k < pc.pieces ? __builtin_amdgcn_exp2f(x[k].x - ref) : 0.0f;
+        if (k0 + k < pc.pieces) {
+          sum += f * x[k].y;
+          acc += f * y[k];
+        }
+      }
+    }
+    const int rr = pc.rg * S::ROWS + r;
+    store_out<D>(a, q.r0 + rr / a.group, h * a.group + rr % a.group, d, acc, sum, m, d == 0);
+  }
 }
+
 int most_rows(int rows, int max_new, int group) {
   return int(std::min<int64_t>(int64_t(std::min(rows, max_new)) * group, INT32_MAX));
 }
+int row_waves(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
 }  // namespace
 
 size_t kv_attend_workspace(int rows, int max_new, int B, int Hq, int heads, int dim) {
   if (rows < 0 || max_new < 0 || B < 0 || heads < 1 || Hq < heads || dim < 1) return 0;
-  return split_shape(dim, most_rows(rows, max_new, Hq / heads)).slots() * (size_t(dim) + 2) * sizeof(float);
+  const int rw = row_waves(most_rows(rows, max_new, Hq / heads));
+  return kCounterBytes + size_t(slots_of(rw)) * 16 * rw * (size_t(dim) + 2) * sizeof(float);
 }
 
 void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks,
@@ -550,25 +529,26 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
   if (!aligned16(ws)) fail("workspace not 16-byte aligned");
   if (ws_bytes < need) fail("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
 
-  Attend a{q, out, lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E, nullptr, nullptr};
+  Attend a{q, out, lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E, kTarget, 1, nullptr,
+           nullptr, nullptr};
   while (1 << a.page_shift < c.page) ++a.page_shift;
-  const SplitShape shape = split_shape(c.dim, most_rows(s.rows, s.max_new, a.group));
-  a.po = static_cast<float*>(ws);
-  a.pml = a.po + shape.slots() * c.dim;
-  const auto go = [&]<int D, int RT>() {
-    kv_split_kernel<D, RT><<<unsigned(shape.wgs), AT_NT, 0, st>>>(a);
-    UH_CHECK_LAUNCH();
-    kv_join_kernel<D, 16 * RT><<<dim3(unsigned(s.rows), unsigned(Hq)), AT_NT, 0, st>>>(a, shape.wgs);
-    UH_CHECK_LAUNCH();
+  const int rows = most_rows(s.rows, s.max_new, a.group), rw = row_waves(rows);
+  a.counters = static_cast<uint32_t*>(ws);
+  a.po = reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes);
+  a.pml = a.po + size_t(slots_of(rw)) * 16 * rw * c.dim;
+  a.rounds = rounds_of(rw);
+  const int64_t segs = int64_t(s.B) * c.heads * cdiv(rows, 16 * rw);  // at most; each is a piece too many at most
+  if (segs + kMostSlots > INT32_MAX) fail("too many rows");
+  const unsigned grid = unsigned(segs + a.target * a.rounds);
+  const auto by_rw = [&]<int D>() {
+    if (rw == 1) kv_split_kernel<D, 1><<<grid, AT_NT, 0, st>>>(a);
+    else if (rw == 2) kv_split_kernel<D, 2><<<grid, AT_NT, 0, st>>>(a);
+    else kv_split_kernel<D, 4><<<grid, AT_NT, 0, st>>>(a);
   };
-  const auto by_rt = [&]<int D>() {
-    if (shape.rt == 1) go.template operator()<D, 1>();
-    else if (shape.rt == 2 || D == 256) go.template operator()<D, 2>();
-    else if constexpr (D < 256) go.template operator()<D, 4>();
-  };
-  if (c.dim == 64) by_rt.template operator()<64>();
-  else if (c.dim == 128) by_rt.template operator()<128>();
-  else by_rt.template operator()<256>();
+  if (c.dim == 64) by_rw.template operator()<64>();
+  else if (c.dim == 128) by_rw.template operator()<128>();
+  else by_rw.template operator()<256>();
+  UH_CHECK_LAUNCH();
 }
 
 }  // namespace unholy::kernels
