@@ -5,6 +5,7 @@
 
 #include "kv_internal.hpp"
 #include "numerics.hpp"
+#include "pipe.hpp"
 
 namespace unholy::kernels {
 
@@ -23,7 +24,7 @@ __device__ __forceinline__ uint32_t first_bits(int n) { return (1u << min(max(n,
 // Which of the 16 tokens from t on a row at position p sees.
 __device__ __forceinline__ uint32_t seen_bits(int p, int t, int window, int sinks) {
   uint32_t see = first_bits(p - t + 1);
-  if (window > 0) see &= ~first_bits(int(min(int64_t(p) - window - t + 1, int64_t(16)))) | first_bits(sinks - t);
+  if (window > 0) see &= ~first_bits(int(max(min(int64_t(p) - window - t + 1, int64_t(16)), int64_t(0)))) | first_bits(sinks - t);
   return see;
 }
 // Inclusive sum over the wave's lanes (all active): DPP shifts within rows of 16, then the rows' last lanes.
@@ -50,9 +51,9 @@ struct Attend {
   KvCache c;
   int ldq, ldo, group, page_shift, window, sinks;
   float scale2;  // scale * log2(e): the kernels take powers of two
-  int target;    // workgroups that the chip holds at a time
-  int rounds;    // of them, where segments are many
-  uint32_t* counters;  // of finished pieces, [slot]; zero between launches
+  int few;             // sequences of up to this many rows are the split kernel's, the others the tiled kernel's
+  uint32_t target;     // workgroups that the chip holds at a time
+  uint32_t* counters;  // of finished parts, by the workgroup of the first; zero between launches
   float *po, *pml;     // partial sums: values [slot][ROWS][D]; maximum and weight sum [slot][ROWS][2]
 };
 
@@ -76,73 +77,120 @@ __device__ __forceinline__ Tiles tiles_of(const Attend& a, const Seq& q) {
 }
 __device__ __forceinline__ int row_groups(int rows, int per) { return (rows + per - 1) / per; }
 
-// The split of a launch's work, worked out by every workgroup from the lengths, which only the device knows: a segment is
-// a (sequence, key / value head, row group) and its tiles; each is cut into pieces of at most `share` tiles, as equal as
-// they can be, a workgroup each. share makes about `target` pieces, so that long and short sequences load the chip evenly.
-// A segment of several pieces leaves partial sums in slots slot0 .. slot0 + pieces - 1: with u the tiles before it in the
-// launch and f = u / share, slots from 2 f on, of which there are 2 (f' - f) >= 2 floor(tiles / share) >= pieces before the
-// next segment's.
-struct Piece {
-  int b, h, rg, index, pieces, i0, i1, slot0;
+// The split of a launch's work, worked out by every workgroup from the lengths, which only the device knows. A segment is a
+// (sequence, key / value head, row group) and its tiles.
+// Many segments: workgroup w takes the tiles [w share, (w + 1) share) of all segments in order, so that long and short
+// sequences load the chip evenly; it may end one segment, do some whole ones and begin another.
+// Few segments (each would cost a workgroup that has the end of one and the beginning of another a start more than
+// those next to it): each is cut into parts as equal as they can be, a workgroup each.
+// The parts of a segment are those of consecutive workgroups; the part of workgroup w that begins a segment leaves its sums
+// in slot 2 w + 1, one that goes on with it in slot 2 w.
+struct Walk {
+  int b, segs, rgs, seg;  // the sequence, its segments, its row groups, the segment
+  uint32_t at;            // where the segment begins, in units (tiles, or parts of equal segments)
+  Seq q;
+  Tiles t;
 };
-__device__ __forceinline__ uint32_t pieces_of(uint32_t tiles, uint32_t share) {
-  return max((tiles + share - 1) / share, 1u);  // (no tiles: a piece that writes zeros)
+struct Part {
+  int h, rg, i0, i1, index, parts;
+};
+constexpr uint32_t START = 2;  // a segment's start, in tiles: the time that its first loads and its end take
+struct Split {
+  bool whole;            // few segments
+  uint32_t share, unit;  // tiles of a part at most; units of a workgroup
+};
+__device__ __forceinline__ uint32_t units_of(const Split& s, uint32_t tiles) {
+  return s.whole ? max((tiles + s.share - 1) / s.share, 1u) : tiles + START;  // (no tiles: a part that writes zeros)
 }
-// Every wave for itself, a sequence a lane: no barriers, and for up to 64 sequences one pass over registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+template <int ROWS>
+__device__ __forceinline__ int segs_of(const Attend& a, const Seq& q) {
+  const int rows = (q.r1 - q.r0) * a.group;
+  return rows <= a.few ? row_groups(rows, ROWS) * a.c.heads : 0;
+}
+// The segment that holds the workgroup's first unit. Every wave for itself, a sequence a lane: no barriers, and for up to 64
+// sequences one pass over registers.
 template <int ROWS, int LEAST>
-__device__ __forceinline__ bool find_piece(const Attend& a, Piece& p, Seq& q, Tiles& t) {
+__device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w) {
   const int lane = threadIdx.x & 63;
-  Tiles mt{0, 0, 0};
   uint32_t segs = 0;  // of this lane's sequence
   const auto look = [&](int b) {
     segs = 0;
-    mt = Tiles{0, 0, 0};
+    w.t = Tiles{0, 0, 0};
     if (b < a.st.B) {
-      q = seq_of(a.st, b);
-      segs = uint32_t(row_groups((q.r1 - q.r0) * a.group, ROWS)) * a.c.heads;
-      if (segs) mt = tiles_of(a, q);
+      w.q = seq_of(a.st, b);
+      segs = uint32_t(segs_of<ROWS>(a, w.q));
+      if (segs) w.t = tiles_of(a, w.q);
     }
   };
-  float tiles = 0.0f;
-  uint32_t all = 0;
+  uint32_t tiles = 0, all = 0;
   for (int b0 = 0; b0 < a.st.B; b0 += 64) {
     look(b0 + lane);
-    tiles += wave_sum(float(mt.count) * float(segs));
+    tiles += lane_of(wave_scan(segs * (uint32_t(w.t.count) + START)), 63);
     all += lane_of(wave_scan(segs), 63);
   }
-  // about `target` pieces where the segments are few, one round of the chip; else more and smaller ones than it holds, which
-  // even out as they come and go
-  const float want = float(all <= uint32_t(a.target) / 2 ? a.target - int(all) : a.target * a.rounds);
-  // (past 2^31 tiles the prefix below would wrap: no segment is cut then)
-  const uint32_t share = tiles < 2.0e9f ? max(uint32_t(ceilf(tiles * 1.0001f / want)), uint32_t(LEAST)) : 1u << 30;
-  uint32_t wg0 = 0, u0 = 0;
+  s.whole = all * 8 <= a.target;
+  const uint32_t wgs = s.whole ? a.target - all : a.target;
+  s.share = max((tiles + wgs - 1) / wgs, uint32_t(LEAST));
+  s.unit = s.whole ? 1 : s.share;
+  const uint32_t u = blockIdx.x * s.unit;
+  uint32_t from = 0;
   for (int b0 = 0; b0 < a.st.B; b0 += 64) {
     if (a.st.B > 64) look(b0 + lane);
-    const uint32_t n = segs * pieces_of(uint32_t(mt.count), share), u = segs * uint32_t(mt.count);
-    const uint32_t wg_end = wg0 + wave_scan(n), u_end = u0 + wave_scan(u);
-    const uint64_t hit = __ballot(blockIdx.x < wg_end);
+    const uint32_t each = units_of(s, uint32_t(w.t.count)), n = segs * each, end = from + wave_scan(n);
+    const uint64_t hit = __ballot(u < end);
     if (hit) {
       const int l = __ffsll((unsigned long long)hit) - 1;  // (a lane of no segments ends where the one before it does)
-      p.b = b0 + l;
-      q = Seq{int(lane_of(q.r0, l)), int(lane_of(q.r1, l)), int(lane_of(q.len, l)), int(lane_of(q.first, l))};
-      t = Tiles{int(lane_of(mt.sink_tiles, l)), int(lane_of(mt.skip, l)), int(lane_of(mt.count, l))};
-      const uint32_t sg = lane_of(segs, l), first = lane_of(wg_end - n, l), ut = lane_of(u_end - u, l);
-      const uint32_t rgs = sg / uint32_t(a.c.heads), pieces = pieces_of(uint32_t(t.count), share);
-      const uint32_t in = blockIdx.x - first, seg = in / pieces, i = in % pieces;
-      const uint32_t each = uint32_t(t.count) / pieces, more = uint32_t(t.count) % pieces;
-      p.index = int(i);
-      p.pieces = int(pieces);
-      p.h = int(seg / rgs);
-      p.rg = int(seg % rgs);
-      p.i0 = int(i * each + min(i, more));
-      p.i1 = p.i0 + int(each + (i < more ? 1 : 0));
-      p.slot0 = int((ut + seg * uint32_t(t.count)) / share * 2);
+      w.b = b0 + l;
+      w.q = Seq{int(lane_of(w.q.r0, l)), int(lane_of(w.q.r1, l)), int(lane_of(w.q.len, l)), int(lane_of(w.q.first, l))};
+      w.t = Tiles{int(lane_of(w.t.sink_tiles, l)), int(lane_of(w.t.skip, l)), int(lane_of(w.t.count, l))};
+      w.segs = int(lane_of(segs, l));
+      w.rgs = w.segs / a.c.heads;
+      const uint32_t first = lane_of(end - n, l), size = lane_of(each, l);
+      w.seg = int((u - first) / size);
+      w.at = first + uint32_t(w.seg) * size;
       return true;
     }
-    wg0 = lane_of(wg_end, 63);
-    u0 = lane_of(u_end, 63);
+    from = lane_of(end, 63);
   }
   return false;
+}
+// The workgroup's part of the segment, from unit u on.
+__device__ __forceinline__ Part part_of(const Split& s, const Walk& w, uint32_t u) {
+  Part p;
+  const uint32_t count = uint32_t(w.t.count), size = units_of(s, count), w0 = w.at / s.unit;
+  p.h = w.seg / w.rgs;
+  p.rg = w.seg % w.rgs;
+  p.index = int(blockIdx.x - w0);
+  p.parts = int((w.at + size - 1) / s.unit - w0 + 1);
+  if (s.whole) {
+    const uint32_t each = count / size, more = count % size, i = uint32_t(p.index);
+    p.i0 = int(i * each + min(i, more));
+    p.i1 = p.i0 + int(each + (i < more ? 1 : 0));
+  } else {
+    const uint32_t i0 = u - w.at, i1 = min(size, (blockIdx.x + 1) * s.unit - w.at);  // the start's units hold no tile
+    p.i0 = int(max(i0, START) - START);
+    p.i1 = int(max(i1, START) - START);
+  }
+  return p;
+}
+// The next segment, if the workgroup's units reach it.
+template <int ROWS>
+__device__ __forceinline__ bool next_segment(const Attend& a, const Split& s, Walk& w) {
+  w.at += units_of(s, uint32_t(w.t.count));
+  if (s.whole || w.at >= (blockIdx.x + 1) * s.unit) return false;
+  if (++w.seg < w.segs) return true;
+  w.seg = 0;
+  do {
+    if (++w.b >= a.st.B) return false;
+    const Seq q = seq_of(a.st, w.b);
+    w.q = Seq{uniform(q.r0), uniform(q.r1), uniform(q.len), uniform(q.first)};
+    w.segs = segs_of<ROWS>(a, w.q);
+  } while (w.segs == 0);
+  w.rgs = w.segs / a.c.heads;
+  w.t = tiles_of(a, w.q);
+  return true;
 }
 
 __device__ __forceinline__ bf16x8 bf16x8_of(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
@@ -151,12 +199,21 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {  // the high bit of 
   return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
+// The first n bytes of four.
+__device__ __forceinline__ uint32_t first_bytes(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1; }
+// Eight bf16, 1 where the lowest bit is set, else 0.
+__device__ __forceinline__ bf16x8 ones(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g,
+                                       uint32_t h) {
+  const auto two = [](uint32_t x, uint32_t y) { return int((x & 1) * 0x3f80u | (y & 1) * 0x3f800000u); };
+  return __builtin_bit_cast(bf16x8, v4i{two(a, b), two(c, d), two(e, f), two(g, h)});
+}
+
 // ---- few rows a sequence: decode and verify steps ---------------------------------------------------------------------
 // Bound by reading the cache once. A wave takes 16 rows ((token, query head) pairs that share a key / value head) and
-// 16 J tokens at a time straight from the cache into registers, no LDS: with S^T = K Q^T the 16x16 product leaves lane
+// 64 tokens at a time straight from the cache into registers, no LDS: with S^T = K Q^T the 16x16 product leaves lane
 // (row c, group g) the scores of tokens 4g .. 4g + 3 of a 16-token tile, and the tiles' rows are taken in such an order of
-// tokens (tile j, row r: token 4J (r / 4) + 4j + r % 4) that over the J tiles these are tokens 4J g .. 4J g + 4J - 1: the
-// very tokens whose values one load of the transposed cache gives it for O^T = V^T P^T. The weights go from one product
+// tokens (tile j, row r: token 16 (r / 4) + 4j + r % 4) that over four tiles these are tokens 16g .. 16g + 15: the very
+// tokens whose values one 16-byte load of the transposed cache gives it for O^T = V^T P^T. The weights go from one product
 // to the other in place, and a row's running maximum and sum are its lane's own.
 // The codes become bf16 exactly (v_cvt_scalef32, the block's scale with them), the products sum in fp32; the weights are
 // rounded to bf16 for the second product (2^-8 of each at most, as much as the output's own rounding), their sum is taken in
@@ -165,9 +222,7 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {  // the high bit of 
 // (4 / RW)-th tile and are joined in LDS. The workgroup that finishes last of those that share rows adds their partial
 // sums, in the order of the tiles whichever it is: the result does not depend on timing.
 template <int D, int RW>
-struct Split {
-  static constexpr int J = D == 256 ? 2 : 4;  // (four tiles of 256 channels do not leave room for two waves)
-  static constexpr int TOK = 16 * J;
+struct Shape {
   static constexpr int TW = AT_WAVES / RW;  // waves that share rows
   static constexpr int ROWS = 16 * RW;
   static constexpr int KL = D / 64;  // 16-byte loads of a key row's quarter
@@ -177,11 +232,10 @@ struct Split {
     float ml[AT_WAVES][16][2];
   };
 };
-constexpr int kTarget = 512;  // two workgroups on each CU
-constexpr int kMostSlots = 4 * kTarget;
-constexpr size_t kCounterBytes = kMostSlots * sizeof(uint32_t);
-constexpr int rounds_of(int rw) { return rw == 4 ? 1 : 2; }
-constexpr int slots_of(int rw) { return 2 * kTarget * rounds_of(rw); }  // two a share of the tiles
+// Workgroups that a CU holds, by their registers.
+constexpr int wgs_per_cu(int dim) { return dim <= 128 ? 2 : 1; }
+constexpr int target_of(int dim) { return 256 * wgs_per_cu(dim); }
+constexpr size_t kCounterBytes = 256 * 2 * sizeof(uint32_t);
 
 // Partial sums pass between workgroups on different XCDs, whose L2 caches do not see each other's lines: stored through
 // to memory and read from there (device-scope accesses), which for these few KiB is far cheaper than the fences that
@@ -220,281 +274,546 @@ __device__ __forceinline__ void store_out(const Attend& a, int row, int hq, int 
 }
 
 template <int D, int RW>
-__global__ __launch_bounds__(AT_NT, 2) void kv_split_kernel(Attend a) {
-  using S = Split<D, RW>;
-  constexpr int J = S::J, TOK = S::TOK, TW = S::TW;
+__global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a) {
+  using S = Shape<D, RW>;
+  constexpr int TW = S::TW;
   __shared__ __align__(16) typename S::Lds lds;
   __shared__ int last;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-  Piece pc;
-  Seq q;
-  Tiles tiles;
-  if (!find_piece<S::ROWS, TW>(a, pc, q, tiles)) return;
-  const int b = pc.b, h = pc.h, nrows = (q.r1 - q.r0) * a.group, row0 = pc.rg * S::ROWS + wave / TW * 16;
-
-  // this lane's row (the last one where there are fewer): its position
-  const int ri = min(row0 + c, nrows - 1), my_row = q.r0 + ri / a.group, my_hq = h * a.group + ri % a.group;
-  const int pos = q.first + ri / a.group;
-  const int pos_lo = q.first + min(row0, nrows - 1) / a.group;  // of the wave's rows
-  const int pos_hi = q.first + min(row0 + 15, nrows - 1) / a.group;
-
-  v4f o[S::DT];
-  float mx = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int d = 0; d < S::DT; ++d) o[d] = v4f{0, 0, 0, 0};
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
+  Split sp;
+  Walk w;
+  if (!find_segment<S::ROWS, TW>(a, sp, w)) return;
+  Part pt = part_of(sp, w, blockIdx.x * sp.unit);
 
   const int mask = a.c.page - 1, sh = a.page_shift;
-  const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
-    pk = page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (t0 + 4 * J * (c >> 2)) >> sh);
-    pv = page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (t0 + 4 * J * g) >> sh);
-  };
-  uint4 kr[J][S::KL];
-  uint32_t vr[S::DT][J];
+  uint4 kr[4][S::KL];
+  uint32_t vr[S::DT][4];
+  bf16x8 qf[2 * S::KL];
   int ksb, vsb;
+  int pos, my_row, my_hq;         // this lane's row (the last one where there are fewer)
+  int pos_lo, pos_hi, nrows, row0;  // of the wave's rows
+  int i, pk, pv, pk1, pv1;
+  const auto token = [&](int i) { return w.t.at(i) * TILE; };
+  const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
+    pk = page_of(a.st.table, a.st.max_blocks, a.c.pages, w.b, (t0 + 16 * (c >> 2)) >> sh);
+    pv = page_of(a.st.table, a.st.max_blocks, a.c.pages, w.b, (t0 + 16 * g) >> sh);
+  };
   const auto load_k = [&](int t0, int pk) {
-    const size_t ph = size_t(max(pk, 0)) * a.c.heads + h;
-    const uint8_t* p = a.c.k + ((ph << sh) + ((t0 + 4 * J * (c >> 2) + (c & 3)) & mask)) * D + 16 * g;
+    const size_t ph = size_t(max(pk, 0)) * a.c.heads + pt.h;
+    const uint8_t* p = a.c.k + ((ph << sh) + ((t0 + 16 * (c >> 2) + (c & 3)) & mask)) * D + 16 * g;
     ksb = a.c.ks[ph];
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int m = 0; m < S::KL; ++m) kr[j][m] = ld16(p + 4 * j * D + 64 * m);
   };
   const auto load_v = [&](int t0, int pv) {
-    const size_t ph = size_t(max(pv, 0)) * a.c.heads + h;
-    const uint8_t* p = a.c.v + ((ph * D + c) << sh) + ((t0 + 4 * J * g) & mask);
+    const size_t ph = size_t(max(pv, 0)) * a.c.heads + pt.h;
+    const uint8_t* p = a.c.v + ((ph * D + c) << sh) + ((t0 + 16 * g) & mask);
     vsb = a.c.vs[ph];
 #pragma unroll
     for (int d = 0; d < S::DT; ++d) {
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+      const uint4 x = ld16(p);
       p += 16 << sh;
-      if constexpr (J == 4) {
-        const uint4 x = *reinterpret_cast<const uint4*>(w);
-        vr[d][0] = x.x, vr[d][1] = x.y, vr[d][2] = x.z, vr[d][3] = x.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(w);
-        vr[d][0] = x.x, vr[d][1] = x.y;
-      }
+      vr[d][0] = x.x, vr[d][1] = x.y, vr[d][2] = x.z, vr[d][3] = x.w;
     }
   };
-  // a 64-token tile is 64 / TOK steps; steps go to the waves in turn
-  constexpr int PER = TILE / TOK;
-  const auto token = [&](int i) { return tiles.at(i / PER) * TILE + i % PER * TOK; };
-  const int i1 = pc.i1 * PER;
-  int i = pc.i0 * PER + wave % TW, pk = 0, pv = 0, pk1 = 0, pv1 = 0;
-  if (row0 >= nrows) i = i1;  // no rows for this wave
-  if (i < i1) lookup(token(i), pk, pv);
-  bf16x8 qf[2 * S::KL];
-  {
+  const auto begin = [&] {  // a part: its rows, and its first loads on their way
+    nrows = (w.q.r1 - w.q.r0) * a.group;
+    row0 = pt.rg * S::ROWS + wave / TW * 16;
+    i = row0 < nrows ? pt.i0 + wave % TW : pt.i1;  // (no rows for this wave)
+    if (i < pt.i1) lookup(token(i), pk, pv);
+    const int ri = min(row0 + c, nrows - 1);
+    my_row = w.q.r0 + ri / a.group, my_hq = pt.h * a.group + ri % a.group;
+    pos = w.q.first + ri / a.group;
+    pos_lo = w.q.first + min(row0, nrows - 1) / a.group;
+    pos_hi = w.q.first + min(row0 + 15, nrows - 1) / a.group;
     const bf16* x = a.q + size_t(my_row) * a.ldq + size_t(my_hq) * D + 16 * g;
 #pragma unroll
     for (int m = 0; m < S::KL; ++m) {
       qf[2 * m] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m));
       qf[2 * m + 1] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m + 8));
     }
-  }
-  if (i < i1) {
-    load_k(token(i), pk);
-    load_v(token(i), pv);
-    if (i + TW < i1) lookup(token(i + TW), pk1, pv1);
-  }
-  for (; i < i1; i += TW) {
-    const int t0 = token(i);
-    const bool more = i + TW < i1;
-    const int tn = token(more ? i + TW : i);
-    const float ks = e8m0_to_f32(uint8_t(ksb));
-    v4f s[J];
+    if (i < pt.i1) {
+      load_k(token(i), pk);
+      load_v(token(i), pv);
+      if (i + TW < pt.i1) lookup(token(i + TW), pk1, pv1);
+    }
+  };
+
+  begin();
+  for (bool again = true; again;) {
+    v4f o[S::DT];
+    float mx = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      s[j] = v4f{0, 0, 0, 0};
+    for (int d = 0; d < S::DT; ++d) o[d] = v4f{0, 0, 0, 0};
+    for (; i < pt.i1; i += TW) {
+      const int t0 = token(i);
+      const bool more = i + TW < pt.i1;
+      const int tn = token(more ? i + TW : i);
+      const float ks = e8m0_to_f32(uint8_t(ksb));
+      v4f s[4];
 #pragma unroll
-      for (int m = 0; m < S::KL; ++m) {
-        s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].x, kr[j][m].y, ks), qf[2 * m], s[j]);
-        s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].z, kr[j][m].w, ks), qf[2 * m + 1], s[j]);
+      for (int j = 0; j < 4; ++j) {
+        s[j] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int m = 0; m < S::KL; ++m) {
+          s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].x, kr[j][m].y, ks), qf[2 * m], s[j]);
+          s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].z, kr[j][m].w, ks), qf[2 * m + 1], s[j]);
+        }
+      }
+      const int pvt = pv;
+      if (more) {
+        pk = pk1, pv = pv1;
+        load_k(tn, pk);
+        if (i + 2 * TW < pt.i1) lookup(token(i + 2 * TW), pk1, pv1);
+      }
+      // what a row does not see: only in the tiles at the ends of what the rows see
+      const bool masked = t0 + TILE - 1 > pos_lo || __any(pvt < 0) ||
+                          (a.window > 0 && int64_t(t0) + a.window <= pos_hi && t0 + TILE > a.sinks);
+      uint32_t see = 0xffff;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] *= a.scale2;
+      if (masked) {
+        see = pvt < 0 ? 0 : seen_bits(pos, t0 + 16 * g, a.window, a.sinks);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) s[k / 4][k % 4] = see >> k & 1 ? s[k / 4][k % 4] : -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k / 4][k % 4]);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float m1 = fmaxf(mx, top), ref = m1 == -INFINITY ? 0.0f : m1;
+      if (__any(m1 != mx)) {
+        const float al = __builtin_amdgcn_exp2f(mx - ref);
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) o[d] *= al;
+        l *= al;
+      }
+      mx = m1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[j][e] = __builtin_amdgcn_exp2f(s[j][e] - ref);
+          l += s[j][e];
+        }
+      const float vs = e8m0_to_f32(uint8_t(vsb));
+      bf16x8 p[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[hf][e] = __bf16(s[2 * hf + e / 4][e % 4]);
+      uint32_t bad = 0;
+      if (masked) {  // slots past the last token hold anything: zero; NaN among the values that some row sees: below
+        const int n = pvt < 0 ? 0 : min(max(w.q.len - (t0 + 16 * g), 0), 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t keep = first_bytes(n - 4 * k);
+#pragma unroll
+          for (int d = 0; d < S::DT; ++d) {
+            vr[d][k] &= keep;
+            bad |= nan_bytes(vr[d][k]);
+          }
+        }
+      }
+      if (__builtin_expect(!__any(bad != 0), 1)) {
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+            o[d] = mfma_bf16(fp8x8_to_bf16(vr[d][2 * hf], vr[d][2 * hf + 1], vs), p[hf], o[d]);
+      } else {
+        // 0 x NaN is NaN: the NaN values are taken out, and a product of 0 / 1 operands counts for each row and channel the
+        // NaN that it sees.
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) {
+          v4f n{0, 0, 0, 0};
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const uint32_t x0 = vr[d][2 * hf], x1 = vr[d][2 * hf + 1], n0 = nan_bytes(x0) >> 7, n1 = nan_bytes(x1) >> 7;
+            const bf16x8 nv = ones(n0, n0 >> 8, n0 >> 16, n0 >> 24, n1, n1 >> 8, n1 >> 16, n1 >> 24);
+            const uint32_t z = see >> (8 * hf);
+            const bf16x8 sv = ones(z, z >> 1, z >> 2, z >> 3, z >> 4, z >> 5, z >> 6, z >> 7);
+            n = mfma_bf16(nv, sv, n);
+            o[d] = mfma_bf16(fp8x8_to_bf16(x0 & ~(n0 * 0xffu), x1 & ~(n1 * 0xffu), vs), p[hf], o[d]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n[e] > 0.0f) o[d][e] = __builtin_nanf("");
+          __builtin_amdgcn_sched_barrier(0);  // (one channel tile at a time: registers)
+        }
+      }
+      if (more) load_v(tn, pv);
+    }
+
+    // the part is summed: the next one's loads go out, then this one is joined
+    const Part done = pt;
+    const uint32_t w0 = blockIdx.x - uint32_t(done.index);
+    const int row = my_row, hq = my_hq, r0 = w.q.r0, left = nrows - done.rg * S::ROWS;  // rows from the group's on
+    const bool mine = wave % TW == 0 && row0 + c < nrows;
+    again = next_segment<S::ROWS>(a, sp, w);
+    if (again) {
+      pt = part_of(sp, w, w.at);
+      begin();
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if constexpr (TW > 1) {
+      pipe::lds_barrier();  // the last part's use of the LDS
+      if (g == 0) lds.ml[wave][c][0] = mx, lds.ml[wave][c][1] = l;
+      pipe::lds_barrier();
+      const int first = wave / TW * TW;
+      float m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < TW; ++k) m = fmaxf(m, lds.ml[first + k][c][0]);
+      const float ref = m == -INFINITY ? 0.0f : m, f = __builtin_amdgcn_exp2f(mx - ref);
+      l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < TW; ++k)
+        l += lds.ml[first + k][c][1] * __builtin_amdgcn_exp2f(lds.ml[first + k][c][0] - ref);
+      mx = m;
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) o[d] *= f;
+      const auto at = [&](int buf, int d) { return reinterpret_cast<v4f*>(&lds.o[buf][(d * 64 + lane) * 4]); };
+#pragma unroll
+      for (int half = TW / 2; half; half /= 2) {  // the upper half of the waves hands its sums to the lower
+        const int k = wave % TW, buf = wave / TW * (TW / 2) + k % half;
+        if (k >= half && k < 2 * half)
+#pragma unroll
+          for (int d = 0; d < S::DT; ++d) *at(buf, d) = o[d];
+        pipe::lds_barrier();
+        if (k < half)
+#pragma unroll
+          for (int d = 0; d < S::DT; ++d) o[d] += *at(buf, d);
+        pipe::lds_barrier();
       }
     }
-    const int pvt = pv;
-    if (more) {
-      pk = pk1, pv = pv1;
-      load_k(tn, pk);
-      if (i + 2 * TW < i1) lookup(token(i + 2 * TW), pk1, pv1);
+    if (done.parts == 1) {
+      if (mine)
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) store_out<D>(a, row, hq, 16 * d + 4 * g, o[d], l, mx, d == 0 && g == 0);
+      continue;
     }
-    // what a row does not see: only in the tiles at the ends of what the rows see
-    const bool masked = t0 + TOK - 1 > pos_lo || __any(pvt < 0) ||
-                        (a.window > 0 && int64_t(t0) + a.window <= pos_hi && t0 + TOK > a.sinks);
-    uint32_t see = 0xffff;
+    if (mine) {
+      const int r = int(blockIdx.x * 2 + (done.index == 0 ? 1 : 0)) * S::ROWS + wave / TW * 16 + c;
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) put4(sums_of(a.po), r * D + 4 * g + 16 * d, o[d]);
+      if (g == 0) put2(sums_of(a.pml), r * 2, mx, l);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
+    __syncthreads();
+    if (tid == 0)
+      last = __hip_atomic_fetch_add(&a.counters[w0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+             uint32_t(done.parts - 1);
+    __syncthreads();
+    if (!last) continue;
+    if (tid == 0)  // as it was found
+      __hip_atomic_store(&a.counters[w0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // a thread per row and four channels, the loads of JOIN parts in flight at a time
+    const int rows = min(S::ROWS, left);
+    for (int it = tid; it < rows * (D / 4); it += AT_NT) {
+      const int r = it / (D / 4), d = it % (D / 4) * 4;
+      float m = -INFINITY, sum = 0.0f;
+      v4f acc{0, 0, 0, 0};
+      for (int k0 = 0; k0 < done.parts; k0 += JOIN) {
+        v4f y[JOIN];
+        float2 x[JOIN];
+#pragma unroll
+        for (int k = 0; k < JOIN; ++k) {
+          const int p = min(k0 + k, done.parts - 1);
+          const int at = (int(w0 + uint32_t(p)) * 2 + (p == 0 ? 1 : 0)) * S::ROWS + r;
+          x[k] = get2(sums_of(a.pml), at * 2);
+          y[k] = get4(sums_of(a.po), at * D + d);
+        }
+        float m1 = m;
+#pragma unroll
+        for (int k = 0; k < JOIN; ++k) m1 = fmaxf(m1, x[k].x);
+        const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m - ref);
+        m = m1;
+        acc *= al;
+        sum *= al;
+#pragma unroll
+        for (int k = 0; k < JOIN; ++k)
+          if (k0 + k < done.parts) {
+            const float f = __builtin_amdgcn_exp2f(x[k].x - ref);
+            sum += f * x[k].y;
+            acc += f * y[k];
+          }
+      }
+      const int rr = done.rg * S::ROWS + r;
+      store_out<D>(a, r0 + rr / a.group, done.h * a.group + rr % a.group, d, acc, sum, m, d == 0);
+    }
+  }
+}
+
+// ---- many rows a sequence: prompts ------------------------------------------------------------------------------------
+// Bound by the matrix rate and by the exponentials and conversions next to it. A workgroup takes 128 rows (4 waves of 32)
+// of one (sequence, key / value head) and goes through the 64-token tiles that they see, which arrive in LDS as codes by
+// direct loads, two tiles ahead, in a ring of three. The 32x32x16 product with the same order of tokens as above: S^T = K Q^T
+// with row 8a + 4h + i of a 32-token half taken as token 16h + 4a + i, so that lane (row, half h) has the scores of 16
+// consecutive tokens and O^T = V^T P^T finds their values in one 16-byte read.
+// LDS: the 16-byte pieces of a key row (D bytes) and of a channel's values (64 bytes) are permuted among themselves such
+// that the sixteen lanes that a read serves at a time find theirs in different banks.
+// Pages and scales are read for 16 tiles at a time: their loads are waited for with all others, direct ones among them.
+// The running maximum is left alone until a row's scores pass it by more than 2^8: the weights stay small enough, and most
+// tiles need no scaling of the sums.
+constexpr int PR_ROWS = 128;
+constexpr int PR_STAGES = 3;
+constexpr int PR_META = 16;  // tiles
+constexpr float PR_LAG = 8.0f;
+
+// The place among a key row's pieces of piece p of row (token) t, and among a channel's pieces of piece p of channel d.
+template <int D>
+__device__ __forceinline__ int key_piece(int t, int p) {
+  const int b1 = t >> 1 & 1, b2 = t >> 2 & 1, b4 = t >> 4 & 1;
+  return p ^ (D == 64 ? b2 | b4 << 1 : D == 128 ? b1 | b2 << 1 | b4 << 2 : (t & 3) | b2 << 2 | b4 << 3);
+}
+__device__ __forceinline__ int value_piece(int d, int p) { return p ^ (d >> 2 & 3); }
+
+template <int D>
+struct Tiled {
+  static constexpr int KV = TILE * D;                   // bytes of a tile's keys, and of its values
+  static constexpr int LOADS = KV / 16 / AT_NT;         // direct loads a thread makes for each
+  static constexpr int DT = D / 32;
+  struct Lds {
+    uint8_t k[PR_STAGES][KV], v[PR_STAGES][KV];
+    int page[2][PR_META * 4];
+    float ks[2][PR_META * 4], vs[2][PR_META * 4];  // of every 16 tokens
+  };
+};
+
+template <int D>
+__global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Attend a) {
+  using S = Tiled<D>;
+  __shared__ __align__(1024) typename S::Lds lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 31, h2 = lane >> 5;
+
+  // Workgroup -> (row block, head): heads inner, so that with 8 heads or a multiple an XCD's workgroups read the same ones'
+  // keys and values; a sequence's last blocks, which see the most, first.
+  const int h = int(blockIdx.x % unsigned(a.c.heads));
+  const uint32_t block = blockIdx.x / unsigned(a.c.heads);
+  Seq q{0, 0, 0, 0};
+  int b = -1, row0 = 0;
+  uint32_t from = 0;
+  for (int b0 = 0; b0 < a.st.B && b < 0; b0 += 64) {
+    uint32_t n = 0;
+    if (b0 + lane < a.st.B) {
+      q = seq_of(a.st, b0 + lane);
+      const int rows = (q.r1 - q.r0) * a.group;
+      n = rows > a.few ? uint32_t(row_groups(rows, PR_ROWS)) : 0;
+    }
+    const uint32_t end = from + wave_scan(n);
+    const uint64_t hit = __ballot(block < end);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      b = b0 + l;
+      q = Seq{int(lane_of(q.r0, l)), int(lane_of(q.r1, l)), int(lane_of(q.len, l)), int(lane_of(q.first, l))};
+      row0 = int(lane_of(end, l) - 1 - block) * PR_ROWS;
+    }
+    from = lane_of(end, 63);
+  }
+  if (b < 0) return;
+  const int nrows = (q.r1 - q.r0) * a.group;
+  Tiles tiles;  // that the workgroup's rows see
+  {
+    const int last = min(row0 + PR_ROWS, nrows) - 1;
+    const Seq mine{0, 0, min(q.len, q.first + last / a.group + 1), q.first + row0 / a.group};
+    tiles = tiles_of(a, Seq{0, 0, max(mine.len, 0), mine.first});
+  }
+
+  // this lane's row
+  const int wrow = row0 + 32 * wave, ri = min(wrow + c, nrows - 1);
+  const int row = q.r0 + ri / a.group, hq = h * a.group + ri % a.group, pos = q.first + ri / a.group;
+  const int pos_lo = q.first + min(wrow, nrows - 1) / a.group, pos_hi = q.first + min(wrow + 31, nrows - 1) / a.group;
+  bf16x8 qf[2 * D / 32];
+  {
+    const bf16* x = a.q + size_t(row) * a.ldq + size_t(hq) * D + 16 * h2;
+#pragma unroll
+    for (int m = 0; m < D / 32; ++m) {
+      const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0;  // scores times |scale|: their largest is the largest weight's
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint4 y = *reinterpret_cast<const uint4*>(x + 32 * m + 8 * e);
+        y.x ^= flip, y.y ^= flip, y.z ^= flip, y.w ^= flip;
+        qf[2 * m + e] = bf16x8_of(y);
+      }
+    }
+  }
+  const float sc = fabsf(a.scale2);
+
+  const auto token = [&](int i) { return tiles.at(i) * TILE; };
+  const auto meta = [&](int chunk) {  // pages and scales of tiles [16 chunk, 16 chunk + 16)
+    if (tid < PR_META * 4) {
+      const int i = chunk * PR_META + tid / 4;
+      const int pg = i < tiles.count ? page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (token(i) + tid % 4 * 16) >> a.page_shift)
+                                     : -1;
+      const size_t ph = size_t(max(pg, 0)) * a.c.heads + h;
+      lds.page[chunk & 1][tid] = pg;
+      lds.ks[chunk & 1][tid] = e8m0_to_f32(a.c.ks[ph]);
+      lds.vs[chunk & 1][tid] = e8m0_to_f32(a.c.vs[ph]);
+    }
+  };
+  const int mask = a.c.page - 1, sh = a.page_shift;
+  const auto fetch = [&](int i) {  // tile i on its way to its stage
+    const int t0 = token(i), st = i % PR_STAGES, mt = i / PR_META & 1, mi = i % PR_META * 4;
+#pragma unroll
+    for (int x = 0; x < S::LOADS; ++x) {
+      const int at = (x * AT_WAVES + wave) * 64 + lane;  // the 16-byte slot that this lane fills
+      const int t = at / (D / 16), p = key_piece<D>(t, at % (D / 16));
+      const size_t ph = size_t(max(lds.page[mt][mi + t / 16], 0)) * a.c.heads + h;
+      pipe::dma16_at(a.c.k + ((ph << sh) + ((t0 + t) & mask)) * D + 16 * p,
+                     pipe::lds_addr(&lds.k[st][(x * AT_WAVES + wave) * 1024]));
+    }
+#pragma unroll
+    for (int x = 0; x < S::LOADS; ++x) {
+      const int at = (x * AT_WAVES + wave) * 64 + lane, d = at / 4, p = value_piece(d, at % 4);
+      const size_t ph = size_t(max(lds.page[mt][mi + p], 0)) * a.c.heads + h;
+      pipe::dma16_at(a.c.v + ((ph * D + d) << sh) + ((t0 + 16 * p) & mask),
+                     pipe::lds_addr(&lds.v[st][(x * AT_WAVES + wave) * 1024]));
+    }
+  };
+
+  pipe::v16f_t o[S::DT];
+#pragma unroll
+  for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+  float ref2 = -INFINITY, l = 0.0f;  // what the weights are relative to (a power of two's exponent); their sum
+  const int n = tiles.count;
+  if (n > 0) {
+    meta(0);
+    __syncthreads();
+    fetch(0);
+    if (n > 1) fetch(1);
+  }
+  const int krow = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);  // the token that is this lane's row of a half
+  const int kat = krow * D + 16 * key_piece<D>(krow, h2), vat = c * 64;
+  for (int t = 0; t < n; ++t) {
+    if (t + 1 < n) pipe::wait_vm<2 * S::LOADS>();
+    else pipe::wait_vm<0>();
+    pipe::lds_barrier();  // tile t is there, and every wave is done with tile t - 1
+    if (t % PR_META == PR_META - 4 && t / PR_META * PR_META + PR_META < n) meta(t / PR_META + 1);
+    if (t + 2 < n) fetch(t + 2);
+    const int t0 = token(t), mt = t / PR_META & 1, mi = t % PR_META * 4;
+    if (wrow >= nrows || t0 > pos_hi) continue;
+    const uint8_t *kt = lds.k[t % PR_STAGES], *vt = lds.v[t % PR_STAGES];
+    const int4 pg = *reinterpret_cast<const int4*>(&lds.page[mt][mi]);
+    const bool missing = uniform((pg.x | pg.y | pg.z | pg.w) < 0);
+    const bool masked = t0 + TILE - 1 > pos_lo || missing ||
+                        (a.window > 0 && int64_t(t0) + a.window <= pos_hi && t0 + TILE > a.sinks);
+
+    pipe::v16f_t s[2];
+#pragma unroll
+    for (int T = 0; T < 2; ++T) {
+      const float ks = lds.ks[mt][mi + 2 * T + (c >> 2 & 1)];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[T][r] = 0.0f;
+#pragma unroll
+      for (int m = 0; m < D / 32; ++m) {
+        const uint4 x = ld16(kt + 32 * T * D + (kat ^ 32 * m));
+        s[T] = pipe::mfma32_bf16(fp8x8_to_bf16(x.x, x.y, ks), qf[2 * m], s[T]);
+        s[T] = pipe::mfma32_bf16(fp8x8_to_bf16(x.z, x.w, ks), qf[2 * m + 1], s[T]);
+      }
+    }
+    uint32_t see[2] = {0xffff, 0xffff};
+    int there[2] = {16, 16};  // of this lane's 16 values, those of tokens that are there
+    if (masked) {
+#pragma unroll
+      for (int T = 0; T < 2; ++T) {
+        const int tt = t0 + 32 * T + 16 * h2;
+        const bool none = lds.page[mt][mi + 2 * T + h2] < 0;
+        see[T] = none ? 0 : seen_bits(pos, tt, a.window, a.sinks);
+        there[T] = none ? 0 : min(max(q.len - tt, 0), 16);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[T][r] = see[T] >> r & 1 ? s[T][r] : -INFINITY;
+      }
+    }
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < J; ++j) s[j] *= a.scale2;
-    if (masked) {
-      see = pvt < 0 ? 0 : seen_bits(pos, t0 + 4 * J * g, a.window, a.sinks);
+    for (int T = 0; T < 2; ++T)
 #pragma unroll
-      for (int k = 0; k < 4 * J; ++k) s[k / 4][k % 4] = see >> k & 1 ? s[k / 4][k % 4] : -INFINITY;
-    }
-#pragma unroll
-    for (int k = 0; k < 4 * J; ++k) top = fmaxf(top, s[k / 4][k % 4]);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float m1 = fmaxf(mx, top), ref = m1 == -INFINITY ? 0.0f : m1;
-    if (__any(m1 != mx)) {
-      const float al = __builtin_amdgcn_exp2f(mx - ref);
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[T][r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
+    if (__any(top > ref2 + PR_LAG)) {
+      const float to = fmaxf(ref2, top), al = __builtin_amdgcn_exp2f(ref2 - (to == -INFINITY ? 0.0f : to));
 #pragma unroll
       for (int d = 0; d < S::DT; ++d) o[d] *= al;
       l *= al;
+      ref2 = to;
     }
-    mx = m1;
+    const float base = ref2 == -INFINITY ? 0.0f : ref2;
 #pragma unroll
-    for (int j = 0; j < J; ++j)
+    for (int T = 0; T < 2; ++T)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[j][e] = __builtin_amdgcn_exp2f(s[j][e] - ref);
-        l += s[j][e];
+      for (int r = 0; r < 16; ++r) {
+        s[T][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[T][r], sc, -base));
+        if (masked) s[T][r] = see[T] >> r & 1 ? s[T][r] : 0.0f;  // (-inf times a scale of 0)
+        l += s[T][r];
       }
-    const float vs = e8m0_to_f32(uint8_t(vsb));
-    bf16x8 p[J / 2];
+    bf16x8 p[2][2];
 #pragma unroll
-    for (int hf = 0; hf < J / 2; ++hf)
+    for (int T = 0; T < 2; ++T)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[hf][e] = __bf16(s[2 * hf + e / 4][e % 4]);
-    uint32_t bad = 0;
-    if (masked) {  // slots past the last token hold anything: zero; NaN among the values that some row sees: below
-      const int n = pvt < 0 ? 0 : min(max(q.len - (t0 + 4 * J * g), 0), 4 * J);
+      for (int e = 0; e < 16; ++e) p[T][e / 8][e % 8] = __bf16(s[T][e]);
+    if (!masked) {
 #pragma unroll
-      for (int k = 0; k < J; ++k) {
-        const uint32_t keep = n >= 4 * k + 4 ? ~0u : n <= 4 * k ? 0u : (1u << (8 * (n - 4 * k))) - 1;
+      for (int T = 0; T < 2; ++T) {
+        const float vs = lds.vs[mt][mi + 2 * T + h2];
+        const uint8_t* at = vt + vat + 16 * value_piece(c, 2 * T + h2);
 #pragma unroll
         for (int d = 0; d < S::DT; ++d) {
-          vr[d][k] &= keep;
-          bad |= nan_bytes(vr[d][k]);
+          const uint4 x = ld16(at + d * 2048);
+          o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(x.x, x.y, vs), p[T][0], o[d]);
+          o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(x.z, x.w, vs), p[T][1], o[d]);
         }
       }
-    }
-    if (__builtin_expect(!__any(bad != 0), 1)) {
+    } else {  // as in the split kernel: what is behind the last token is zero, NaN counted for the rows that see it
 #pragma unroll
-      for (int d = 0; d < S::DT; ++d)
+      for (int T = 0; T < 2; ++T) {
+        const float vs = lds.vs[mt][mi + 2 * T + h2];
+        const uint8_t* at = vt + vat + 16 * value_piece(c, 2 * T + h2);
 #pragma unroll
-        for (int hf = 0; hf < J / 2; ++hf)
-          o[d] = mfma_bf16(fp8x8_to_bf16(vr[d][2 * hf], vr[d][2 * hf + 1], vs), p[hf], o[d]);
-    } else {
-      // 0 x NaN is NaN: the NaN values are taken out, and a product of 0 / 1 operands counts for each row and channel the
-      // NaN that it sees.
+        for (int d = 0; d < S::DT; ++d) {
+          const uint4 y = ld16(at + d * 2048);
+          uint32_t x[4] = {y.x, y.y, y.z, y.w}, nan[4], bad = 0;
 #pragma unroll
-      for (int d = 0; d < S::DT; ++d) {
-        v4f n{0, 0, 0, 0};
-#pragma unroll
-        for (int hf = 0; hf < J / 2; ++hf) {
-          bf16x8 nv, sv;
-          uint32_t x[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t nb = nan_bytes(vr[d][2 * hf + k]) >> 7;  // 0 / 1 in each byte
-            x[k] = vr[d][2 * hf + k] & ~(nb * 0xffu);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              nv[4 * k + e] = __bf16(float(nb >> (8 * e) & 1));
-              sv[4 * k + e] = __bf16(float(see >> (8 * hf + 4 * k + e) & 1));
-            }
+          for (int k = 0; k < 4; ++k) {
+            x[k] &= first_bytes(there[T] - 4 * k);
+            nan[k] = nan_bytes(x[k]) >> 7;
+            bad |= nan[k];
           }
-          n = mfma_bf16(nv, sv, n);
-          o[d] = mfma_bf16(fp8x8_to_bf16(x[0], x[1], vs), p[hf], o[d]);
-        }
+          if (__builtin_expect(__any(bad != 0), 0)) {
+            pipe::v16f_t many;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n[e] > 0.0f) o[d][e] = __builtin_nanf("");
+            for (int r = 0; r < 16; ++r) many[r] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t n0 = nan[2 * e], n1 = nan[2 * e + 1], z = see[T] >> (8 * e);
+              many = pipe::mfma32_bf16(ones(n0, n0 >> 8, n0 >> 16, n0 >> 24, n1, n1 >> 8, n1 >> 16, n1 >> 24),
+                                       ones(z, z >> 1, z >> 2, z >> 3, z >> 4, z >> 5, z >> 6, z >> 7), many);
+              x[2 * e] &= ~(n0 * 0xffu);
+              x[2 * e + 1] &= ~(n1 * 0xffu);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (many[r] > 0.0f) o[d][r] = __builtin_nanf("");
+          }
+          o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(x[0], x[1], vs), p[T][0], o[d]);
+          o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(x[2], x[3], vs), p[T][1], o[d]);
+        }
       }
     }
-    if (more) load_v(tn, pv);
   }
-
-  // join the waves that share rows
-  l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  if constexpr (TW > 1) {
-    if (g == 0) lds.ml[wave][c][0] = mx, lds.ml[wave][c][1] = l;
-    __syncthreads();
-    const int w0 = wave / TW * TW;
-    float m = -INFINITY;
+  if (wrow + c >= nrows) return;
 #pragma unroll
-    for (int w = 0; w < TW; ++w) m = fmaxf(m, lds.ml[w0 + w][c][0]);
-    const float ref = m == -INFINITY ? 0.0f : m, f = __builtin_amdgcn_exp2f(mx - ref);
-    l = 0.0f;
+  for (int d = 0; d < S::DT; ++d)
 #pragma unroll
-    for (int w = 0; w < TW; ++w) l += lds.ml[w0 + w][c][1] * __builtin_amdgcn_exp2f(lds.ml[w0 + w][c][0] - ref);
-    mx = m;
-#pragma unroll
-    for (int d = 0; d < S::DT; ++d) o[d] *= f;
-    const auto at = [&](int buf, int d) { return reinterpret_cast<v4f*>(&lds.o[buf][(d * 64 + lane) * 4]); };
-#pragma unroll
-    for (int half = TW / 2; half; half /= 2) {  // the upper half of the waves hands its sums to the lower
-      const int k = wave % TW, buf = wave / TW * (TW / 2) + k % half;
-      if (k >= half && k < 2 * half)
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) *at(buf, d) = o[d];
-      __syncthreads();
-      if (k < half)
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) o[d] += *at(buf, d);
-      __syncthreads();
-    }
-  }
-  const bool mine = wave % TW == 0 && row0 + c < nrows;
-  if (pc.pieces == 1) {
-    if (mine)
-#pragma unroll
-      for (int d = 0; d < S::DT; ++d) store_out<D>(a, my_row, my_hq, 16 * d + 4 * g, o[d], l, mx, d == 0 && g == 0);
-    return;
-  }
-  if (mine) {
-    const int r = (pc.slot0 + pc.index) * S::ROWS + wave / TW * 16 + c;
-#pragma unroll
-    for (int d = 0; d < S::DT; ++d) put4(sums_of(a.po), r * D + 4 * g + 16 * d, o[d]);
-    if (g == 0) put2(sums_of(a.pml), r * 2, mx, l);
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
-  __syncthreads();
-  if (tid == 0)
-    last = __hip_atomic_fetch_add(&a.counters[pc.slot0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-           uint32_t(pc.pieces - 1);
-  __syncthreads();
-  if (!last) return;
-  if (tid == 0)  // as it was found
-    __hip_atomic_store(&a.counters[pc.slot0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // a thread per row and four channels, the loads of eight pieces in flight at a time
-  const int rows = min(S::ROWS, nrows - pc.rg * S::ROWS);
-  const __amdgpu_buffer_rsrc_t po = sums_of(a.po + size_t(pc.slot0) * S::ROWS * D);
-  const __amdgpu_buffer_rsrc_t pml = sums_of(a.pml + size_t(pc.slot0) * S::ROWS * 2);
-  for (int it = tid; it < rows * (D / 4); it += AT_NT) {
-    const int r = it / (D / 4), d = it % (D / 4) * 4;
-    float m = -INFINITY, sum = 0.0f;
-    v4f acc{0, 0, 0, 0};
-    for (int k0 = 0; k0 < pc.pieces; k0 += JOIN) {
-      v4f y[JOIN];
-      float2 x[JOIN];
-#pragma unroll
-      for (int k = 0; k < JOIN; ++k) {
-        const int at = min(k0 + k, pc.pieces - 1) * S::ROWS + r;
-        x[k] = get2(pml, at * 2);
-        y[k] = get4(po, at * D + d);
-      }
-      float m1 = m;
-#pragma unroll
-      for (int k = 0; k < JOIN; ++k) m1 = fmaxf(m1, x[k].x);
-      const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m - ref);
-      m = m1;
-      acc *= al;
-      sum *= al;
-#pragma unroll
-      for (int k = 0; k < JOIN; ++k) {
-        const float f = k0 + k < pc.pieces ? __builtin_amdgcn_exp2f(x[k].x - ref) : 0.0f;
-        if (k0 + k < pc.pieces) {
-          sum += f * x[k].y;
-          acc += f * y[k];
-        }
-      }
-    }
-    const int rr = pc.rg * S::ROWS + r;
-    store_out<D>(a, q.r0 + rr / a.group, h * a.group + rr % a.group, d, acc, sum, m, d == 0);
-  }
+    for (int r = 0; r < 16; r += 4)
+      store_out<D>(a, row, hq, 32 * d + 2 * r + 4 * h2, v4f{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]}, l, ref2,
+                   d == 0 && r == 0 && h2 == 0);
 }
 
 int most_rows(int rows, int max_new, int group) {
@@ -502,12 +821,27 @@ int most_rows(int rows, int max_new, int group) {
 }
 int row_waves(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
+// Which kernels a step takes. Up to `few` rows a sequence (of a key / value head) the split kernel: it reads the cache once
+// for all of them and spreads a single sequence over the chip, which the tiled kernel does not; past that it would read the
+// cache again for every 64 rows. Where the step's sequences may be of both kinds each kernel takes its own; a single sequence
+// is the tiled kernel's if it may have more.
+struct Way {
+  int few, rw;
+  bool split, tiled;
+};
+Way way_of(int rows, int max_new, int B, int group) {
+  const int most = most_rows(rows, max_new, group), few = std::max(64, group);
+  if (most <= few) return {few, row_waves(most), true, false};
+  if (B == 1) return {0, 1, false, true};
+  return {few, row_waves(group), true, true};
+}
+
 }  // namespace
 
 size_t kv_attend_workspace(int rows, int max_new, int B, int Hq, int heads, int dim) {
   if (rows < 0 || max_new < 0 || B < 0 || heads < 1 || Hq < heads || dim < 1) return 0;
-  const int rw = row_waves(most_rows(rows, max_new, Hq / heads));
-  return kCounterBytes + size_t(slots_of(rw)) * 16 * rw * (size_t(dim) + 2) * sizeof(float);
+  const int rw = way_of(rows, max_new, B, Hq / heads).rw;
+  return kCounterBytes + size_t(2) * target_of(dim) * 16 * rw * (size_t(dim) + 2) * sizeof(float);
 }
 
 void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks,
@@ -529,17 +863,27 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
   if (!aligned16(ws)) fail("workspace not 16-byte aligned");
   if (ws_bytes < need) fail("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
 
-  Attend a{q, out, lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E, kTarget, 1, nullptr,
-           nullptr, nullptr};
+  const Way way = way_of(s.rows, s.max_new, s.B, Hq / c.heads);
+  Attend a{q,       out,   lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E, way.few,
+           unsigned(target_of(c.dim)), nullptr, nullptr, nullptr};
   while (1 << a.page_shift < c.page) ++a.page_shift;
-  const int rows = most_rows(s.rows, s.max_new, a.group), rw = row_waves(rows);
   a.counters = static_cast<uint32_t*>(ws);
   a.po = reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes);
-  a.pml = a.po + size_t(slots_of(rw)) * 16 * rw * c.dim;
-  a.rounds = rounds_of(rw);
-  const int64_t segs = int64_t(s.B) * c.heads * cdiv(rows, 16 * rw);  // at most; each is a piece too many at most
-  if (segs + kMostSlots > INT32_MAX) fail("too many rows");
-  const unsigned grid = unsigned(segs + a.target * a.rounds);
+  a.pml = a.po + size_t(2) * a.target * 16 * way.rw * c.dim;
+  const int rows = std::min(most_rows(s.rows, s.max_new, a.group), way.few), rw = way.rw;
+  const int64_t segs = int64_t(s.B) * c.heads * cdiv(rows, 16 * rw);  // at most
+  const int64_t tiles = std::max<int64_t>(cdiv(size_t(s.max_blocks) * c.page, TILE), 1);
+  const int64_t blocks = (cdiv(size_t(s.rows) * a.group, PR_ROWS) + int64_t(s.B)) * c.heads;  // at most
+  if (segs * 8 > INT32_MAX || segs * (tiles + START) > INT32_MAX || blocks > INT32_MAX) fail("rows times blocks past 31 bits");
+  const unsigned grid = unsigned(std::min<int64_t>(segs * cdiv(tiles, AT_WAVES / rw), a.target));
+  const auto tiled = [&]<int D>() { kv_tiled_kernel<D><<<unsigned(blocks), AT_NT, 0, st>>>(a); };
+  if (way.tiled) {
+    if (c.dim == 64) tiled.template operator()<64>();
+    else if (c.dim == 128) tiled.template operator()<128>();
+    else tiled.template operator()<256>();
+    UH_CHECK_LAUNCH();
+  }
+  if (!way.split) return;
   const auto by_rw = [&]<int D>() {
     if (rw == 1) kv_split_kernel<D, 1><<<grid, AT_NT, 0, st>>>(a);
     else if (rw == 2) kv_split_kernel<D, 2><<<grid, AT_NT, 0, st>>>(a);

@@ -57,6 +57,11 @@ __device__ __forceinline__ void dma16_g(const void* base, uint32_t off16, uint32
   lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(addr), "s"(lds) : "memory", "m0");
 }
+// dma16 from an address per lane.
+__device__ __forceinline__ void dma16_at(const void* addr, uint32_t lds) {
+  lds = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(addr), "s"(lds) : "memory", "m0");
+}
 // The same with 4 bytes per lane (to LDS lds + 4 * lane): a gather of one dword per lane.
 __device__ __forceinline__ void dma4(const void* base, uint32_t voff, uint32_t lds) {
   const uint64_t sbase = uniform_ptr(base);
