@@ -201,12 +201,16 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {  // the high bit of 
 
 // The first n bytes of four.
 __device__ __forceinline__ uint32_t first_bytes(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1; }
-// Eight bf16, 1 where the lowest bit is set, else 0.
-__device__ __forceinline__ bf16x8 ones(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g,
-                                       uint32_t h) {
-  const auto two = [](uint32_t x, uint32_t y) { return int((x & 1) * 0x3f80u | (y & 1) * 0x3f800000u); };
-  return __builtin_bit_cast(bf16x8, v4i{two(a, b), two(c, d), two(e, f), two(g, h)});
+// bf16 operands of 0 and 1: of the NaN among eight codes, and of eight bits; and codes with zeros for their NaN.
+__device__ __forceinline__ uint32_t two_ones(uint32_t x, uint32_t y) { return (x & 1) * 0x3f80u | (y & 1) * 0x3f800000u; }
+__device__ __forceinline__ bf16x8 nan_ones(uint32_t lo, uint32_t hi) {
+  const uint32_t a = nan_bytes(lo) >> 7, b = nan_bytes(hi) >> 7;
+  return bf16x8_of(make_uint4(two_ones(a, a >> 8), two_ones(a >> 16, a >> 24), two_ones(b, b >> 8), two_ones(b >> 16, b >> 24)));
 }
+__device__ __forceinline__ bf16x8 bit_ones(uint32_t z) {
+  return bf16x8_of(make_uint4(two_ones(z, z >> 1), two_ones(z >> 2, z >> 3), two_ones(z >> 4, z >> 5), two_ones(z >> 6, z >> 7)));
+}
+__device__ __forceinline__ uint32_t no_nan(uint32_t x) { return x & ~((nan_bytes(x) >> 7) * 0xffu); }
 
 // ---- few rows a sequence: decode and verify steps ---------------------------------------------------------------------
 // Bound by reading the cache once. A wave takes 16 rows ((token, query head) pairs that share a key / value head) and
@@ -326,8 +330,8 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
     const int ri = min(row0 + c, nrows - 1);
     my_row = w.q.r0 + ri / a.group, my_hq = pt.h * a.group + ri % a.group;
     pos = w.q.first + ri / a.group;
-    pos_lo = w.q.first + min(row0, nrows - 1) / a.group;
-    pos_hi = w.q.first + min(row0 + 15, nrows - 1) / a.group;
+    pos_lo = uniform(w.q.first + min(row0, nrows - 1) / a.group);
+    pos_hi = uniform(w.q.first + min(row0 + 15, nrows - 1) / a.group);
     const bf16* x = a.q + size_t(my_row) * a.ldq + size_t(my_hq) * D + 16 * g;
 #pragma unroll
     for (int m = 0; m < S::KL; ++m) {
@@ -405,46 +409,37 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
       for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[hf][e] = __bf16(s[2 * hf + e / 4][e % 4]);
-      uint32_t bad = 0;
-      if (masked) {  // slots past the last token hold anything: zero; NaN among the values that some row sees: below
+      if (masked) {  // slots past the last token hold anything: zero
         const int n = pvt < 0 ? 0 : min(max(w.q.len - (t0 + 16 * g), 0), 16);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t keep = first_bytes(n - 4 * k);
-#pragma unroll
-          for (int d = 0; d < S::DT; ++d) {
-            vr[d][k] &= keep;
-            bad |= nan_bytes(vr[d][k]);
-          }
-        }
-      }
-      if (__builtin_expect(!__any(bad != 0), 1)) {
+        uint32_t bad = 0;
 #pragma unroll
         for (int d = 0; d < S::DT; ++d)
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
-            o[d] = mfma_bf16(fp8x8_to_bf16(vr[d][2 * hf], vr[d][2 * hf + 1], vs), p[hf], o[d]);
-      } else {
-        // 0 x NaN is NaN: the NaN values are taken out, and a product of 0 / 1 operands counts for each row and channel the
-        // NaN that it sees.
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) {
-          v4f n{0, 0, 0, 0};
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const uint32_t x0 = vr[d][2 * hf], x1 = vr[d][2 * hf + 1], n0 = nan_bytes(x0) >> 7, n1 = nan_bytes(x1) >> 7;
-            const bf16x8 nv = ones(n0, n0 >> 8, n0 >> 16, n0 >> 24, n1, n1 >> 8, n1 >> 16, n1 >> 24);
-            const uint32_t z = see >> (8 * hf);
-            const bf16x8 sv = ones(z, z >> 1, z >> 2, z >> 3, z >> 4, z >> 5, z >> 6, z >> 7);
-            n = mfma_bf16(nv, sv, n);
-            o[d] = mfma_bf16(fp8x8_to_bf16(x0 & ~(n0 * 0xffu), x1 & ~(n1 * 0xffu), vs), p[hf], o[d]);
+          for (int k = 0; k < 4; ++k) {
+            vr[d][k] &= first_bytes(n - 4 * k);
+            bad |= nan_bytes(vr[d][k]);
           }
+        if (__builtin_expect(__any(bad != 0), 0)) {
+          // NaN among the values that some row sees, and 0 x NaN is NaN: they are taken out, and a product of 0 / 1 operands
+          // counts for each row and channel the NaN that it sees.
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n[e] > 0.0f) o[d][e] = __builtin_nanf("");
-          __builtin_amdgcn_sched_barrier(0);  // (one channel tile at a time: registers)
+          for (int d = 0; d < S::DT; ++d) {
+            v4f many = mfma_bf16(nan_ones(vr[d][0], vr[d][1]), bit_ones(see), v4f{0, 0, 0, 0});
+            many = mfma_bf16(nan_ones(vr[d][2], vr[d][3]), bit_ones(see >> 8), many);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              vr[d][k] = no_nan(vr[d][k]);
+              if (many[k] > 0.0f) o[d][k] = __builtin_nanf("");
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (one channel tile at a time: registers)
+          }
         }
       }
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          o[d] = mfma_bf16(fp8x8_to_bf16(vr[d][2 * hf], vr[d][2 * hf + 1], vs), p[hf], o[d]);
       if (more) load_v(tn, pv);
     }
 
@@ -621,12 +616,14 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
     const int last = min(row0 + PR_ROWS, nrows) - 1;
     const Seq mine{0, 0, min(q.len, q.first + last / a.group + 1), q.first + row0 / a.group};
     tiles = tiles_of(a, Seq{0, 0, max(mine.len, 0), mine.first});
+    tiles = Tiles{uniform(tiles.sink_tiles), uniform(tiles.skip), uniform(tiles.count)};
   }
 
   // this lane's row
   const int wrow = row0 + 32 * wave, ri = min(wrow + c, nrows - 1);
   const int row = q.r0 + ri / a.group, hq = h * a.group + ri % a.group, pos = q.first + ri / a.group;
-  const int pos_lo = q.first + min(wrow, nrows - 1) / a.group, pos_hi = q.first + min(wrow + 31, nrows - 1) / a.group;
+  const int pos_lo = uniform(q.first + min(wrow, nrows - 1) / a.group);
+  const int pos_hi = uniform(q.first + min(wrow + 31, nrows - 1) / a.group);
   bf16x8 qf[2 * D / 32];
   {
     const bf16* x = a.q + size_t(row) * a.ldq + size_t(hq) * D + 16 * h2;
@@ -641,7 +638,7 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
       }
     }
   }
-  const float sc = fabsf(a.scale2);
+  const float sc = fmaxf(fabsf(a.scale2), 0x1p-126f);  // (not 0: hidden scores are -inf, and stay so)
 
   const auto token = [&](int i) { return tiles.at(i) * TILE; };
   const auto meta = [&](int chunk) {  // pages and scales of tiles [16 chunk, 16 chunk + 16)
@@ -656,22 +653,42 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
     }
   };
   const int mask = a.c.page - 1, sh = a.page_shift;
-  const auto fetch = [&](int i) {  // tile i on its way to its stage
-    const int t0 = token(i), st = i % PR_STAGES, mt = i / PR_META & 1, mi = i % PR_META * 4;
+  // Tile i on its way to its stage; pg: its page, where a page holds whole tiles (then only the base differs from tile to
+  // tile), else its four groups of tokens are looked up by their lanes.
+  uint32_t koff[S::LOADS], voff[S::LOADS];
 #pragma unroll
-    for (int x = 0; x < S::LOADS; ++x) {
-      const int at = (x * AT_WAVES + wave) * 64 + lane;  // the 16-byte slot that this lane fills
-      const int t = at / (D / 16), p = key_piece<D>(t, at % (D / 16));
-      const size_t ph = size_t(max(lds.page[mt][mi + t / 16], 0)) * a.c.heads + h;
-      pipe::dma16_at(a.c.k + ((ph << sh) + ((t0 + t) & mask)) * D + 16 * p,
-                     pipe::lds_addr(&lds.k[st][(x * AT_WAVES + wave) * 1024]));
-    }
+  for (int x = 0; x < S::LOADS; ++x) {  // the 16-byte slots that this lane fills
+    const int at = (x * AT_WAVES + wave) * 64 + lane, t = at / (D / 16), d = at / 4;
+    koff[x] = uint32_t(t * D + 16 * key_piece<D>(t, at % (D / 16)));
+    voff[x] = uint32_t((d << sh) + 16 * value_piece(d, at % 4));
+  }
+  const bool whole = a.c.page >= TILE;
+  const auto page_at = [&](int i) { return lds.page[i / PR_META & 1][i % PR_META * 4]; };
+  const auto fetch = [&](int i, int pg) {
+    const int t0 = token(i), st = i % PR_STAGES;
+    const auto to = [&](uint8_t* stage, int x) { return pipe::lds_addr(stage + (x * AT_WAVES + wave) * 1024); };
+    if (whole) {
+      const size_t ph = size_t(uniform(max(pg, 0))) * a.c.heads + h;
+      const uint8_t* kb = a.c.k + ((ph << sh) + (t0 & mask)) * D;
+      const uint8_t* vb = a.c.v + ((ph * D) << sh) + (t0 & mask);
 #pragma unroll
-    for (int x = 0; x < S::LOADS; ++x) {
-      const int at = (x * AT_WAVES + wave) * 64 + lane, d = at / 4, p = value_piece(d, at % 4);
-      const size_t ph = size_t(max(lds.page[mt][mi + p], 0)) * a.c.heads + h;
-      pipe::dma16_at(a.c.v + ((ph * D + d) << sh) + ((t0 + 16 * p) & mask),
-                     pipe::lds_addr(&lds.v[st][(x * AT_WAVES + wave) * 1024]));
+      for (int x = 0; x < S::LOADS; ++x) pipe::dma16(kb, koff[x], to(lds.k[st], x));
+#pragma unroll
+      for (int x = 0; x < S::LOADS; ++x) pipe::dma16(vb, voff[x], to(lds.v[st], x));
+    } else {
+      const int* pages = &lds.page[i / PR_META & 1][i % PR_META * 4];
+#pragma unroll
+      for (int x = 0; x < S::LOADS; ++x) {
+        const uint32_t t = koff[x] / D;
+        const size_t ph = size_t(max(pages[t / 16], 0)) * a.c.heads + h;
+        pipe::dma16_at(a.c.k + ((ph << sh) + ((t0 + t) & mask)) * D + koff[x] % D, to(lds.k[st], x));
+      }
+#pragma unroll
+      for (int x = 0; x < S::LOADS; ++x) {
+        const int d = ((x * AT_WAVES + wave) * 64 + lane) / 4, p = int(voff[x] - (uint32_t(d) << sh)) / 16;
+        const size_t ph = size_t(max(pages[p], 0)) * a.c.heads + h;
+        pipe::dma16_at(a.c.v + ((ph * D + d) << sh) + ((t0 + 16 * p) & mask), to(lds.v[st], x));
+      }
     }
   };
 
@@ -682,11 +699,13 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
   float ref2 = -INFINITY, l = 0.0f;  // what the weights are relative to (a power of two's exponent); their sum
   const int n = tiles.count;
+  int next = 0;  // the page of the next tile to fetch, read ahead
   if (n > 0) {
     meta(0);
     __syncthreads();
-    fetch(0);
-    if (n > 1) fetch(1);
+    fetch(0, page_at(0));
+    if (n > 1) fetch(1, page_at(1));
+    if (n > 2) next = page_at(2);
   }
   const int krow = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);  // the token that is this lane's row of a half
   const int kat = krow * D + 16 * key_piece<D>(krow, h2), vat = c * 64;
@@ -695,7 +714,8 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
     else pipe::wait_vm<0>();
     pipe::lds_barrier();  // tile t is there, and every wave is done with tile t - 1
     if (t % PR_META == PR_META - 4 && t / PR_META * PR_META + PR_META < n) meta(t / PR_META + 1);
-    if (t + 2 < n) fetch(t + 2);
+    if (t + 2 < n) fetch(t + 2, next);
+    if (t + 3 < n) next = page_at(t + 3);
     const int t0 = token(t), mt = t / PR_META & 1, mi = t % PR_META * 4;
     if (wrow >= nrows || t0 > pos_hi) continue;
     const uint8_t *kt = lds.k[t % PR_STAGES], *vt = lds.v[t % PR_STAGES];
@@ -704,19 +724,33 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
     const bool masked = t0 + TILE - 1 > pos_lo || missing ||
                         (a.window > 0 && int64_t(t0) + a.window <= pos_hi && t0 + TILE > a.sinks);
 
+    uint4 kx[2][D / 32];
+    float ks[2], vs[2];
+#pragma unroll
+    for (int T = 0; T < 2; ++T) {
+      ks[T] = lds.ks[mt][mi + 2 * T + (c >> 2 & 1)];
+      vs[T] = lds.vs[mt][mi + 2 * T + h2];
+#pragma unroll
+      for (int m = 0; m < D / 32; ++m) kx[T][m] = ld16(kt + 32 * T * D + (kat ^ 32 * m));
+    }
+    __builtin_amdgcn_sched_barrier(0);  // every read on its way before the first product waits for one
     pipe::v16f_t s[2];
 #pragma unroll
     for (int T = 0; T < 2; ++T) {
-      const float ks = lds.ks[mt][mi + 2 * T + (c >> 2 & 1)];
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[T][r] = 0.0f;
 #pragma unroll
       for (int m = 0; m < D / 32; ++m) {
-        const uint4 x = ld16(kt + 32 * T * D + (kat ^ 32 * m));
-        s[T] = pipe::mfma32_bf16(fp8x8_to_bf16(x.x, x.y, ks), qf[2 * m], s[T]);
-        s[T] = pipe::mfma32_bf16(fp8x8_to_bf16(x.z, x.w, ks), qf[2 * m + 1], s[T]);
+        s[T] = pipe::mfma32_bf16(fp8x8_to_bf16(kx[T][m].x, kx[T][m].y, ks[T]), qf[2 * m], s[T]);
+        s[T] = pipe::mfma32_bf16(fp8x8_to_bf16(kx[T][m].z, kx[T][m].w, ks[T]), qf[2 * m + 1], s[T]);
       }
     }
+    uint4 vx[2][S::DT];
+#pragma unroll
+    for (int T = 0; T < 2; ++T)
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) vx[T][d] = ld16(vt + vat + 16 * value_piece(c, 2 * T + h2) + d * 2048);
+    __builtin_amdgcn_sched_barrier(0);
     uint32_t see[2] = {0xffff, 0xffff};
     int there[2] = {16, 16};  // of this lane's 16 values, those of tokens that are there
     if (masked) {
@@ -749,7 +783,6 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[T][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[T][r], sc, -base));
-        if (masked) s[T][r] = see[T] >> r & 1 ? s[T][r] : 0.0f;  // (-inf times a scale of 0)
         l += s[T][r];
       }
     bf16x8 p[2][2];
@@ -757,54 +790,54 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
     for (int T = 0; T < 2; ++T)
 #pragma unroll
       for (int e = 0; e < 16; ++e) p[T][e / 8][e % 8] = __bf16(s[T][e]);
-    if (!masked) {
+    if (masked) {  // slots past the last token hold anything: zero
+      uint32_t bad = 0;
 #pragma unroll
-      for (int T = 0; T < 2; ++T) {
-        const float vs = lds.vs[mt][mi + 2 * T + h2];
-        const uint8_t* at = vt + vat + 16 * value_piece(c, 2 * T + h2);
+      for (int T = 0; T < 2; ++T)
 #pragma unroll
         for (int d = 0; d < S::DT; ++d) {
-          const uint4 x = ld16(at + d * 2048);
-          o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(x.x, x.y, vs), p[T][0], o[d]);
-          o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(x.z, x.w, vs), p[T][1], o[d]);
+          uint4& x = vx[T][d];
+          x.x &= first_bytes(there[T]), x.y &= first_bytes(there[T] - 4), x.z &= first_bytes(there[T] - 8);
+          x.w &= first_bytes(there[T] - 12);
+          bad |= nan_bytes(x.x) | nan_bytes(x.y) | nan_bytes(x.z) | nan_bytes(x.w);
         }
-      }
-    } else {  // as in the split kernel: what is behind the last token is zero, NaN counted for the rows that see it
+      if (__builtin_expect(__any(bad != 0), 0)) {
+        // 0 x NaN is NaN: the NaN among the values are taken out, and each is set by itself in the sums of the rows that see
+        // it, from the codes in LDS (few registers; how long it takes does not matter).
 #pragma unroll
-      for (int T = 0; T < 2; ++T) {
-        const float vs = lds.vs[mt][mi + 2 * T + h2];
-        const uint8_t* at = vt + vat + 16 * value_piece(c, 2 * T + h2);
+        for (int d = 0; d < S::DT; ++d)
+          for (int k = 0; k < 8; ++k) {
+            const int T = k >> 2, j = 4 * (k & 3);  // tokens j .. j + 3 of the lane's 16
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(vt + vat + 16 * value_piece(c, 2 * T + h2) + d * 2048 + j);
+            const uint32_t nan = nan_bytes(x & first_bytes((T ? there[1] : there[0]) - j));
+            for (uint64_t left = __ballot(nan != 0); left; left &= left - 1) {
+              const int from = __ffsll((unsigned long long)left) - 1;  // its channel: row 8a + 4h + i of the products
+              const uint32_t bits = lane_of(nan, from);
+              for (int e = 0; e < 4; ++e) {
+                if (!(bits >> (8 * e + 7) & 1)) continue;
+                const int tok = t0 + 32 * T + (from & 32) / 2 + j + e, to = from / 8 % 4 * 4 + from % 4;
+                const bool hit = h2 == (from >> 2 & 1) && (seen_bits(pos, tok, a.window, a.sinks) & 1);
 #pragma unroll
-        for (int d = 0; d < S::DT; ++d) {
-          const uint4 y = ld16(at + d * 2048);
-          uint32_t x[4] = {y.x, y.y, y.z, y.w}, nan[4], bad = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[k] &= first_bytes(there[T] - 4 * k);
-            nan[k] = nan_bytes(x[k]) >> 7;
-            bad |= nan[k];
-          }
-          if (__builtin_expect(__any(bad != 0), 0)) {
-            pipe::v16f_t many;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) many[r] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t n0 = nan[2 * e], n1 = nan[2 * e + 1], z = see[T] >> (8 * e);
-              many = pipe::mfma32_bf16(ones(n0, n0 >> 8, n0 >> 16, n0 >> 24, n1, n1 >> 8, n1 >> 16, n1 >> 24),
-                                       ones(z, z >> 1, z >> 2, z >> 3, z >> 4, z >> 5, z >> 6, z >> 7), many);
-              x[2 * e] &= ~(n0 * 0xffu);
-              x[2 * e + 1] &= ~(n1 * 0xffu);
+                for (int r = 0; r < 16; ++r) o[d][r] = hit && r == to ? __builtin_nanf("") : o[d][r];
+              }
             }
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (many[r] > 0.0f) o[d][r] = __builtin_nanf("");
           }
-          o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(x[0], x[1], vs), p[T][0], o[d]);
-          o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(x[2], x[3], vs), p[T][1], o[d]);
-        }
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int d = 0; d < S::DT; ++d) {
+            uint4& x = vx[T][d];
+            x = make_uint4(no_nan(x.x), no_nan(x.y), no_nan(x.z), no_nan(x.w));
+          }
       }
     }
+#pragma unroll
+    for (int T = 0; T < 2; ++T)
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) {
+        o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(vx[T][d].x, vx[T][d].y, vs[T]), p[T][0], o[d]);
+        o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(vx[T][d].z, vx[T][d].w, vs[T]), p[T][1], o[d]);
+      }
   }
   l += __shfl_xor(l, 32, 64);
   if (wrow + c >= nrows) return;
