@@ -17,6 +17,7 @@ namespace {
 constexpr int TILE = 64;          // tokens a wave takes at a time
 constexpr int AT_NT = 256;        // threads of a workgroup
 constexpr int AT_WAVES = AT_NT / 64;
+constexpr int FEW = 16;           // rows (of a key / value head) of a sequence that the split kernel takes
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 // Bits of the first n of up to 16 tokens.
@@ -51,10 +52,10 @@ struct Attend {
   KvCache c;
   int ldq, ldo, group, page_shift, window, sinks;
   float scale2;  // scale * log2(e): the kernels take powers of two
-  int few;             // sequences of up to this many rows are the split kernel's, the others the tiled kernel's
+  int few;  // sequences of up to this many rows (FEW or none) are the split kernel's, the others the tiled kernel's
   uint32_t target;     // workgroups that the chip holds at a time
   uint32_t* counters;  // of finished parts, by the workgroup of the first; zero between launches
-  float *po, *pml;     // partial sums: values [slot][ROWS][D]; maximum and weight sum [slot][ROWS][2]
+  float *po, *pml;     // partial sums: values [slot][rows][D]; maximum and weight sum [slot][rows][2]
 };
 
 // The 64-token tiles that some row of a sequence sees: with a window the sinks' tiles [0, sink_tiles) and those from
@@ -78,40 +79,57 @@ __device__ __forceinline__ Tiles tiles_of(const Attend& a, const Seq& q) {
 __device__ __forceinline__ int row_groups(int rows, int per) { return (rows + per - 1) / per; }
 
 // The split of a launch's work, worked out by every workgroup from the lengths, which only the device knows. A segment is a
-// (sequence, key / value head, row group) and its tiles.
+// (sequence, key / value head) and its tiles.
 // Many segments: workgroup w takes the tiles [w share, (w + 1) share) of all segments in order, so that long and short
-// sequences load the chip evenly; it may end one segment, do some whole ones and begin another.
-// Few segments (each would cost a workgroup that has the end of one and the beginning of another a start more than
-// those next to it): each is cut into parts as equal as they can be, a workgroup each.
+// sequences load the chip evenly; it may end one segment, do some whole ones and begin another, and each beginning costs it
+// START tiles' time. Few segments (an eighth of the workgroups): each is cut into parts as equal as they can be, a workgroup
+// each, and no workgroup has two beginnings. (256 segments of 18 tiles under a window, four layers: 68 us cut anywhere, 74 in
+// two equal parts, each joined, 72 whole; 8 of 65 tiles, sixteen layers: 298 us cut anywhere, 186 in equal parts.)
 // The parts of a segment are those of consecutive workgroups; the part of workgroup w that begins a segment leaves its sums
 // in slot 2 w + 1, one that goes on with it in slot 2 w.
 struct Walk {
-  int b, segs, rgs, seg;  // the sequence, its segments, its row groups, the segment
-  uint32_t at;            // where the segment begins, in units (tiles, or parts of equal segments)
+  int b, h;     // the sequence and the head
+  uint32_t at;  // where the segment begins, in units (tiles, or parts of equal segments)
   Seq q;
   Tiles t;
 };
 struct Part {
-  int h, rg, i0, i1, index, parts;
+  int i0, i1, index, parts;
 };
 constexpr uint32_t START = 2;  // a segment's start, in tiles: the time that its first loads and its end take
+// The parts that n tiles make.
+__device__ __forceinline__ uint32_t parts_of(uint32_t tiles, uint32_t share) {
+  return max((tiles + share - 1) / share, 1u);  // (no tiles: a part that writes zeros)
+}
+// The smallest share, `least` at least, with which n things of `tiles` tiles in each lane make `target` parts or fewer: all
+// is their number over the lanes (<= target), sum their tiles. ceil(sum / target) is too small or right, and
+// ceil(sum / (target - all)) is large enough: each adds a part at most to its exact share.
+__device__ __forceinline__ uint32_t smallest_share(uint32_t n, uint32_t tiles, uint32_t sum, uint32_t all, uint32_t target,
+                                                   uint32_t least) {
+  uint32_t lo = max((sum + target - 1) / target, least);
+  uint32_t hi = max(all < target ? (sum + target - all - 1) / (target - all) : wave_reduce_u32<true>(tiles), least);
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (lane_of(wave_scan(n * parts_of(tiles, mid)), 63) <= target) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
 struct Split {
-  bool whole;            // few segments
+  bool whole;            // equal parts of each segment
   uint32_t share, unit;  // tiles of a part at most; units of a workgroup
 };
 __device__ __forceinline__ uint32_t units_of(const Split& s, uint32_t tiles) {
-  return s.whole ? max((tiles + s.share - 1) / s.share, 1u) : tiles + START;  // (no tiles: a part that writes zeros)
+  return s.whole ? parts_of(tiles, s.share) : tiles + START;
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-template <int ROWS>
-__device__ __forceinline__ int segs_of(const Attend& a, const Seq& q) {
-  const int rows = (q.r1 - q.r0) * a.group;
-  return rows <= a.few ? row_groups(rows, ROWS) * a.c.heads : 0;
+__device__ __forceinline__ bool is_few(const Attend& a, const Seq& q) {
+  return q.r1 > q.r0 && (q.r1 - q.r0) * a.group <= a.few;
 }
 // The segment that holds the workgroup's first unit. Every wave for itself, a sequence a lane: no barriers, and for up to 64
 // sequences one pass over registers.
-template <int ROWS, int LEAST>
 __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w) {
   const int lane = threadIdx.x & 63;
   uint32_t segs = 0;  // of this lane's sequence
@@ -120,8 +138,10 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w)
     w.t = Tiles{0, 0, 0};
     if (b < a.st.B) {
       w.q = seq_of(a.st, b);
-      segs = uint32_t(segs_of<ROWS>(a, w.q));
-      if (segs) w.t = tiles_of(a, w.q);
+      if (is_few(a, w.q)) {
+        segs = uint32_t(a.c.heads);
+        w.t = tiles_of(a, w.q);
+      }
     }
   };
   uint32_t tiles = 0, all = 0;
@@ -131,8 +151,9 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w)
     all += lane_of(wave_scan(segs), 63);
   }
   s.whole = all * 8 <= a.target;
-  const uint32_t wgs = s.whole ? a.target - all : a.target;
-  s.share = max((tiles + wgs - 1) / wgs, uint32_t(LEAST));
+  if (!s.whole) s.share = max((tiles + a.target - 1) / a.target, uint32_t(AT_WAVES));
+  else if (a.st.B <= 64) s.share = smallest_share(segs, uint32_t(w.t.count), tiles - START * all, all, a.target, AT_WAVES);
+  else s.share = max((tiles + a.target - all - 1) / (a.target - all), uint32_t(AT_WAVES));  // one that is large enough
   s.unit = s.whole ? 1 : s.share;
   const uint32_t u = blockIdx.x * s.unit;
   uint32_t from = 0;
@@ -145,11 +166,9 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w)
       w.b = b0 + l;
       w.q = Seq{int(lane_of(w.q.r0, l)), int(lane_of(w.q.r1, l)), int(lane_of(w.q.len, l)), int(lane_of(w.q.first, l))};
       w.t = Tiles{int(lane_of(w.t.sink_tiles, l)), int(lane_of(w.t.skip, l)), int(lane_of(w.t.count, l))};
-      w.segs = int(lane_of(segs, l));
-      w.rgs = w.segs / a.c.heads;
       const uint32_t first = lane_of(end - n, l), size = lane_of(each, l);
-      w.seg = int((u - first) / size);
-      w.at = first + uint32_t(w.seg) * size;
+      w.h = int((u - first) / size);
+      w.at = first + uint32_t(w.h) * size;
       return true;
     }
     from = lane_of(end, 63);
@@ -160,8 +179,6 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w)
 __device__ __forceinline__ Part part_of(const Split& s, const Walk& w, uint32_t u) {
   Part p;
   const uint32_t count = uint32_t(w.t.count), size = units_of(s, count), w0 = w.at / s.unit;
-  p.h = w.seg / w.rgs;
-  p.rg = w.seg % w.rgs;
   p.index = int(blockIdx.x - w0);
   p.parts = int((w.at + size - 1) / s.unit - w0 + 1);
   if (s.whole) {
@@ -176,19 +193,16 @@ __device__ __forceinline__ Part part_of(const Split& s, const Walk& w, uint32_t 
   return p;
 }
 // The next segment, if the workgroup's units reach it.
-template <int ROWS>
 __device__ __forceinline__ bool next_segment(const Attend& a, const Split& s, Walk& w) {
   w.at += units_of(s, uint32_t(w.t.count));
   if (s.whole || w.at >= (blockIdx.x + 1) * s.unit) return false;
-  if (++w.seg < w.segs) return true;
-  w.seg = 0;
+  if (++w.h < a.c.heads) return true;
+  w.h = 0;
   do {
     if (++w.b >= a.st.B) return false;
     const Seq q = seq_of(a.st, w.b);
     w.q = Seq{uniform(q.r0), uniform(q.r1), uniform(q.len), uniform(q.first)};
-    w.segs = segs_of<ROWS>(a, w.q);
-  } while (w.segs == 0);
-  w.rgs = w.segs / a.c.heads;
+  } while (!is_few(a, w.q));
   w.t = tiles_of(a, w.q);
   return true;
 }
@@ -222,24 +236,21 @@ __device__ __forceinline__ uint32_t no_nan(uint32_t x) { return x & ~((nan_bytes
 // The codes become bf16 exactly (v_cvt_scalef32, the block's scale with them), the products sum in fp32; the weights are
 // rounded to bf16 for the second product (2^-8 of each at most, as much as the output's own rounding), their sum is taken in
 // fp32 before that.
-// The four waves are RW sets of 16 rows (they read the same tokens, which L1 serves) times 4 / RW that take every
-// (4 / RW)-th tile and are joined in LDS. The workgroup that finishes last of those that share rows adds their partial
-// sums, in the order of the tiles whichever it is: the result does not depend on timing.
-template <int D, int RW>
+// The four waves take every fourth tile and are joined in LDS. The workgroup that finishes last of those that share rows adds
+// their partial sums, in the order of the tiles whichever it is: the result does not depend on timing.
+template <int D>
 struct Shape {
-  static constexpr int TW = AT_WAVES / RW;  // waves that share rows
-  static constexpr int ROWS = 16 * RW;
   static constexpr int KL = D / 64;  // 16-byte loads of a key row's quarter
   static constexpr int DT = D / 16;  // 16-channel tiles
   struct Lds {
-    float o[TW > 1 ? AT_WAVES / 2 : 1][16 * D];
-    float ml[AT_WAVES][16][2];
+    float o[AT_WAVES / 2][FEW * D];
+    float ml[AT_WAVES][FEW][2];
   };
 };
 // Workgroups that a CU holds, by their registers.
 constexpr int wgs_per_cu(int dim) { return dim <= 128 ? 2 : 1; }
 constexpr int target_of(int dim) { return 256 * wgs_per_cu(dim); }
-constexpr size_t kCounterBytes = 256 * 2 * sizeof(uint32_t);
+constexpr size_t kCounterBytes = 512 * sizeof(uint32_t);
 
 // Partial sums pass between workgroups on different XCDs, whose L2 caches do not see each other's lines: stored through
 // to memory and read from there (device-scope accesses), which for these few KiB is far cheaper than the fences that
@@ -277,16 +288,15 @@ __device__ __forceinline__ void store_out(const Attend& a, int row, int hq, int 
   if (first && a.lse) a.lse[size_t(row) * (a.group * a.c.heads) + hq] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
 }
 
-template <int D, int RW>
+template <int D>
 __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a) {
-  using S = Shape<D, RW>;
-  constexpr int TW = S::TW;
+  using S = Shape<D>;
   __shared__ __align__(16) typename S::Lds lds;
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
   Split sp;
   Walk w;
-  if (!find_segment<S::ROWS, TW>(a, sp, w)) return;
+  if (!find_segment(a, sp, w)) return;
   Part pt = part_of(sp, w, blockIdx.x * sp.unit);
 
   const int mask = a.c.page - 1, sh = a.page_shift;
@@ -294,8 +304,8 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
   uint32_t vr[S::DT][4];
   bf16x8 qf[2 * S::KL];
   int ksb, vsb;
-  int pos, my_row, my_hq;         // this lane's row (the last one where there are fewer)
-  int pos_lo, pos_hi, nrows, row0;  // of the wave's rows
+  int pos, my_row, my_hq;     // this lane's row (the last one where there are fewer)
+  int pos_lo, pos_hi, nrows;  // of all rows
   int i, pk, pv, pk1, pv1;
   const auto token = [&](int i) { return w.t.at(i) * TILE; };
   const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
@@ -303,7 +313,7 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
     pv = page_of(a.st.table, a.st.max_blocks, a.c.pages, w.b, (t0 + 16 * g) >> sh);
   };
   const auto load_k = [&](int t0, int pk) {
-    const size_t ph = size_t(max(pk, 0)) * a.c.heads + pt.h;
+    const size_t ph = size_t(max(pk, 0)) * a.c.heads + w.h;
     const uint8_t* p = a.c.k + ((ph << sh) + ((t0 + 16 * (c >> 2) + (c & 3)) & mask)) * D + 16 * g;
     ksb = a.c.ks[ph];
 #pragma unroll
@@ -312,7 +322,7 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
       for (int m = 0; m < S::KL; ++m) kr[j][m] = ld16(p + 4 * j * D + 64 * m);
   };
   const auto load_v = [&](int t0, int pv) {
-    const size_t ph = size_t(max(pv, 0)) * a.c.heads + pt.h;
+    const size_t ph = size_t(max(pv, 0)) * a.c.heads + w.h;
     const uint8_t* p = a.c.v + ((ph * D + c) << sh) + ((t0 + 16 * g) & mask);
     vsb = a.c.vs[ph];
 #pragma unroll
@@ -324,14 +334,13 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
   };
   const auto begin = [&] {  // a part: its rows, and its first loads on their way
     nrows = (w.q.r1 - w.q.r0) * a.group;
-    row0 = pt.rg * S::ROWS + wave / TW * 16;
-    i = row0 < nrows ? pt.i0 + wave % TW : pt.i1;  // (no rows for this wave)
+    i = pt.i0 + wave;
     if (i < pt.i1) lookup(token(i), pk, pv);
-    const int ri = min(row0 + c, nrows - 1);
-    my_row = w.q.r0 + ri / a.group, my_hq = pt.h * a.group + ri % a.group;
+    const int ri = min(c, nrows - 1);
+    my_row = w.q.r0 + ri / a.group, my_hq = w.h * a.group + ri % a.group;
     pos = w.q.first + ri / a.group;
-    pos_lo = uniform(w.q.first + min(row0, nrows - 1) / a.group);
-    pos_hi = uniform(w.q.first + min(row0 + 15, nrows - 1) / a.group);
+    pos_lo = w.q.first;
+    pos_hi = w.q.first + (w.q.r1 - w.q.r0) - 1;
     const bf16* x = a.q + size_t(my_row) * a.ldq + size_t(my_hq) * D + 16 * g;
 #pragma unroll
     for (int m = 0; m < S::KL; ++m) {
@@ -341,7 +350,7 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
     if (i < pt.i1) {
       load_k(token(i), pk);
       load_v(token(i), pv);
-      if (i + TW < pt.i1) lookup(token(i + TW), pk1, pv1);
+      if (i + AT_WAVES < pt.i1) lookup(token(i + AT_WAVES), pk1, pv1);
     }
   };
 
@@ -351,10 +360,10 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
     float mx = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int d = 0; d < S::DT; ++d) o[d] = v4f{0, 0, 0, 0};
-    for (; i < pt.i1; i += TW) {
+    for (; i < pt.i1; i += AT_WAVES) {
       const int t0 = token(i);
-      const bool more = i + TW < pt.i1;
-      const int tn = token(more ? i + TW : i);
+      const bool more = i + AT_WAVES < pt.i1;
+      const int tn = token(more ? i + AT_WAVES : i);
       const float ks = e8m0_to_f32(uint8_t(ksb));
       v4f s[4];
 #pragma unroll
@@ -370,7 +379,7 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
       if (more) {
         pk = pk1, pv = pv1;
         load_k(tn, pk);
-        if (i + 2 * TW < pt.i1) lookup(token(i + 2 * TW), pk1, pv1);
+        if (i + 2 * AT_WAVES < pt.i1) lookup(token(i + 2 * AT_WAVES), pk1, pv1);
       }
       // what a row does not see: only in the tiles at the ends of what the rows see
       const bool masked = t0 + TILE - 1 > pos_lo || __any(pvt < 0) ||
@@ -446,44 +455,39 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
     // the part is summed: the next one's loads go out, then this one is joined
     const Part done = pt;
     const uint32_t w0 = blockIdx.x - uint32_t(done.index);
-    const int row = my_row, hq = my_hq, r0 = w.q.r0, left = nrows - done.rg * S::ROWS;  // rows from the group's on
-    const bool mine = wave % TW == 0 && row0 + c < nrows;
-    again = next_segment<S::ROWS>(a, sp, w);
+    const int row = my_row, hq = my_hq, r0 = w.q.r0, h = w.h, rows = nrows;
+    const bool mine = wave == 0 && c < nrows;
+    again = next_segment(a, sp, w);
     if (again) {
       pt = part_of(sp, w, w.at);
       begin();
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    if constexpr (TW > 1) {
-      pipe::lds_barrier();  // the last part's use of the LDS
-      if (g == 0) lds.ml[wave][c][0] = mx, lds.ml[wave][c][1] = l;
+    pipe::lds_barrier();  // the last part's use of the LDS
+    if (g == 0) lds.ml[wave][c][0] = mx, lds.ml[wave][c][1] = l;
+    pipe::lds_barrier();
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < AT_WAVES; ++k) m = fmaxf(m, lds.ml[k][c][0]);
+    const float ref = m == -INFINITY ? 0.0f : m, f = __builtin_amdgcn_exp2f(mx - ref);
+    l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < AT_WAVES; ++k) l += lds.ml[k][c][1] * __builtin_amdgcn_exp2f(lds.ml[k][c][0] - ref);
+    mx = m;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) o[d] *= f;
+    const auto at = [&](int buf, int d) { return reinterpret_cast<v4f*>(&lds.o[buf][(d * 64 + lane) * 4]); };
+#pragma unroll
+    for (int half = AT_WAVES / 2; half; half /= 2) {  // the upper half of the waves hands its sums to the lower
+      if (wave >= half && wave < 2 * half)
+#pragma unroll
+        for (int d = 0; d < S::DT; ++d) *at(wave - half, d) = o[d];
       pipe::lds_barrier();
-      const int first = wave / TW * TW;
-      float m = -INFINITY;
+      if (wave < half)
 #pragma unroll
-      for (int k = 0; k < TW; ++k) m = fmaxf(m, lds.ml[first + k][c][0]);
-      const float ref = m == -INFINITY ? 0.0f : m, f = __builtin_amdgcn_exp2f(mx - ref);
-      l = 0.0f;
-#pragma unroll
-      for (int k = 0; k < TW; ++k)
-        l += lds.ml[first + k][c][1] * __builtin_amdgcn_exp2f(lds.ml[first + k][c][0] - ref);
-      mx = m;
-#pragma unroll
-      for (int d = 0; d < S::DT; ++d) o[d] *= f;
-      const auto at = [&](int buf, int d) { return reinterpret_cast<v4f*>(&lds.o[buf][(d * 64 + lane) * 4]); };
-#pragma unroll
-      for (int half = TW / 2; half; half /= 2) {  // the upper half of the waves hands its sums to the lower
-        const int k = wave % TW, buf = wave / TW * (TW / 2) + k % half;
-        if (k >= half && k < 2 * half)
-#pragma unroll
-          for (int d = 0; d < S::DT; ++d) *at(buf, d) = o[d];
-        pipe::lds_barrier();
-        if (k < half)
-#pragma unroll
-          for (int d = 0; d < S::DT; ++d) o[d] += *at(buf, d);
-        pipe::lds_barrier();
-      }
+        for (int d = 0; d < S::DT; ++d) o[d] += *at(wave, d);
+      pipe::lds_barrier();
     }
     if (done.parts == 1) {
       if (mine)
@@ -492,7 +496,7 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
       continue;
     }
     if (mine) {
-      const int r = int(blockIdx.x * 2 + (done.index == 0 ? 1 : 0)) * S::ROWS + wave / TW * 16 + c;
+      const int r = int(blockIdx.x * 2 + (done.index == 0 ? 1 : 0)) * FEW + c;
 #pragma unroll
       for (int d = 0; d < S::DT; ++d) put4(sums_of(a.po), r * D + 4 * g + 16 * d, o[d]);
       if (g == 0) put2(sums_of(a.pml), r * 2, mx, l);
@@ -507,7 +511,6 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
     if (tid == 0)  // as it was found
       __hip_atomic_store(&a.counters[w0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // a thread per row and four channels, the loads of JOIN parts in flight at a time
-    const int rows = min(S::ROWS, left);
     for (int it = tid; it < rows * (D / 4); it += AT_NT) {
       const int r = it / (D / 4), d = it % (D / 4) * 4;
       float m = -INFINITY, sum = 0.0f;
@@ -518,7 +521,7 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
 #pragma unroll
         for (int k = 0; k < JOIN; ++k) {
           const int p = min(k0 + k, done.parts - 1);
-          const int at = (int(w0 + uint32_t(p)) * 2 + (p == 0 ? 1 : 0)) * S::ROWS + r;
+          const int at = (int(w0 + uint32_t(p)) * 2 + (p == 0 ? 1 : 0)) * FEW + r;
           x[k] = get2(sums_of(a.pml), at * 2);
           y[k] = get4(sums_of(a.po), at * D + d);
         }
@@ -537,8 +540,7 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
             acc += f * y[k];
           }
       }
-      const int rr = done.rg * S::ROWS + r;
-      store_out<D>(a, r0 + rr / a.group, done.h * a.group + rr % a.group, d, acc, sum, m, d == 0);
+      store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
     }
   }
 }
@@ -559,6 +561,12 @@ constexpr int PR_STAGES = 3;
 constexpr int PR_META = 16;  // tiles
 constexpr float PR_LAG = 8.0f;
 
+// The larger of a lane's value and its counterpart's in the wave's other half.
+__device__ __forceinline__ float max_halves(float v) {
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+
 // The place among a key row's pieces of piece p of row (token) t, and among a channel's pieces of piece p of channel d.
 template <int D>
 __device__ __forceinline__ int key_piece(int t, int p) {
@@ -575,49 +583,93 @@ struct Tiled {
   struct Lds {
     uint8_t k[PR_STAGES][KV], v[PR_STAGES][KV];
     int page[2][PR_META * 4];
+    uint64_t missing[2];  // a bit for every 16 tokens without a page
     float ks[2][PR_META * 4], vs[2][PR_META * 4];  // of every 16 tokens
   };
 };
 
+// A workgroup's rows and tiles. The row blocks of all sequences times the heads, and where these do not fill the chip each
+// block's tiles are cut into parts of at most `share`: as few as still fill it. A sequence's last blocks, which see the most,
+// come first; the heads are inner, so that with 8 heads or a multiple an XCD's workgroups read the same ones' keys and
+// values.
+struct BlockPart {
+  int b, h, row0;
+  Seq q;
+  Tiles t;                       // that the block's rows see
+  int i0, i1;                    // the part's of them
+  int index, parts, first;       // which part of how many, and the workgroup of the first
+};
+__device__ __forceinline__ Tiles block_tiles(const Attend& a, const Seq& q, int row0) {
+  const int last = min(row0 + PR_ROWS, (q.r1 - q.r0) * a.group) - 1;
+  return tiles_of(a, Seq{0, 0, max(min(q.len, q.first + last / a.group + 1), 0), q.first + row0 / a.group});
+}
+__device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p) {
+  constexpr uint32_t LEAST = 4, NONE = 1u << 30;
+  const int lane = threadIdx.x & 63;
+  const uint32_t heads = uint32_t(a.c.heads);
+  Seq q{0, 0, 0, 0};
+  uint32_t blocks = 0, most = 0, all = 0;  // of this lane's sequence, tiles of its last block; of all, times the heads
+  const auto look = [&](int b) {
+    blocks = most = 0;
+    if (b < a.st.B) {
+      q = seq_of(a.st, b);
+      const int rows = (q.r1 - q.r0) * a.group;
+      if (rows > a.few) {
+        blocks = uint32_t(row_groups(rows, PR_ROWS));
+        most = uint32_t(block_tiles(a, q, int(blocks - 1) * PR_ROWS).count);
+      }
+    }
+  };
+  uint32_t tiles = 0;  // (a block's taken as the last one's; as long as the blocks are few)
+  for (int b0 = 0; b0 < a.st.B; b0 += 64) {
+    look(b0 + lane);
+    all += lane_of(wave_scan(blocks), 63) * heads;
+    if (all < a.target) tiles += lane_of(wave_scan(blocks * most), 63) * heads;
+  }
+  uint32_t share = NONE;
+  if (all < a.target && a.st.B <= 64) share = smallest_share(blocks * heads, most, tiles, all, a.target, LEAST);
+  else if (all < a.target) share = max((tiles + a.target - all - 1) / (a.target - all), LEAST);  // one that is large enough
+  uint32_t from = 0;
+  for (int b0 = 0; b0 < a.st.B; b0 += 64) {
+    if (a.st.B > 64) look(b0 + lane);
+    const uint32_t parts = parts_of(most, share), n = blocks * parts * heads, end = from + wave_scan(n);
+    const uint64_t hit = __ballot(blockIdx.x < end);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      p.b = b0 + l;
+      p.q = Seq{int(lane_of(q.r0, l)), int(lane_of(q.r1, l)), int(lane_of(q.len, l)), int(lane_of(q.first, l))};
+      const uint32_t in = blockIdx.x - lane_of(end - n, l), np = lane_of(parts, l);
+      p.h = int(in % heads);
+      p.index = int(in / heads % np);
+      const int block = int(lane_of(blocks, l) - 1 - in / heads / np);
+      p.row0 = block * PR_ROWS;
+      const Tiles t = block_tiles(a, p.q, p.row0);
+      p.t = Tiles{uniform(t.sink_tiles), uniform(t.skip), uniform(t.count)};
+      p.parts = int(parts_of(uint32_t(p.t.count), share));
+      if (p.index >= p.parts) return false;  // (a block that sees less than the sequence's last)
+      p.first = int(blockIdx.x) - p.index * int(heads);
+      const int each = p.t.count / p.parts, more = p.t.count % p.parts;
+      p.i0 = p.index * each + min(p.index, more);
+      p.i1 = p.i0 + each + (p.index < more ? 1 : 0);
+      return true;
+    }
+    from = lane_of(end, 63);
+  }
+  return false;
+}
+
 template <int D>
-__global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Attend a) {
+__global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tiled_kernel(Attend a) {
   using S = Tiled<D>;
   __shared__ __align__(1024) typename S::Lds lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 31, h2 = lane >> 5;
 
-  // Workgroup -> (row block, head): heads inner, so that with 8 heads or a multiple an XCD's workgroups read the same ones'
-  // keys and values; a sequence's last blocks, which see the most, first.
-  const int h = int(blockIdx.x % unsigned(a.c.heads));
-  const uint32_t block = blockIdx.x / unsigned(a.c.heads);
-  Seq q{0, 0, 0, 0};
-  int b = -1, row0 = 0;
-  uint32_t from = 0;
-  for (int b0 = 0; b0 < a.st.B && b < 0; b0 += 64) {
-    uint32_t n = 0;
-    if (b0 + lane < a.st.B) {
-      q = seq_of(a.st, b0 + lane);
-      const int rows = (q.r1 - q.r0) * a.group;
-      n = rows > a.few ? uint32_t(row_groups(rows, PR_ROWS)) : 0;
-    }
-    const uint32_t end = from + wave_scan(n);
-    const uint64_t hit = __ballot(block < end);
-    if (hit) {
-      const int l = __ffsll((unsigned long long)hit) - 1;
-      b = b0 + l;
-      q = Seq{int(lane_of(q.r0, l)), int(lane_of(q.r1, l)), int(lane_of(q.len, l)), int(lane_of(q.first, l))};
-      row0 = int(lane_of(end, l) - 1 - block) * PR_ROWS;
-    }
-    from = lane_of(end, 63);
-  }
-  if (b < 0) return;
-  const int nrows = (q.r1 - q.r0) * a.group;
-  Tiles tiles;  // that the workgroup's rows see
-  {
-    const int last = min(row0 + PR_ROWS, nrows) - 1;
-    const Seq mine{0, 0, min(q.len, q.first + last / a.group + 1), q.first + row0 / a.group};
-    tiles = tiles_of(a, Seq{0, 0, max(mine.len, 0), mine.first});
-    tiles = Tiles{uniform(tiles.sink_tiles), uniform(tiles.skip), uniform(tiles.count)};
-  }
+  BlockPart bp;
+  if (!find_block(a, bp)) return;
+  const int b = bp.b, h = bp.h, row0 = bp.row0;
+  const Seq q = bp.q;
+  const Tiles tiles = bp.t;
+  const int nrows = (q.r1 - q.r0) * a.group, parts = bp.parts;
 
   // this lane's row
   const int wrow = row0 + 32 * wave, ri = min(wrow + c, nrows - 1);
@@ -640,13 +692,15 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
   }
   const float sc = fmaxf(fabsf(a.scale2), 0x1p-126f);  // (not 0: hidden scores are -inf, and stay so)
 
-  const auto token = [&](int i) { return tiles.at(i) * TILE; };
+  const auto token = [&](int i) { return tiles.at(bp.i0 + i) * TILE; };
   const auto meta = [&](int chunk) {  // pages and scales of tiles [16 chunk, 16 chunk + 16)
     if (tid < PR_META * 4) {
       const int i = chunk * PR_META + tid / 4;
-      const int pg = i < tiles.count ? page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (token(i) + tid % 4 * 16) >> a.page_shift)
+      const int pg = i < bp.i1 - bp.i0 ? page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (token(i) + tid % 4 * 16) >> a.page_shift)
                                      : -1;
       const size_t ph = size_t(max(pg, 0)) * a.c.heads + h;
+      const uint64_t none = __ballot(pg < 0);
+      if (tid == 0) lds.missing[chunk & 1] = none;
       lds.page[chunk & 1][tid] = pg;
       lds.ks[chunk & 1][tid] = e8m0_to_f32(a.c.ks[ph]);
       lds.vs[chunk & 1][tid] = e8m0_to_f32(a.c.vs[ph]);
@@ -698,8 +752,9 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
   float ref2 = -INFINITY, l = 0.0f;  // what the weights are relative to (a power of two's exponent); their sum
-  const int n = tiles.count;
+  const int n = bp.i1 - bp.i0;
   int next = 0;  // the page of the next tile to fetch, read ahead
+  uint64_t missing = 0;
   if (n > 0) {
     meta(0);
     __syncthreads();
@@ -717,11 +772,13 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
     if (t + 2 < n) fetch(t + 2, next);
     if (t + 3 < n) next = page_at(t + 3);
     const int t0 = token(t), mt = t / PR_META & 1, mi = t % PR_META * 4;
+    if (t % PR_META == 0) {
+      const uint64_t x = lds.missing[mt];
+      missing = uint64_t(uint32_t(uniform(int(x >> 32)))) << 32 | uint32_t(uniform(int(x)));
+    }
     if (wrow >= nrows || t0 > pos_hi) continue;
     const uint8_t *kt = lds.k[t % PR_STAGES], *vt = lds.v[t % PR_STAGES];
-    const int4 pg = *reinterpret_cast<const int4*>(&lds.page[mt][mi]);
-    const bool missing = uniform((pg.x | pg.y | pg.z | pg.w) < 0);
-    const bool masked = t0 + TILE - 1 > pos_lo || missing ||
+    const bool masked = t0 + TILE - 1 > pos_lo || (missing >> mi & 15) != 0 ||
                         (a.window > 0 && int64_t(t0) + a.window <= pos_hi && t0 + TILE > a.sinks);
 
     uint4 kx[2][D / 32];
@@ -734,16 +791,17 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
       for (int m = 0; m < D / 32; ++m) kx[T][m] = ld16(kt + 32 * T * D + (kat ^ 32 * m));
     }
     __builtin_amdgcn_sched_barrier(0);  // every read on its way before the first product waits for one
-    pipe::v16f_t s[2];
+    pipe::v16f_t s[2];  // (products that follow one another add to different sums: none waits for the one before)
 #pragma unroll
-    for (int T = 0; T < 2; ++T) {
+    for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[T][r] = 0.0f;
+    for (int m = 0; m < D / 32; ++m) {
 #pragma unroll
-      for (int m = 0; m < D / 32; ++m) {
+      for (int T = 0; T < 2; ++T)
         s[T] = pipe::mfma32_bf16(fp8x8_to_bf16(kx[T][m].x, kx[T][m].y, ks[T]), qf[2 * m], s[T]);
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
         s[T] = pipe::mfma32_bf16(fp8x8_to_bf16(kx[T][m].z, kx[T][m].w, ks[T]), qf[2 * m + 1], s[T]);
-      }
     }
     uint4 vx[2][S::DT];
 #pragma unroll
@@ -757,7 +815,7 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
 #pragma unroll
       for (int T = 0; T < 2; ++T) {
         const int tt = t0 + 32 * T + 16 * h2;
-        const bool none = lds.page[mt][mi + 2 * T + h2] < 0;
+        const bool none = missing >> (mi + 2 * T + h2) & 1;
         see[T] = none ? 0 : seen_bits(pos, tt, a.window, a.sinks);
         there[T] = none ? 0 : min(max(q.len - tt, 0), 16);
 #pragma unroll
@@ -769,7 +827,7 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
     for (int T = 0; T < 2; ++T)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[T][r]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
+    top = max_halves(top) * sc;
     if (__any(top > ref2 + PR_LAG)) {
       const float to = fmaxf(ref2, top), al = __builtin_amdgcn_exp2f(ref2 - (to == -INFINITY ? 0.0f : to));
 #pragma unroll
@@ -783,7 +841,7 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[T][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[T][r], sc, -base));
-        l += s[T][r];
+        l += s[T][r];  // (before the rounding to bf16: lse is as exact as fp32 is)
       }
     bf16x8 p[2][2];
 #pragma unroll
@@ -832,49 +890,122 @@ __global__ __launch_bounds__(AT_NT, D == 256 ? 1 : 2) void kv_tiled_kernel(Atten
       }
     }
 #pragma unroll
-    for (int T = 0; T < 2; ++T)
+    for (int T = 0; T < 2; ++T) {
 #pragma unroll
-      for (int d = 0; d < S::DT; ++d) {
+      for (int d = 0; d < S::DT; ++d)
         o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(vx[T][d].x, vx[T][d].y, vs[T]), p[T][0], o[d]);
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d)
         o[d] = pipe::mfma32_bf16(fp8x8_to_bf16(vx[T][d].z, vx[T][d].w, vs[T]), p[T][1], o[d]);
-      }
+    }
   }
   l += __shfl_xor(l, 32, 64);
-  if (wrow + c >= nrows) return;
+  const auto four = [&](int d, int r) { return v4f{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]}; };
+  if (parts == 1) {
+    if (wrow + c >= nrows) return;
 #pragma unroll
-  for (int d = 0; d < S::DT; ++d)
+    for (int d = 0; d < S::DT; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      store_out<D>(a, row, hq, 32 * d + 2 * r + 4 * h2, v4f{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]}, l, ref2,
-                   d == 0 && r == 0 && h2 == 0);
+      for (int r = 0; r < 4; ++r)
+        store_out<D>(a, row, hq, 32 * d + 8 * r + 4 * h2, four(d, r), l, ref2, d == 0 && r == 0 && h2 == 0);
+    return;
+  }
+  // Partial sums as the lanes hold them: [slot][wave][four channels of a lane][lane], whole lines.
+  constexpr int QUADS = PR_ROWS * D / 4;
+  const int slot0 = bp.first, step = a.c.heads;  // of part 0; from part to part
+  if (wrow < nrows) {
+    const int slot = slot0 + bp.index * step;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        put4(sums_of(a.po), (slot * QUADS + ((wave * S::DT + d) * 4 + r) * 64 + lane) * 4, four(d, r));
+    if (h2 == 0) put2(sums_of(a.pml), (slot * PR_ROWS + 32 * wave + c) * 2, ref2, l);
+  }
+  __shared__ int last;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
+  __syncthreads();
+  if (tid == 0)
+    last = __hip_atomic_fetch_add(&a.counters[slot0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           uint32_t(parts - 1);
+  __syncthreads();
+  if (!last) return;
+  if (tid == 0)  // as it was found
+    __hip_atomic_store(&a.counters[slot0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // Four quads a thread and four parts of each at a time, all their loads in flight: one CU reads all the sums of a block,
+  // and what it has in flight sets its rate.
+  const int quads = min(row_groups(nrows - row0, 32), AT_WAVES) * (S::DT * 256);  // of the waves that have rows
+  for (int at0 = 0; at0 < quads; at0 += 4 * AT_NT) {
+    float m[4], sum[4];
+    v4f acc[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = -INFINITY, sum[e] = 0.0f, acc[e] = v4f{0, 0, 0, 0};
+    for (int k0 = 0; k0 < parts; k0 += 4) {
+      v4f y[4][4];
+      float2 x[4][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = min(at0 + e * AT_NT + tid, quads - 1), r = at / (S::DT * 256) * 32 + (at & 31);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int slot = slot0 + min(k0 + k, parts - 1) * step;
+          x[e][k] = get2(sums_of(a.pml), (slot * PR_ROWS + r) * 2);
+          y[e][k] = get4(sums_of(a.po), (slot * QUADS + at) * 4);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float m1 = m[e];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m1 = fmaxf(m1, x[e][k].x);
+        const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m[e] - ref);
+        m[e] = m1;
+        acc[e] *= al;
+        sum[e] *= al;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k0 + k < parts) {
+            const float f = __builtin_amdgcn_exp2f(x[e][k].x - ref);
+            sum[e] += f * x[e][k].y;
+            acc[e] += f * y[e][k];
+          }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = at0 + e * AT_NT + tid, w = at / (S::DT * 256), quad = at / 64 % (S::DT * 4);
+      const int rr = row0 + 32 * w + (at & 31), d = quad / 4 * 32 + quad % 4 * 8 + (at & 32) / 8;
+      if (at < quads && rr < nrows)
+        store_out<D>(a, q.r0 + rr / a.group, h * a.group + rr % a.group, d, acc[e], sum[e], m[e], d == 0);
+    }
+  }
 }
 
 int most_rows(int rows, int max_new, int group) {
   return int(std::min<int64_t>(int64_t(std::min(rows, max_new)) * group, INT32_MAX));
 }
-int row_waves(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
-
-// Which kernels a step takes. Up to `few` rows a sequence (of a key / value head) the split kernel: it reads the cache once
-// for all of them and spreads a single sequence over the chip, which the tiled kernel does not; past that it would read the
-// cache again for every 64 rows. Where the step's sequences may be of both kinds each kernel takes its own; a single sequence
-// is the tiled kernel's if it may have more.
+// Which kernels a step takes: up to FEW rows a sequence (of a key / value head) the split kernel, past that the tiled one.
+// Where the step's sequences may be of both kinds each kernel takes its own; a single sequence is the tiled kernel's if it may
+// have more.
 struct Way {
-  int few, rw;
+  int few;
   bool split, tiled;
 };
 Way way_of(int rows, int max_new, int B, int group) {
-  const int most = most_rows(rows, max_new, group), few = std::max(64, group);
-  if (most <= few) return {few, row_waves(most), true, false};
-  if (B == 1) return {0, 1, false, true};
-  return {few, row_waves(group), true, true};
+  if (most_rows(rows, max_new, group) <= FEW) return {FEW, true, false};
+  if (B == 1 || group > FEW) return {0, false, true};
+  return {FEW, true, true};
+}
+// Partial sums of one launch: 2 target of FEW rows, or target of a row block.
+size_t sum_rows(const Way& way, int dim) {
+  return size_t(target_of(dim)) * (way.tiled ? PR_ROWS : 2 * FEW);
 }
 
 }  // namespace
 
 size_t kv_attend_workspace(int rows, int max_new, int B, int Hq, int heads, int dim) {
   if (rows < 0 || max_new < 0 || B < 0 || heads < 1 || Hq < heads || dim < 1) return 0;
-  const int rw = way_of(rows, max_new, B, Hq / heads).rw;
-  return kCounterBytes + size_t(2) * target_of(dim) * 16 * rw * (size_t(dim) + 2) * sizeof(float);
+  return kCounterBytes + sum_rows(way_of(rows, max_new, B, Hq / heads), dim) * (size_t(dim) + 2) * sizeof(float);
 }
 
 void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks,
@@ -902,30 +1033,25 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
   while (1 << a.page_shift < c.page) ++a.page_shift;
   a.counters = static_cast<uint32_t*>(ws);
   a.po = reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes);
-  a.pml = a.po + size_t(2) * a.target * 16 * way.rw * c.dim;
-  const int rows = std::min(most_rows(s.rows, s.max_new, a.group), way.few), rw = way.rw;
-  const int64_t segs = int64_t(s.B) * c.heads * cdiv(rows, 16 * rw);  // at most
+  a.pml = a.po + sum_rows(way, c.dim) * c.dim;
+  const int64_t segs = int64_t(s.B) * c.heads;
   const int64_t tiles = std::max<int64_t>(cdiv(size_t(s.max_blocks) * c.page, TILE), 1);
   const int64_t blocks = (cdiv(size_t(s.rows) * a.group, PR_ROWS) + int64_t(s.B)) * c.heads;  // at most
   if (segs * 8 > INT32_MAX || segs * (tiles + START) > INT32_MAX || blocks > INT32_MAX) fail("rows times blocks past 31 bits");
-  const unsigned grid = unsigned(std::min<int64_t>(segs * cdiv(tiles, AT_WAVES / rw), a.target));
-  const auto tiled = [&]<int D>() { kv_tiled_kernel<D><<<unsigned(blocks), AT_NT, 0, st>>>(a); };
   if (way.tiled) {
-    if (c.dim == 64) tiled.template operator()<64>();
-    else if (c.dim == 128) tiled.template operator()<128>();
-    else tiled.template operator()<256>();
+    const unsigned grid = std::max(unsigned(blocks), a.target);
+    if (c.dim == 64) kv_tiled_kernel<64><<<grid, AT_NT, 0, st>>>(a);
+    else if (c.dim == 128) kv_tiled_kernel<128><<<grid, AT_NT, 0, st>>>(a);
+    else kv_tiled_kernel<256><<<grid, AT_NT, 0, st>>>(a);
     UH_CHECK_LAUNCH();
   }
-  if (!way.split) return;
-  const auto by_rw = [&]<int D>() {
-    if (rw == 1) kv_split_kernel<D, 1><<<grid, AT_NT, 0, st>>>(a);
-    else if (rw == 2) kv_split_kernel<D, 2><<<grid, AT_NT, 0, st>>>(a);
-    else kv_split_kernel<D, 4><<<grid, AT_NT, 0, st>>>(a);
-  };
-  if (c.dim == 64) by_rw.template operator()<64>();
-  else if (c.dim == 128) by_rw.template operator()<128>();
-  else by_rw.template operator()<256>();
-  UH_CHECK_LAUNCH();
+  if (way.split) {
+    const unsigned grid = unsigned(std::min<int64_t>(segs * cdiv(tiles, AT_WAVES), a.target));
+    if (c.dim == 64) kv_split_kernel<64><<<grid, AT_NT, 0, st>>>(a);
+    else if (c.dim == 128) kv_split_kernel<128><<<grid, AT_NT, 0, st>>>(a);
+    else kv_split_kernel<256><<<grid, AT_NT, 0, st>>>(a);
+    UH_CHECK_LAUNCH();
+  }
 }
 
 }  // namespace unholy::kernels
