@@ -18,6 +18,8 @@ constexpr int TILE = 64;          // tokens a wave takes at a time
 constexpr int AT_NT = 256;        // threads of a workgroup
 constexpr int AT_WAVES = AT_NT / 64;
 constexpr int FEW = 16;           // rows (of a key / value head) of a sequence that the split kernel takes
+constexpr int JOIN = 8;           // partial sums that a thread reads at a time
+constexpr int JOIN_QUADS = 2;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 // Bits of the first n of up to 16 tokens.
@@ -43,6 +45,14 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return uint32_t(__builtin_amdgcn_readlane(int(v), lane)); }
 
+// Rows whose sums the parts [slot, slot + step, ...) of a launch hold.
+struct Block {
+  int parts, step;
+  int row0, rows;  // from the sequence's first (row, query head) on
+  int r0, h;       // the sequence's first row, the head
+  int pad[2];
+};
+
 // What every workgroup knows of the call.
 struct Attend {
   const bf16* q;
@@ -54,7 +64,8 @@ struct Attend {
   float scale2;  // scale * log2(e): the kernels take powers of two
   int few;  // sequences of up to this many rows (FEW or none) are the split kernel's, the others the tiled kernel's
   uint32_t target;     // workgroups that the chip holds at a time
-  uint32_t* counters;  // of finished parts, by the workgroup of the first; zero between launches
+  uint32_t* counters;  // of finished parts, by the workgroup of the first; zero between launches (split kernel)
+  Block* blocks;       // by the workgroup of the first part (tiled kernel)
   float *po, *pml;     // partial sums: values [slot][rows][D]; maximum and weight sum [slot][rows][2]
 };
 
@@ -250,14 +261,13 @@ struct Shape {
 // Workgroups that a CU holds, by their registers.
 constexpr int wgs_per_cu(int dim) { return dim <= 128 ? 2 : 1; }
 constexpr int target_of(int dim) { return 256 * wgs_per_cu(dim); }
-constexpr size_t kCounterBytes = 512 * sizeof(uint32_t);
+constexpr size_t kHeadBytes = 512 * (sizeof(uint32_t) + sizeof(Block));  // counters and blocks
 
 // Partial sums pass between workgroups on different XCDs, whose L2 caches do not see each other's lines: stored through
 // to memory and read from there (device-scope accesses), which for these few KiB is far cheaper than the fences that
 // write back and invalidate a whole L2 (a layer of a single-token step over 4097 tokens, 17 pieces a
 // head: 25.0 us with fences, 13.9 with these).
 constexpr int SC1 = 16;  // the cache policy of a device-scope access
-constexpr int JOIN = 8;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t sums_of(float* p) {
   return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00027000);
 }
@@ -597,7 +607,7 @@ struct BlockPart {
   Seq q;
   Tiles t;                       // that the block's rows see
   int i0, i1;                    // the part's of them
-  int index, parts, first;       // which part of how many, and the workgroup of the first
+  int index, parts;              // which part of how many
 };
 __device__ __forceinline__ Tiles block_tiles(const Attend& a, const Seq& q, int row0) {
   const int last = min(row0 + PR_ROWS, (q.r1 - q.r0) * a.group) - 1;
@@ -647,7 +657,6 @@ __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p) {
       p.t = Tiles{uniform(t.sink_tiles), uniform(t.skip), uniform(t.count)};
       p.parts = int(parts_of(uint32_t(p.t.count), share));
       if (p.index >= p.parts) return false;  // (a block that sees less than the sequence's last)
-      p.first = int(blockIdx.x) - p.index * int(heads);
       const int each = p.t.count / p.parts, more = p.t.count % p.parts;
       p.i0 = p.index * each + min(p.index, more);
       p.i1 = p.i0 + each + (p.index < more ? 1 : 0);
@@ -665,7 +674,13 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 31, h2 = lane >> 5;
 
   BlockPart bp;
-  if (!find_block(a, bp)) return;
+  const bool some = find_block(a, bp);
+  if (tid == 0 && blockIdx.x < a.target)
+    a.blocks[blockIdx.x] = some && bp.index == 0
+                               ? Block{bp.parts, int(a.c.heads), bp.row0, min(PR_ROWS, (bp.q.r1 - bp.q.r0) * a.group - bp.row0),
+                                       bp.q.r0, bp.h, {}}
+                               : Block{};
+  if (!some) return;
   const int b = bp.b, h = bp.h, row0 = bp.row0;
   const Seq q = bp.q;
   const Tiles tiles = bp.t;
@@ -911,73 +926,70 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
     return;
   }
   // Partial sums as the lanes hold them: [slot][wave][four channels of a lane][lane], whole lines.
-  constexpr int QUADS = PR_ROWS * D / 4;
-  const int slot0 = bp.first, step = a.c.heads;  // of part 0; from part to part
-  if (wrow < nrows) {
-    const int slot = slot0 + bp.index * step;
+  if (wrow >= nrows) return;
 #pragma unroll
-    for (int d = 0; d < S::DT; ++d)
+  for (int d = 0; d < S::DT; ++d)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        put4(sums_of(a.po), (slot * QUADS + ((wave * S::DT + d) * 4 + r) * 64 + lane) * 4, four(d, r));
-    if (h2 == 0) put2(sums_of(a.pml), (slot * PR_ROWS + 32 * wave + c) * 2, ref2, l);
-  }
-  __shared__ int last;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
-  __syncthreads();
-  if (tid == 0)
-    last = __hip_atomic_fetch_add(&a.counters[slot0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-           uint32_t(parts - 1);
-  __syncthreads();
-  if (!last) return;
-  if (tid == 0)  // as it was found
-    __hip_atomic_store(&a.counters[slot0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // Four quads a thread and four parts of each at a time, all their loads in flight: one CU reads all the sums of a block,
-  // and what it has in flight sets its rate.
-  const int quads = min(row_groups(nrows - row0, 32), AT_WAVES) * (S::DT * 256);  // of the waves that have rows
-  for (int at0 = 0; at0 < quads; at0 += 4 * AT_NT) {
-    float m[4], sum[4];
-    v4f acc[4];
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<v4f*>(a.po + (size_t(blockIdx.x) * (PR_ROWS * D / 4) + ((wave * S::DT + d) * 4 + r) * 64 + lane) * 4) =
+          four(d, r);
+  if (h2 == 0) *reinterpret_cast<float2*>(a.pml + (size_t(blockIdx.x) * PR_ROWS + 32 * wave + c) * 2) = make_float2(ref2, l);
+}
+
+// The parts of the tiled kernel's blocks, in order. A thread per row and four channels, two of them and eight parts of each at
+// a time: what takes time are the rounds of loads, 3 us each from memory that no L2 holds (16 blocks x 4 heads of 40 rows in 7
+// or 8 parts: %J1% us; by the last workgroup of each block, as in the split kernel, 14 us).
+template <int D>
+__global__ __launch_bounds__(AT_NT) void kv_join_kernel(Attend a) {
+  constexpr int WAVE_QUADS = D / 32 * 256;  // of 32 rows
+  const Block k = a.blocks[blockIdx.x];
+  if (k.parts <= 1) return;
+  const int at0 = blockIdx.y * JOIN_QUADS * AT_NT + threadIdx.x;
+  if (at0 / WAVE_QUADS * 32 >= k.rows) return;
+  float m[JOIN_QUADS], sum[JOIN_QUADS];
+  v4f acc[JOIN_QUADS];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) m[e] = -INFINITY, sum[e] = 0.0f, acc[e] = v4f{0, 0, 0, 0};
-    for (int k0 = 0; k0 < parts; k0 += 4) {
-      v4f y[4][4];
-      float2 x[4][4];
+  for (int e = 0; e < JOIN_QUADS; ++e) m[e] = -INFINITY, sum[e] = 0.0f, acc[e] = v4f{0, 0, 0, 0};
+  for (int p0 = 0; p0 < k.parts; p0 += JOIN) {
+    v4f y[JOIN_QUADS][JOIN];
+    float2 x[JOIN_QUADS][JOIN];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int at = min(at0 + e * AT_NT + tid, quads - 1), r = at / (S::DT * 256) * 32 + (at & 31);
+    for (int p = 0; p < JOIN; ++p) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int slot = slot0 + min(k0 + k, parts - 1) * step;
-          x[e][k] = get2(sums_of(a.pml), (slot * PR_ROWS + r) * 2);
-          y[e][k] = get4(sums_of(a.po), (slot * QUADS + at) * 4);
+      for (int e = 0; e < JOIN_QUADS; ++e) x[e][p] = make_float2(-INFINITY, 0.0f), y[e][p] = v4f{0, 0, 0, 0};
+      if (p0 + p >= k.parts) continue;
+      const size_t slot = size_t(blockIdx.x) + size_t(p0 + p) * k.step;
+#pragma unroll
+      for (int e = 0; e < JOIN_QUADS; ++e) {
+        const int at = at0 + e * AT_NT, r = at / WAVE_QUADS * 32 + (at & 31);
+        x[e][p] = *reinterpret_cast<const float2*>(a.pml + (slot * PR_ROWS + r) * 2);
+        y[e][p] = *reinterpret_cast<const v4f*>(a.po + (slot * (PR_ROWS * D / 4) + at) * 4);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < JOIN_QUADS; ++e) {
+      float m1 = m[e];
+#pragma unroll
+      for (int p = 0; p < JOIN; ++p) m1 = fmaxf(m1, x[e][p].x);
+      const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m[e] - ref);
+      m[e] = m1;
+      acc[e] *= al;
+      sum[e] *= al;
+#pragma unroll
+      for (int p = 0; p < JOIN; ++p)
+        if (p0 + p < k.parts) {
+          const float f = __builtin_amdgcn_exp2f(x[e][p].x - ref);
+          sum[e] += f * x[e][p].y;
+          acc[e] += f * y[e][p];
         }
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float m1 = m[e];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) m1 = fmaxf(m1, x[e][k].x);
-        const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m[e] - ref);
-        m[e] = m1;
-        acc[e] *= al;
-        sum[e] *= al;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k0 + k < parts) {
-            const float f = __builtin_amdgcn_exp2f(x[e][k].x - ref);
-            sum[e] += f * x[e][k].y;
-            acc[e] += f * y[e][k];
-          }
-      }
     }
+  }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int at = at0 + e * AT_NT + tid, w = at / (S::DT * 256), quad = at / 64 % (S::DT * 4);
-      const int rr = row0 + 32 * w + (at & 31), d = quad / 4 * 32 + quad % 4 * 8 + (at & 32) / 8;
-      if (at < quads && rr < nrows)
-        store_out<D>(a, q.r0 + rr / a.group, h * a.group + rr % a.group, d, acc[e], sum[e], m[e], d == 0);
-    }
+  for (int e = 0; e < JOIN_QUADS; ++e) {
+    const int at = at0 + e * AT_NT, quad = at / 64 % (D / 8), r = at / WAVE_QUADS * 32 + (at & 31), rr = k.row0 + r;
+    const int d = quad / 4 * 32 + quad % 4 * 8 + (at & 32) / 8;
+    if (r < k.rows)
+      store_out<D>(a, k.r0 + rr / a.group, k.h * a.group + rr % a.group, d, acc[e], sum[e], m[e], d == 0);
   }
 }
 
@@ -985,15 +997,16 @@ int most_rows(int rows, int max_new, int group) {
   return int(std::min<int64_t>(int64_t(std::min(rows, max_new)) * group, INT32_MAX));
 }
 // Which kernels a step takes: up to FEW rows a sequence (of a key / value head) the split kernel, past that the tiled one.
-// Where the step's sequences may be of both kinds each kernel takes its own; a single sequence is the tiled kernel's if it may
-// have more.
+// Where the step's sequences may be of both kinds each kernel takes its own, at the price of a launch (3 us where it has
+// nothing); not where no sequence has more rows than one block: the tiled kernel's parts are as good for the few rows among
+// them; and a single sequence is the tiled kernel's if it may have more.
 struct Way {
   int few;
   bool split, tiled;
 };
 Way way_of(int rows, int max_new, int B, int group) {
   if (most_rows(rows, max_new, group) <= FEW) return {FEW, true, false};
-  if (B == 1 || group > FEW) return {0, false, true};
+  if (B == 1 || group > FEW || most_rows(rows, max_new, group) <= PR_ROWS) return {0, false, true};
   return {FEW, true, true};
 }
 // Partial sums of one launch: 2 target of FEW rows, or target of a row block.
@@ -1005,7 +1018,7 @@ size_t sum_rows(const Way& way, int dim) {
 
 size_t kv_attend_workspace(int rows, int max_new, int B, int Hq, int heads, int dim) {
   if (rows < 0 || max_new < 0 || B < 0 || heads < 1 || Hq < heads || dim < 1) return 0;
-  return kCounterBytes + sum_rows(way_of(rows, max_new, B, Hq / heads), dim) * (size_t(dim) + 2) * sizeof(float);
+  return kHeadBytes + sum_rows(way_of(rows, max_new, B, Hq / heads), dim) * (size_t(dim) + 2) * sizeof(float);
 }
 
 void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks,
@@ -1029,10 +1042,11 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
 
   const Way way = way_of(s.rows, s.max_new, s.B, Hq / c.heads);
   Attend a{q,       out,   lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E, way.few,
-           unsigned(target_of(c.dim)), nullptr, nullptr, nullptr};
+           unsigned(target_of(c.dim)), nullptr, nullptr, nullptr, nullptr};
   while (1 << a.page_shift < c.page) ++a.page_shift;
   a.counters = static_cast<uint32_t*>(ws);
-  a.po = reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes);
+  a.blocks = reinterpret_cast<Block*>(a.counters + 512);
+  a.po = reinterpret_cast<float*>(static_cast<char*>(ws) + kHeadBytes);
   a.pml = a.po + sum_rows(way, c.dim) * c.dim;
   const int64_t segs = int64_t(s.B) * c.heads;
   const int64_t tiles = std::max<int64_t>(cdiv(size_t(s.max_blocks) * c.page, TILE), 1);
@@ -1043,6 +1057,11 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
     if (c.dim == 64) kv_tiled_kernel<64><<<grid, AT_NT, 0, st>>>(a);
     else if (c.dim == 128) kv_tiled_kernel<128><<<grid, AT_NT, 0, st>>>(a);
     else kv_tiled_kernel<256><<<grid, AT_NT, 0, st>>>(a);
+    UH_CHECK_LAUNCH();
+    const dim3 join(a.target, unsigned(PR_ROWS * c.dim / 4 / AT_NT / JOIN_QUADS));
+    if (c.dim == 64) kv_join_kernel<64><<<join, AT_NT, 0, st>>>(a);
+    else if (c.dim == 128) kv_join_kernel<128><<<join, AT_NT, 0, st>>>(a);
+    else kv_join_kernel<256><<<join, AT_NT, 0, st>>>(a);
     UH_CHECK_LAUNCH();
   }
   if (way.split) {
