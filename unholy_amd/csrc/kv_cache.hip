@@ -256,30 +256,40 @@ __global__ __launch_bounds__(PL_NT) void kv_reserve_kernel(KvSeqs s, const int32
   }
   __syncthreads();  // every decision above is made on refs as they were
   const int lane = tid & 63;
-  for (int b = tid >> 6; b < s.B; b += PL_NT / 64) {  // a wave per sequence
-    const int64_t len = max(s.lens[b], 0), g = max(grow[b], 0);
-    const int64_t held64 = (len + page - 1) / page, want64 = (len + g + page - 1) / page;
-    const int src = w.b[b], begin = w.a[b], extra = src >= 0;
-    const bool fits = want64 <= s.max_blocks;
-    const int held = int(held64), count = fits ? int(want64 - held64) : 0;
-    const bool served = fits && (count + extra == 0 || begin + count + extra <= found);
-    if (served) {
-      const int* list = w.a + s.B + begin;
-      for (int j = lane; j < count; j += 64) {
-        const int p = list[extra + j];
-        s.table[size_t(b) * s.max_blocks + held + j] = p;
-        refs[p] = 1;
-      }
-      if (extra && lane == 0) {
-        s.table[size_t(b) * s.max_blocks + held - 1] = list[0];
-        refs[list[0]] = 1;
-        atomicSub(&refs[src], 1);
-        w.pairs[atomicAdd(&copies, 1)] = make_int2(src, list[0]);  // in any order: they touch different pages
+  for (int b0 = tid & ~63; b0 < s.B; b0 += PL_NT) {  // a sequence a thread, and where it gets many pages its wave
+    const int b = b0 + lane;
+    int held = 0, count = 0, first = 0;
+    if (b < s.B) {
+      const int64_t len = max(s.lens[b], 0), g = max(grow[b], 0);
+      const int64_t held64 = (len + page - 1) / page, want64 = (len + g + page - 1) / page;
+      const int src = w.b[b], begin = w.a[b], extra = src >= 0;
+      const bool fits = want64 <= s.max_blocks;
+      const int more = fits ? int(want64 - held64) : 0;
+      const bool served = fits && (more + extra == 0 || begin + more + extra <= found);
+      ok[b] = served;
+      if (served) {
+        held = int(held64);
+        count = more;
+        first = begin + extra;
+        if (g > 0) s.lens[b] = int(len + g);
+        if (extra) {
+          const int to = w.a[s.B + begin];
+          s.table[size_t(b) * s.max_blocks + held - 1] = to;
+          refs[to] = 1;
+          atomicSub(&refs[src], 1);
+          w.pairs[atomicAdd(&copies, 1)] = make_int2(src, to);  // in any order: they touch different pages
+        }
       }
     }
-    if (lane == 0) {
-      ok[b] = served;
-      if (served) s.lens[b] = int(len + g);
+    for (uint64_t some = __ballot(count > 0); some; some &= some - 1) {
+      const int l = __ffsll((unsigned long long)some) - 1;
+      const int c = __builtin_amdgcn_readlane(count, l), h = __builtin_amdgcn_readlane(held, l);
+      const int* list = w.a + s.B + __builtin_amdgcn_readlane(first, l);
+      for (int j = lane; j < c; j += 64) {
+        const int p = list[j];
+        s.table[size_t(b0 + l) * s.max_blocks + h + j] = p;
+        refs[p] = 1;
+      }
     }
   }
   __syncthreads();
@@ -305,13 +315,14 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(KvCache c, int layers, Pag
     const uint4* src = reinterpret_cast<const uint4*>(data + (base + pair.x) * bytes + size_t(part) * CP_BYTES);
     uint4* dst = reinterpret_cast<uint4*>(data + (base + pair.y) * bytes + size_t(part) * CP_BYTES);
     const int vecs = int(min(bytes - size_t(part) * CP_BYTES, size_t(CP_BYTES)) / 16);
-    uint4 v[CP_BYTES / 16 / 256] = {};
-#pragma unroll
-    for (int i = 0; i < CP_BYTES / 16 / 256; ++i)
-      if (int(threadIdx.x) + i * 256 < vecs) v[i] = src[threadIdx.x + i * 256];
-#pragma unroll
-    for (int i = 0; i < CP_BYTES / 16 / 256; ++i)
-      if (int(threadIdx.x) + i * 256 < vecs) dst[threadIdx.x + i * 256] = v[i];
+    if (vecs == CP_BYTES / 16) {
+      const v4i *from = reinterpret_cast<const v4i*>(src) + threadIdx.x;
+      v4i* to = reinterpret_cast<v4i*>(dst) + threadIdx.x;
+      const v4i v0 = from[0], v1 = from[256], v2 = from[512], v3 = from[768];
+      to[0] = v0, to[256] = v1, to[512] = v2, to[768] = v3;
+    } else {
+      for (int i = threadIdx.x; i < vecs; i += 256) dst[i] = src[i];
+    }
     if (part == 0) {
       uint8_t* sc = which ? c.vs : c.ks;
       for (int h = threadIdx.x; h < c.heads; h += 256)
@@ -449,12 +460,12 @@ void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& s, 
 
 size_t kv_pages_workspace(int B, int pages) { return B < 0 || pages < 0 ? 0 : carve_pages(nullptr, B, pages).bytes; }
 
-// The copies: enough workgroups to fill the chip, and no more than there can be pieces.
+// The copies, by at most `wgs` workgroups and no more than there can be pieces.
 static void launch_copies(const KvCache& c, int layers, size_t most, const PagesWs& w, const int32_t* table,
-                          int32_t* table_out, size_t entries, hipStream_t st) {
+                          int32_t* table_out, size_t entries, size_t wgs, hipStream_t st) {
   const size_t per = (size_t(c.heads) * c.page * c.dim + CP_BYTES - 1) / CP_BYTES;
   const size_t want = std::max(most * layers * 2 * per, (entries + 255) / 256);
-  const unsigned grid = unsigned(std::clamp<size_t>(want, 1, 2048));
+  const unsigned grid = unsigned(std::clamp<size_t>(want, 1, wgs));
   kv_copy_kernel<<<grid, 256, 0, st>>>(c, layers, w, table, table_out, entries);
   UH_CHECK_LAUNCH();
 }
@@ -470,7 +481,7 @@ void kv_reserve(const KvSeqs& s, const int32_t* grow, int32_t* refs, const KvCac
   const PagesWs w = carve_pages(ws, s.B, c.pages);
   kv_reserve_kernel<<<1, PL_NT, 0, st>>>(s, grow, refs, c.pages, c.page, ok, w);
   UH_CHECK_LAUNCH();
-  launch_copies(c, layers, size_t(s.B), w, nullptr, nullptr, 0, st);
+  launch_copies(c, layers, size_t(s.B), w, nullptr, nullptr, 0, 2048, st);  // (most steps copy nothing)
 }
 
 void kv_fork(const KvSeqs& s, const int32_t* from, int32_t* refs, int pages, int page, int32_t* done, hipStream_t st) {
@@ -502,7 +513,7 @@ void kv_compact(const int32_t* table, int32_t* table_out, int max_blocks, int B,
   const PagesWs w = carve_pages(ws, B, c.pages);
   kv_compact_kernel<<<1, PL_NT, 0, st>>>(refs, refs_out, c.pages, live, w);
   UH_CHECK_LAUNCH();
-  launch_copies(c, layers, size_t(c.pages) / 2, w, table, table_out, entries, st);
+  launch_copies(c, layers, size_t(c.pages) / 2, w, table, table_out, entries, 8192, st);  // (2048: 3% longer)
 }
 
 }  // namespace unholy::kernels
