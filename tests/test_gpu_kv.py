@@ -205,6 +205,100 @@ def test_attend_is_the_same_every_time_and_without_lse():
     assert np.array_equal(first, attend(c, q, 8, 0.1, lse=False)[0])
 
 
+@pytest.mark.parametrize("B,tokens", [(100, 256), (70, 128), (300, 64), (65, 448)])
+def test_tables_that_are_full(B, tokens):
+    """Many sequences as long as the table: every workgroup that the launch may have is needed."""
+    rng = np.random.default_rng(B)
+    check_attend(kv_ref.Step(rng, [1] * B, [tokens - 1] * B, 1, 64, 64, spare_blocks=0), 2)
+
+
+@pytest.mark.parametrize("Hkv", [1, 2])
+@pytest.mark.parametrize("n,ctx,window", [(129, 600, 190), (129, 600, 200), (300, 1000, 255), (257, 63, 130), (130, 800, 1)])
+def test_last_rows_that_see_fewer_tiles(n, ctx, window, Hkv):
+    """A window that is cut finer for a sequence's whole row blocks than for the few rows of its last."""
+    rng = np.random.default_rng(n + window)
+    check_attend(kv_ref.Step(rng, [n], [ctx], Hkv, 64, 32), Hkv, window=window, sinks=2)
+
+
+@pytest.mark.parametrize("window", [0, 77])
+@pytest.mark.parametrize("n", [[1, 2] * 65, [0] * 60 + [1, 3] + [0] * 70 + [2, 0], [20] * 70, [0] * 67 + [150, 18],
+                               [1] * 50 + [19, 0] * 15 + [140] + [2] * 20])
+def test_more_sequences_than_lanes(n, window):
+    """Past 64 sequences the work is cut in several passes; some with rows for one kernel, some for both."""
+    rng = np.random.default_rng(len(n))
+    ctx = [int(x) for x in rng.integers(0, 400, len(n))]
+    ctx[60], ctx[-2] = 3000, 1700
+    check_attend(kv_ref.Step(rng, n, ctx, 1, 64, 64), 1, window=window, sinks=window // 20)
+
+
+@pytest.mark.parametrize("n", [[1, 1], [5, 130], [40]])
+def test_windows_past_any_length(n):
+    rng = np.random.default_rng(2)
+    s = kv_ref.Step(rng, n, [300] * len(n), 1, 64, 16)
+    check_attend(s, 4, window=2 ** 31 - 1)
+    check_attend(s, 4, window=50, sinks=2 ** 31 - 1)
+    check_attend(s, 4, window=-1, sinks=3)  # none
+
+
+@pytest.mark.parametrize("D,page,Hq,Hkv", [(64, 16, 128, 8), (128, 64, 64, 4), (256, 128, 64, 4)])
+@pytest.mark.parametrize("window", [0, 1500])
+def test_many_rows_over_many_tiles(D, page, Hq, Hkv, window):
+    """Enough row blocks to fill the chip, each over the tiles of a long context, a block without a page far into it; some
+    rows of them, each against a sequence of its own that ends there."""
+    rng = np.random.default_rng(D)
+    n, ctx = 1100, 2000
+    s = kv_ref.Step(rng, [n], [ctx], Hkv, D, page)
+    s.table[0, 2300 // page] = -1
+    q = randn_bf16(rng, (n, Hq, D))
+    got, lse = attend(Cache(s), q, Hq, D ** -0.5, window, 3)
+    rows = [0, 1, 127, 128, 300, 511, 777, n - 1]
+    s.n, s.B, s.cu, s.rows = [1] * len(rows), len(rows), np.arange(len(rows) + 1), len(rows)
+    s.lens, s.table = np.array([ctx + 1 + r for r in rows]), np.repeat(s.table, len(rows), 0)
+    ref, rlse, tol, ltol = kv_ref.attend(s, from_bf16(q[rows]).astype(np.float64), Hq, D ** -0.5, window, 3)
+    assert (np.abs(from_bf16(got[rows]) - ref) <= tol).all() and (np.abs(lse[rows] - rlse) <= ltol).all()
+
+
+def test_one_workspace_for_calls_of_any_shape():
+    """The workspace of the largest call serves the others in any order, and each gives what it gives with its own."""
+    rng = np.random.default_rng(21)
+    steps = [(kv_ref.Step(rng, n, ctx, Hkv, D, 32), Hq) for n, ctx, Hkv, D, Hq in
+             [([1] * 3, [2000, 5, 900], 2, 128, 8), ([150, 1], [700, 90], 1, 64, 4), ([20, 18], [1500, 3], 2, 256, 2),
+              ([1] * 90, [70] * 90, 1, 64, 1), ([40] * 3, [800, 0, 64], 2, 128, 4)]]
+    calls = [(Cache(s), s, Hq, randn_bf16(rng, (s.rows, Hq, s.D))) for s, Hq in steps]
+    want = [attend(c, q, Hq, 0.1)[0] for c, s, Hq, q in calls]
+    need = max(call("uh_kv_attend_workspace_size", s.rows, max(s.n), s.B, Hq, s.Hkv, s.D) for s, Hq in steps)
+    ws = dev(np.zeros(need, np.uint8))
+    for i in [0, 1, 0, 2, 3, 4, 1, 3, 2, 0, 4]:
+        c, s, Hq, q = calls[i]
+        out = dev(np.zeros(q.shape, np.uint16))
+        call("uh_kv_attend", dev(q), Hq * s.D, c.cu, s.rows, max(s.n), c.lens, c.table, s.max_blocks, s.B, *c.arrays(),
+             s.pages, s.page, Hq, s.Hkv, s.D, 0.1, 0, 0, out, Hq * s.D, None, ws, need, None)
+        synchronize()
+        assert np.array_equal(out.download(q.shape, np.uint16), want[i]), i
+
+
+def test_calls_on_two_streams_at_once():
+    """A decode step and a prompt on streams of their own, with workspaces of their own, over the same cache."""
+    rng = np.random.default_rng(22)
+    s = kv_ref.Step(rng, [1, 1], [4000, 900], 2, 128, 64)
+    t = kv_ref.Step.__new__(kv_ref.Step)
+    t.__dict__.update(s.__dict__)
+    t.n, t.rows, t.cu = [150, 33], 183, np.array([0, 150, 183], np.int32)
+    calls = []
+    for x in (s, t):
+        c, q = Cache(x), randn_bf16(rng, (x.rows, 8, 128))
+        need = call("uh_kv_attend_workspace_size", x.rows, max(x.n), 2, 8, 2, 128)
+        calls.append((c, x, dev(q), dev(np.zeros(q.shape, np.uint16)), dev(np.zeros(need, np.uint8)), need, Stream(),
+                      attend(c, q, 8, 0.1)[0]))
+    for _ in range(20):
+        for c, x, q, out, ws, need, st, _ in calls:
+            call("uh_kv_attend", q, 1024, c.cu, x.rows, max(x.n), c.lens, c.table, x.max_blocks, 2, *c.arrays(), x.pages,
+                 x.page, 8, 2, 128, 0.1, 0, 0, out, 1024, None, ws, need, st.handle)
+    for c, x, q, out, ws, need, st, want in calls:
+        st.synchronize()
+        assert np.array_equal(out.download(want.shape, np.uint16), want)
+
+
 def test_large_page_numbers():
     """A pool past 4 GiB: pages whose bytes lie beyond 32-bit offsets."""
     rng = np.random.default_rng(8)
@@ -541,3 +635,33 @@ def test_captured_step_replays_with_new_lengths():
         ref, _, tol, _ = kv_ref.attend(s, from_bf16(x).astype(np.float64), Hq, 0.09)
         assert (np.abs(from_bf16(out.download((4, Hq, 128), np.uint16)) - ref) <= tol).all()
         synchronize()
+
+
+def test_captured_prompts_replay_with_other_rows():
+    """A step of prompts and decode rows captured once: each replay takes the rows and lengths that are there then, and leaves
+    the workspace for the next."""
+    rng = np.random.default_rng(13)
+    s = kv_ref.Step(rng, [100, 100, 100], [400, 1500, 20], 2, 64, 32)
+    st, Hq, rows, most = Stream(), 8, 300, 300
+    c, q, out = Cache(s), dev(np.zeros((rows, Hq, 64), np.uint16)), dev(np.zeros((rows, Hq, 64), np.uint16))
+    need = call("uh_kv_attend_workspace_size", rows, most, 3, Hq, 2, 64)
+    ws = dev(np.zeros(need, np.uint8))
+    g = Graph(st, lambda: call("uh_kv_attend", q, Hq * 64, c.cu, rows, most, c.lens, c.table, s.max_blocks, 3, *c.arrays(),
+                               s.pages, 32, Hq, 2, 64, 0.125, 0, 0, out, Hq * 64, None, ws, need, st.handle))
+    for n in ([100, 100, 100], [1, 298, 1], [0, 3, 5], [300, 0, 0], [2, 2, 2], [64, 1, 120], [0, 0, 0], [1, 298, 1]):
+        s.n = n
+        s.cu = np.concatenate(([0], np.cumsum(n))).astype(np.int32)
+        s.lens = np.array([max(500, n[0]), 1600, max(120, n[2])], np.int32)
+        x = randn_bf16(rng, (rows, Hq, 64))
+        q.upload(x)
+        c.cu.upload(s.cu)
+        c.lens.upload(s.lens)
+        out.upload(np.full((rows, Hq, 64), 0x7FC1, np.uint16))
+        synchronize()
+        g.launch()
+        st.synchronize()
+        got = out.download((rows, Hq, 64), np.uint16)
+        ref, _, tol, _ = kv_ref.attend(s, from_bf16(x).astype(np.float64), Hq, 0.125)
+        m = sum(n)
+        assert (np.abs(from_bf16(got[:m]) - ref[:m]) <= tol[:m]).all() and (got[m:] == 0x7FC1).all()
+        attend(c, x[:max(m, 1)], Hq, 0.125, max_new=300)  # eager work between the replays

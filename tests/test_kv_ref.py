@@ -38,7 +38,11 @@ REFUSED = (
     + [(c, {"ws": None}, "null workspace") for c in CALLS if "ws" in CALLS[c]]
     + [("uh_kv_append", {f: n}, "ldk / ldv") for f in ("ldk", "ldv") for n in (1016, 1028, 0)]
     + [("uh_kv_attend", {f: n}, "ldq / ldo") for f in ("ldq", "ldo") for n in (4088, 4100, 0)]
-    + [("uh_kv_attend", {"Hq": n}, "Hq must be") for n in (0, 12, -8)]
+    + [("uh_kv_attend", {"Hq": n}, "Hq must be") for n in (0, 12, -8, 1 << 16)]
+    + [("uh_kv_attend", {"rows": (1 << 31) // 32, "max_new": 5}, "rows * Hq")]
+    + [("uh_kv_attend", {"B": 1 << 20, "max_blocks": 1 << 12}, "31 bits")]
+    + [("uh_kv_attend", {"B": 1, "Hkv": 1, "rows": 1 << 14, "max_new": 1 << 14, "max_blocks": 1 << 23, "ws_bytes": 1 << 40},
+        "31 bits")]
     + [("uh_kv_attend", {"sinks": -1}, "sinks"), ("uh_kv_attend", {"scale": float("nan")}, "scale"),
        ("uh_kv_attend", {"scale": float("inf")}, "scale")]
 )

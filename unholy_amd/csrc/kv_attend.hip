@@ -655,8 +655,8 @@ __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p) {
       p.row0 = block * PR_ROWS;
       const Tiles t = block_tiles(a, p.q, p.row0);
       p.t = Tiles{uniform(t.sink_tiles), uniform(t.skip), uniform(t.count)};
-      p.parts = int(parts_of(uint32_t(p.t.count), share));
-      if (p.index >= p.parts) return false;  // (a block that sees less than the sequence's last)
+      p.parts = int(min(parts_of(uint32_t(p.t.count), share), np));  // (under a window the last block may see fewer tiles)
+      if (p.index >= p.parts) return false;  // a block that sees less than the sequence's last
       const int each = p.t.count / p.parts, more = p.t.count % p.parts;
       p.i0 = p.index * each + min(p.index, more);
       p.i1 = p.i0 + each + (p.index < more ? 1 : 0);
@@ -1051,7 +1051,9 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
   const int64_t segs = int64_t(s.B) * c.heads;
   const int64_t tiles = std::max<int64_t>(cdiv(size_t(s.max_blocks) * c.page, TILE), 1);
   const int64_t blocks = (cdiv(size_t(s.rows) * a.group, PR_ROWS) + int64_t(s.B)) * c.heads;  // at most
-  if (segs * 8 > INT32_MAX || segs * (tiles + START) > INT32_MAX || blocks > INT32_MAX) fail("rows times blocks past 31 bits");
+  if (segs * 8 > INT32_MAX || std::max(segs, std::min<int64_t>(blocks, a.target)) * (tiles + START) > INT32_MAX ||
+      blocks > INT32_MAX)
+    fail("rows times blocks past 31 bits");
   if (way.tiled) {
     const unsigned grid = std::max(unsigned(blocks), a.target);
     if (c.dim == 64) kv_tiled_kernel<64><<<grid, AT_NT, 0, st>>>(a);
@@ -1065,7 +1067,7 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
     UH_CHECK_LAUNCH();
   }
   if (way.split) {
-    const unsigned grid = unsigned(std::min<int64_t>(segs * cdiv(tiles, AT_WAVES), a.target));
+    const unsigned grid = unsigned(std::min<int64_t>(segs * cdiv(tiles + START, AT_WAVES), a.target));
     if (c.dim == 64) kv_split_kernel<64><<<grid, AT_NT, 0, st>>>(a);
     else if (c.dim == 128) kv_split_kernel<128><<<grid, AT_NT, 0, st>>>(a);
     else kv_split_kernel<256><<<grid, AT_NT, 0, st>>>(a);
