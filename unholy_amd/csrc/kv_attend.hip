@@ -15,11 +15,9 @@ using namespace kv;
 namespace {
 
 constexpr int TILE = 64;          // tokens a wave takes at a time
-constexpr int AT_NT = 256;        // threads of a workgroup
+constexpr int AT_NT = 256;        // threads of a workgroup: four waves
 constexpr int AT_WAVES = AT_NT / 64;
 constexpr int FEW = 16;           // rows (of a key / value head) of a sequence that the split kernel takes
-constexpr int JOIN = 8;           // partial sums that a thread reads at a time
-constexpr int JOIN_QUADS = 2;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 // Bits of the first n of up to 16 tokens.
@@ -248,19 +246,22 @@ __device__ __forceinline__ uint32_t no_nan(uint32_t x) { return x & ~((nan_bytes
 // rounded to bf16 for the second product (2^-8 of each at most, as much as the output's own rounding), their sum is taken in
 // fp32 before that.
 // The four waves take every fourth tile and are joined in LDS. The workgroup that finishes last of those that share rows adds
-// their partial sums, in the order of the tiles whichever it is: the result does not depend on timing.
+// their partial sums, in the same order whichever it is: the result does not depend on timing. (Workgroups of eight waves, one
+// a CU, have half as many parts to join, but a CU then waits for twice the bytes: sixteen layers of one token over 4097 take
+// 202 us for 160.)
 template <int D>
 struct Shape {
   static constexpr int KL = D / 64;  // 16-byte loads of a key row's quarter
   static constexpr int DT = D / 16;  // 16-channel tiles
+  static constexpr int QUADS = FEW * D / 4;  // four channels of a row
   struct Lds {
-    float o[AT_WAVES / 2][FEW * D];
-    float ml[AT_WAVES][FEW][2];
+    v4f o[AT_WAVES * QUADS];  // the waves' sums, later the groups' (of the join)
+    float2 ml[AT_WAVES][FEW], group_ml[AT_NT];
   };
 };
-// Workgroups that a CU holds, by their registers.
-constexpr int wgs_per_cu(int dim) { return dim <= 128 ? 2 : 1; }
-constexpr int target_of(int dim) { return 256 * wgs_per_cu(dim); }
+// Workgroups that the chip holds, two a CU or, by their registers, one.
+constexpr int target_of(int dim) { return dim <= 128 ? 512 : 256; }
+constexpr int FLIGHT = 10;  // partial sums that a thread reads at a time
 constexpr size_t kHeadBytes = 512 * (sizeof(uint32_t) + sizeof(Block));  // counters and blocks
 
 // Partial sums pass between workgroups on different XCDs, whose L2 caches do not see each other's lines: stored through
@@ -299,7 +300,7 @@ __device__ __forceinline__ void store_out(const Attend& a, int row, int hq, int 
 }
 
 template <int D>
-__global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a) {
+__global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Attend a) {
   using S = Shape<D>;
   __shared__ __align__(16) typename S::Lds lds;
   __shared__ int last;
@@ -462,11 +463,11 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
       if (more) load_v(tn, pv);
     }
 
-    // the part is summed: the next one's loads go out, then this one is joined
+    // the part is summed: the next one's loads go out, then the waves' sums of this one are joined, four channels of a row
+    // a thread
     const Part done = pt;
     const uint32_t w0 = blockIdx.x - uint32_t(done.index);
-    const int row = my_row, hq = my_hq, r0 = w.q.r0, h = w.h, rows = nrows;
-    const bool mine = wave == 0 && c < nrows;
+    const int r0 = w.q.r0, h = w.h, rows = nrows;
     again = next_segment(a, sp, w);
     if (again) {
       pt = part_of(sp, w, w.at);
@@ -475,42 +476,38 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     pipe::lds_barrier();  // the last part's use of the LDS
-    if (g == 0) lds.ml[wave][c][0] = mx, lds.ml[wave][c][1] = l;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) lds.o[wave * S::QUADS + d * 64 + lane] = o[d];
+    if (g == 0) lds.ml[wave][c] = make_float2(mx, l);
     pipe::lds_barrier();
-    float m = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < AT_WAVES; ++k) m = fmaxf(m, lds.ml[k][c][0]);
-    const float ref = m == -INFINITY ? 0.0f : m, f = __builtin_amdgcn_exp2f(mx - ref);
-    l = 0.0f;
+    for (int e = 0; e < S::QUADS; e += AT_NT) {
+      const int at = e + tid, r = at & 15, d = at / 64 * 16 + (at >> 4 & 3) * 4;
+      if (r >= rows) continue;
+      float2 ml[AT_WAVES];  // of the waves: maximum and sum
+      float m = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < AT_WAVES; ++k) l += lds.ml[k][c][1] * __builtin_amdgcn_exp2f(lds.ml[k][c][0] - ref);
-    mx = m;
+      for (int k = 0; k < AT_WAVES; ++k) {
+        ml[k] = lds.ml[k][r];
+        m = fmaxf(m, ml[k].x);
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      v4f acc{0, 0, 0, 0};
 #pragma unroll
-    for (int d = 0; d < S::DT; ++d) o[d] *= f;
-    const auto at = [&](int buf, int d) { return reinterpret_cast<v4f*>(&lds.o[buf][(d * 64 + lane) * 4]); };
-#pragma unroll
-    for (int half = AT_WAVES / 2; half; half /= 2) {  // the upper half of the waves hands its sums to the lower
-      if (wave >= half && wave < 2 * half)
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) *at(wave - half, d) = o[d];
-      pipe::lds_barrier();
-      if (wave < half)
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) o[d] += *at(wave, d);
-      pipe::lds_barrier();
+      for (int k = 0; k < AT_WAVES; ++k) {
+        const float f = __builtin_amdgcn_exp2f(ml[k].x - ref);
+        sum += f * ml[k].y;
+        acc += f * lds.o[k * S::QUADS + at];
+      }
+      if (done.parts == 1) {
+        store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
+      } else {
+        const int slot = int(blockIdx.x * 2 + (done.index == 0 ? 1 : 0)) * FEW + r;
+        put4(sums_of(a.po), slot * D + d, acc);
+        if (d == 0) put2(sums_of(a.pml), slot * 2, m, sum);
+      }
     }
-    if (done.parts == 1) {
-      if (mine)
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) store_out<D>(a, row, hq, 16 * d + 4 * g, o[d], l, mx, d == 0 && g == 0);
-      continue;
-    }
-    if (mine) {
-      const int r = int(blockIdx.x * 2 + (done.index == 0 ? 1 : 0)) * FEW + c;
-#pragma unroll
-      for (int d = 0; d < S::DT; ++d) put4(sums_of(a.po), r * D + 4 * g + 16 * d, o[d]);
-      if (g == 0) put2(sums_of(a.pml), r * 2, mx, l);
-    }
+    if (done.parts == 1) continue;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
     __syncthreads();
     if (tid == 0)
@@ -520,36 +517,63 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
     if (!last) continue;
     if (tid == 0)  // as it was found
       __hip_atomic_store(&a.counters[w0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // a thread per row and four channels, the loads of JOIN parts in flight at a time
-    for (int it = tid; it < rows * (D / 4); it += AT_NT) {
+    // The parts are dealt to `groups` of threads, four channels of a row a thread, and the groups joined in LDS. What takes
+    // time are the rounds of reads, about a microsecond each: as many in flight as the registers hold, but not ten where
+    // there are two (sixteen layers of one token over 4097: 160 us; by a group of all threads, eight at a time, 183).
+    const int items = rows * (D / 4), groups = min(max(AT_NT / items, 1), AT_WAVES), gi = tid / items;
+    for (int it = gi < groups ? tid - gi * items : items; it < items; it += AT_NT) {
       const int r = it / (D / 4), d = it % (D / 4) * 4;
       float m = -INFINITY, sum = 0.0f;
       v4f acc{0, 0, 0, 0};
-      for (int k0 = 0; k0 < done.parts; k0 += JOIN) {
-        v4f y[JOIN];
-        float2 x[JOIN];
+      const auto add = [&]<int N>(int k0) {  // parts k0, k0 + groups, ... (N of them)
+        v4f y[N];
+        float2 x[N];
 #pragma unroll
-        for (int k = 0; k < JOIN; ++k) {
-          const int p = min(k0 + k, done.parts - 1);
+        for (int k = 0; k < N; ++k) {
+          const int p = min(k0 + k * groups, done.parts - 1);
           const int at = (int(w0 + uint32_t(p)) * 2 + (p == 0 ? 1 : 0)) * FEW + r;
           x[k] = get2(sums_of(a.pml), at * 2);
           y[k] = get4(sums_of(a.po), at * D + d);
         }
         float m1 = m;
 #pragma unroll
-        for (int k = 0; k < JOIN; ++k) m1 = fmaxf(m1, x[k].x);
+        for (int k = 0; k < N; ++k) m1 = fmaxf(m1, x[k].x);
         const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m - ref);
         m = m1;
         acc *= al;
         sum *= al;
 #pragma unroll
-        for (int k = 0; k < JOIN; ++k)
-          if (k0 + k < done.parts) {
+        for (int k = 0; k < N; ++k)
+          if (k0 + k * groups < done.parts) {
             const float f = __builtin_amdgcn_exp2f(x[k].x - ref);
             sum += f * x[k].y;
             acc += f * y[k];
           }
+      };
+      if (done.parts <= 2 * groups) add.template operator()<2>(gi % groups);
+      else
+        for (int k0 = gi % groups; k0 < done.parts; k0 += FLIGHT * groups) add.template operator()<FLIGHT>(k0);
+      if (groups == 1) {
+        store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
+      } else {
+        lds.o[tid] = acc;  // (the waves' sums were read before the counter was)
+        lds.group_ml[tid] = make_float2(m, sum);
       }
+    }
+    if (groups == 1) continue;
+    pipe::lds_barrier();
+    if (tid < items) {
+      float m = -INFINITY, sum = 0.0f;
+      v4f acc{0, 0, 0, 0};
+      for (int k = 0; k < groups; ++k) m = fmaxf(m, lds.group_ml[k * items + tid].x);
+      const float ref = m == -INFINITY ? 0.0f : m;
+      for (int k = 0; k < groups; ++k) {
+        const float2 x = lds.group_ml[k * items + tid];
+        const float f = __builtin_amdgcn_exp2f(x.x - ref);
+        sum += f * x.y;
+        acc += f * lds.o[k * items + tid];
+      }
+      const int r = tid / (D / 4), d = tid % (D / 4) * 4;
       store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
     }
   }
@@ -567,6 +591,7 @@ __global__ __launch_bounds__(AT_NT, wgs_per_cu(D)) void kv_split_kernel(Attend a
 // The running maximum is left alone until a row's scores pass it by more than 2^8: the weights stay small enough, and most
 // tiles need no scaling of the sums.
 constexpr int PR_ROWS = 128;
+constexpr int JOIN = 8, JOIN_QUADS = 2;  // partial sums that a thread of the join reads at a time, of each of its quads
 constexpr int PR_STAGES = 3;
 constexpr int PR_META = 16;  // tiles
 constexpr float PR_LAG = 8.0f;
