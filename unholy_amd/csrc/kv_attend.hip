@@ -591,7 +591,6 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
 // The running maximum is left alone until a row's scores pass it by more than 2^8: the weights stay small enough, and most
 // tiles need no scaling of the sums.
 constexpr int PR_ROWS = 128;
-constexpr int JOIN = 8, JOIN_QUADS = 2;  // partial sums that a thread of the join reads at a time, of each of its quads
 constexpr int PR_STAGES = 3;
 constexpr int PR_META = 16;  // tiles
 constexpr float PR_LAG = 8.0f;
@@ -961,61 +960,48 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
   if (h2 == 0) *reinterpret_cast<float2*>(a.pml + (size_t(blockIdx.x) * PR_ROWS + 32 * wave + c) * 2) = make_float2(ref2, l);
 }
 
-// The parts of the tiled kernel's blocks, in order. A thread per row and four channels, two of them and eight parts of each at
-// a time: what takes time are the rounds of loads, 3 us each from memory that no L2 holds (16 blocks x 4 heads of 40 rows in 7
-// or 8 parts: %J1% us; by the last workgroup of each block, as in the split kernel, 14 us).
+// The parts of the tiled kernel's blocks, in order. A thread per row and four channels, JOIN parts at a time: what takes time
+// are the rounds of loads, 3 us each from memory that no L2 holds, so few registers and many threads rather than many parts in
+// flight (eight parts of two quads a thread: 5% more for a step of 256 blocks in two parts each, 1% for 64 blocks in 7 or 8
+// parts, 6% less for four blocks in 16). 64 blocks of 40 rows: 7 us; by the last workgroup of each block, as in the split
+// kernel, 14.
+constexpr int JOIN = 4;
 template <int D>
 __global__ __launch_bounds__(AT_NT) void kv_join_kernel(Attend a) {
   constexpr int WAVE_QUADS = D / 32 * 256;  // of 32 rows
   const Block k = a.blocks[blockIdx.x];
   if (k.parts <= 1) return;
-  const int at0 = blockIdx.y * JOIN_QUADS * AT_NT + threadIdx.x;
-  if (at0 / WAVE_QUADS * 32 >= k.rows) return;
-  float m[JOIN_QUADS], sum[JOIN_QUADS];
-  v4f acc[JOIN_QUADS];
-#pragma unroll
-  for (int e = 0; e < JOIN_QUADS; ++e) m[e] = -INFINITY, sum[e] = 0.0f, acc[e] = v4f{0, 0, 0, 0};
+  const int at = blockIdx.y * AT_NT + threadIdx.x, r = at / WAVE_QUADS * 32 + (at & 31), rr = k.row0 + r;
+  if (r >= k.rows) return;
+  float m = -INFINITY, sum = 0.0f;
+  v4f acc{0, 0, 0, 0};
   for (int p0 = 0; p0 < k.parts; p0 += JOIN) {
-    v4f y[JOIN_QUADS][JOIN];
-    float2 x[JOIN_QUADS][JOIN];
+    v4f y[JOIN];
+    float2 x[JOIN];
 #pragma unroll
     for (int p = 0; p < JOIN; ++p) {
-#pragma unroll
-      for (int e = 0; e < JOIN_QUADS; ++e) x[e][p] = make_float2(-INFINITY, 0.0f), y[e][p] = v4f{0, 0, 0, 0};
+      x[p] = make_float2(-INFINITY, 0.0f), y[p] = v4f{0, 0, 0, 0};
       if (p0 + p >= k.parts) continue;
       const size_t slot = size_t(blockIdx.x) + size_t(p0 + p) * k.step;
-#pragma unroll
-      for (int e = 0; e < JOIN_QUADS; ++e) {
-        const int at = at0 + e * AT_NT, r = at / WAVE_QUADS * 32 + (at & 31);
-        x[e][p] = *reinterpret_cast<const float2*>(a.pml + (slot * PR_ROWS + r) * 2);
-        y[e][p] = *reinterpret_cast<const v4f*>(a.po + (slot * (PR_ROWS * D / 4) + at) * 4);
-      }
+      x[p] = *reinterpret_cast<const float2*>(a.pml + (slot * PR_ROWS + r) * 2);
+      y[p] = *reinterpret_cast<const v4f*>(a.po + (slot * (PR_ROWS * D / 4) + at) * 4);
     }
+    float m1 = m;
 #pragma unroll
-    for (int e = 0; e < JOIN_QUADS; ++e) {
-      float m1 = m[e];
+    for (int p = 0; p < JOIN; ++p) m1 = fmaxf(m1, x[p].x);
+    const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m - ref);
+    m = m1;
+    acc *= al;
+    sum *= al;
 #pragma unroll
-      for (int p = 0; p < JOIN; ++p) m1 = fmaxf(m1, x[e][p].x);
-      const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m[e] - ref);
-      m[e] = m1;
-      acc[e] *= al;
-      sum[e] *= al;
-#pragma unroll
-      for (int p = 0; p < JOIN; ++p)
-        if (p0 + p < k.parts) {
-          const float f = __builtin_amdgcn_exp2f(x[e][p].x - ref);
-          sum[e] += f * x[e][p].y;
-          acc[e] += f * y[e][p];
-        }
+    for (int p = 0; p < JOIN; ++p) {
+      const float f = __builtin_amdgcn_exp2f(x[p].x - ref);
+      sum += f * x[p].y;
+      acc += f * y[p];
     }
   }
-#pragma unroll
-  for (int e = 0; e < JOIN_QUADS; ++e) {
-    const int at = at0 + e * AT_NT, quad = at / 64 % (D / 8), r = at / WAVE_QUADS * 32 + (at & 31), rr = k.row0 + r;
-    const int d = quad / 4 * 32 + quad % 4 * 8 + (at & 32) / 8;
-    if (r < k.rows)
-      store_out<D>(a, k.r0 + rr / a.group, k.h * a.group + rr % a.group, d, acc[e], sum[e], m[e], d == 0);
-  }
+  const int quad = at / 64 % (D / 8), d = quad / 4 * 32 + quad % 4 * 8 + (at & 32) / 8;
+  store_out<D>(a, k.r0 + rr / a.group, k.h * a.group + rr % a.group, d, acc, sum, m, d == 0);
 }
 
 int most_rows(int rows, int max_new, int group) {
@@ -1085,7 +1071,7 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
     else if (c.dim == 128) kv_tiled_kernel<128><<<grid, AT_NT, 0, st>>>(a);
     else kv_tiled_kernel<256><<<grid, AT_NT, 0, st>>>(a);
     UH_CHECK_LAUNCH();
-    const dim3 join(a.target, unsigned(PR_ROWS * c.dim / 4 / AT_NT / JOIN_QUADS));
+    const dim3 join(a.target, unsigned(PR_ROWS * c.dim / 4 / AT_NT));
     if (c.dim == 64) kv_join_kernel<64><<<join, AT_NT, 0, st>>>(a);
     else if (c.dim == 128) kv_join_kernel<128><<<join, AT_NT, 0, st>>>(a);
     else kv_join_kernel<256><<<join, AT_NT, 0, st>>>(a);
