@@ -231,6 +231,13 @@ def test_more_sequences_than_lanes(n, window):
     check_attend(kv_ref.Step(rng, n, ctx, 1, 64, 64), 1, window=window, sinks=window // 20)
 
 
+@pytest.mark.parametrize("n", [[1] * 39 + [60], [1] * 20 + [0] * 15 + [3, 17, 100, 0, 16], [20] * 33, [2] * 31 + [30]])
+def test_few_and_many_rows_in_no_more_than_a_block(n):
+    """Steps that the two kernels share, and steps that are the tiled one's, by rows on average and sequences."""
+    rng = np.random.default_rng(sum(n))
+    check_attend(kv_ref.Step(rng, n, rng.integers(0, 300, len(n)).tolist(), 8, 64, 64), 8)
+
+
 @pytest.mark.parametrize("n", [[1, 1], [5, 130], [40]])
 def test_windows_past_any_length(n):
     rng = np.random.default_rng(2)

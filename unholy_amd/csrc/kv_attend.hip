@@ -92,8 +92,9 @@ __device__ __forceinline__ int row_groups(int rows, int per) { return (rows + pe
 // Many segments: workgroup w takes the tiles [w share, (w + 1) share) of all segments in order, so that long and short
 // sequences load the chip evenly; it may end one segment, do some whole ones and begin another, and each beginning costs it
 // START tiles' time. Few segments (an eighth of the workgroups): each is cut into parts as equal as they can be, a workgroup
-// each, and no workgroup has two beginnings. (256 segments of 18 tiles under a window, four layers: 68 us cut anywhere, 74 in
-// two equal parts, each joined, 72 whole; 8 of 65 tiles, sixteen layers: 298 us cut anywhere, 186 in equal parts.)
+// each, and no workgroup has two beginnings. (256 segments of 18 tiles under a window, four layers: 67 us cut anywhere, 75 in
+// two equal parts, each joined, 71 whole; 8 of 65 tiles, sixteen layers: 203 us cut anywhere, 159 in equal parts; between
+// them, 32 of some 1700 tiles are 176 and 178.)
 // The parts of a segment are those of consecutive workgroups; the part of workgroup w that begins a segment leaves its sums
 // in slot 2 w + 1, one that goes on with it in slot 2 w.
 struct Walk {
@@ -266,8 +267,8 @@ constexpr size_t kHeadBytes = 512 * (sizeof(uint32_t) + sizeof(Block));  // coun
 
 // Partial sums pass between workgroups on different XCDs, whose L2 caches do not see each other's lines: stored through
 // to memory and read from there (device-scope accesses), which for these few KiB is far cheaper than the fences that
-// write back and invalidate a whole L2 (a layer of a single-token step over 4097 tokens, 17 pieces a
-// head: 25.0 us with fences, 13.9 with these).
+// write back and invalidate a whole L2 (sixteen layers of one token over 4097 tokens, 17 parts a head: 375 us with fences,
+// 159 with these).
 constexpr int SC1 = 16;  // the cache policy of a device-scope access
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t sums_of(float* p) {
   return __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00027000);
@@ -1007,17 +1008,21 @@ __global__ __launch_bounds__(AT_NT) void kv_join_kernel(Attend a) {
 int most_rows(int rows, int max_new, int group) {
   return int(std::min<int64_t>(int64_t(std::min(rows, max_new)) * group, INT32_MAX));
 }
-// Which kernels a step takes: up to FEW rows a sequence (of a key / value head) the split kernel, past that the tiled one.
-// Where the step's sequences may be of both kinds each kernel takes its own, at the price of a launch (3 us where it has
-// nothing); not where no sequence has more rows than one block: the tiled kernel's parts are as good for the few rows among
-// them; and a single sequence is the tiled kernel's if it may have more.
+// Which kernels a step takes: up to FEW rows a sequence (of a key / value head) the split kernel (64 sequences of one token
+// 105 us, by the tiled one 161), past that the tiled one, and where the step's sequences may be of both kinds each its own
+// (eight tokens and a chunk of 1000: 111 us, all by the tiled one 128). The second way costs launches, though, 8 us or so: not
+// taken for a single sequence, where every sequence of the step is past FEW by its group alone, and, if none has more rows
+// than one block, where they are past FEW on average (16 x 5 draft tokens, four layers: 129 us, with the launches 139) or few
+// (31 tokens and a chunk of 30, 8 heads: 51 us and 62; 63 tokens and a chunk of 30: 113 and 90).
 struct Way {
   int few;
   bool split, tiled;
 };
-Way way_of(int rows, int max_new, int B, int group) {
-  if (most_rows(rows, max_new, group) <= FEW) return {FEW, true, false};
-  if (B == 1 || group > FEW || most_rows(rows, max_new, group) <= PR_ROWS) return {0, false, true};
+Way way_of(int rows, int max_new, int B, int group, int heads) {
+  const int most = most_rows(rows, max_new, group);
+  if (most <= FEW) return {FEW, true, false};
+  if (B == 1 || group > FEW) return {0, false, true};
+  if (most <= PR_ROWS && (int64_t(rows) * group > int64_t(FEW) * B || int64_t(B) * heads <= 256)) return {0, false, true};
   return {FEW, true, true};
 }
 // Partial sums of one launch: 2 target of FEW rows, or target of a row block.
@@ -1029,7 +1034,7 @@ size_t sum_rows(const Way& way, int dim) {
 
 size_t kv_attend_workspace(int rows, int max_new, int B, int Hq, int heads, int dim) {
   if (rows < 0 || max_new < 0 || B < 0 || heads < 1 || Hq < heads || dim < 1) return 0;
-  return kHeadBytes + sum_rows(way_of(rows, max_new, B, Hq / heads), dim) * (size_t(dim) + 2) * sizeof(float);
+  return kHeadBytes + sum_rows(way_of(rows, max_new, B, Hq / heads, heads), dim) * (size_t(dim) + 2) * sizeof(float);
 }
 
 void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks,
@@ -1051,7 +1056,7 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
   if (!aligned16(ws)) fail("workspace not 16-byte aligned");
   if (ws_bytes < need) fail("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
 
-  const Way way = way_of(s.rows, s.max_new, s.B, Hq / c.heads);
+  const Way way = way_of(s.rows, s.max_new, s.B, Hq / c.heads, c.heads);
   Attend a{q,       out,   lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E, way.few,
            unsigned(target_of(c.dim)), nullptr, nullptr, nullptr, nullptr};
   while (1 << a.page_shift < c.page) ++a.page_shift;

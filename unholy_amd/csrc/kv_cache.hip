@@ -439,6 +439,7 @@ void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& s, 
   if (int64_t(s.B) * nblk > INT32_MAX) throw std::runtime_error("kv_append: B * blocks past 31 bits");
   const dim3 grid(unsigned(s.B) * unsigned(nblk), unsigned(c.heads), 2);
   // A wave holds 128 pieces of 8 channels x 4 tokens: enough for `most` tokens, wherever they begin, or a workgroup of four
+  // (64 sequences of one token in eight layers: 50 us by waves, 59 by workgroups)
   const bool few = ((most + 2) / 4 + 1) * (c.dim / 8) <= 64 * pieces_of(c.dim, c.page, 64);
   const auto go = [&]<int D, int PAGE>() {
     if (few) kv_append_kernel<D, PAGE, 64><<<grid, 64, 0, st>>>(k, ldk, v, ldv, s, c, nblk);
