@@ -69,8 +69,8 @@ struct KvSeqs {
 // (refs > 1) and not full is replaced by a copy in all `layers` of the cache, so that the sequence may append to it. Free
 // pages go to the sequences in order, lowest first, the copy before the new ones; from the first sequence on whose pages
 // no longer suffice, none that needs a page is served. ok[b] = 1: served; 0: untouched (no pages left, or more blocks than
-// the table has). Pages that this call frees by copying them for every user are free afterwards. ws: kv_pages_workspace
-// bytes, 16-byte aligned, any contents.
+// the table has): such a sequence must bring no rows to the step, they would take its last tokens' places. Pages that this
+// call frees by copying them for every user are free afterwards. ws: kv_pages_workspace bytes, 16-byte aligned, any contents.
 size_t kv_pages_workspace(int B, int pages);
 void kv_reserve(const KvSeqs& seqs, const int32_t* grow, int32_t* refs, const KvCache& cache, int layers, int32_t* ok,
                 void* ws, size_t ws_bytes, hipStream_t st);

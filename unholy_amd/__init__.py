@@ -1,4 +1,5 @@
-"""gfx950 quantized-MoE hot path: MXFP4 routed experts and the fp8 block-scaled dense GEMM.
+"""gfx950 quantized-MoE hot path: MXFP4 routed experts, the fp8 block-scaled dense GEMM, and the attention between them over
+an 8-bit paged key / value cache.
 
 The compute lives in libunholy_amd.so (hand-written HIP for gfx950 behind a C ABI, include/unholy_amd.h; the C++
 drop-ins of the reference's src/kernels entry points are declared under include/unholy/kernels/). This package is
