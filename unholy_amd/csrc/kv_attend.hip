@@ -965,11 +965,10 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
   if (h2 == 0) *reinterpret_cast<float2*>(a.pml + (size_t(blockIdx.x) * PR_ROWS + 32 * wave + c) * 2) = make_float2(ref2, l);
 }
 
-// The parts of the tiled kernel's blocks, in order. A thread per row and four channels, JOIN parts at a time: what takes time
-// are the rounds of loads, 3 us each from memory that no L2 holds, so few registers and many threads rather than many parts in
-// flight (eight parts of two quads a thread: 5% more for a step of 256 blocks in two parts each, 1% for 64 blocks in 7 or 8
-// parts, 6% less for four blocks in 16). 64 blocks of 40 rows: 7 us; by the last workgroup of each block, as in the split
-// kernel, 14.
+// The parts of the tiled kernel's blocks, in order. A thread per row and four channels, JOIN parts at a time: few registers and
+// many threads rather than many parts in flight (eight parts of two quads a thread: 5% more for a step of 256 blocks in two
+// parts each, 1% for 64 blocks in 7 or 8 parts; 5% less for four blocks in 16). 64 blocks of 40 rows: 7 us; by the last workgroup
+// of each block, as in the split kernel, 14.
 constexpr int JOIN = 4;
 template <int D>
 __global__ __launch_bounds__(AT_NT) void kv_join_kernel(Attend a) {
