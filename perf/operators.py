@@ -378,6 +378,7 @@ def own_step(s):
         s["graph"].launch()
     else:
         from unholy_amd.device import Graph
+        torch.cuda.current_stream().synchronize()  # the other stream's first step comes after the inputs and the workspace's zeros
         own_layers(s, stream().handle)
         s["graph"] = Graph(stream(), lambda: own_layers(s, stream().handle))
 
