@@ -50,8 +50,9 @@ void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& ste
 // out zero and lse -inf for a row whose visible tokens have no s above -inf. Values of tokens that a row does not see do
 // not reach it, NaN among them.
 // q bf16 [rows, Hq, dim] and out the same (row strides ldq, ldo >= Hq * dim, % 8; 16-byte aligned), lse fp32 [rows, Hq].
-// ws: device workspace of kv_attend_workspace bytes, 16-byte aligned, zeroed before its first call; a call leaves it as the
-// next one, of any shape, needs it. Calls that may overlap need one each.
+// ws: device workspace of kv_attend_workspace bytes, 16-byte aligned, zeroed before its first call (finished, or earlier on
+// the same stream); a call leaves it as the next one, of any shape, needs it, and nothing else may write it meanwhile. Calls
+// that may overlap need one each.
 size_t kv_attend_workspace(int rows, int max_new, int B, int Hq, int heads, int dim);
 void kv_attend(const bf16* q, int ldq, const KvStep& step, const KvCache& cache, int Hq, float scale, int window,
                int sinks, bf16* out, int ldo, float* lse, void* ws, size_t ws_bytes, hipStream_t st);

@@ -119,6 +119,14 @@ def test_long_contexts(D):
     check_attend(kv_ref.Step(rng, [1, 1, 1, 3, 1], [9000, 3, 2500, 4000, 0], 1, D, 64), 4)
 
 
+@pytest.mark.parametrize("n,Hq", [(1, 1), (1, 16), (5, 16), (2, 40)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_long_context(n, Hq, D):
+    """One sequence and one key / value head, with as many parts as are worth their join."""
+    rng = np.random.default_rng(n * Hq)
+    check_attend(kv_ref.Step(rng, [n], [20000], 1, D, 64), Hq, max_new=max(n, 3) if Hq == 1 else 2 ** 31 - 1)
+
+
 @pytest.mark.parametrize("n", [[0, 0], [0, 3, 0], [1, 0, 0, 150, 0, 1], [0, 200]])
 def test_sequences_without_rows(n):
     rng = np.random.default_rng(len(n))

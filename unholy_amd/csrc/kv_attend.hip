@@ -126,6 +126,11 @@ __device__ __forceinline__ uint32_t smallest_share(uint32_t n, uint32_t tiles, u
   return lo;
 }
 
+// The root of a times n items' average of `sum`.
+__device__ __forceinline__ uint32_t root(float a, uint32_t sum, uint32_t n) {
+  return uint32_t(__builtin_amdgcn_sqrtf(a * float(sum) * __builtin_amdgcn_rcpf(float(max(n, 1u)))));
+}
+
 struct Split {
   bool whole;            // equal parts of each segment
   uint32_t share, unit;  // tiles of a part at most; units of a workgroup
@@ -161,9 +166,12 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w)
     all += lane_of(wave_scan(segs), 63);
   }
   s.whole = all * 8 <= a.target;
+  // Equal parts have a tile a wave at least, and where segments are long so many that they (0.35 us each) balance the join by
+  // one workgroup (0.014 us a part and row): 16 rows over 131,000 tokens take 45 us a call, in 512 parts of four tiles 99.
+  const uint32_t lo = max(uint32_t(AT_WAVES), root(0.04f * float(min(min(a.st.max_new, FEW) * a.group, FEW)), tiles, all));
   if (!s.whole) s.share = max((tiles + a.target - 1) / a.target, uint32_t(AT_WAVES));
-  else if (a.st.B <= 64) s.share = smallest_share(segs, uint32_t(w.t.count), tiles - START * all, all, a.target, AT_WAVES);
-  else s.share = max((tiles + a.target - all - 1) / (a.target - all), uint32_t(AT_WAVES));  // one that is large enough
+  else if (a.st.B <= 64) s.share = smallest_share(segs, uint32_t(w.t.count), tiles - START * all, all, a.target, lo);
+  else s.share = max((tiles + a.target - all - 1) / (a.target - all), lo);  // one that is large enough
   s.unit = s.whole ? 1 : s.share;
   const uint32_t u = blockIdx.x * s.unit;
   uint32_t from = 0;
@@ -583,8 +591,8 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
 }
 
 // ---- many rows a sequence: prompts ------------------------------------------------------------------------------------
-// Bound by the matrix rate and by the exponentials and conversions next to it: 8192 rows of 32 heads of 128 take 530 to 540 us,
-// 1.02 to 1.04 PFLOP/s (a large bf16 product reaches 1.17 here), the matrix units busy for half of the cycles and the vector units
+// Bound by the matrix rate and by the exponentials and conversions next to it: 8192 rows of 32 heads of 128 take 527 to 550 us,
+// 1.00 to 1.04 PFLOP/s (a large bf16 product reaches 1.17 here), the matrix units busy for half of the cycles and the vector units
 // for 70%; with 64 channels, where an exponential comes with half as many products, 0.57 PFLOP/s. A workgroup takes 128 rows (4 waves of 32)
 // of one (sequence, key / value head) and goes through the 64-token tiles that they see, which arrive in LDS as codes by
 // direct loads, two tiles ahead, in a ring of three. The 32x32x16 product with the same order of tokens as above: S^T = K Q^T
@@ -643,7 +651,7 @@ __device__ __forceinline__ Tiles block_tiles(const Attend& a, const Seq& q, int 
   return tiles_of(a, Seq{0, 0, max(min(q.len, q.first + last / a.group + 1), 0), q.first + row0 / a.group});
 }
 __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p) {
-  constexpr uint32_t LEAST = 4, NONE = 1u << 30;
+  constexpr uint32_t NONE = 1u << 30;
   const int lane = threadIdx.x & 63;
   const uint32_t heads = uint32_t(a.c.heads);
   Seq q{0, 0, 0, 0};
@@ -665,9 +673,12 @@ __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p) {
     all += lane_of(wave_scan(blocks), 63) * heads;
     if (all < a.target) tiles += lane_of(wave_scan(blocks * most), 63) * heads;
   }
+  // A part has 4 tiles at least, and where blocks see many so many that they (1.5 us each) balance the join (0.3 us a part):
+  // 80 rows of 128 over 131,000 tokens take 63 us a call, in 512 parts of four tiles 164.
+  const uint32_t least = max(4u, root(0.2f, tiles, all));
   uint32_t share = NONE;
-  if (all < a.target && a.st.B <= 64) share = smallest_share(blocks * heads, most, tiles, all, a.target, LEAST);
-  else if (all < a.target) share = max((tiles + a.target - all - 1) / (a.target - all), LEAST);  // one that is large enough
+  if (all < a.target && a.st.B <= 64) share = smallest_share(blocks * heads, most, tiles, all, a.target, least);
+  else if (all < a.target) share = max((tiles + a.target - all - 1) / (a.target - all), least);  // one that is large enough
   uint32_t from = 0;
   for (int b0 = 0; b0 < a.st.B; b0 += 64) {
     if (a.st.B > 64) look(b0 + lane);
