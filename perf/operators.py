@@ -340,7 +340,7 @@ _stream = None
 
 
 def stream():
-    """The program's one stream for captured work."""
+    """The stream that steps are captured on. Nothing runs there: a captured step is replayed on torch's current stream."""
     global _stream
     if _stream is None:
         from unholy_amd.device import Stream
@@ -371,15 +371,17 @@ def own_layers(s, st):
 
 
 def own_step(s):
-    """A step through the layers: captured in the program's first step of a shape, replayed in the next ones."""
-    if not s["case"]["graph"]:
-        own_layers(s, torch.cuda.current_stream().cuda_stream)
-    elif s["graph"] is not None:
-        s["graph"].launch()
-    else:
+    """A step through the layers: call by call the first time, and captured then where the program replays it in the next
+    ones. All of it runs on torch's current stream, so that it comes after what writes its inputs, zeroes its workspace or
+    used their memory before, and what reads its results, or is given its memory, comes after it."""
+    from unholy_amd import call
+    now = torch.cuda.current_stream().cuda_stream
+    if s["graph"] is not None:
+        call("uh_graph_launch", s["graph"].handle, now)
+        return
+    own_layers(s, now)
+    if s["case"]["graph"]:
         from unholy_amd.device import Graph
-        torch.cuda.current_stream().synchronize()  # the other stream's first step comes after the inputs and the workspace's zeros
-        own_layers(s, stream().handle)
         s["graph"] = Graph(stream(), lambda: own_layers(s, stream().handle))
 
 
