@@ -4,7 +4,8 @@
 // One layer's cache is pages of `page` tokens (16, 32, 64 or 128), for each page and key / value head
 //   k  e4m3 [page, dim], one row a token,
 //   v  e4m3 [dim, page], transposed: consecutive tokens of a channel, as the value product's matrix operand wants them,
-//   ks, vs  e8m0, the power-of-two scale of the block's keys and of its values,
+//   ks, vs  e8m0, the power-of-two scale of the block's keys and of its values (kv_append's are 2^119 at most; 255 is NaN,
+//           and so are the keys or values of its block then),
 // each array [pages, heads, ...] (pool-wide calls: [layers, pages, heads, ...]); dim 64, 128 or 256; k and v 16-byte
 // aligned. Position t of sequence b lies in slot t % page of page table[b * max_blocks + t / page]; an entry that is no
 // page number (-1) holds nothing.
@@ -48,7 +49,7 @@ void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& ste
 // if p - t < window or t < sinks, and only if its page exists;
 //   s = scale q . k,  out = sum softmax(s) v,  lse = ln(sum e^s) (may be null),
 // out zero and lse -inf for a row whose visible tokens have no s above -inf. Values of tokens that a row does not see do
-// not reach it, NaN among them.
+// not reach it, NaN among them, nor do the scales of blocks that it sees nothing of, whatever they hold.
 // q bf16 [rows, Hq, dim] and out the same (row strides ldq, ldo >= Hq * dim, % 8; 16-byte aligned), lse fp32 [rows, Hq].
 // ws: device workspace of kv_attend_workspace bytes, 16-byte aligned, zeroed before its first call (finished, or earlier on
 // the same stream); a call leaves it as the next one, of any shape, needs it, and nothing else may write it meanwhile. Calls

@@ -202,6 +202,64 @@ def test_nan_reaches_only_the_rows_that_see_it(n, page):
     assert np.array_equal(from_bf16(got)[fine], want[fine])
 
 
+def spare_page_0(s):
+    """Page 0 of a step changes places with a page that no sequence has; the pages that none has then, page 0 first."""
+    free = np.setdiff1d(np.arange(s.pages), s.table)
+    if free[0] != 0:
+        s.table[s.table == 0] = free[0]
+        for x in (s.k, s.v, s.ks, s.vs):
+            x[free[0]] = x[0]
+        free[0] = 0
+    return free
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
+@pytest.mark.parametrize("D,page,n", [(64, 16, 1), (64, 64, 3), (128, 32, 5), (256, 128, 1), (64, 16, 140), (128, 64, 140),
+                                      (256, 32, 140)])
+def test_scales_of_pages_that_no_row_sees(D, page, n, window, sinks):
+    """Not a number (byte 255): the scales of every page that holds no token of a sequence. One stands in the table behind
+    each sequence's last token, and page 0 is one, next to blocks that have no page."""
+    rng = np.random.default_rng(page + n)
+    s = kv_ref.Step(rng, [n, n], [400, 130], 2, D, page, spare_blocks=4)
+    free = spare_page_0(s)
+    s.ks[free], s.vs[free] = 255, 255
+    for b in range(2):
+        blocks = -(-int(s.lens[b]) // page)
+        s.table[b, blocks:blocks + 2] = free[1]
+    s.table[0, 130 // page] = -1
+    check_attend(s, 4, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("n", [1, 3, 140])
+@pytest.mark.parametrize("side", ["ks", "vs"])
+def test_a_scale_that_is_nan_reaches_only_the_rows_that_see_it(side, n, page):
+    """Not a number (byte 255): the scale of sequence 0's first block and of sequence 1's third, of one head. Every value of
+    it is NaN for the rows that see one of its tokens, and nothing for the others."""
+    rng = np.random.default_rng(n + page)
+    s = kv_ref.Step(rng, [n, n], [400, 130], 2, 64, page)
+    q = randn_bf16(rng, (s.rows, 4, 64))
+    for window in (0, 60):
+        clean, clse = attend(Cache(s), q, 4, 0.1, window)
+        kept = getattr(s, side).copy()
+        getattr(s, side)[s.table[0, 0], 1] = getattr(s, side)[s.table[1, 2], 0] = 255
+        got, lse = attend(Cache(s), q, 4, 0.1, window)
+        setattr(s, side, kept)
+        want, wlse = from_bf16(clean).copy(), clse.copy()
+        for b, blk, heads in ((0, 0, slice(2, 4)), (1, 2, slice(0, 2))):
+            for i in range(n):
+                p = s.position(b, i)
+                first, last = (max(p - window + 1, 0) if window else 0), p  # what the row sees
+                if first < (blk + 1) * page and last >= blk * page:
+                    want[b * n + i, heads] = np.nan
+                    if side == "ks":
+                        wlse[b * n + i, heads] = np.nan
+        assert (np.isnan(from_bf16(got)) == np.isnan(want)).all()
+        fine = ~np.isnan(want)
+        assert np.array_equal(from_bf16(got)[fine], want[fine])
+        assert np.array_equal(lse, wlse, equal_nan=True)
+
+
 def test_attend_is_the_same_every_time_and_without_lse():
     rng = np.random.default_rng(3)
     s = kv_ref.Step(rng, [1, 1, 40, 1], [3000, 0, 500, 1500], 2, 128, 64)

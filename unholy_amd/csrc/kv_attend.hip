@@ -231,6 +231,11 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {  // the high bit of 
   return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
+// A scale byte that is no number, as e8m0 has it (in fp32: infinity; the products' conversions make NaN of any code with
+// it), and four codes that are none.
+constexpr int NAN_SCALE = 0xff;
+constexpr uint32_t NAN_CODES = 0x7f7f7f7fu;
+
 // The first n bytes of four.
 __device__ __forceinline__ uint32_t first_bytes(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1; }
 // bf16 operands of 0 and 1: of the NaN among eight codes, and of eight bits; and codes with zeros for their NaN.
@@ -434,7 +439,6 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
           s[j][e] = __builtin_amdgcn_exp2f(s[j][e] - ref);
           l += s[j][e];
         }
-      const float vs = e8m0_to_f32(uint8_t(vsb));
       bf16x8 p[2];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf)
@@ -442,12 +446,14 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
         for (int e = 0; e < 8; ++e) p[hf][e] = __bf16(s[2 * hf + e / 4][e % 4]);
       if (masked) {  // slots past the last token hold anything: zero
         const int n = pvt < 0 ? 0 : min(max(w.q.len - (t0 + 16 * g), 0), 16);
+        const uint32_t all = vsb == NAN_SCALE ? NAN_CODES : 0;  // its codes are NaN, under a scale that is a number then
+        vsb = all ? 127 : vsb;
         uint32_t bad = 0;
 #pragma unroll
         for (int d = 0; d < S::DT; ++d)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            vr[d][k] &= first_bytes(n - 4 * k);
+            vr[d][k] = (vr[d][k] | all) & first_bytes(n - 4 * k);
             bad |= nan_bytes(vr[d][k]);
           }
         if (__builtin_expect(__any(bad != 0), 0)) {
@@ -466,6 +472,7 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
           }
         }
       }
+      const float vs = e8m0_to_f32(uint8_t(vsb));
 #pragma unroll
       for (int d = 0; d < S::DT; ++d)
 #pragma unroll
@@ -904,6 +911,13 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
 #pragma unroll
       for (int e = 0; e < 16; ++e) p[T][e / 8][e % 8] = __bf16(s[T][e]);
     if (masked) {  // slots past the last token hold anything: zero
+      if (__builtin_expect(__any(fmaxf(vs[0], vs[1]) == INFINITY), 0)) {  // NAN_SCALE: its codes are NaN
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int d = 0; d < S::DT; ++d)
+            if (vs[T] == INFINITY) vx[T][d] = make_uint4(NAN_CODES, NAN_CODES, NAN_CODES, NAN_CODES);
+      }
       uint32_t bad = 0;
 #pragma unroll
       for (int T = 0; T < 2; ++T)
@@ -921,7 +935,8 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
         for (int d = 0; d < S::DT; ++d)
           for (int k = 0; k < 8; ++k) {
             const int T = k >> 2, j = 4 * (k & 3);  // tokens j .. j + 3 of the lane's 16
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(vt + vat + 16 * value_piece(c, 2 * T + h2) + d * 2048 + j);
+            uint32_t x = *reinterpret_cast<const uint32_t*>(vt + vat + 16 * value_piece(c, 2 * T + h2) + d * 2048 + j);
+            if ((T ? vs[1] : vs[0]) == INFINITY) x = NAN_CODES;
             const uint32_t nan = nan_bytes(x & first_bytes((T ? there[1] : there[0]) - j));
             for (uint64_t left = __ballot(nan != 0); left; left &= left - 1) {
               const int from = __ffsll((unsigned long long)left) - 1;  // its channel: row 8a + 4h + i of the products
@@ -943,6 +958,8 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
             x = make_uint4(no_nan(x.x), no_nan(x.y), no_nan(x.z), no_nan(x.w));
           }
       }
+#pragma unroll
+      for (int T = 0; T < 2; ++T) vs[T] = vs[T] == INFINITY ? 1.0f : vs[T];
     }
 #pragma unroll
     for (int T = 0; T < 2; ++T) {
