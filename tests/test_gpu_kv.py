@@ -448,6 +448,22 @@ def test_append_values_at_the_borders():
     check_append(s, x, x[::-1].copy())
 
 
+@pytest.mark.parametrize("rows", [2 ** 31 - 1, 2 ** 31 - 64, (1 << 29) - 3, (1 << 26) + 1])
+@pytest.mark.parametrize("D", [64, 256])
+def test_append_for_any_number_of_rows(D, rows):
+    """A launch that is sized for as many rows as an int counts, of which the step brings a few hundred (none past them is
+    read)."""
+    rng = np.random.default_rng(7)
+    s = kv_ref.Step(rng, [150, 1, 64], [5, 130, 0], 2, D, 64)
+    c, width = Cache(s), 2 * D
+    knew, vnew = (randn_bf16(rng, (s.rows, 2, D)) for _ in range(2))
+    call("uh_kv_append", dev(knew), width, dev(vnew), width, c.cu, rows, rows, c.lens, c.table, s.max_blocks, s.B,
+         *c.arrays(), s.pages, s.page, 2, D, None)
+    synchronize()
+    for got, want in zip(c.down(), kv_ref.append(s, knew, vnew)):
+        assert np.array_equal(got, want)
+
+
 def test_append_skips_what_has_no_slot():
     rng = np.random.default_rng(2)
     s = kv_ref.Step(rng, [5, 40, 3, 70], [0, 20, 30, 0], 2, 64, 16, spare_blocks=0)

@@ -435,8 +435,8 @@ void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& s, 
   if (int64_t(ldk) < int64_t(c.heads) * c.dim || int64_t(ldv) < int64_t(c.heads) * c.dim || ldk % 8 || ldv % 8)
     throw std::runtime_error("kv_append: ldk / ldv >= heads * dim, % 8");
   if (!aligned16(k) || !aligned16(v)) throw std::runtime_error("kv_append: rows not 16-byte aligned");
-  const int most = std::min(s.max_new, s.rows);
-  const int nblk = std::min((most - 1 + c.page - 1) / c.page + 1, s.max_blocks);  // blocks that `most` tokens can reach
+  const int64_t most = std::min(s.max_new, s.rows);  // (up to 2^31 - 1)
+  const int nblk = int(std::min<int64_t>((most - 1 + c.page - 1) / c.page + 1, s.max_blocks));  // that they can reach
   if (int64_t(s.B) * nblk > INT32_MAX) throw std::runtime_error("kv_append: B * blocks past 31 bits");
   const dim3 grid(unsigned(s.B) * unsigned(nblk), unsigned(c.heads), 2);
   // A wave holds 128 pieces of 8 channels x 4 tokens: enough for `most` tokens, wherever they begin, or a workgroup of four
