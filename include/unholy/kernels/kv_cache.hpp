@@ -13,7 +13,9 @@
 // A step brings rows cu[b] .. cu[b + 1] of sequence b (cu [B + 1], ascending); lens[b] counts the sequence's tokens, the
 // new ones included, so row i of its n is the token at position lens[b] - n + i. cu, lens and table are read on the
 // device: a captured step replays with what they hold then. `rows` is how many rows the row arrays have, `max_new` at
-// least the rows of any one sequence. Rows that no sequence has are left as they are.
+// least the rows of any one sequence: a sequence that brings more all the same (a launch captured for fewer, say) is taken
+// as one that brings none, none of its rows is appended, and their attention is what a row is given that sees nothing. Rows
+// that no sequence has are left as they are. No sequences, no rows or max_new 0: nothing is launched.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -369,7 +369,8 @@ int uh_mx_moe_forward_noalloc(const uint16_t* x, const float* logits, int T, int
  * full contracts; no reference counterpart). One layer: kc e4m3 [pages, Hkv, page, D], vc e4m3 [pages, Hkv, D, page], ks / vs
  * e8m0 [pages, Hkv]; page 16, 32, 64 or 128 tokens, D 64, 128 or 256. table int32 [B, max_blocks] (page numbers, -1: none),
  * lens int32 [B] (tokens of a sequence, the step's new ones included), cu int32 [B + 1] (the step's rows of each sequence),
- * all on the device; rows: of the row arrays; max_new: at least any sequence's rows. ---- */
+ * all on the device; rows: of the row arrays; max_new: at least any sequence's rows (of one that brings more, nothing is appended
+ * and the rows' attention is zero). ---- */
 /* The new rows' keys / values k, v bf16 [rows, Hkv, D] (row strides ldk, ldv) quantized into their slots, a power-of-two
  * scale for each block and head that only grows while the block fills. */
 int uh_kv_append(const uint16_t* k, int ldk, const uint16_t* v, int ldv, const int32_t* cu, int rows, int max_new,

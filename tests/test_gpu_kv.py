@@ -495,6 +495,56 @@ def test_append_then_attend_step_by_step():
         s.ctx = [x + 1 for x in s.ctx]
 
 
+@pytest.mark.parametrize("Hq,max_new,n,mode", [
+    (4, 1, [1, 3, 1, 0, 2], "few rows"), (2, 3, [4, 3, 0, 200], "few rows"), (1, 2, [1] * 70 + [3, 2, 9], "few rows"),
+    (4, 20, [20, 30, 5], "many rows"), (40, 1, [1, 2, 1], "many rows"), (4, 40, [41], "many rows"),
+    (4, 130, [1, 131, 130, 2], "both"), (2, 150, [1] * 66 + [151, 9, 700, 140], "both")])
+def test_sequences_of_more_rows_than_max_new(Hq, max_new, n, mode):
+    """Steps captured for max_new rows a sequence, replayed with more: the others' results are theirs, of these sequences
+    nothing is appended, and their rows come back as rows that see nothing, not with what was there."""
+    rng = np.random.default_rng(len(n))
+    s = kv_ref.Step(rng, n, rng.integers(0, 150, len(n)).tolist(), 1, 64, 32, spare_rows=2)
+    c, st, D = Cache(s), Stream(), 64
+    q, new = randn_bf16(rng, (s.rows, Hq, D)), randn_bf16(rng, (s.rows, 1, D))
+    dq, dn, out = dev(q), dev(new), dev(np.full(q.shape, 0x7FC1, np.uint16))
+    lse = dev(np.full((s.rows, Hq), np.nan, np.float32))
+    need = call("uh_kv_attend_workspace_size", s.rows, max_new, s.B, Hq, 1, D)
+    ws = dev(np.zeros(need, np.uint8))
+    c.cu.upload(np.zeros(s.B + 1, np.int32))  # captured, and run once, without rows
+
+    def work():
+        call("uh_kv_append", dn, D, dn, D, c.cu, s.rows, max_new, c.lens, c.table, s.max_blocks, s.B, *c.arrays(), s.pages,
+             s.page, 1, D, st.handle)
+        call("uh_kv_attend", dq, Hq * D, c.cu, s.rows, max_new, c.lens, c.table, s.max_blocks, s.B, *c.arrays(), s.pages,
+             s.page, Hq, 1, D, 0.125, 0, 0, out, Hq * D, lse, ws, need, st.handle)
+
+    synchronize()
+    work()
+    g = Graph(st, work)
+    st.synchronize()
+    c.cu.upload(s.cu)
+    synchronize()
+    taken = kv_ref.Step.__new__(kv_ref.Step)
+    taken.__dict__.update(s.__dict__)
+    taken.n = [k if k <= max_new else 0 for k in n]
+    for _ in range(2):
+        g.launch()
+        st.synchronize()
+        want = kv_ref.append(taken, new, new)
+        for got, x in zip(c.down(), want):
+            assert np.array_equal(got, x)
+        taken.k, taken.v, taken.ks, taken.vs = want
+        ref, rlse, tol, ltol = kv_ref.attend(taken, from_bf16(q).astype(np.float64), Hq, 0.125)
+        got, gl = out.download(q.shape, np.uint16), lse.download((s.rows, Hq), np.float32)
+        for b, k in enumerate(n):
+            r = slice(int(s.cu[b]), int(s.cu[b]) + k)
+            if k > max_new:
+                assert (got[r] == 0).all() and np.isneginf(gl[r]).all(), b
+            else:
+                assert (np.abs(from_bf16(got[r]) - ref[r]) <= tol[r]).all() and (np.abs(gl[r] - rlse[r]) <= ltol[r]).all(), b
+        assert (got[sum(n):] == 0x7FC1).all() and np.isnan(gl[sum(n):]).all()
+
+
 # ---- pages -----------------------------------------------------------------------------------------------------------
 class Pool:
     """Tables, lengths and reference counts of B slots over a pool, host and device."""

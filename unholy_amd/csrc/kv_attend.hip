@@ -48,7 +48,7 @@ struct Block {
   int parts, step;
   int row0, rows;  // from the sequence's first (row, query head) on
   int r0, h;       // the sequence's first row, the head
-  int pad[2];
+  int over, pad;   // some sequence brings more than max_new rows
 };
 
 // What every workgroup knows of the call.
@@ -60,6 +60,7 @@ struct Attend {
   KvCache c;
   int ldq, ldo, group, page_shift, window, sinks;
   float scale2;  // scale * log2(e): the kernels take powers of two
+  bool clears;   // the rows of sequences with more than max_new are the split kernel's to clear (else the join's)
   int few;  // sequences of up to this many rows (FEW or none) are the split kernel's, the others the tiled kernel's
   uint32_t target;     // workgroups that the chip holds at a time
   uint32_t* counters;  // of finished parts, by the workgroup of the first; zero between launches (split kernel)
@@ -140,19 +141,35 @@ __device__ __forceinline__ uint32_t units_of(const Split& s, uint32_t tiles) {
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Zeros (lse: -inf) in the rows of the sequences that bring more than max_new, which see nothing: workgroup w's of n.
+__device__ __forceinline__ void clear_rows(const Attend& a, int w, int n) {
+  const int heads = a.group * a.c.heads, quads = heads * a.c.dim / 8;
+  for (int b = 0; b < a.st.B; ++b) {
+    int past;
+    const Seq q = seq_of(a.st, b, &past);
+    for (int i = w; i < past; i += n) {
+      uint4* out = reinterpret_cast<uint4*>(a.out + size_t(q.r0 + i) * a.ldo);
+      for (int j = int(threadIdx.x); j < quads; j += AT_NT) out[j] = make_uint4(0, 0, 0, 0);
+      if (a.lse)
+        for (int j = int(threadIdx.x); j < heads; j += AT_NT) a.lse[size_t(q.r0 + i) * heads + j] = -INFINITY;
+    }
+  }
+}
+
 __device__ __forceinline__ bool is_few(const Attend& a, const Seq& q) {
   return q.r1 > q.r0 && (q.r1 - q.r0) * a.group <= a.few;
 }
 // The segment that holds the workgroup's first unit. Every wave for itself, a sequence a lane: no barriers, and for up to 64
-// sequences one pass over registers.
-__device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w) {
+// sequences one pass over registers. over: some sequence brings more than max_new rows.
+__device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w, bool& over) {
   const int lane = threadIdx.x & 63;
   uint32_t segs = 0;  // of this lane's sequence
+  int past = 0;       // rows of it past what the launch takes
   const auto look = [&](int b) {
     segs = 0;
     w.t = Tiles{0, 0, 0};
     if (b < a.st.B) {
-      w.q = seq_of(a.st, b);
+      w.q = seq_of(a.st, b, &past);
       if (is_few(a, w.q)) {
         segs = uint32_t(a.c.heads);
         w.t = tiles_of(a, w.q);
@@ -160,8 +177,10 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w)
     }
   };
   uint32_t tiles = 0, all = 0;
+  over = false;
   for (int b0 = 0; b0 < a.st.B; b0 += 64) {
     look(b0 + lane);
+    over |= __any(past > 0) != 0;
     tiles += lane_of(wave_scan(segs * (uint32_t(w.t.count) + START)), 63);
     all += lane_of(wave_scan(segs), 63);
   }
@@ -323,7 +342,10 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
   Split sp;
   Walk w;
-  if (!find_segment(a, sp, w)) return;
+  bool over;
+  const bool some = find_segment(a, sp, w, over);
+  if (__builtin_expect(over && a.clears, 0)) clear_rows(a, int(blockIdx.x), int(gridDim.x));
+  if (!some) return;
   Part pt = part_of(sp, w, blockIdx.x * sp.unit);
 
   const int mask = a.c.page - 1, sh = a.page_shift;
@@ -657,16 +679,17 @@ __device__ __forceinline__ Tiles block_tiles(const Attend& a, const Seq& q, int 
   const int last = min(row0 + PR_ROWS, (q.r1 - q.r0) * a.group) - 1;
   return tiles_of(a, Seq{0, 0, max(min(q.len, q.first + last / a.group + 1), 0), q.first + row0 / a.group});
 }
-__device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p) {
+__device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p, bool& over) {
   constexpr uint32_t NONE = 1u << 30;
   const int lane = threadIdx.x & 63;
   const uint32_t heads = uint32_t(a.c.heads);
   Seq q{0, 0, 0, 0};
   uint32_t blocks = 0, most = 0, all = 0;  // of this lane's sequence, tiles of its last block; of all, times the heads
+  int past = 0;                            // as in find_segment
   const auto look = [&](int b) {
     blocks = most = 0;
     if (b < a.st.B) {
-      q = seq_of(a.st, b);
+      q = seq_of(a.st, b, &past);
       const int rows = (q.r1 - q.r0) * a.group;
       if (rows > a.few) {
         blocks = uint32_t(row_groups(rows, PR_ROWS));
@@ -675,8 +698,10 @@ __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p) {
     }
   };
   uint32_t tiles = 0;  // (a block's taken as the last one's; as long as the blocks are few)
+  over = false;
   for (int b0 = 0; b0 < a.st.B; b0 += 64) {
     look(b0 + lane);
+    over |= __any(past > 0) != 0;
     all += lane_of(wave_scan(blocks), 63) * heads;
     if (all < a.target) tiles += lane_of(wave_scan(blocks * most), 63) * heads;
   }
@@ -721,12 +746,13 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 31, h2 = lane >> 5;
 
   BlockPart bp;
-  const bool some = find_block(a, bp);
+  bool over;
+  const bool some = find_block(a, bp, over);
   if (tid == 0 && blockIdx.x < a.target)
     a.blocks[blockIdx.x] = some && bp.index == 0
                                ? Block{bp.parts, int(a.c.heads), bp.row0, min(PR_ROWS, (bp.q.r1 - bp.q.r0) * a.group - bp.row0),
-                                       bp.q.r0, bp.h, {}}
-                               : Block{};
+                                       bp.q.r0, bp.h, over, 0}
+                               : Block{0, 0, 0, 0, 0, 0, over, 0};
   if (!some) return;
   const int b = bp.b, h = bp.h, row0 = bp.row0;
   const Seq q = bp.q;
@@ -1002,6 +1028,7 @@ template <int D>
 __global__ __launch_bounds__(AT_NT) void kv_join_kernel(Attend a) {
   constexpr int WAVE_QUADS = D / 32 * 256;  // of 32 rows
   const Block k = a.blocks[blockIdx.x];
+  if (__builtin_expect(k.over, 0)) clear_rows(a, int(blockIdx.x * gridDim.y + blockIdx.y), int(gridDim.x * gridDim.y));
   if (k.parts <= 1) return;
   const int at = blockIdx.y * AT_NT + threadIdx.x, r = at / WAVE_QUADS * 32 + (at & 31), rr = k.row0 + r;
   if (r >= k.rows) return;
@@ -1088,8 +1115,8 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
   if (ws_bytes < need) fail("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
 
   const Way way = way_of(s.rows, s.max_new, s.B, Hq / c.heads, c.heads);
-  Attend a{q,       out,   lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E, way.few,
-           unsigned(target_of(c.dim)), nullptr, nullptr, nullptr, nullptr};
+  Attend a{q,       out,   lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E,
+           !way.tiled, way.few, unsigned(target_of(c.dim)), nullptr, nullptr, nullptr, nullptr};
   while (1 << a.page_shift < c.page) ++a.page_shift;
   a.counters = static_cast<uint32_t*>(ws);
   a.blocks = reinterpret_cast<Block*>(a.counters + 512);
