@@ -39,10 +39,11 @@ struct KvStep {
 // The new rows' keys and values k, v bf16 [rows, heads, dim] (row strides ldk, ldv >= heads * dim, % 8; 16-byte aligned)
 // quantized into their slots. A block's scale is the smallest power of two 2^e, e <= 119, with amax <= 448 2^e over its
 // new tokens' finite values (amax floored at 1e-4); where the block holds earlier tokens of the sequence it is at least
-// the block's scale so far, and if it grows their codes are rounded to the new one (a shift by a power of two: exact but
-// for codes that become subnormal). Codes: round to nearest even, saturating at 448 2^e; a NaN stays one. Tokens at
-// negative positions, past the table or without a page are skipped. A page that the step writes must belong to one
-// sequence (kv_reserve sees to that). Nothing but the slots of the sequence's tokens and the block's scales is written.
+// the block's scale so far (kv_append's own: 2^119 at most), and if it grows their codes are rounded to the new one (a shift
+// by a power of two: exact but for codes that become subnormal). Codes: round to nearest even, saturating at 448 2^e; a NaN
+// stays one. Tokens at negative positions, past the table or without a page are skipped. A page that the step writes must
+// belong to one sequence (kv_reserve sees to that). Nothing but the slots of the sequence's tokens and the block's scales
+// is written.
 void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& step, const KvCache& cache,
                hipStream_t st);
 

@@ -372,6 +372,35 @@ def test_calls_on_two_streams_at_once():
         assert np.array_equal(out.download(want.shape, np.uint16), want)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (500, 4)])
+def test_readers_of_one_cache_on_two_streams(window, sinks):
+    """The device arrays of one cache, its tables and lengths read by a decode step, drafts and a prompt at once, each on a
+    stream and with rows, output and workspace of its own."""
+    rng = np.random.default_rng(23)
+    s = kv_ref.Step(rng, [1, 1], [4000, 900], 2, 128, 64)
+    c, calls = Cache(s), []
+    for n in ([1, 1], [150, 33], [6, 5]):
+        x = Cache.__new__(Cache)
+        x.__dict__.update(c.__dict__)
+        x.step = kv_ref.Step.__new__(kv_ref.Step)
+        x.step.__dict__.update(s.__dict__)
+        x.step.n, x.step.rows, x.step.cu = n, sum(n), np.concatenate(([0], np.cumsum(n))).astype(np.int32)
+        x.cu = dev(x.step.cu)
+        q = randn_bf16(rng, (sum(n), 8, 128))
+        need = call("uh_kv_attend_workspace_size", sum(n), max(n), 2, 8, 2, 128)
+        calls.append((x, n, dev(q), dev(np.zeros(q.shape, np.uint16)), dev(np.zeros(need, np.uint8)), need, Stream(),
+                      attend(x, q, 8, 0.1, window, sinks)[0]))
+    for _ in range(20):
+        for x, n, q, out, ws, need, st, _ in calls:
+            call("uh_kv_attend", q, 1024, x.cu, sum(n), max(n), c.lens, c.table, s.max_blocks, 2, *c.arrays(), s.pages,
+                 s.page, 8, 2, 128, 0.1, window, sinks, out, 1024, None, ws, need, st.handle)
+    for x, n, q, out, ws, need, st, want in calls:
+        st.synchronize()
+        assert np.array_equal(out.download(want.shape, np.uint16), want)
+    for got, want in zip(c.down(), (s.k, s.v, s.ks, s.vs)):
+        assert np.array_equal(got, want)
+
+
 def test_large_page_numbers():
     """A pool past 4 GiB: pages whose bytes lie beyond 32-bit offsets."""
     rng = np.random.default_rng(8)
