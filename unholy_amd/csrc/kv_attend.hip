@@ -60,11 +60,10 @@ struct Attend {
   KvCache c;
   int ldq, ldo, group, page_shift, window, sinks;
   float scale2;  // scale * log2(e): the kernels take powers of two
-  bool clears;   // the rows of sequences with more than max_new are the split kernel's to clear (else the join's)
   int few;  // sequences of up to this many rows (FEW or none) are the split kernel's, the others the tiled kernel's
   uint32_t target;     // workgroups that the chip holds at a time
   uint32_t* counters;  // of finished parts, by the workgroup of the first; zero between launches (split kernel)
-  Block* blocks;       // by the workgroup of the first part (tiled kernel)
+  Block* blocks;       // by the workgroup of the first part (tiled kernel; null where it is not launched)
   float *po, *pml;     // partial sums: values [slot][rows][D]; maximum and weight sum [slot][rows][2]
 };
 
@@ -145,9 +144,9 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ void clear_rows(const Attend& a, int w, int n) {
   const int heads = a.group * a.c.heads, quads = heads * a.c.dim / 8;
   for (int b = 0; b < a.st.B; ++b) {
-    int past;
-    const Seq q = seq_of(a.st, b, &past);
-    for (int i = w; i < past; i += n) {
+    const Seq q = seq_of(a.st, b);
+    if (!too_many(a.st, q)) continue;
+    for (int i = w; i < q.r1 - q.r0; i += n) {
       uint4* out = reinterpret_cast<uint4*>(a.out + size_t(q.r0 + i) * a.ldo);
       for (int j = int(threadIdx.x); j < quads; j += AT_NT) out[j] = make_uint4(0, 0, 0, 0);
       if (a.lse)
@@ -157,19 +156,21 @@ __device__ __forceinline__ void clear_rows(const Attend& a, int w, int n) {
 }
 
 __device__ __forceinline__ bool is_few(const Attend& a, const Seq& q) {
-  return q.r1 > q.r0 && (q.r1 - q.r0) * a.group <= a.few;
+  return q.r1 > q.r0 && (q.r1 - q.r0) * a.group <= a.few && !too_many(a.st, q);
 }
 // The segment that holds the workgroup's first unit. Every wave for itself, a sequence a lane: no barriers, and for up to 64
 // sequences one pass over registers. over: some sequence brings more than max_new rows.
 __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w, bool& over) {
   const int lane = threadIdx.x & 63;
   uint32_t segs = 0;  // of this lane's sequence
-  int past = 0;       // rows of it past what the launch takes
+  int rows = 0;
   const auto look = [&](int b) {
     segs = 0;
+    rows = 0;
     w.t = Tiles{0, 0, 0};
     if (b < a.st.B) {
-      w.q = seq_of(a.st, b, &past);
+      w.q = seq_of(a.st, b);
+      rows = w.q.r1 - w.q.r0;
       if (is_few(a, w.q)) {
         segs = uint32_t(a.c.heads);
         w.t = tiles_of(a, w.q);
@@ -180,7 +181,7 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w,
   over = false;
   for (int b0 = 0; b0 < a.st.B; b0 += 64) {
     look(b0 + lane);
-    over |= __any(past > 0) != 0;
+    over |= __ballot(rows > a.st.max_new) != 0;
     tiles += lane_of(wave_scan(segs * (uint32_t(w.t.count) + START)), 63);
     all += lane_of(wave_scan(segs), 63);
   }
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
   Walk w;
   bool over;
   const bool some = find_segment(a, sp, w, over);
-  if (__builtin_expect(over && a.clears, 0)) clear_rows(a, int(blockIdx.x), int(gridDim.x));
+  if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(blockIdx.x), int(gridDim.x));  // (else the join's to do)
   if (!some) return;
   Part pt = part_of(sp, w, blockIdx.x * sp.unit);
 
@@ -685,14 +686,15 @@ __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p, bool& 
   const uint32_t heads = uint32_t(a.c.heads);
   Seq q{0, 0, 0, 0};
   uint32_t blocks = 0, most = 0, all = 0;  // of this lane's sequence, tiles of its last block; of all, times the heads
-  int past = 0;                            // as in find_segment
+  int rows = 0;
   const auto look = [&](int b) {
     blocks = most = 0;
+    rows = 0;
     if (b < a.st.B) {
-      q = seq_of(a.st, b, &past);
-      const int rows = (q.r1 - q.r0) * a.group;
-      if (rows > a.few) {
-        blocks = uint32_t(row_groups(rows, PR_ROWS));
+      q = seq_of(a.st, b);
+      rows = q.r1 - q.r0;
+      if (rows * a.group > a.few && rows <= a.st.max_new) {
+        blocks = uint32_t(row_groups(rows * a.group, PR_ROWS));
         most = uint32_t(block_tiles(a, q, int(blocks - 1) * PR_ROWS).count);
       }
     }
@@ -701,7 +703,7 @@ __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p, bool& 
   over = false;
   for (int b0 = 0; b0 < a.st.B; b0 += 64) {
     look(b0 + lane);
-    over |= __any(past > 0) != 0;
+    over |= __ballot(rows > a.st.max_new) != 0;
     all += lane_of(wave_scan(blocks), 63) * heads;
     if (all < a.target) tiles += lane_of(wave_scan(blocks * most), 63) * heads;
   }
@@ -1115,11 +1117,11 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
   if (ws_bytes < need) fail("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
 
   const Way way = way_of(s.rows, s.max_new, s.B, Hq / c.heads, c.heads);
-  Attend a{q,       out,   lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E,
-           !way.tiled, way.few, unsigned(target_of(c.dim)), nullptr, nullptr, nullptr, nullptr};
+  Attend a{q,       out,   lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E, way.few,
+           unsigned(target_of(c.dim)), nullptr, nullptr, nullptr, nullptr};
   while (1 << a.page_shift < c.page) ++a.page_shift;
   a.counters = static_cast<uint32_t*>(ws);
-  a.blocks = reinterpret_cast<Block*>(a.counters + 512);
+  if (way.tiled) a.blocks = reinterpret_cast<Block*>(a.counters + 512);
   a.po = reinterpret_cast<float*>(static_cast<char*>(ws) + kHeadBytes);
   a.pml = a.po + sum_rows(way, c.dim) * c.dim;
   const int64_t segs = int64_t(s.B) * c.heads;

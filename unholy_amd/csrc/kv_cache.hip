@@ -58,7 +58,7 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(const bf16* __restrict__ 
   const int blk = max(q.first, 0) / PAGE + int(blockIdx.x % nblk), lo = blk * PAGE;
   if (lo >= q.len || blk >= st.max_blocks) return;
   const int p0 = max(max(q.first, lo), 0), s0 = p0 - lo, n = min(lo + PAGE, q.len) - p0, end = s0 + n;  // new: [s0, end)
-  if (n <= 0) return;
+  if (n <= 0 || too_many(st, q)) return;
   const int page = st.table[size_t(b) * st.max_blocks + blk];
   const int ld = values ? ldv : ldk;
   const bf16* x = (values ? vx : kx) + size_t(q.r0 + (p0 - q.first)) * ld + size_t(h) * D;

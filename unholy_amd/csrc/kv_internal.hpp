@@ -10,22 +10,21 @@
 namespace unholy::kernels::kv {
 
 // Sequence b's rows [r0, r1) of the step, kept inside the row arrays whatever cu holds, its length and the position of
-// row r0 (below 0 where more rows come than tokens are counted). A launch is sized for max_new rows of a sequence: one that
-// has more is taken as one without rows (past, if it is asked for: their number), not as the first of them.
+// row r0 (below 0 where more rows come than tokens are counted).
 struct Seq {
   int r0, r1, len, first;
 };
-__device__ __forceinline__ Seq seq_of(const KvStep& s, int b, int* past = nullptr) {
+__device__ __forceinline__ Seq seq_of(const KvStep& s, int b) {
   Seq q;
   q.r0 = min(max(s.cu[b], 0), s.rows);
   q.r1 = min(max(s.cu[b + 1], q.r0), s.rows);
-  const bool many = q.r1 - q.r0 > s.max_new;
-  if (past) *past = many ? q.r1 - q.r0 : 0;
-  if (many) q.r1 = q.r0;
   q.len = max(s.lens[b], 0);
   q.first = q.len - (q.r1 - q.r0);
   return q;
 }
+
+// A launch is sized for max_new rows of a sequence: one that has more is taken as one without rows, not as the first of them.
+__device__ __forceinline__ bool too_many(const KvStep& s, const Seq& q) { return q.r1 - q.r0 > s.max_new; }
 
 // The page of block blk of sequence b, or -1.
 __device__ __forceinline__ int page_of(const int32_t* table, int max_blocks, int pages, int b, int blk) {
