@@ -61,7 +61,7 @@ struct Attend {
   int ldq, ldo, group, page_shift, window, sinks;
   float scale2;  // scale * log2(e): the kernels take powers of two
   int few;  // sequences of up to this many rows (FEW or none) are the split kernel's, the others the tiled kernel's
-  uint32_t target;     // workgroups that the chip holds at a time
+  uint32_t target;     // workgroups that the work is cut for
   uint32_t* counters;  // of finished parts, by the workgroup of the first; zero between launches (split kernel)
   Block* blocks;       // by the workgroup of the first part (tiled kernel; null where it is not launched)
   float *po, *pml;     // partial sums: values [slot][rows][D]; maximum and weight sum [slot][rows][2]
@@ -272,12 +272,12 @@ __device__ __forceinline__ uint32_t no_nan(uint32_t x) { return x & ~((nan_bytes
 // ---- few rows a sequence: decode and verify steps ---------------------------------------------------------------------
 // Bound by reading the cache once (64 sequences of 0 to 8190 tokens, 8 heads of 128: 105 us, 5.3 TB/s; four of 90,000 to
 // 131,000: 178 us, 5.4 TB/s; a sum over a large array reads 6.1 TB/s here), and where there is little of it by the chain of
-// loads that depend on each other: lengths, table, keys, partial sums. A wave takes 16 rows ((token, query head) pairs that share a key / value head) and
-// 64 tokens at a time straight from the cache into registers, no LDS: with S^T = K Q^T the 16x16 product leaves lane
-// (row c, group g) the scores of tokens 4g .. 4g + 3 of a 16-token tile, and the tiles' rows are taken in such an order of
-// tokens (tile j, row r: token 16 (r / 4) + 4j + r % 4) that over four tiles these are tokens 16g .. 16g + 15: the very
-// tokens whose values one 16-byte load of the transposed cache gives it for O^T = V^T P^T. The weights go from one product
-// to the other in place, and a row's running maximum and sum are its lane's own.
+// loads that depend on each other: lengths, table, keys, partial sums. A wave takes 16 rows ((token, query head) pairs that
+// share a key / value head) and 64 tokens at a time straight from the cache into registers, no LDS: with S^T = K Q^T the
+// 16x16 product leaves lane (row c, group g) the scores of tokens 4g .. 4g + 3 of a 16-token tile, and the tiles' rows are
+// taken in such an order of tokens (tile j, row r: token 16 (r / 4) + 4j + r % 4) that over four tiles these are tokens
+// 16g .. 16g + 15: the very tokens whose values one 16-byte load of the transposed cache gives it for O^T = V^T P^T. The
+// weights go from one product to the other in place, and a row's running maximum and sum are its lane's own.
 // The codes become bf16 exactly (v_cvt_scalef32, the block's scale with them), the products sum in fp32; the weights are
 // rounded to bf16 for the second product (2^-8 of each at most, as much as the output's own rounding), their sum is taken in
 // fp32 before that.
@@ -295,7 +295,8 @@ struct Shape {
     float2 ml[AT_WAVES][FEW], group_ml[AT_NT];
   };
 };
-// Workgroups that the chip holds, two a CU or, by their registers, one.
+// Workgroups that a launch's work is cut for: two a CU, by their registers, or one (and two for 64 channels, of whose tiled
+// kernel a CU holds three).
 constexpr int target_of(int dim) { return dim <= 128 ? 512 : 256; }
 constexpr int FLIGHT = 10;  // partial sums that a thread reads at a time
 constexpr size_t kHeadBytes = 512 * (sizeof(uint32_t) + sizeof(Block));  // counters and blocks
@@ -621,18 +622,21 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
 }
 
 // ---- many rows a sequence: prompts ------------------------------------------------------------------------------------
-// Bound by the matrix rate and by the exponentials and conversions next to it: 8192 rows of 32 heads of 128 take 527 to 550 us,
-// 1.00 to 1.04 PFLOP/s (a large bf16 product reaches 1.17 here), the matrix units busy for half of the cycles and the vector units
-// for 70%; with 64 channels, where an exponential comes with half as many products, 0.57 PFLOP/s. A workgroup takes 128 rows (4 waves of 32)
-// of one (sequence, key / value head) and goes through the 64-token tiles that they see, which arrive in LDS as codes by
-// direct loads, two tiles ahead, in a ring of three. The 32x32x16 product with the same order of tokens as above: S^T = K Q^T
+// Bound by the matrix rate and by the vector work next to it: 8192 rows of 32 heads of 128 take 527 to 562 us, 0.98 to 1.04
+// PFLOP/s (a large bf16 product reaches 1.17 here), the matrix units busy for half of the cycles and the vector units for 72%;
+// with 64 channels, where a score's exponential, scaling and sum come with half as many products, 0.56 PFLOP/s (28%, 78%). With
+// 256 the registers do not suffice (14 are spilled), and in pages of 16 and 32 tokens each tile's reload waits for the direct
+// loads as well: 4096 rows of 32 heads over 4 take 355 us, in pages of 16 396 (128 channels: 153 and 166).
+// A workgroup takes 128 rows (4 waves of 32) of one (sequence, key / value head) and goes through the 64-token tiles that they
+// see, which arrive in LDS as codes by direct loads, two tiles ahead, in a ring of three. The 32x32x16 product with the same order of tokens as above: S^T = K Q^T
 // with row 8a + 4h + i of a 32-token half taken as token 16h + 4a + i, so that lane (row, half h) has the scores of 16
 // consecutive tokens and O^T = V^T P^T finds their values in one 16-byte read.
 // LDS: the 16-byte pieces of a key row (D bytes) and of a channel's values (64 bytes) are permuted among themselves such
 // that the sixteen lanes that a read serves at a time find theirs in different banks.
 // Pages and scales are read for 16 tiles at a time: their loads are waited for with all others, direct ones among them.
 // The running maximum is left alone until a row's scores pass it by more than 2^8: the weights stay small enough, and most
-// tiles need no scaling of the sums.
+// tiles need no scaling of the sums. The largest weight is not 1 then, as it is above, but rounded to bf16 like the others: an
+// output is off by 2.2e-3 of its norm, the split kernel's by 1.8e-3, and the output's own rounding alone is 1.65e-3.
 constexpr int PR_ROWS = 128;
 constexpr int PR_STAGES = 3;
 constexpr int PR_META = 16;  // tiles

@@ -18,7 +18,9 @@ namespace {
 // thread takes 8 channels of a token, lanes along the rows. Values, whose tokens lie a byte apart: 8 channels of the four
 // tokens of a dword, lanes along the tokens, so that a wave reads 64-byte pieces of 16 rows and writes whole 64-byte rows of
 // channels (12,002 tokens of 8 heads of 128: 16.8 us, 4.4 TB/s; through an LDS tile of bytes 25.8). A step of few tokens is
-// bound by its three dependent loads (lengths, page, scale): 6.3 us a layer.
+// bound by its three dependent loads (lengths, page, scale): 6.3 us a layer, while no block's scale grows. Where one does, its
+// earlier codes are read and written by the byte, one after the other, and the launch waits for that: 43 us a layer for 64
+// tokens in full use, of whose blocks a sixth grow (prompts, which write whole blocks, lose some 5 us).
 // A power-of-two scale, as everywhere in this library, so that a block whose scale grows keeps its codes: rne(c 2^-g) is
 // exact unless the result is subnormal, and then off by at most 2^-10 of the new scale's unit. (A scale with a mantissa
 // would round every code of the block again, each time that it grows.)
