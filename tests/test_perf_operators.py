@@ -1,5 +1,6 @@
 """The calls that perf/operators.py makes of the library: a step runs on torch's current stream, whether call by call or
 replayed, in order with what writes its inputs and reads its results."""
+import pathlib
 import subprocess
 import sys
 import types
@@ -89,5 +90,6 @@ print("in order")
 def test_steps_run_in_order_with_torch():
     """Rows written by torch just before a step, and results read by torch just after it, without a wait of the host. (In a
     process of its own, where torch comes first and the library takes torch's HIP runtime.)"""
-    done = subprocess.run([sys.executable, "-u", "-c", ORDER], capture_output=True, text=True, timeout=100)
+    done = subprocess.run([sys.executable, "-u", "-c", ORDER], cwd=pathlib.Path(__file__).resolve().parents[1],
+                          capture_output=True, text=True, timeout=100)
     assert done.returncode == 0 and "in order" in done.stdout, done.stderr[-2000:]

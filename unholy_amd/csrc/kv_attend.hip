@@ -628,9 +628,9 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
 // 256 the registers do not suffice (14 are spilled), and in pages of 16 and 32 tokens each tile's reload waits for the direct
 // loads as well: 4096 rows of 32 heads over 4 take 355 us, in pages of 16 396 (128 channels: 153 and 166).
 // A workgroup takes 128 rows (4 waves of 32) of one (sequence, key / value head) and goes through the 64-token tiles that they
-// see, which arrive in LDS as codes by direct loads, two tiles ahead, in a ring of three. The 32x32x16 product with the same order of tokens as above: S^T = K Q^T
-// with row 8a + 4h + i of a 32-token half taken as token 16h + 4a + i, so that lane (row, half h) has the scores of 16
-// consecutive tokens and O^T = V^T P^T finds their values in one 16-byte read.
+// see, which arrive in LDS as codes by direct loads, two tiles ahead, in a ring of three. The 32x32x16 product with the same
+// order of tokens as above: S^T = K Q^T with row 8a + 4h + i of a 32-token half taken as token 16h + 4a + i, so that lane
+// (row, half h) has the scores of 16 consecutive tokens and O^T = V^T P^T finds their values in one 16-byte read.
 // LDS: the 16-byte pieces of a key row (D bytes) and of a channel's values (64 bytes) are permuted among themselves such
 // that the sixteen lanes that a read serves at a time find theirs in different banks.
 // Pages and scales are read for 16 tiles at a time: their loads are waited for with all others, direct ones among them.
