@@ -23,6 +23,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "unholy/kernels/rope.hpp"
+
 namespace unholy::kernels {
 
 using bf16 = uint16_t;
@@ -46,6 +48,17 @@ struct KvStep {
 // is written.
 void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& step, const KvCache& cache,
                hipStream_t st);
+
+// The step between the projections and the cache in one launch: queries q [rows, Hq, dim] and keys k [rows, heads, dim] of each
+// row normalised by head (wq, wk bf16 [dim], eps; null: not) and rotated to the row's position, as qk_norm_rope (rope, where
+// the weights are null) does it at positions lens[b] - n + i; the queries into qo, the keys, rounded to bf16, and the values v
+// into the cache as kv_append does it: all results are those of the two calls, bit for bit. Hq 0: no queries. qo may be q (with
+// its stride), otherwise they share no element. Rows that no sequence has, and those of one with more than max_new, are left as
+// they are in qo; queries are also rotated where their token has no page. Strides and alignment as in kv_append (q, qo and the
+// weights too); r.rot % 16, r.first % 8.
+void kv_append_rope(const bf16* q, int ldq, bf16* qo, int ldqo, int Hq, const bf16* wq, const bf16* k, int ldk, const bf16* wk,
+                    float eps, const bf16* v, int ldv, const KvStep& step, const Rope& r, const KvCache& cache,
+                    hipStream_t st);
 
 // Causal attention of the step's rows over their sequences' cached tokens (the new ones among them: kv_append goes
 // before). Query head h reads key / value head h / (Hq / heads). Row at position p sees token t <= p, with window > 0 only

@@ -365,6 +365,23 @@ int uh_mx_moe_forward_noalloc(const uint16_t* x, const float* logits, int T, int
                               const uint8_t* const* tab, float limit, uint16_t* out, int32_t* sel, float* wt,
                               void* stream);
 
+/* ---- rotary positions of heads, alone and behind the norms of queries and keys (include/unholy/kernels/rope.hpp has the
+ * contracts; no reference counterpart). Channels [first, first + rot) of a head in pairs, interleaved (2i, 2i + 1) or in halves
+ * (i, i + rot / 2), pair i turned by pos * freq[i] (freq double [rot / 2], device: radians a position) and times mscale. ---- */
+/* Frequencies on the host: base^(-2i / rot), slowed by `factor` for a longer context: scaling 0 none, 1 all, 2 in proportion
+ * between those that turn `low` times over `trained` positions (slowed) and `high` times (kept), 3 between the same two, by
+ * pair number. */
+int uh_rope_frequencies(double* h_freq, int rot, double base, int scaling, double factor, double low, double high,
+                        double trained);
+/* x [rows, heads, dim] at positions pos int32 [rows] into y (which may be x); inverse: the transpose, its gradient. dim <= 1024. */
+int uh_rope(const uint16_t* x, int ldx, uint16_t* y, int ldy, const int32_t* pos, int rows, int heads, int dim,
+            const double* freq, int first, int rot, int interleaved, float mscale, int inverse, void* stream);
+/* Each head of q [rows, Hq, dim] and k [rows, Hkv, dim] over its root mean square, times wq / wk bf16 [dim], then rotated, into
+ * qo / ko (which may be q / k). */
+int uh_qk_norm_rope(const uint16_t* q, int ldq, uint16_t* qo, int ldqo, int Hq, const uint16_t* wq, const uint16_t* k, int ldk,
+                    uint16_t* ko, int ldko, int Hkv, const uint16_t* wk, float eps, const int32_t* pos, int rows, int dim,
+                    const double* freq, int first, int rot, int interleaved, float mscale, void* stream);
+
 /* ---- the 8-bit paged key / value cache and its attention (include/unholy/kernels/kv_cache.hpp has the layout and the
  * full contracts; no reference counterpart). One layer: kc e4m3 [pages, Hkv, page, D], vc e4m3 [pages, Hkv, D, page], ks / vs
  * e8m0 [pages, Hkv]; page 16, 32, 64 or 128 tokens, D 64, 128 or 256. table int32 [B, max_blocks] (page numbers, -1: none),
@@ -376,6 +393,14 @@ int uh_mx_moe_forward_noalloc(const uint16_t* x, const float* logits, int T, int
 int uh_kv_append(const uint16_t* k, int ldk, const uint16_t* v, int ldv, const int32_t* cu, int rows, int max_new,
                  const int32_t* lens, const int32_t* table, int max_blocks, int B, uint8_t* kc, uint8_t* vc, uint8_t* ks,
                  uint8_t* vs, int pages, int page, int Hkv, int D, void* stream);
+/* uh_qk_norm_rope of a step's queries (into qo, which may be q) and keys at their rows' positions (wq / wk NULL: no norm) and
+ * uh_kv_append of those keys and of v, in one launch: the same results, bit for bit. Hq 0: keys and values only. rot % 16,
+ * first % 8. */
+int uh_kv_append_rope(const uint16_t* q, int ldq, uint16_t* qo, int ldqo, int Hq, const uint16_t* wq, const uint16_t* k,
+                      int ldk, const uint16_t* wk, float eps, const uint16_t* v, int ldv, const int32_t* cu, int rows,
+                      int max_new, const int32_t* lens, const int32_t* table, int max_blocks, int B, const double* freq,
+                      int first, int rot, int interleaved, float mscale, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs,
+                      int pages, int page, int Hkv, int D, void* stream);
 /* Causal attention of the rows q bf16 [rows, Hq, D] over the cached tokens into out (the same shape): every token up to
  * the row's own, with window > 0 the last `window` of them and the first `sinks` tokens of the sequence. lse (may be NULL)
  * fp32 [rows, Hq]. ws: uh_kv_attend_workspace_size bytes, 16-byte aligned, zeroed before its first call

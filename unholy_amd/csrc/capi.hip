@@ -19,6 +19,7 @@
 #include "unholy/kernels/moe_dispatch.hpp"
 #include "unholy/kernels/mx_moe.hpp"
 #include "unholy/kernels/ref.hpp"
+#include "unholy/kernels/rope.hpp"
 #include "unholy_amd.h"
 #include "mx_internal.hpp"
 
@@ -943,6 +944,37 @@ int uh_mx_moe_forward_noalloc(const uint16_t* x, const float* logits, int T, int
   return uh_mx_moe_forward_ev(x, logits, T, K, E, D, I, tab, limit, ws, kScratchBytes, out, sel, wt, stream, nullptr);
 }
 
+int uh_rope_frequencies(double* h_freq, int rot, double base, int scaling, double factor, double low, double high,
+                        double trained) {
+  return guard([&] {
+    k::rope_frequencies(h_freq, rot, base, static_cast<k::RopeScaling>(scaling), factor, low, high, trained);
+  });
+}
+int uh_rope(const uint16_t* x, int ldx, uint16_t* y, int ldy, const int32_t* pos, int rows, int heads, int dim,
+            const double* freq, int first, int rot, int interleaved, float mscale, int inverse, void* st) {
+  return guard([&] {
+    k::rope(x, ldx, y, ldy, pos, rows, heads, dim, {freq, first, rot, interleaved != 0, mscale}, inverse != 0, S(st));
+  });
+}
+int uh_qk_norm_rope(const uint16_t* q, int ldq, uint16_t* qo, int ldqo, int Hq, const uint16_t* wq, const uint16_t* kx, int ldk,
+                    uint16_t* ko, int ldko, int Hkv, const uint16_t* wk, float eps, const int32_t* pos, int rows, int dim,
+                    const double* freq, int first, int rot, int interleaved, float mscale, void* st) {
+  return guard([&] {
+    k::qk_norm_rope(q, ldq, qo, ldqo, Hq, wq, kx, ldk, ko, ldko, Hkv, wk, eps, pos, rows, dim,
+                    {freq, first, rot, interleaved != 0, mscale}, S(st));
+  });
+}
+
+int uh_kv_append_rope(const uint16_t* q, int ldq, uint16_t* qo, int ldqo, int Hq, const uint16_t* wq, const uint16_t* kx,
+                      int ldk, const uint16_t* wk, float eps, const uint16_t* vx, int ldv, const int32_t* cu, int rows,
+                      int max_new, const int32_t* lens, const int32_t* table, int max_blocks, int B, const double* freq,
+                      int first, int rot, int interleaved, float mscale, uint8_t* kc, uint8_t* vc, uint8_t* ks, uint8_t* vs,
+                      int pages, int page, int Hkv, int D, void* st) {
+  return guard([&] {
+    k::kv_append_rope(q, ldq, qo, ldqo, Hq, wq, kx, ldk, wk, eps, vx, ldv, {cu, lens, table, B, max_blocks, rows, max_new},
+                      {freq, first, rot, interleaved != 0, mscale}, {kc, vc, ks, vs, pages, page, Hkv, D}, S(st));
+  });
+}
 int uh_kv_append(const uint16_t* kx, int ldk, const uint16_t* vx, int ldv, const int32_t* cu, int rows, int max_new,
                  const int32_t* lens, const int32_t* table, int max_blocks, int B, uint8_t* kc, uint8_t* vc, uint8_t* ks,
                  uint8_t* vs, int pages, int page, int Hkv, int D, void* st) {

@@ -4,6 +4,7 @@
 
 #include "kv_internal.hpp"
 #include "numerics.hpp"
+#include "turn.hpp"
 
 namespace unholy::kernels {
 
@@ -49,11 +50,80 @@ __device__ __forceinline__ uint32_t kv_codes4(float a, float b, float c, float d
 // Pieces of 8 channels x 4 tokens that a thread holds; a workgroup of one wave takes steps of few tokens.
 constexpr int pieces_of(int dim, int page, int nt) { return nt == 64 ? 2 : std::max(1, page * dim / 32 / nt); }
 
-template <int D, int PAGE, int NT>
+// What kv_append_rope does besides: the queries, and how queries and keys are normalised (no weights: they are not) and rotated.
+struct AppendTurn {
+  const bf16* q;
+  bf16* qo;
+  const bf16 *wq, *wk;
+  int ldq, ldqo, Hq, row_wgs;  // workgroups of a row
+  float eps;
+  Rope r;
+};
+
+// Eight channels and their partners of a head, in the workgroup's form (D / 16 lanes a head, all of them here together).
+template <int D>
+__device__ __forceinline__ void turn_slot(uint4& a, uint4& b, const turn::Slot& s, const bf16* w, const float2* cs, const Rope& r,
+                                          float eps) {
+  float v[16];
+  turn::unpack<8>(a, v);
+  turn::unpack<8>(b, v + 8);
+  if (w) {
+    float ss = turn::sum_squares<8>(v, 0.0f), ww[16];
+#pragma unroll
+    for (int o = D / 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    turn::unpack<8>(*reinterpret_cast<const uint4*>(w + s.a), ww);
+    turn::unpack<8>(*reinterpret_cast<const uint4*>(w + s.b), ww + 8);
+    turn::scale<8>(v, ww, turn::rms_scale(ss, D, eps));
+  }
+  if (s.turned) turn::rotate<8>(v, cs, r.interleaved, false);
+  a = turn::pack<8>(v);
+  b = turn::pack<8>(v + 8);
+}
+
+// The sequence that has row r of the step, or B: how many end before it.
+__device__ __forceinline__ int seq_of_row(const KvStep& st, int r) {
+  int n = 0;
+  for (int b0 = 0; b0 < st.B; b0 += 64) {
+    const int b = b0 + int(threadIdx.x & 63);
+    n += __popcll(__ballot(b < st.B && st.cu[b + 1] <= r));
+  }
+  return n;
+}
+
+// The queries of a row: workgroup `at` of row_wgs for each.
+template <int D, int NT>
+__device__ __forceinline__ void turn_queries(const KvStep& st, const AppendTurn& t, size_t at) {
+  constexpr int L = D / 16, G = NT / L;
+  __shared__ float2 cs[D / 2];
+  if (at >= size_t(st.rows) * t.row_wgs) return;
+  const int row = int(at / t.row_wgs), tid = threadIdx.x, lane = tid % L, pairs = t.r.rot / 2;
+  const int first = int(at % t.row_wgs) * G + tid / L, step = t.row_wgs * G;
+  const turn::Slot s = turn::slot_of<8>(lane, D, t.r.first, t.r.rot, t.r.interleaved);
+  const int b = seq_of_row(st, row);
+  if (b >= st.B) return;
+  const Seq q = seq_of(st, b);
+  if (row < q.r0 || too_many(st, q)) return;
+  for (int i = tid; i < pairs; i += NT) cs[i] = turn::turn_of(q.first + row - q.r0, t.r.freq[i], t.r.mscale);
+  __syncthreads();
+  for (int h = first; h < t.Hq; h += step) {
+    const bf16* x = t.q + size_t(row) * t.ldq + size_t(h) * D;
+    uint4 va = *reinterpret_cast<const uint4*>(x + s.a), vb = *reinterpret_cast<const uint4*>(x + s.b);
+    turn_slot<D>(va, vb, s, t.wq, cs + lane * 8, t.r, t.eps);
+    bf16* y = t.qo + size_t(row) * t.ldqo + size_t(h) * D;
+    *reinterpret_cast<uint4*>(y + s.a) = va;
+    *reinterpret_cast<uint4*>(y + s.b) = vb;
+  }
+}
+
+// TURN: kv_append_rope's, whose grid has further layers of workgroups for the queries.
+template <int D, int PAGE, int NT, bool TURN>
 __global__ __launch_bounds__(NT) void kv_append_kernel(const bf16* __restrict__ kx, int ldk, const bf16* __restrict__ vx,
-                                                       int ldv, KvStep st, KvCache c, int nblk) {
+                                                       int ldv, KvStep st, KvCache c, int nblk, AppendTurn t) {
   constexpr int CH = D / 8, Q = pieces_of(D, PAGE, NT);
   __shared__ float red[NT / 64];
+  if constexpr (TURN)
+    if (blockIdx.z >= 2)
+      return turn_queries<D, NT>(st, t, (size_t(blockIdx.z - 2) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x);
   const int b = blockIdx.x / nblk, h = blockIdx.y, tid = threadIdx.x;
   const bool values = blockIdx.z != 0;
   const Seq q = seq_of(st, b);
@@ -86,6 +156,16 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(const bf16* __restrict__ 
         if (t >= 0 && t < n) raw[4 * i + e] = *reinterpret_cast<const uint4*>(x + size_t(t) * ld + d);
       }
     }
+  } else if constexpr (TURN) {  // a slot of a head: pieces 2 i and 2 i + 1
+#pragma unroll
+    for (int i = 0; i < 2 * Q; ++i) {
+      const int at = tid + i * NT;
+      if (at >= n * (CH / 2)) continue;
+      const turn::Slot s = turn::slot_of<8>(at % (CH / 2), D, t.r.first, t.r.rot, t.r.interleaved);
+      const bf16* y = x + size_t(at / (CH / 2)) * ld;
+      raw[2 * i] = *reinterpret_cast<const uint4*>(y + s.a);
+      raw[2 * i + 1] = *reinterpret_cast<const uint4*>(y + s.b);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 4 * Q; ++i) {
@@ -98,6 +178,21 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(const bf16* __restrict__ 
   uint8_t* codes = (values ? c.v : c.k) + ph * (size_t(D) * PAGE);
   uint8_t* scale = (values ? c.vs : c.ks) + ph;
   const int old = s0 ? *scale : 0;
+
+  if constexpr (TURN)
+    if (!values) {
+#pragma unroll
+      for (int i = 0; i < 2 * Q; ++i) {
+        const int at = tid + i * NT, token = at / (CH / 2), sl = at % (CH / 2);
+        const turn::Slot s = turn::slot_of<8>(sl, D, t.r.first, t.r.rot, t.r.interleaved);
+        if (i * NT >= n * (CH / 2)) break;  // (a head's lanes are here together, or none)
+        float2 cs[8] = {};
+        if (s.turned && token < n)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) cs[j] = turn::turn_of(p0 + token, t.r.freq[sl * 8 + j], t.r.mscale);
+        turn_slot<D>(raw[2 * i], raw[2 * i + 1], s, t.wk, cs, t.r, t.eps);
+      }
+    }
 
   float am = 0.0f;
   bool odd = false;
@@ -137,6 +232,22 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(const bf16* __restrict__ 
           for (int e = 0; e < 4; ++e)
             if (4 * u + e >= s0 && 4 * u + e < end) y[e] = uint8_t(w >> (8 * e));
         }
+      }
+    }
+  } else if constexpr (TURN) {
+#pragma unroll
+    for (int i = 0; i < 2 * Q; ++i) {
+      const int at = tid + i * NT;
+      if (at >= n * (CH / 2)) continue;
+      const turn::Slot s = turn::slot_of<8>(at % (CH / 2), D, t.r.first, t.r.rot, t.r.interleaved);
+      uint8_t* y = codes + size_t(s0 + at / (CH / 2)) * D;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = half_of(raw[2 * i + e], j);
+        *reinterpret_cast<uint2*>(y + (e ? s.b : s.a)) =
+            make_uint2(kv_codes4(v[0], v[1], v[2], v[3], inv, odd), kv_codes4(v[4], v[5], v[6], v[7], inv, odd));
       }
     }
   } else {
@@ -429,24 +540,33 @@ void check_ws(const char* who, const void* ws, size_t bytes, size_t need) {
 
 }  // namespace
 
-void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& s, const KvCache& c, hipStream_t st) {
-  check_cache("kv_append", c);
-  check_step("kv_append", s);
-  if (s.B == 0 || s.rows == 0 || s.max_new == 0 || s.max_blocks == 0) return;
-  if (!k || !v) throw std::runtime_error("kv_append: null operand");
+// The launch of kv_append, and with t of kv_append_rope.
+template <bool TURN>
+static void append(const char* who, const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& s, const KvCache& c,
+                   AppendTurn t, hipStream_t st) {
+  const auto fail = [&](const char* what) { throw std::runtime_error(std::string(who) + ": " + what); };
+  if (!k || !v) fail("null operand");
   if (int64_t(ldk) < int64_t(c.heads) * c.dim || int64_t(ldv) < int64_t(c.heads) * c.dim || ldk % 8 || ldv % 8)
-    throw std::runtime_error("kv_append: ldk / ldv >= heads * dim, % 8");
-  if (!aligned16(k) || !aligned16(v)) throw std::runtime_error("kv_append: rows not 16-byte aligned");
+    fail("ldk / ldv >= heads * dim, % 8");
+  if (!aligned16(k) || !aligned16(v)) fail("rows not 16-byte aligned");
   const int64_t most = std::min(s.max_new, s.rows);  // (up to 2^31 - 1)
-  const int nblk = int(std::min<int64_t>((most - 1 + c.page - 1) / c.page + 1, s.max_blocks));  // that they can reach
-  if (int64_t(s.B) * nblk > INT32_MAX) throw std::runtime_error("kv_append: B * blocks past 31 bits");
-  const dim3 grid(unsigned(s.B) * unsigned(nblk), unsigned(c.heads), 2);
+  const int reach = int(std::min<int64_t>((most - 1 + c.page - 1) / c.page + 1, s.max_blocks));
+  const int nblk = std::max(reach, 1);  // blocks that they can reach (none: the queries' workgroups are laid out by it all the same)
+  if (int64_t(s.B) * nblk > INT32_MAX) fail("B * blocks past 31 bits");
+  dim3 grid(unsigned(s.B) * unsigned(nblk), unsigned(c.heads), 2);
   // A wave holds 128 pieces of 8 channels x 4 tokens: enough for `most` tokens, wherever they begin, or a workgroup of four
   // (64 sequences of one token in eight layers: 50 us by waves, 59 by workgroups)
   const bool few = ((most + 2) / 4 + 1) * (c.dim / 8) <= 64 * pieces_of(c.dim, c.page, 64);
+  if constexpr (TURN) {
+    const int heads = (few ? 64 : 256) / (c.dim / 16);  // of a workgroup at a time
+    t.row_wgs = few ? int(cdiv(t.Hq, heads)) : 1;
+    const size_t layer = size_t(grid.x) * grid.y, wgs = t.Hq ? size_t(s.rows) * t.row_wgs : 0;
+    if ((wgs + layer - 1) / layer > 65533) fail("rows past what a launch takes");
+    grid.z += unsigned((wgs + layer - 1) / layer);
+  }
   const auto go = [&]<int D, int PAGE>() {
-    if (few) kv_append_kernel<D, PAGE, 64><<<grid, 64, 0, st>>>(k, ldk, v, ldv, s, c, nblk);
-    else kv_append_kernel<D, PAGE, 256><<<grid, 256, 0, st>>>(k, ldk, v, ldv, s, c, nblk);
+    if (few) kv_append_kernel<D, PAGE, 64, TURN><<<grid, 64, 0, st>>>(k, ldk, v, ldv, s, c, nblk, t);
+    else kv_append_kernel<D, PAGE, 256, TURN><<<grid, 256, 0, st>>>(k, ldk, v, ldv, s, c, nblk, t);
   };
   const auto by_page = [&]<int D>() {
     switch (c.page) {
@@ -460,6 +580,35 @@ void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& s, 
   else if (c.dim == 128) by_page.template operator()<128>();
   else by_page.template operator()<256>();
   UH_CHECK_LAUNCH();
+}
+
+void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& s, const KvCache& c, hipStream_t st) {
+  check_cache("kv_append", c);
+  check_step("kv_append", s);
+  if (s.B == 0 || s.rows == 0 || s.max_new == 0 || s.max_blocks == 0) return;
+  append<false>("kv_append", k, ldk, v, ldv, s, c, AppendTurn{}, st);
+}
+
+void kv_append_rope(const bf16* q, int ldq, bf16* qo, int ldqo, int Hq, const bf16* wq, const bf16* k, int ldk, const bf16* wk,
+                    float eps, const bf16* v, int ldv, const KvStep& s, const Rope& r, const KvCache& c, hipStream_t st) {
+  const char* who = "kv_append_rope";
+  const auto fail = [&](const char* what) { throw std::runtime_error(std::string(who) + ": " + what); };
+  check_cache(who, c);
+  check_step(who, s);
+  turn::check_rope(who, r, c.dim);
+  if (r.rot % 16 || r.first % 8) fail("rot % 16, first % 8 (qk_norm_rope and kv_append take others)");
+  if (Hq < 0 || Hq > 65535) fail("Hq must be in [0, 65535]");
+  if (!(eps >= 0.0f) || eps - eps != 0.0f) fail("eps must be finite and not negative");
+  if (s.B == 0 || s.rows == 0 || s.max_new == 0) return;
+  if (Hq) {
+    if (!q || !qo) fail("null operand");
+    const int64_t width = int64_t(Hq) * c.dim;
+    if (ldq < width || ldqo < width || ldq % 8 || ldqo % 8) fail("ldq / ldqo >= Hq * dim, % 8");
+    if (!aligned16(q) || !aligned16(qo)) fail("rows not 16-byte aligned");
+    if (q == qo && ldq != ldqo) fail("in place with two strides");
+  }
+  if (!aligned16(wq) || !aligned16(wk)) fail("weights not 16-byte aligned");
+  append<true>(who, k, ldk, v, ldv, s, c, AppendTurn{q, qo, wq, wk, ldq, ldqo, Hq, 0, eps, r}, st);
 }
 
 size_t kv_pages_workspace(int B, int pages) { return B < 0 || pages < 0 ? 0 : carve_pages(nullptr, B, pages).bytes; }

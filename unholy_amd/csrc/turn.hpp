@@ -1,0 +1,126 @@
+// Heads as the kernels that rotate them hold them: slots of twice V channels, which a lane reads, normalises and rotates by
+// itself.
+#pragma once
+
+#include "common.hpp"
+#include "numerics.hpp"
+#include "unholy/kernels/rope.hpp"
+
+namespace unholy::kernels::turn {
+
+using namespace uh;
+
+// V values of bf16, as one load.
+template <int V>
+struct Raw;
+template <>
+struct Raw<8> { using type = uint4; };
+template <>
+struct Raw<4> { using type = uint2; };
+template <>
+struct Raw<2> { using type = uint32_t; };
+template <>
+struct Raw<1> { using type = uint16_t; };
+template <int V>
+using raw_t = typename Raw<V>::type;
+
+template <int V>
+__device__ __forceinline__ void unpack(const raw_t<V>& x, float* v) {
+  if constexpr (V == 1) {
+    v[0] = bf16_to_f32(x);
+  } else {
+    uint32_t w[V / 2];
+    __builtin_memcpy(w, &x, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ raw_t<V> pack(const float* v) {
+  if constexpr (V == 1) {
+    return f32_to_bf16(v[0]);
+  } else {
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) w[i] = uint32_t(f32_to_bf16(v[2 * i])) | uint32_t(f32_to_bf16(v[2 * i + 1])) << 16;
+    raw_t<V> x;
+    __builtin_memcpy(&x, w, sizeof(w));
+    return x;
+  }
+}
+
+// A head's slots: first those of the rotated part, each V pairs (pair V s + j of slot s: halves: channel j of both pieces;
+// interleaved: channels 2j and 2j + 1 of the two pieces side by side), then the other channels, two pieces a slot, of which the
+// last may be alone. rot % 2V, first % V and dim % V are 0.
+struct Slot {
+  int a, b;  // the first channels of its pieces; b < 0: none
+  bool turned;
+};
+template <int V>
+__host__ __device__ __forceinline__ int slots_of(int dim, int rot) {
+  return rot / (2 * V) + (dim - rot + 2 * V - 1) / (2 * V);
+}
+template <int V>
+__device__ __forceinline__ Slot slot_of(int s, int dim, int first, int rot, bool interleaved) {
+  const int turned = rot / (2 * V);
+  if (s < turned) return interleaved ? Slot{first + 2 * V * s, first + 2 * V * s + V, true} : Slot{first + V * s, first + rot / 2 + V * s, true};
+  const int u = 2 * V * (s - turned), w = u + V;  // of the channels that are not rotated
+  return Slot{u < first ? u : u + rot, w >= dim - rot ? -1 : w < first ? w : w + rot, false};
+}
+
+// The two products of a rotation: (cos, sin) of pos * freq, times mscale. The angle in turns: 64 bits, whole turns cut off, what is
+// left of one (at most a half) rounded to fp32, which is off by 2^-25 turns, 2e-7 radians.
+__device__ __forceinline__ float2 turn_of(int pos, double freq, float mscale) {
+  constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
+  const double t = double(pos) * (freq * kTurn);
+  float s, c;
+  sincospif(2.0f * float(t - rint(t)), &s, &c);
+  return make_float2(c * mscale, s * mscale);
+}
+
+// The slot's V pairs rotated; cs: (cos, sin) of each. v: the two pieces one after the other.
+template <int V>
+__device__ __forceinline__ void rotate(float (&v)[2 * V], const float2* cs, bool interleaved, bool inverse) {
+#pragma clang fp contract(off)  // (each product and sum as written: every kernel that rotates rounds alike)
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float c = cs[j].x, s = inverse ? -cs[j].y : cs[j].y;
+    float& a = interleaved ? v[2 * j] : v[j];
+    float& b = interleaved ? v[2 * j + 1] : v[V + j];
+    const float x = a, y = b;
+    a = __builtin_fmaf(x, c, -(y * s));
+    b = __builtin_fmaf(x, s, y * c);
+  }
+}
+
+// 1 / root of the mean square of a head whose channels' squares sum to ss.
+__device__ __forceinline__ float rms_scale(float ss, int dim, float eps) {
+#pragma clang fp contract(off)
+  return 1.0f / sqrtf(ss / float(dim) + eps);
+}
+template <int V>
+__device__ __forceinline__ float sum_squares(const float (&v)[2 * V], float ss) {
+#pragma unroll
+  for (int j = 0; j < 2 * V; ++j) ss = __builtin_fmaf(v[j], v[j], ss);
+  return ss;
+}
+template <int V>
+__device__ __forceinline__ void scale(float (&v)[2 * V], const float (&w)[2 * V], float r) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int j = 0; j < 2 * V; ++j) v[j] = w[j] * (v[j] * r);
+}
+
+// Argument checks of every entry that rotates.
+inline void check_rope(const char* who, const Rope& r, int dim) {
+  const auto fail = [&](const char* what) { throw std::runtime_error(std::string(who) + ": " + what); };
+  if (r.rot < 0 || r.rot % 2 || r.first < 0 || r.first > dim || r.rot > dim - r.first) fail("rot even, first + rot <= dim");
+  if (!(r.mscale - r.mscale == 0.0f)) fail("mscale is not finite");
+  if (r.rot && !r.freq) fail("null frequencies");
+  if (reinterpret_cast<uintptr_t>(r.freq) % 8) fail("frequencies not 8-byte aligned");
+}
+
+}  // namespace unholy::kernels::turn
