@@ -410,6 +410,20 @@ int uh_kv_attend(const uint16_t* q, int ldq, const int32_t* cu, int rows, int ma
                  const int32_t* table, int max_blocks, int B, const uint8_t* kc, const uint8_t* vc, const uint8_t* ks,
                  const uint8_t* vs, int pages, int page, int Hq, int Hkv, int D, float scale, int window, int sinks,
                  uint16_t* out, int ldo, float* lse, void* ws, size_t ws_bytes, void* stream);
+/* Sequences whose tables begin with the same pages: uh_kv_share finds them on the device, once for the layers of a step, and
+ * uh_kv_attend_shared is uh_kv_attend with that plan, which reads those pages once for all rows of a group (the same results but
+ * for the order of sums). group int32 [B] (may be NULL: those with the same first page): sequences with the same number in
+ * [0, B) may be taken together, -1: alone. plan: uh_kv_share_plan_size bytes, 16-byte aligned. ws:
+ * uh_kv_attend_shared_workspace_size bytes, as uh_kv_attend's. */
+size_t uh_kv_share_plan_size(int B, int rows);
+int uh_kv_share(const int32_t* group, const int32_t* cu, int rows, int max_new, const int32_t* lens, const int32_t* table,
+                int max_blocks, int B, int pages, int page, void* plan, size_t plan_bytes, void* stream);
+size_t uh_kv_attend_shared_workspace_size(int rows, int max_new, int B, int Hq, int Hkv, int D);
+int uh_kv_attend_shared(const uint16_t* q, int ldq, const int32_t* cu, int rows, int max_new, const int32_t* lens,
+                        const int32_t* table, int max_blocks, int B, const uint8_t* kc, const uint8_t* vc, const uint8_t* ks,
+                        const uint8_t* vs, int pages, int page, int Hq, int Hkv, int D, float scale, int window, int sinks,
+                        uint16_t* out, int ldo, float* lse, const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes,
+                        void* stream);
 /* Pages, on the device: refs int32 [pages] counts the table entries that name a page (0: free); the caches here are all
  * layers' [layers, pages, ...]. reserve: pages for the next grow[b] tokens, lens[b] += grow[b], a shared last page that is
  * not full copied first; ok[b] 0: untouched, no pages left. fork: empty slot b becomes a fork of sequence from[b] (-1:

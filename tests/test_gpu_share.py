@@ -1,0 +1,391 @@
+"""Attention of sequences that begin alike on the GPU: the plan against a plain restatement, the attention against the 64-bit
+reference within the bounds that hold for kv_attend (its products and roundings are the same; sums join in another order)."""
+import numpy as np
+import pytest
+
+from tests import kv_ref
+from tests.helpers import from_bf16, randn_bf16
+from tests.test_gpu_kv import Cache, Pool, attend, dev
+from unholy_amd import call
+from unholy_amd.device import DeviceBuffer, Graph, Stream, synchronize
+
+pytestmark = pytest.mark.gpu
+
+GUARD = 0xA5
+
+
+def step_of(rng, groups, alone, Hkv, D, page, n=1, order=None, spare_rows=0):
+    """A step of groups [(tokens that begin alike, [further tokens of each])] and sequences alone [tokens], n rows each (or a list
+    in the order of the sequences), in slots by `order`; and each slot's group (-1: alone)."""
+    ctx = [p + o for p, own in groups for o in own] + list(alone)
+    label = [g for g, (_, own) in enumerate(groups) for _ in own] + [-1] * len(alone)
+    ns = [n] * len(ctx) if isinstance(n, int) else list(n)
+    order = np.arange(len(ctx)) if order is None else np.asarray(order)
+    s = kv_ref.Step(rng, [ns[i] for i in order], [ctx[i] for i in order], Hkv, D, page, spare_rows=spare_rows)
+    label = np.array([label[i] for i in order], np.int32)
+    for g, (p, _) in enumerate(groups):
+        slots = np.flatnonzero(label == g)
+        s.table[slots, :p // page] = s.table[slots[0], :p // page]
+    return s, label
+
+
+def share_ref(s, group=None, max_new=None):
+    """tiles of each sequence, and the groups as [(tiles, slots)]."""
+    most = max(s.n + [0]) if max_new is None else max_new
+    limit = [min(max(int(s.lens[b]) - s.n[b], 0) // s.page, s.max_blocks) for b in range(s.B)]
+    classes = {}
+    for b in range(s.B):
+        key = int(s.table[b, 0]) if group is None else int(group[b])
+        ok = 0 <= key < (s.pages if group is None else s.B) and 1 <= s.n[b] <= min(16, most) and limit[b] * s.page >= 64
+        if ok:
+            classes.setdefault(key, []).append(b)
+    tiles, groups = np.zeros(s.B, int), []
+    for slots in classes.values():
+        r, long = slots[0], {}
+        for b in slots:
+            k = 0
+            while k < min(limit[b], limit[r]) and s.table[b, k] == s.table[r, k] and 0 <= s.table[b, k] < s.pages:
+                k += 1
+            long[b] = k * s.page // 64
+        saved, t = max(((sum(x >= t for x in long.values()) - 1) * t, t) for t in long.values())
+        if saved > 0:
+            groups.append((t, [b for b in slots if long[b] >= t]))
+    for t, slots in groups:
+        tiles[slots] = t
+    return tiles, sorted(groups, key=lambda g: g[1][0])
+
+
+def plan_of(c, group=None, most=None, stream=None):
+    s = c.step
+    most = max(s.n + [0]) if most is None else most
+    need = call("uh_kv_share_plan_size", s.B, s.rows)
+    plan = dev(np.full(need + 64, GUARD, np.uint8))
+    g = None if group is None else dev(np.asarray(group, np.int32))
+    call("uh_kv_share", g, c.cu, s.rows, most, c.lens, c.table, s.max_blocks, s.B, s.pages, s.page, plan, need, stream)
+    synchronize()
+    assert (plan.download(need + 64, np.uint8)[need:] == GUARD).all()
+    return plan, need
+
+
+def check_plan(c, plan, group=None, most=None):
+    s = c.step
+    got = plan.download(16 + 4 * s.B, np.int32)
+    tiles, groups = share_ref(s, group, most)
+    head, seqs = got[:16], got[16:].reshape(s.B, 4)
+    assert head[1:6].tolist() == [s.B, s.rows, max(s.n + [0]) if most is None else most, s.max_blocks, s.page]
+    assert seqs[:, 0].tolist() == tiles.tolist()
+    assert head[6:8].tolist() == [len(groups), sum(s.n[b] for _, slots in groups for b in slots)]
+    row0 = 0
+    for g, (_, slots) in enumerate(groups):
+        at = 0
+        for b in slots:
+            assert seqs[b].tolist()[1:] == [at, row0, g]
+            at += s.n[b]
+        row0 += at
+    return tiles, groups
+
+
+def shared(c, q, Hq, scale, plan, need_plan, window=0, sinks=0, pad=0, most=None, stream=None, lse=True, ws=None):
+    s = c.step
+    rows, width = q.shape[0], Hq * s.D
+    ld, most = width + pad, max(s.n + [0]) if most is None else most
+    x = np.full((rows, ld), 0x7FC0, np.uint16)
+    x[:, :width] = q.reshape(rows, width)
+    dq, out = dev(x), dev(np.full((rows, ld), 0x7FC1, np.uint16))
+    dl = dev(np.full((rows, Hq), np.nan, np.float32))
+    need = call("uh_kv_attend_shared_workspace_size", rows, most, s.B, Hq, s.Hkv, s.D)
+    if ws is None:
+        ws = DeviceBuffer(need + 64)
+        ws.zero()
+        call("uh_memcpy_h2d", ws.ptr + need, np.full(64, GUARD, np.uint8).ctypes.data, 64)
+    call("uh_kv_attend_shared", dq, ld, c.cu, rows, most, c.lens, c.table, s.max_blocks, s.B, *c.arrays(), s.pages, s.page, Hq,
+         s.Hkv, s.D, scale, window, sinks, out, ld, dl if lse else None, plan, need_plan, ws, need, stream)
+    synchronize()
+    assert (ws.download(64, np.uint8, need) == GUARD).all()
+    got = out.download((rows, ld), np.uint16)
+    assert (got[:, width:] == 0x7FC1).all()
+    return got[:, :width].reshape(rows, Hq, s.D), dl.download((rows, Hq), np.float32)
+
+
+def check(s, Hq, group=None, window=0, sinks=0, pad=0, scale=None, qscale=1.0, most=None, seed=1, expect=None, gone=()):
+    """gone: sequences with more rows than the launch is sized for."""
+    c, scale = Cache(s), s.D ** -0.5 if scale is None else scale
+    plan, need = plan_of(c, group, most)
+    _, groups = check_plan(c, plan, group, most)
+    if expect is not None:
+        assert len(groups) == expect
+    q = randn_bf16(np.random.default_rng(seed), (s.rows, Hq, s.D), qscale)
+    got, lse = shared(c, q, Hq, scale, plan, need, window, sinks, pad, most)
+    ref, rlse, tol, ltol = kv_ref.attend(s, from_bf16(q).astype(np.float64), Hq, scale, window, sinks)
+    for b in gone:
+        r = slice(int(s.cu[b]), int(s.cu[b + 1]))
+        ref[r], rlse[r], tol[r], ltol[r] = 0.0, -np.inf, 0.0, 0.0
+    untouched = np.ones(s.rows, bool)
+    untouched[:s.cu[-1]] = False
+    assert (got[untouched] == 0x7FC1).all() and np.isnan(lse[untouched]).all()
+    out, ref, rlse, tol, ltol = (x[~untouched] for x in (from_bf16(got).astype(np.float64), ref, rlse, tol, ltol))
+    lse = lse[~untouched]
+    assert np.array_equal(np.isnan(out), np.isnan(ref)) and np.array_equal(np.isnan(lse), np.isnan(rlse))
+    fine, near = ~np.isnan(ref), np.isfinite(rlse)
+    err = np.abs(out - ref)[fine]
+    print(f"shared rows={s.rows} worst error {np.max(err / np.maximum(tol[fine], 1e-30), initial=0):.3f} of bound")
+    assert (err <= tol[fine]).all()
+    assert (np.isneginf(lse) == np.isneginf(rlse)).all()
+    assert (np.abs(lse[near] - rlse[near]) <= ltol[near]).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("Hq,Hkv", [(2, 2), (8, 1), (6, 2)])
+def test_decode(D, page, Hq, Hkv):
+    """A group, one more, and sequences that share nothing."""
+    rng = np.random.default_rng(D + page + Hq)
+    s, label = step_of(rng, [(300, [0, 1, 65, 40]), (128, [10, 200])], [0, 5, 700], Hkv, D, page, order=rng.permutation(9))
+    check(s, Hq, expect=2)
+    check(s, Hq, label, expect=2)
+
+
+@pytest.mark.parametrize("n", [2, 5, 16])
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(8, 1, 64, 16), (16, 1, 128, 64), (6, 2, 128, 32), (4, 2, 256, 128), (1, 1, 64, 64)])
+def test_drafts(n, Hq, Hkv, D, page):
+    """Several rows a sequence: parts of 16 of them, blocks of 128 that end inside a sequence."""
+    rng = np.random.default_rng(n + Hq)
+    s, _ = step_of(rng, [(400, [3, 90, 0, 17, 64])], [33], Hkv, D, page, n=n, spare_rows=3)
+    check(s, Hq, expect=1, pad=8)
+
+
+@pytest.mark.parametrize("n", [[1, 16, 17, 3, 1, 40], [5, 0, 1, 2, 0, 1], [200, 1, 1, 1, 1, 1], [17, 300, 20, 18, 30, 19]])
+def test_steps_of_many_kinds(n):
+    """Sequences with more than 16 rows, or none, among the others: they are in no group."""
+    rng = np.random.default_rng(sum(n))
+    s, label = step_of(rng, [(200, [5, 60, 9, 100])], [70, 0], 2, 64, 16, n=n, spare_rows=4)
+    check(s, 6)
+    check(s, 6, label, most=max(n) + 5)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (64, 4), (100, 70), (150, 0), (400, 64), (5000, 3), (2 ** 31 - 1, 0), (90, 2 ** 31 - 1)])
+@pytest.mark.parametrize("D,page,n", [(64, 16, 1), (128, 64, 3)])
+def test_window_and_sinks(window, sinks, D, page, n):
+    rng = np.random.default_rng(window % 1000 + sinks % 1000)
+    s, _ = step_of(rng, [(330, [0, 40, 90, 300]), (128, [2, 5])], [450], 2, D, page, n=n)
+    check(s, 4, window=window, sinks=sinks, expect=2)
+
+
+@pytest.mark.parametrize("scale,qscale", [(0.0, 1.0), (-0.1, 1.0), (1.0, 8.0), (30.0, 1.0)])
+def test_scales(scale, qscale):
+    rng = np.random.default_rng(9)
+    s, _ = step_of(rng, [(200, [5, 60, 9])], [70], 2, 64, 32, n=2)
+    check(s, 4, scale=scale, qscale=qscale, expect=1)
+
+
+@pytest.mark.parametrize("each,Hq", [(40, 4), (33, 8), (70, 16)])
+def test_blocks_of_rows(each, Hq):
+    """More rows than one block, the last of them not full."""
+    rng = np.random.default_rng(each)
+    s, _ = step_of(rng, [(256, [int(x) for x in rng.integers(0, 30, each)])], [], 1, 64, 64)
+    check(s, Hq, expect=1)
+
+
+@pytest.mark.parametrize("groups,each", [(70, 2), (3, 50), (130, 3)])
+def test_more_sequences_than_lanes(groups, each):
+    rng = np.random.default_rng(groups)
+    s, label = step_of(rng, [(64 + 16 * int(rng.integers(0, 6)), rng.integers(0, 20, each).tolist()) for _ in range(groups)], [10, 100],
+                       1, 64, 16, order=rng.permutation(groups * each + 2))
+    check(s, 2, expect=groups)
+    check(s, 2, label, expect=groups)
+
+
+def test_a_block_of_a_group_for_every_workgroup():
+    """More blocks than the chip has places: none is cut."""
+    rng = np.random.default_rng(70)
+    s, _ = step_of(rng, [(64, [1, 2])] * 20, [], 32, 64, 64)
+    check(s, 32, expect=20)
+
+
+@pytest.mark.parametrize("D,parts", [(64, 9000), (128, 5000), (256, 3000)])
+def test_long_common_parts(D, parts):
+    """Contexts that are split over many workgroups, in two forms."""
+    rng = np.random.default_rng(D)
+    s, _ = step_of(rng, [(parts, [7, 700, 0])], [1500], 1, D, 64)
+    check(s, 4, expect=1)
+
+
+def test_the_plan_takes_what_saves_most():
+    """Three begin alike for long, six for a little: of 5 x 2 tiles and 2 x 9 the second; and with numbers that say so, both."""
+    rng = np.random.default_rng(3)
+    s, label = step_of(rng, [(640, [0, 5, 9]), (128, [300, 2, 70])], [], 1, 64, 64)
+    s.table[3:, :2] = s.table[0, :2]
+    plan = plan_of(Cache(s))[0]
+    assert check_plan(Cache(s), plan)[1] == [(10, [0, 1, 2])]
+    check(s, 2, expect=1)
+    check(s, 2, label, expect=2)
+    check(s, 2, [0, 1, 2, 3, 4, 5], expect=0)  # nobody with anybody
+    check(s, 2, [0, 0, 9, -5, 6, 2 ** 31 - 1], expect=1)  # numbers out of range: alone
+    check(s, 2, [4] * 6, expect=1)
+
+
+def test_pages_that_are_missing_or_differ():
+    """The common part ends where tables have no page, or not the same one."""
+    rng = np.random.default_rng(4)
+    s, label = step_of(rng, [(640, [0, 5, 9, 33])], [], 1, 64, 16)
+    s.table[:, 25] = -1
+    check(s, 2, expect=1)
+    s.table[2, 13] = s.table[2, 39]
+    check(s, 2, label, expect=1)
+    s.table[:, 0] = s.pages + 3
+    check(s, 2, label, expect=0)
+    s.table[:] = -1
+    check(s, 2, label, expect=0)
+
+
+def test_lengths_that_end_the_common_part():
+    """No tile of which a new row is a token, or comes before it, is common; nothing past the table is."""
+    rng = np.random.default_rng(5)
+    s, _ = step_of(rng, [(200, [0, 0, 0])], [], 1, 64, 16)
+    s.table[1:] = s.table[0]  # the new tokens' page too
+    for lens in ([201, 193, 129], [64, 65, 66], [1, 0, 200], [129, 129, 129], [500, 500, 500]):
+        s.lens = np.array(lens, np.int32)
+        check(s, 2)
+
+
+@pytest.mark.parametrize("most", [4, 16])
+def test_more_rows_than_the_launch_is_sized_for(most):
+    rng = np.random.default_rng(6)
+    n = [1, most + 1, 2, 3]
+    s, label = step_of(rng, [(150, [0, 4, 8, 70])], [], 2, 64, 16, n=n, spare_rows=2)
+    check(s, 4, label, most=most, expect=1, gone=[1])
+
+
+def test_nan_reaches_the_rows_that_see_it():
+    """A NaN in a common value: that channel of every row of the group; in a common key: every row; under a window, the rows
+    that still see it. What follows the last tokens is NaN throughout."""
+    rng = np.random.default_rng(7)
+    s, _ = step_of(rng, [(256, [3, 60, 100])], [90], 2, 64, 64)
+    for b in range(s.B):
+        for t in range(int(s.lens[b]), -(-int(s.lens[b]) // 64) * 64):
+            s.k[s.table[b, t // 64], :, t % 64] = 0xFF
+            s.v[s.table[b, t // 64], :, :, t % 64] = 0x7F
+    check(s, 4, expect=1)
+    s.v[s.table[0, 1], 0, 5, 9] = 0x7F  # token 73
+    s.k[s.table[0, 2], 1, 3, 7] = 0xFF  # token 131
+    c = Cache(s)
+    plan, need = plan_of(c)
+    q = randn_bf16(rng, (s.rows, 4, 64))
+    for window in (0, 240):
+        got = np.isnan(from_bf16(shared(c, q, 4, 0.1, plan, need, window)[0]))
+        want = np.isnan(from_bf16(attend(c, q, 4, 0.1, window)[0]))
+        assert np.array_equal(got, want) and got[0, 0, 5] and got[0, 2:].all()
+
+
+def test_scales_that_are_no_number():
+    rng = np.random.default_rng(8)
+    s, _ = step_of(rng, [(256, [3, 60, 100])], [90], 2, 64, 64)
+    s.ks[s.table[0, 1], 0] = s.vs[s.table[0, 2], 1] = 255
+    c = Cache(s)
+    plan, need = plan_of(c)
+    q = randn_bf16(rng, (s.rows, 4, 64))
+    for window in (0, 150, 20):
+        got, want = (np.isnan(from_bf16(x[0])) for x in (shared(c, q, 4, 0.1, plan, need, window), attend(c, q, 4, 0.1, window)))
+        assert np.array_equal(got, want)
+
+
+def test_a_plan_of_other_sizes_is_not_used():
+    """Of a step with another number of rows, sequences or blocks, or of no step: every sequence reads its own."""
+    rng = np.random.default_rng(10)
+    s, _ = step_of(rng, [(300, [3, 60, 100])], [90], 2, 64, 64, n=2)
+    t, _ = step_of(rng, [(300, [3, 60, 100])], [90, 5], 2, 64, 64, n=1)
+    c, q = Cache(s), randn_bf16(rng, (s.rows, 4, 64))
+    ref, _, tol, _ = kv_ref.attend(s, from_bf16(q).astype(np.float64), 4, 0.1)
+    need = call("uh_kv_share_plan_size", s.B, s.rows)
+    other, size = plan_of(Cache(t))
+    for plan, n in ((other, max(size, need)), (dev(np.zeros(need, np.uint8)), need), (dev(np.full(need, 0xFF, np.uint8)), need)):
+        if plan.nbytes < n:
+            continue
+        got, _ = shared(c, q, 4, 0.1, plan, n)
+        assert (np.abs(from_bf16(got) - ref) <= tol).all()
+
+
+def test_the_same_every_time_and_without_lse():
+    rng = np.random.default_rng(11)
+    s, _ = step_of(rng, [(2000, [3, 700, 100, 0])], [900], 2, 128, 64)
+    c, q = Cache(s), randn_bf16(rng, (s.rows, 8, 128))
+    plan, need = plan_of(c)
+    first, lse = shared(c, q, 8, 0.1, plan, need)
+    for _ in range(3):
+        again, l2 = shared(c, q, 8, 0.1, plan, need)
+        assert np.array_equal(first, again) and np.array_equal(lse, l2)
+    assert np.array_equal(first, shared(c, q, 8, 0.1, plan, need, lse=False)[0])
+
+
+def test_one_sequence():
+    rng = np.random.default_rng(12)
+    check(kv_ref.Step(rng, [1], [300], 1, 64, 16), 4, expect=0)
+    check(kv_ref.Step(rng, [20], [300], 1, 64, 16), 4, expect=0)
+
+
+def test_captured_steps_replay_with_other_tables():
+    """The plan and two layers captured once, replayed with other rows, lengths and tables, eager work between; one workspace."""
+    rng = np.random.default_rng(13)
+    st, Hq, B, rows = Stream(), 8, 6, 8
+    steps = []
+    for groups, alone, n in (([(300, [0, 9, 40, 100])], [7, 200], [1, 1, 2, 1, 2, 1]), ([(128, [5, 5]), (400, [1, 2, 3])], [50], 1),
+                             ([], [300, 0, 10, 500, 64, 70], 1), ([(450, [0, 1, 2, 3, 4, 5])], [], [2, 1, 1, 2, 1, 1])):
+        s, _ = step_of(rng, groups, alone, 2, 128, 64, n=n)
+        s.rows = rows
+        steps.append(s)
+    width, pages = max(s.max_blocks for s in steps), max(s.pages for s in steps)
+    for s in steps:
+        s.table = np.concatenate([s.table, np.full((B, width - s.max_blocks), -1, np.int32)], 1)
+        extra = pages - s.pages
+        s.k, s.v, s.ks, s.vs = (np.concatenate([x, np.zeros((extra,) + x.shape[1:], np.uint8)]) for x in (s.k, s.v, s.ks, s.vs))
+        s.max_blocks, s.pages = width, pages
+    c = Cache(steps[0])
+    need_p = call("uh_kv_share_plan_size", B, rows)
+    need = call("uh_kv_attend_shared_workspace_size", rows, 2, B, Hq, 2, 128)
+    plan, ws = dev(np.zeros(need_p, np.uint8)), dev(np.zeros(need, np.uint8))
+    q, out = [dev(np.zeros((rows, Hq, 128), np.uint16)) for _ in range(2)], [dev(np.zeros((rows, Hq, 128), np.uint16)) for _ in range(2)]
+
+    def work():
+        call("uh_kv_share", None, c.cu, rows, 2, c.lens, c.table, width, B, pages, 64, plan, need_p, st.handle)
+        for a, b in zip(q, out):
+            call("uh_kv_attend_shared", a, Hq * 128, c.cu, rows, 2, c.lens, c.table, width, B, *c.arrays(), pages, 64, Hq, 2, 128,
+                 0.09, 0, 0, b, Hq * 128, None, plan, need_p, ws, need, st.handle)
+
+    g = Graph(st, work)
+    for s in steps + steps[:2]:
+        for buf, a in zip((c.k, c.v, c.ks, c.vs, c.cu, c.lens, c.table), (s.k, s.v, s.ks, s.vs, s.cu, s.lens, s.table)):
+            buf.upload(a)
+        x = [randn_bf16(rng, (rows, Hq, 128)) for _ in range(2)]
+        for a, b, o in zip(q, x, out):
+            a.upload(b)
+            o.upload(np.full((rows, Hq, 128), 0x7FC1, np.uint16))
+        synchronize()
+        g.launch()
+        st.synchronize()
+        c.step = s
+        used = int(s.cu[-1])
+        for b, o in zip(x, out):
+            got = o.download((rows, Hq, 128), np.uint16)
+            ref, _, tol, _ = kv_ref.attend(s, from_bf16(b).astype(np.float64), Hq, 0.09)
+            assert (np.abs(from_bf16(got[:used]) - ref[:used]) <= tol[:used]).all() and (got[used:] == 0x7FC1).all()
+        eager = plan_of(c, most=2)
+        shared(c, x[0], Hq, 0.09, *eager, most=2)
+
+
+def test_after_forks():
+    """As an engine makes them: prompts, forks of them, pages for the next tokens, then the plan by the forks' sources."""
+    rng = np.random.default_rng(14)
+    page, Hkv, Hq, D, B = 16, 2, 8, 64, 7
+    p = Pool(rng, [200, 0, 0, 0, 90, 0, 40], 80, page, 20, layers=1, Hkv=Hkv, D=D)
+    p.fork([-1, 0, 0, 0, -1, 4, -1])
+    assert p.reserve([1, 2, 1, 1, 1, 1, 1]).all()
+    s = kv_ref.Step.__new__(kv_ref.Step)
+    s.n, s.B, s.Hkv, s.D, s.page, s.pages = [1, 2, 1, 1, 1, 1, 1], B, Hkv, D, page, p.pages
+    s.lens, s.table, s.max_blocks = p.lens, p.table, p.table.shape[1]
+    s.cu = np.concatenate(([0], np.cumsum(s.n))).astype(np.int32)
+    s.rows = int(s.cu[-1])
+    shapes = ((p.pages, Hkv, page, D), (p.pages, Hkv, D, page))
+    s.k, s.v = (kv_ref.encode(rng.standard_normal(x) * 64) for x in shapes)
+    s.ks, s.vs = (rng.integers(118, 124, (p.pages, Hkv), dtype=np.uint8) for _ in range(2))
+    check(s, Hq, [0, 0, 0, 0, 4, 4, 6], expect=2)
+    check(s, Hq, expect=2)

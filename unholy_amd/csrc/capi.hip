@@ -997,6 +997,28 @@ int uh_kv_attend(const uint16_t* q, int ldq, const int32_t* cu, int rows, int ma
                  ws_bytes, S(st));
   });
 }
+size_t uh_kv_share_plan_size(int B, int rows) { return k::kv_share_plan(B, rows); }
+int uh_kv_share(const int32_t* group, const int32_t* cu, int rows, int max_new, const int32_t* lens, const int32_t* table,
+                int max_blocks, int B, int pages, int page, void* plan, size_t plan_bytes, void* st) {
+  return guard([&] {
+    k::kv_share(group, {cu, lens, table, B, max_blocks, rows, max_new}, pages, page, plan, plan_bytes, S(st));
+  });
+}
+size_t uh_kv_attend_shared_workspace_size(int rows, int max_new, int B, int Hq, int Hkv, int D) {
+  return k::kv_attend_shared_workspace(rows, max_new, B, Hq, Hkv, D);
+}
+int uh_kv_attend_shared(const uint16_t* q, int ldq, const int32_t* cu, int rows, int max_new, const int32_t* lens,
+                        const int32_t* table, int max_blocks, int B, const uint8_t* kc, const uint8_t* vc, const uint8_t* ks,
+                        const uint8_t* vs, int pages, int page, int Hq, int Hkv, int D, float scale, int window, int sinks,
+                        uint16_t* out, int ldo, float* lse, const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes,
+                        void* st) {
+  return guard([&] {
+    const auto rw = [](const uint8_t* p) { return const_cast<uint8_t*>(p); };  // read only
+    k::kv_attend_shared(q, ldq, {cu, lens, table, B, max_blocks, rows, max_new},
+                        {rw(kc), rw(vc), rw(ks), rw(vs), pages, page, Hkv, D}, Hq, scale, window, sinks, out, ldo, lse, plan,
+                        plan_bytes, ws, ws_bytes, S(st));
+  });
+}
 size_t uh_kv_pages_workspace_size(int B, int pages) { return k::kv_pages_workspace(B, pages); }
 int uh_kv_reserve(int32_t* table, int max_blocks, int32_t* lens, const int32_t* grow, int B, int32_t* refs, uint8_t* kc,
                   uint8_t* vc, uint8_t* ks, uint8_t* vs, int layers, int pages, int page, int Hkv, int D, int32_t* ok,

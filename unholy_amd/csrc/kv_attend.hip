@@ -18,6 +18,7 @@ constexpr int TILE = 64;          // tokens a wave takes at a time
 constexpr int AT_NT = 256;        // threads of a workgroup: four waves
 constexpr int AT_WAVES = AT_NT / 64;
 constexpr int FEW = 16;           // rows (of a key / value head) of a sequence that the split kernel takes
+constexpr int PR_ROWS = 128;      // rows of a workgroup of the tiled kernel
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 // Bits of the first n of up to 16 tokens.
@@ -51,6 +52,11 @@ struct Block {
   int over, pad;   // some sequence brings more than max_new rows
 };
 
+// Where the partial sums of a block of a group's rows begin, of how many parts.
+struct Common {
+  int row, parts;
+};
+
 // What every workgroup knows of the call.
 struct Attend {
   const bf16* q;
@@ -65,22 +71,27 @@ struct Attend {
   uint32_t* counters;  // of finished parts, by the workgroup of the first; zero between launches (split kernel)
   Block* blocks;       // by the workgroup of the first part (tiled kernel; null where it is not launched)
   float *po, *pml;     // partial sums: values [slot][rows][D]; maximum and weight sum [slot][rows][2]
+  // kv_attend_shared's
+  Share share;
+  Common* common;      // by block of a group and head
+  float *so, *sml;     // the groups' partial sums: values [row][D]; maximum and weight sum [row][2]
 };
 
-// The 64-token tiles that some row of a sequence sees: with a window the sinks' tiles [0, sink_tiles) and those from
+// The 64-token tiles from `from` on that some row of a sequence sees: with a window sink_tiles of the sinks' and those from
 // `skip` on, else all; count of them, numbered in order.
 struct Tiles {
-  int sink_tiles, skip, count;
-  __device__ __forceinline__ int at(int i) const { return i < sink_tiles ? i : i - sink_tiles + skip; }
+  int sink_tiles, skip, count, from;
+  __device__ __forceinline__ int at(int i) const { return i < sink_tiles ? from + i : i - sink_tiles + skip; }
 };
-__device__ __forceinline__ Tiles tiles_of(const Attend& a, const Seq& q) {
+__device__ __forceinline__ Tiles tiles_of(const Attend& a, const Seq& q, int from = 0) {
   const int64_t cap = int64_t(a.st.max_blocks) << a.page_shift;
   const int end = int((min(int64_t(q.len), cap) + TILE - 1) / TILE);
-  Tiles t{0, 0, end};
+  from = min(from, end);
+  Tiles t{0, from, end - from, from};
   if (a.window > 0) {
     const int64_t lo = int64_t(q.first) - a.window + 1;  // the first token in the first row's window
-    t.skip = min(int(max(lo, int64_t(0)) / TILE), end);
-    t.sink_tiles = min(int((int64_t(a.sinks) + TILE - 1) / TILE), t.skip);
+    t.skip = max(min(int(max(lo, int64_t(0)) / TILE), end), from);
+    t.sink_tiles = max(min(int((int64_t(a.sinks) + TILE - 1) / TILE), t.skip) - from, 0);
     t.count = end - t.skip + t.sink_tiles;
   }
   return t;
@@ -99,6 +110,7 @@ __device__ __forceinline__ int row_groups(int rows, int per) { return (rows + pe
 // in slot 2 w + 1, one that goes on with it in slot 2 w.
 struct Walk {
   int b, h;     // the sequence and the head
+  int part;     // kv_attend_shared: which FEW of the sequence's rows
   uint32_t at;  // where the segment begins, in units (tiles, or parts of equal segments)
   Seq q;
   Tiles t;
@@ -155,11 +167,23 @@ __device__ __forceinline__ void clear_rows(const Attend& a, int w, int n) {
   }
 }
 
+// A sequence's segments: its heads, times (kv_attend_shared) the parts of FEW rows that it brings.
+template <bool SH>
+__device__ __forceinline__ int segments_of(const Attend& a, const Seq& q) {
+  return SH ? a.c.heads * (((q.r1 - q.r0) * a.group + FEW - 1) / FEW) : a.c.heads;
+}
+// Tiles of sequence b that are read with its group.
+template <bool SH>
+__device__ __forceinline__ int common_tiles(const Attend& a, int b) {
+  if constexpr (SH) return share_fits(a.share.head, a.st, a.c.page) ? a.share.seqs[b].tiles : 0;
+  return 0;
+}
 __device__ __forceinline__ bool is_few(const Attend& a, const Seq& q) {
   return q.r1 > q.r0 && (q.r1 - q.r0) * a.group <= a.few && !too_many(a.st, q);
 }
 // The segment that holds the workgroup's first unit. Every wave for itself, a sequence a lane: no barriers, and for up to 64
 // sequences one pass over registers. over: some sequence brings more than max_new rows.
+template <bool SH>
 __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w, bool& over) {
   const int lane = threadIdx.x & 63;
   uint32_t segs = 0;  // of this lane's sequence
@@ -167,13 +191,13 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w,
   const auto look = [&](int b) {
     segs = 0;
     rows = 0;
-    w.t = Tiles{0, 0, 0};
+    w.t = Tiles{0, 0, 0, 0};
     if (b < a.st.B) {
       w.q = seq_of(a.st, b);
       rows = w.q.r1 - w.q.r0;
       if (is_few(a, w.q)) {
-        segs = uint32_t(a.c.heads);
-        w.t = tiles_of(a, w.q);
+        segs = uint32_t(segments_of<SH>(a, w.q));
+        w.t = tiles_of(a, w.q, common_tiles<SH>(a, b));
       }
     }
   };
@@ -203,10 +227,13 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w,
       const int l = __ffsll((unsigned long long)hit) - 1;  // (a lane of no segments ends where the one before it does)
       w.b = b0 + l;
       w.q = Seq{int(lane_of(w.q.r0, l)), int(lane_of(w.q.r1, l)), int(lane_of(w.q.len, l)), int(lane_of(w.q.first, l))};
-      w.t = Tiles{int(lane_of(w.t.sink_tiles, l)), int(lane_of(w.t.skip, l)), int(lane_of(w.t.count, l))};
+      w.t = Tiles{int(lane_of(w.t.sink_tiles, l)), int(lane_of(w.t.skip, l)), int(lane_of(w.t.count, l)),
+                  SH ? int(lane_of(w.t.from, l)) : 0};
       const uint32_t first = lane_of(end - n, l), size = lane_of(each, l);
       w.h = int((u - first) / size);
       w.at = first + uint32_t(w.h) * size;
+      w.part = SH ? w.h / a.c.heads : 0;
+      if (SH) w.h %= a.c.heads;
       return true;
     }
     from = lane_of(end, 63);
@@ -231,17 +258,20 @@ __device__ __forceinline__ Part part_of(const Split& s, const Walk& w, uint32_t 
   return p;
 }
 // The next segment, if the workgroup's units reach it.
+template <bool SH>
 __device__ __forceinline__ bool next_segment(const Attend& a, const Split& s, Walk& w) {
   w.at += units_of(s, uint32_t(w.t.count));
   if (s.whole || w.at >= (blockIdx.x + 1) * s.unit) return false;
   if (++w.h < a.c.heads) return true;
   w.h = 0;
+  if (SH && ++w.part * FEW < (w.q.r1 - w.q.r0) * a.group) return true;
+  w.part = 0;
   do {
     if (++w.b >= a.st.B) return false;
     const Seq q = seq_of(a.st, w.b);
     w.q = Seq{uniform(q.r0), uniform(q.r1), uniform(q.len), uniform(q.first)};
   } while (!is_few(a, w.q));
-  w.t = tiles_of(a, w.q);
+  w.t = tiles_of(a, w.q, SH ? uniform(common_tiles<SH>(a, w.b)) : 0);
   return true;
 }
 
@@ -336,7 +366,9 @@ __device__ __forceinline__ void store_out(const Attend& a, int row, int hq, int 
   if (first && a.lse) a.lse[size_t(row) * (a.group * a.c.heads) + hq] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
 }
 
-template <int D>
+// SH (kv_attend_shared): the tiles that a group has in common are left out; what launches before this one made of them joins the
+// sums as further parts. A sequence's rows, up to SHARE_ROWS times the query heads of a head, go FEW at a time.
+template <int D, bool SH>
 __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Attend a) {
   using S = Shape<D>;
   __shared__ __align__(16) typename S::Lds lds;
@@ -345,7 +377,7 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
   Split sp;
   Walk w;
   bool over;
-  const bool some = find_segment(a, sp, w, over);
+  const bool some = find_segment<SH>(a, sp, w, over);
   if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(blockIdx.x), int(gridDim.x));  // (else the join's to do)
   if (!some) return;
   Part pt = part_of(sp, w, blockIdx.x * sp.unit);
@@ -357,6 +389,8 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
   int ksb, vsb;
   int pos, my_row, my_hq;     // this lane's row (the last one where there are fewer)
   int pos_lo, pos_hi, nrows;  // of all rows
+  int row0 = 0;               // the first of them, from the sequence's first (row, query head) on
+  [[maybe_unused]] ShareSeq mine{};
   int i, pk, pv, pk1, pv1;
   const auto token = [&](int i) { return w.t.at(i) * TILE; };
   const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
@@ -385,9 +419,14 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
   };
   const auto begin = [&] {  // a part: its rows, and its first loads on their way
     nrows = (w.q.r1 - w.q.r0) * a.group;
+    if constexpr (SH) {
+      row0 = w.part * FEW;
+      nrows = min(nrows - row0, FEW);
+      if (w.t.from) mine = a.share.seqs[w.b];
+    }
     i = pt.i0 + wave;
     if (i < pt.i1) lookup(token(i), pk, pv);
-    const int ri = min(c, nrows - 1);
+    const int ri = row0 + min(c, nrows - 1);
     my_row = w.q.r0 + ri / a.group, my_hq = w.h * a.group + ri % a.group;
     pos = w.q.first + ri / a.group;
     pos_lo = w.q.first;
@@ -509,8 +548,19 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
     // a thread
     const Part done = pt;
     const uint32_t w0 = blockIdx.x - uint32_t(done.index);
-    const int r0 = w.q.r0, h = w.h, rows = nrows;
-    again = next_segment(a, sp, w);
+    const int r0 = w.q.r0, h = w.h, rows = nrows, part0 = SH ? row0 : 0;
+    // the group's sums of these rows: as many parts for each, which begin at rows of one block or of the next
+    int more = 0, upto = 0, begin0 = 0, begin1 = 0;
+    if constexpr (SH)
+      if (w.t.from) {
+        const int list = mine.at * a.group + row0, block = list / PR_ROWS;
+        const Common* k = a.common + (size_t(mine.row0) * a.group / PR_ROWS + mine.group + block) * a.c.heads + h;
+        more = k->parts;
+        begin0 = k->row + list % PR_ROWS;
+        upto = (block + 1) * PR_ROWS - list;  // rows in that block
+        begin1 = upto < rows ? k[a.c.heads].row - upto : 0;
+      }
+    again = next_segment<SH>(a, sp, w);
     if (again) {
       pt = part_of(sp, w, w.at);
       begin();
@@ -541,27 +591,29 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
         sum += f * ml[k].y;
         acc += f * lds.o[k * S::QUADS + at];
       }
-      if (done.parts == 1) {
-        store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
+      if (done.parts == 1 && more == 0) {
+        store_out<D>(a, r0 + (part0 + r) / a.group, h * a.group + (part0 + r) % a.group, d, acc, sum, m, d == 0);
       } else {
         const int slot = int(blockIdx.x * 2 + (done.index == 0 ? 1 : 0)) * FEW + r;
         put4(sums_of(a.po), slot * D + d, acc);
         if (d == 0) put2(sums_of(a.pml), slot * 2, m, sum);
       }
     }
-    if (done.parts == 1) continue;
+    if (done.parts == 1 && more == 0) continue;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
     __syncthreads();
     if (tid == 0)
-      last = __hip_atomic_fetch_add(&a.counters[w0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+      last = done.parts == 1 ||
+              __hip_atomic_fetch_add(&a.counters[w0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
              uint32_t(done.parts - 1);
     __syncthreads();
     if (!last) continue;
-    if (tid == 0)  // as it was found
+    if (tid == 0 && done.parts > 1)  // as it was found
       __hip_atomic_store(&a.counters[w0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // The parts are dealt to `groups` of threads, four channels of a row a thread, and the groups joined in LDS. What takes
     // time are the rounds of reads, about a microsecond each: as many in flight as the registers hold, but not ten where
     // there are two (sixteen layers of one token over 4097: 160 us; by a group of all threads, eight at a time, 183).
+    const int all_parts = done.parts + more;
     const int items = rows * (D / 4), groups = min(max(AT_NT / items, 1), AT_WAVES), gi = tid / items;
     for (int it = gi < groups ? tid - gi * items : items; it < items; it += AT_NT) {
       const int r = it / (D / 4), d = it % (D / 4) * 4;
@@ -572,8 +624,14 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
         float2 x[N];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-          const int p = min(k0 + k * groups, done.parts - 1);
+          const int p = min(k0 + k * groups, all_parts - 1);
           const int at = (int(w0 + uint32_t(p)) * 2 + (p == 0 ? 1 : 0)) * FEW + r;
+          if (SH && p >= done.parts) {
+            const size_t row = size_t((r < upto ? begin0 : begin1) + r) + size_t(p - done.parts) * a.c.heads * PR_ROWS;
+            x[k] = *reinterpret_cast<const float2*>(a.sml + row * 2);
+            y[k] = *reinterpret_cast<const v4f*>(a.so + row * D + d);
+            continue;
+          }
           x[k] = get2(sums_of(a.pml), at * 2);
           y[k] = get4(sums_of(a.po), at * D + d);
         }
@@ -586,17 +644,17 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
         sum *= al;
 #pragma unroll
         for (int k = 0; k < N; ++k)
-          if (k0 + k * groups < done.parts) {
+          if (k0 + k * groups < all_parts) {
             const float f = __builtin_amdgcn_exp2f(x[k].x - ref);
             sum += f * x[k].y;
             acc += f * y[k];
           }
       };
-      if (done.parts <= 2 * groups) add.template operator()<2>(gi % groups);
+      if (all_parts <= 2 * groups) add.template operator()<2>(gi % groups);
       else
-        for (int k0 = gi % groups; k0 < done.parts; k0 += FLIGHT * groups) add.template operator()<FLIGHT>(k0);
+        for (int k0 = gi % groups; k0 < all_parts; k0 += FLIGHT * groups) add.template operator()<FLIGHT>(k0);
       if (groups == 1) {
-        store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
+        store_out<D>(a, r0 + (part0 + r) / a.group, h * a.group + (part0 + r) % a.group, d, acc, sum, m, d == 0);
       } else {
         lds.o[tid] = acc;  // (the waves' sums were read before the counter was)
         lds.group_ml[tid] = make_float2(m, sum);
@@ -615,7 +673,7 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
         sum += f * x.y;
         acc += f * lds.o[k * items + tid];
       }
-      const int r = tid / (D / 4), d = tid % (D / 4) * 4;
+      const int r = part0 + tid / (D / 4), d = tid % (D / 4) * 4;
       store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
     }
   }
@@ -637,7 +695,6 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
 // The running maximum is left alone until a row's scores pass it by more than 2^8: the weights stay small enough, and most
 // tiles need no scaling of the sums. The largest weight is not 1 then, as it is above, but rounded to bf16 like the others: an
 // output is off by 2.2e-3 of its norm, the split kernel's by 1.8e-3, and the output's own rounding alone is 1.65e-3.
-constexpr int PR_ROWS = 128;
 constexpr int PR_STAGES = 3;
 constexpr int PR_META = 16;  // tiles
 constexpr float PR_LAG = 8.0f;
@@ -745,7 +802,64 @@ __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p, bool& 
   return false;
 }
 
-template <int D>
+// The same of the groups' blocks (kv_attend_shared): the rows of a group's list, and the tiles that they have in common. Every
+// block's sums are partial ones. `single`: as many blocks as fill the chip, whole ones, and the sums of a head's rows follow each
+// other in the order of the list; else a workgroup's have PR_ROWS places of their own.
+__device__ __forceinline__ bool find_common(const Attend& a, BlockPart& p, int& sums) {
+  constexpr uint32_t NONE = 1u << 30;
+  const int lane = threadIdx.x & 63;
+  const uint32_t heads = uint32_t(a.c.heads);
+  const int n = share_fits(a.share.head, a.st, a.c.page) ? a.share.head->groups : 0;
+  ShareGroup g{};
+  uint32_t blocks = 0, count = 0, all = 0, tiles = 0;
+  const auto look = [&](int i) {
+    blocks = count = 0;
+    if (i < n) {
+      g = a.share.groups[i];
+      blocks = uint32_t(row_groups(g.rows * a.group, PR_ROWS));
+      count = uint32_t(tiles_of(a, Seq{0, 0, g.tiles * TILE, g.first}).count);
+    }
+  };
+  for (int b0 = 0; b0 < n; b0 += 64) {
+    look(b0 + lane);
+    all += lane_of(wave_scan(blocks), 63) * heads;
+    if (all < a.target) tiles += lane_of(wave_scan(blocks * count), 63) * heads;
+  }
+  const bool single = all >= a.target;
+  const uint32_t least = max(4u, root(0.2f, tiles, all));
+  uint32_t share = NONE;
+  if (!single && n <= 64) share = smallest_share(blocks * heads, count, tiles, all, a.target, least);
+  else if (!single) share = max((tiles + a.target - all - 1) / (a.target - all), least);
+  uint32_t from = 0;
+  for (int b0 = 0; b0 < n; b0 += 64) {
+    if (n > 64) look(b0 + lane);
+    const uint32_t parts = parts_of(count, share), wgs = blocks * parts * heads, end = from + wave_scan(wgs);
+    const uint64_t hit = __ballot(blockIdx.x < end);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      const uint32_t in = blockIdx.x - lane_of(end - wgs, l), np = lane_of(parts, l);
+      const int row0 = int(lane_of(g.row0, l)), block = int(in / heads / np);
+      p.b = int(lane_of(g.seq, l));
+      p.h = int(in % heads);
+      p.index = int(in / heads % np);
+      p.parts = int(np);
+      p.row0 = block * PR_ROWS;
+      p.q = Seq{row0, row0 + int(lane_of(g.rows, l)), int(lane_of(g.tiles, l)) * TILE, int(lane_of(g.first, l))};
+      p.t = tiles_of(a, p.q);
+      const int each = p.t.count / p.parts, more = p.t.count % p.parts;
+      p.i0 = p.index * each + min(p.index, more);
+      p.i1 = p.i0 + each + (p.index < more ? 1 : 0);
+      sums = single ? (p.h * a.share.head->list + row0) * a.group + p.row0 : int(blockIdx.x) * PR_ROWS;
+      if (threadIdx.x == 0 && p.index == 0)
+        a.common[(size_t(row0) * a.group / PR_ROWS + (b0 + l) + block) * heads + p.h] = Common{sums, p.parts};
+      return true;
+    }
+    from = lane_of(end, 63);
+  }
+  return false;
+}
+
+template <int D, bool COMMON>
 __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tiled_kernel(Attend a) {
   using S = Tiled<D>;
   __shared__ __align__(1024) typename S::Lds lds;
@@ -753,8 +867,9 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
 
   BlockPart bp;
   bool over;
-  const bool some = find_block(a, bp, over);
-  if (tid == 0 && blockIdx.x < a.target)
+  [[maybe_unused]] int sums = 0;
+  const bool some = COMMON ? find_common(a, bp, sums) : find_block(a, bp, over);
+  if (!COMMON && tid == 0 && blockIdx.x < a.target)
     a.blocks[blockIdx.x] = some && bp.index == 0
                                ? Block{bp.parts, int(a.c.heads), bp.row0, min(PR_ROWS, (bp.q.r1 - bp.q.r0) * a.group - bp.row0),
                                        bp.q.r0, bp.h, over, 0}
@@ -767,9 +882,15 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
 
   // this lane's row
   const int wrow = row0 + 32 * wave, ri = min(wrow + c, nrows - 1);
-  const int row = q.r0 + ri / a.group, hq = h * a.group + ri % a.group, pos = q.first + ri / a.group;
-  const int pos_lo = uniform(q.first + min(wrow, nrows - 1) / a.group);
-  const int pos_hi = uniform(q.first + min(wrow + 31, nrows - 1) / a.group);
+  int row = q.r0 + ri / a.group, pos = q.first + ri / a.group;
+  const int hq = h * a.group + ri % a.group;
+  if constexpr (COMMON) {
+    const int2 listed = a.share.list[row];
+    row = listed.x, pos = listed.y;
+  }
+  // (a group's tiles lie before all of its rows)
+  const int pos_lo = COMMON ? INT32_MAX : uniform(q.first + min(wrow, nrows - 1) / a.group);
+  const int pos_hi = COMMON ? INT32_MAX : uniform(q.first + min(wrow + 31, nrows - 1) / a.group);
   bf16x8 qf[2 * D / 32];
   {
     const bf16* x = a.q + size_t(row) * a.ldq + size_t(hq) * D + 16 * h2;
@@ -1005,6 +1126,16 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
   }
   l += __shfl_xor(l, 32, 64);
   const auto four = [&](int d, int r) { return v4f{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]}; };
+  if constexpr (COMMON) {  // [row][D]: kv_split_kernel takes the rows of one sequence
+    if (wrow + c >= nrows) return;
+    const size_t at = size_t(sums) + 32 * wave + c;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) *reinterpret_cast<v4f*>(a.so + at * D + 32 * d + 8 * r + 4 * h2) = four(d, r);
+    if (h2 == 0) *reinterpret_cast<float2*>(a.sml + at * 2) = make_float2(ref2, l);
+    return;
+  }
   if (parts == 1) {
     if (wrow + c >= nrows) return;
 #pragma unroll
@@ -1094,6 +1225,29 @@ size_t sum_rows(const Way& way, int dim) {
   return size_t(target_of(dim)) * (way.tiled ? PR_ROWS : 2 * FEW);
 }
 
+// kv_attend_shared: sequences of up to SHARE_ROWS rows, in a group or alone, are the split kernel's, the others the tiled kernel's.
+Way shared_way(int rows, int max_new, int group) {
+  return {SHARE_ROWS * group, true, std::min(rows, max_new) > SHARE_ROWS};
+}
+// Its workspace: counters and blocks, the groups' blocks, their sums, the split kernel's, the tiled kernel's (which is launched
+// first: its sums lie where the groups' do).
+struct SharedWs {
+  int64_t blocks;    // of the groups, times heads, at most
+  int64_t sum_rows;  // of the groups' sums
+  size_t split, common, bytes;  // offsets; all
+};
+SharedWs carve_shared(int rows, int max_new, int B, int Hq, int heads, int dim) {
+  SharedWs w;
+  const int64_t group = Hq / heads, list = std::min<int64_t>(rows, int64_t(SHARE_ROWS) * B);
+  w.blocks = (list * group / PR_ROWS + B / 2 + 1) * heads;
+  w.sum_rows = std::max<int64_t>(int64_t(target_of(dim)) * PR_ROWS, list * Hq);
+  w.common = kHeadBytes;
+  w.split = (w.common + size_t(w.blocks) * sizeof(Common) + 15) / 16 * 16;
+  const size_t row = (size_t(dim) + 2) * sizeof(float);
+  w.bytes = w.split + size_t(target_of(dim)) * 2 * FEW * row + size_t(w.sum_rows) * row;
+  return w;
+}
+
 }  // namespace
 
 size_t kv_attend_workspace(int rows, int max_new, int B, int Hq, int heads, int dim) {
@@ -1101,31 +1255,66 @@ size_t kv_attend_workspace(int rows, int max_new, int B, int Hq, int heads, int 
   return kHeadBytes + sum_rows(way_of(rows, max_new, B, Hq / heads, heads), dim) * (size_t(dim) + 2) * sizeof(float);
 }
 
-void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks,
-               bf16* out, int ldo, float* lse, void* ws, size_t ws_bytes, hipStream_t st) {
-  const auto fail = [](const std::string& what) { throw std::runtime_error("kv_attend: " + what); };
-  check_cache("kv_attend", c);
-  check_step("kv_attend", s);
+size_t kv_attend_shared_workspace(int rows, int max_new, int B, int Hq, int heads, int dim) {
+  if (rows < 0 || max_new < 0 || B < 0 || heads < 1 || Hq < heads || dim < 1) return 0;
+  return std::max(carve_shared(rows, max_new, B, Hq, heads, dim).bytes, kv_attend_workspace(rows, max_new, B, Hq, heads, dim));
+}
+
+namespace {
+
+// The operands' checks; false: there is nothing to do.
+bool check_attend(const char* who, const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int sinks,
+                  const bf16* out, int ldo, const void* ws, size_t ws_bytes, size_t need) {
+  const auto fail = [&](const std::string& what) { throw std::runtime_error(std::string(who) + ": " + what); };
+  check_cache(who, c);
+  check_step(who, s);
   if (Hq < 1 || Hq % c.heads || Hq > 65535) fail("Hq must be a multiple of heads, up to 65535");
   if (sinks < 0) fail("sinks < 0");
   if (!std::isfinite(scale)) fail("scale is not finite");
-  if (s.B == 0 || s.rows == 0 || s.max_new == 0) return;
+  if (s.B == 0 || s.rows == 0 || s.max_new == 0) return false;
   if (!q || !out) fail("null operand");
   const int64_t width = int64_t(Hq) * c.dim;
   if (ldq < width || ldo < width || ldq % 8 || ldo % 8) fail("ldq / ldo >= Hq * dim, % 8");
   if (!aligned16(q) || !aligned16(out)) fail("rows not 16-byte aligned");
   if (int64_t(s.rows) * Hq > INT32_MAX) fail("rows * Hq past 31 bits");
-  const size_t need = kv_attend_workspace(s.rows, s.max_new, s.B, Hq, c.heads, c.dim);
   if (!ws) fail("null workspace");
   if (!aligned16(ws)) fail("workspace not 16-byte aligned");
   if (ws_bytes < need) fail("workspace of " + std::to_string(ws_bytes) + " bytes, " + std::to_string(need) + " needed");
-
-  const Way way = way_of(s.rows, s.max_new, s.B, Hq / c.heads, c.heads);
-  Attend a{q,       out,   lse, s, c, ldq, ldo, Hq / c.heads, 0, window, sinks, scale * LOG2E, way.few,
-           unsigned(target_of(c.dim)), nullptr, nullptr, nullptr, nullptr};
+  return true;
+}
+Attend attend_of(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks, bf16* out,
+                 int ldo, float* lse, const Way& way, void* ws) {
+  Attend a{};
+  a.q = q, a.out = out, a.lse = lse, a.st = s, a.c = c, a.ldq = ldq, a.ldo = ldo, a.group = Hq / c.heads;
+  a.window = window, a.sinks = sinks, a.scale2 = scale * LOG2E, a.few = way.few, a.target = unsigned(target_of(c.dim));
   while (1 << a.page_shift < c.page) ++a.page_shift;
   a.counters = static_cast<uint32_t*>(ws);
   if (way.tiled) a.blocks = reinterpret_cast<Block*>(a.counters + 512);
+  return a;
+}
+// f.operator()<D>() for the cache's dim.
+template <class F>
+void by_dim(int dim, F&& f) {
+  if (dim == 64) f.template operator()<64>();
+  else if (dim == 128) f.template operator()<128>();
+  else f.template operator()<256>();
+  UH_CHECK_LAUNCH();
+}
+void launch_tiled(const Attend& a, int64_t blocks, hipStream_t st) {
+  const unsigned grid = std::max(unsigned(blocks), a.target);
+  by_dim(a.c.dim, [&]<int D>() { kv_tiled_kernel<D, false><<<grid, AT_NT, 0, st>>>(a); });
+  const dim3 join(a.target, unsigned(PR_ROWS * a.c.dim / 4 / AT_NT));
+  by_dim(a.c.dim, [&]<int D>() { kv_join_kernel<D><<<join, AT_NT, 0, st>>>(a); });
+}
+
+}  // namespace
+
+void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks,
+               bf16* out, int ldo, float* lse, void* ws, size_t ws_bytes, hipStream_t st) {
+  const size_t need = kv_attend_workspace(s.rows, s.max_new, s.B, Hq, c.heads, c.dim);
+  if (!check_attend("kv_attend", q, ldq, s, c, Hq, scale, sinks, out, ldo, ws, ws_bytes, need)) return;
+  const Way way = way_of(s.rows, s.max_new, s.B, Hq / c.heads, c.heads);
+  Attend a = attend_of(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, way, ws);
   a.po = reinterpret_cast<float*>(static_cast<char*>(ws) + kHeadBytes);
   a.pml = a.po + sum_rows(way, c.dim) * c.dim;
   const int64_t segs = int64_t(s.B) * c.heads;
@@ -1133,26 +1322,52 @@ void kv_attend(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq
   const int64_t blocks = (cdiv(size_t(s.rows) * a.group, PR_ROWS) + int64_t(s.B)) * c.heads;  // at most
   if (segs * 8 > INT32_MAX || std::max(segs, std::min<int64_t>(blocks, a.target)) * (tiles + START) > INT32_MAX ||
       blocks > INT32_MAX)
-    fail("rows times blocks past 31 bits");
-  if (way.tiled) {
-    const unsigned grid = std::max(unsigned(blocks), a.target);
-    if (c.dim == 64) kv_tiled_kernel<64><<<grid, AT_NT, 0, st>>>(a);
-    else if (c.dim == 128) kv_tiled_kernel<128><<<grid, AT_NT, 0, st>>>(a);
-    else kv_tiled_kernel<256><<<grid, AT_NT, 0, st>>>(a);
-    UH_CHECK_LAUNCH();
-    const dim3 join(a.target, unsigned(PR_ROWS * c.dim / 4 / AT_NT));
-    if (c.dim == 64) kv_join_kernel<64><<<join, AT_NT, 0, st>>>(a);
-    else if (c.dim == 128) kv_join_kernel<128><<<join, AT_NT, 0, st>>>(a);
-    else kv_join_kernel<256><<<join, AT_NT, 0, st>>>(a);
-    UH_CHECK_LAUNCH();
-  }
+    throw std::runtime_error("kv_attend: rows times blocks past 31 bits");
+  if (way.tiled) launch_tiled(a, blocks, st);
   if (way.split) {
     const unsigned grid = unsigned(std::min<int64_t>(segs * cdiv(tiles + START, AT_WAVES), a.target));
-    if (c.dim == 64) kv_split_kernel<64><<<grid, AT_NT, 0, st>>>(a);
-    else if (c.dim == 128) kv_split_kernel<128><<<grid, AT_NT, 0, st>>>(a);
-    else kv_split_kernel<256><<<grid, AT_NT, 0, st>>>(a);
-    UH_CHECK_LAUNCH();
+    by_dim(c.dim, [&]<int D>() { kv_split_kernel<D, false><<<grid, AT_NT, 0, st>>>(a); });
   }
+}
+
+void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks,
+                      bf16* out, int ldo, float* lse, const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes,
+                      hipStream_t st) {
+  const char* who = "kv_attend_shared";
+  const auto fail = [&](const char* what) { throw std::runtime_error(std::string(who) + ": " + what); };
+  const size_t need = kv_attend_shared_workspace(s.rows, s.max_new, s.B, Hq, c.heads, c.dim);
+  if (!check_attend(who, q, ldq, s, c, Hq, scale, sinks, out, ldo, ws, ws_bytes, need)) return;
+  if (!plan) fail("null plan");
+  if (!aligned16(plan)) fail("plan not 16-byte aligned");
+  if (plan_bytes < kv_share_plan(s.B, s.rows)) fail("plan too small");
+  const Way way = shared_way(s.rows, s.max_new, Hq / c.heads);
+  Attend a = attend_of(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, way, ws);
+  const SharedWs w = carve_shared(s.rows, s.max_new, s.B, Hq, c.heads, c.dim);
+  const int64_t most = std::min<int64_t>(std::min(s.rows, s.max_new), SHARE_ROWS);
+  const int64_t segs = int64_t(s.B) * c.heads * cdiv(size_t(most) * a.group, FEW);
+  const int64_t tiles = std::max<int64_t>(cdiv(size_t(s.max_blocks) * c.page, TILE), 1);
+  const int64_t blocks = (cdiv(size_t(s.rows) * a.group, PR_ROWS) + int64_t(s.B)) * c.heads;
+  if (segs * 8 > INT32_MAX || std::max(segs, std::min<int64_t>(std::max(blocks, w.blocks), a.target)) * (tiles + START) > INT32_MAX ||
+      blocks > INT32_MAX || w.blocks > INT32_MAX || w.sum_rows > INT32_MAX)
+    fail("rows times blocks past 31 bits");
+  a.share = carve_share(const_cast<void*>(plan), s.B, s.rows);
+  char* base = static_cast<char*>(ws);
+  a.common = reinterpret_cast<Common*>(base + w.common);
+  a.so = reinterpret_cast<float*>(base + w.split) + size_t(a.target) * 2 * FEW * (c.dim + 2);
+  a.sml = a.so + size_t(w.sum_rows) * c.dim;
+  if (way.tiled) {
+    a.po = a.so;
+    a.pml = a.po + size_t(a.target) * PR_ROWS * c.dim;
+    launch_tiled(a, blocks, st);
+  }
+  a.po = reinterpret_cast<float*>(base + w.split);
+  a.pml = a.po + size_t(a.target) * 2 * FEW * c.dim;
+  if (s.B > 1) {
+    const unsigned grid = unsigned(std::max<int64_t>(w.blocks, a.target));
+    by_dim(c.dim, [&]<int D>() { kv_tiled_kernel<D, true><<<grid, AT_NT, 0, st>>>(a); });
+  }
+  const unsigned grid = unsigned(std::min<int64_t>(segs * cdiv(tiles + START, AT_WAVES), a.target));
+  by_dim(c.dim, [&]<int D>() { kv_split_kernel<D, true><<<grid, AT_NT, 0, st>>>(a); });
 }
 
 }  // namespace unholy::kernels

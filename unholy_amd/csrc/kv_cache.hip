@@ -522,6 +522,132 @@ __global__ __launch_bounds__(64) void kv_free_kernel(KvSeqs s, const int32_t* __
   if (lane == 0 && left != len) s.lens[b] = left;
 }
 
+// ---- sequences that begin alike --------------------------------------------------------------------------------------
+// One workgroup: which sequences may share (by number or first page, through a hash table), how far the tables of each and of the
+// lowest of them agree (a wave a sequence), then for each such class the length that saves the most tiles' reads, and the lists.
+// The loops over all pairs of sequences are in LDS up to SH_LDS of them (the scratch in the plan past that).
+constexpr int SH_LDS = 1024;
+
+template <bool LDS>
+__global__ __launch_bounds__(PL_NT) void kv_share_kernel(const int32_t* __restrict__ group, KvStep st, int pages, int page,
+                                                         Share sh, int hash) {
+  __shared__ int wsum[PL_NT / 64];
+  __shared__ __align__(8) int own[LDS ? 8 * SH_LDS + 4 * SH_LDS : 2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int* p = LDS ? own : sh.scratch;
+  unsigned long long* best = reinterpret_cast<unsigned long long*>(p);  // by the class's lowest: saved, then tiles (25 bits)
+  int *rep = p + 2 * st.B, *tiles = rep + st.B, *rows = tiles + st.B, *first = rows + st.B, *limit = first + st.B,
+      *base = limit + st.B, *keys = base + st.B, *low = keys + hash;
+  for (int i = tid; i < hash; i += PL_NT) keys[i] = -1, low[i] = INT32_MAX;
+  __syncthreads();
+
+  // classes: base[b] holds the place of the sequence's key for now
+  for (int b = tid; b < st.B; b += PL_NT) {
+    const Seq q = seq_of(st, b);
+    const int n = q.r1 - q.r0, blocks = min(max(q.first, 0) / page, st.max_blocks);
+    int key = -1;
+    if (n >= 1 && n <= SHARE_ROWS && !too_many(st, q) && int64_t(blocks) * page >= SHARE_TILE) {
+      key = group ? group[b] : page_of(st.table, st.max_blocks, pages, b, 0);
+      if (group && (key < 0 || key >= st.B)) key = -1;
+    }
+    int at = -1;
+    if (key >= 0) {
+      at = int(uint32_t(key) * 2654435761u >> 8) & (hash - 1);
+      for (;; at = (at + 1) & (hash - 1)) {  // (twice as many places as keys: one is free)
+        const int was = atomicCAS(&keys[at], -1, key);
+        if (was == -1 || was == key) break;
+      }
+      atomicMin(&low[at], b);
+    }
+    base[b] = at;
+    rows[b] = n;
+    first[b] = q.first;
+    limit[b] = blocks;
+    best[b] = 0;
+  }
+  __syncthreads();
+  for (int b = tid; b < st.B; b += PL_NT) rep[b] = base[b] < 0 ? -1 : low[base[b]];
+  __syncthreads();
+
+  // tiles that each has in common with the lowest of its class
+  for (int b = wave; b < st.B; b += PL_NT / 64) {
+    const int r = rep[b];
+    int same = 0;
+    if (r >= 0) {
+      const int most = min(limit[b], limit[r]);
+      const int32_t *x = st.table + size_t(b) * st.max_blocks, *y = st.table + size_t(r) * st.max_blocks;
+      constexpr int AHEAD = 4;
+      for (bool all = true; all && same < most;) {
+        int u[AHEAD], v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const int j = min(same + k * 64 + lane, most - 1);
+          u[k] = x[j], v[k] = y[j];
+        }
+        const int from = same;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const bool ok = from + k * 64 + lane < most && u[k] == v[k] && u[k] >= 0 && u[k] < pages;
+          const uint64_t bad = ~__ballot(ok);
+          if (all) same += bad ? __ffsll((unsigned long long)bad) - 1 : 64;
+          all = all && !bad;
+        }
+      }
+    }
+    if (lane == 0) tiles[b] = int(int64_t(same) * page / SHARE_TILE);
+  }
+  __syncthreads();
+
+  // what each length would save: the tiles of all but one of the sequences that are as long
+  for (int b = tid; b < st.B; b += PL_NT) {
+    const int r = rep[b], t = tiles[b];
+    if (r < 0 || t == 0) continue;
+    int64_t count = 0;
+    for (int i = 0; i < st.B; ++i) count += rep[i] == r && tiles[i] >= t;
+    if (count > 1) atomicMax(&best[r], (unsigned long long)min((count - 1) * t, int64_t(1) << 38) << 25 | (unsigned long long)t);
+  }
+  __syncthreads();
+
+  // places: the groups in the order of their lowest sequences, their rows in the order of the slots
+  int groups = 0, list = 0;
+  for (int b0 = 0; b0 < st.B; b0 += PL_NT) {
+    const int b = b0 + tid, r = b < st.B ? rep[b] : -1;
+    const int t = r >= 0 ? int(best[r] & 0x1ffffff) : 0;
+    const bool member = t > 0 && tiles[b] >= t;
+    int at = 0, all = 0, lowest = INT32_MAX;
+    if (member)
+      for (int i = 0; i < st.B; ++i) {
+        const bool in = rep[i] == r && tiles[i] >= t;
+        at += in && i < b ? rows[i] : 0;
+        all += in ? rows[i] : 0;
+        lowest = in ? min(lowest, first[i]) : lowest;
+      }
+    const bool head = member && r == b;  // (the lowest of a class is as long as any of it)
+    int sum, many;
+    const int g = groups + block_scan(head, wsum, many), row0 = list + block_scan(head ? all : 0, wsum, sum);
+    groups += many;
+    list += sum;
+    if (head) {
+      sh.groups[g] = ShareGroup{row0, all, t, b, lowest, {0, 0, 0}};
+      base[b] = g;
+      limit[b] = row0;
+    }
+    if (b < st.B) sh.seqs[b] = ShareSeq{member ? t : 0, at, 0, 0};
+  }
+  __syncthreads();
+  for (int b = tid; b < st.B; b += PL_NT) {
+    ShareSeq s = sh.seqs[b];
+    if (s.tiles == 0) continue;
+    s.group = base[rep[b]];
+    s.row0 = limit[rep[b]];
+    sh.seqs[b] = s;
+    const int r0 = seq_of(st, b).r0;
+    for (int i = 0; i < rows[b]; ++i) sh.list[s.row0 + s.at + i] = make_int2(r0 + i, first[b] + i);
+  }
+  if (tid == 0)
+    *sh.head = ShareHead{SHARE_MAGIC, st.B, st.rows, st.max_new, st.max_blocks, page, groups, list, {}};
+}
+
 void check_seqs(const char* who, const KvSeqs& s, const int32_t* more, const int32_t* refs, int pages, int page) {
   const auto fail = [&](const char* what) { throw std::runtime_error(std::string(who) + ": " + what); };
   if (s.B < 0 || s.max_blocks < 0) fail("negative size");
@@ -609,6 +735,24 @@ void kv_append_rope(const bf16* q, int ldq, bf16* qo, int ldqo, int Hq, const bf
   }
   if (!aligned16(wq) || !aligned16(wk)) fail("weights not 16-byte aligned");
   append<true>(who, k, ldk, v, ldv, s, c, AppendTurn{q, qo, wq, wk, ldq, ldqo, Hq, 0, eps, r}, st);
+}
+
+size_t kv_share_plan(int B, int rows) { return B < 0 || rows < 0 ? 0 : carve_share(nullptr, B, rows).bytes; }
+
+void kv_share(const int32_t* group, const KvStep& s, int pages, int page, void* plan, size_t plan_bytes, hipStream_t st) {
+  const auto fail = [](const char* what) { throw std::runtime_error(std::string("kv_share: ") + what); };
+  check_step("kv_share", s);
+  check_pages("kv_share", pages);
+  if (page != 16 && page != 32 && page != 64 && page != 128) fail("page must be 16, 32, 64 or 128");
+  if (s.B > (1 << 24)) fail("B > 2^24");
+  if (!plan) fail("null plan");
+  if (!aligned16(plan)) fail("plan not 16-byte aligned");
+  if (plan_bytes < kv_share_plan(s.B, s.rows)) fail("plan too small");
+  if (s.B == 0 || s.rows == 0 || s.max_new == 0) return;
+  const Share sh = carve_share(plan, s.B, s.rows);
+  if (s.B <= SH_LDS) kv_share_kernel<true><<<1, PL_NT, 0, st>>>(group, s, pages, page, sh, int(share_hash(s.B)));
+  else kv_share_kernel<false><<<1, PL_NT, 0, st>>>(group, s, pages, page, sh, int(share_hash(s.B)));
+  UH_CHECK_LAUNCH();
 }
 
 size_t kv_pages_workspace(int B, int pages) { return B < 0 || pages < 0 ? 0 : carve_pages(nullptr, B, pages).bytes; }

@@ -33,6 +33,62 @@ __device__ __forceinline__ int page_of(const int32_t* table, int max_blocks, int
   return p >= 0 && p < pages ? p : -1;
 }
 
+// What kv_share writes and kv_attend_shared reads (device). Sequences of a group read the first `tiles` tiles of SHARE_TILE tokens,
+// whose pages they have in common, together: all rows of its sequences, in the order of the slots, are the group's list.
+constexpr int SHARE_TILE = 64;
+constexpr int SHARE_ROWS = 16;  // a sequence that brings more rows is left alone: they fill tiles of rows by themselves
+struct ShareHead {
+  int magic, B, rows, max_new, max_blocks, page;
+  int groups, list;  // their number, rows in the list
+  int pad[8];
+};
+struct ShareSeq {
+  int tiles;  // 0: alone
+  int at;     // its first row, from the group's first on
+  int row0, group;
+};
+struct ShareGroup {
+  int row0, rows, tiles;
+  int seq;    // whose table is read
+  int first;  // the lowest position of its rows
+  int pad[3];
+};
+struct Share {
+  ShareHead* head;
+  ShareSeq* seqs;      // [B]
+  ShareGroup* groups;  // [B / 2 + 1]
+  int2* list;          // [rows] {row of the step, position}
+  int* scratch;        // kv_share's own: 8 B + 2 hash_size(B) ints
+  size_t bytes;
+};
+constexpr int SHARE_MAGIC = 0x5ea4ed01;
+inline size_t share_hash(int B) {  // a power of two, twice the sequences at least
+  size_t n = 64;
+  while (n < 2 * size_t(B)) n *= 2;
+  return n;
+}
+inline Share carve_share(void* plan, int B, int rows) {
+  Share s;
+  char* p = static_cast<char*>(plan);
+  const auto take = [&](size_t bytes) {
+    char* at = p;
+    p += (bytes + 15) / 16 * 16;
+    return at;
+  };
+  s.head = reinterpret_cast<ShareHead*>(take(sizeof(ShareHead)));
+  s.seqs = reinterpret_cast<ShareSeq*>(take(sizeof(ShareSeq) * size_t(B)));
+  s.groups = reinterpret_cast<ShareGroup*>(take(sizeof(ShareGroup) * (size_t(B) / 2 + 1)));
+  s.list = reinterpret_cast<int2*>(take(sizeof(int2) * size_t(rows)));
+  s.scratch = reinterpret_cast<int*>(take(sizeof(int) * (8 * size_t(B) + 2 * share_hash(B))));
+  s.bytes = size_t(p - static_cast<char*>(plan));
+  return s;
+}
+// Whether a plan was made for a step of these sizes: another one is not used.
+__device__ __forceinline__ bool share_fits(const ShareHead* h, const KvStep& s, int page) {
+  return h->magic == SHARE_MAGIC && h->B == s.B && h->rows == s.rows && h->max_new == s.max_new &&
+         h->max_blocks == s.max_blocks && h->page == page;
+}
+
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 inline void check_pages(const char* who, int pages) {
