@@ -83,7 +83,7 @@ void kv_attend(const bf16* q, int ldq, const KvStep& step, const KvCache& cache,
 // those with the same first page. Of such sequences those that bring 1 to 16 rows and have the same pages as the lowest of
 // them for long enough (in whole pages before any new row, and in multiples of 64 tokens) become a group, as many of them and as
 // long as saves the most; the others are alone. Wrong numbers cost time, never results: what is shared is read off the table.
-// plan: kv_share_plan bytes, 16-byte aligned, any contents before. It holds for the step's cu, lens and table as they were when it
+// plan: kv_share_plan bytes, 16-byte aligned, zeroed before the first call that makes one in it. It holds for the step's cu, lens and table as they were when it
 // was made, and stays valid while sequences only grow and none of its pages is changed, moved (kv_compact) or given up.
 size_t kv_share_plan(int B, int rows);
 void kv_share(const int32_t* group, const KvStep& step, int pages, int page, void* plan, size_t plan_bytes, hipStream_t st);

@@ -59,7 +59,7 @@ def plan_of(c, group=None, most=None, stream=None):
     s = c.step
     most = max(s.n + [0]) if most is None else most
     need = call("uh_kv_share_plan_size", s.B, s.rows)
-    plan = dev(np.full(need + 64, GUARD, np.uint8))
+    plan = dev(np.concatenate([np.zeros(need, np.uint8), np.full(64, GUARD, np.uint8)]))
     g = None if group is None else dev(np.asarray(group, np.int32))
     call("uh_kv_share", g, c.cu, s.rows, most, c.lens, c.table, s.max_blocks, s.B, s.pages, s.page, plan, need, stream)
     synchronize()

@@ -40,7 +40,8 @@ constexpr int SHARE_ROWS = 16;  // a sequence that brings more rows is left alon
 struct ShareHead {
   int magic, B, rows, max_new, max_blocks, page;
   int groups, list;  // their number, rows in the list
-  int pad[8];
+  int pad[7];
+  unsigned done;     // kv_share's workgroups that are done; zero between launches
 };
 struct ShareSeq {
   int tiles;  // 0: alone
@@ -58,15 +59,12 @@ struct Share {
   ShareSeq* seqs;      // [B]
   ShareGroup* groups;  // [B / 2 + 1]
   int2* list;          // [rows] {row of the step, position}
-  int* scratch;        // kv_share's own: 8 B + 2 hash_size(B) ints
+  int4* found;         // [B, up to a multiple of SHARE_AHEAD] kv_share's own: what it knows of each sequence
+  unsigned long long* best;  // [B] the same of each class
   size_t bytes;
 };
+constexpr int SHARE_AHEAD = 16;
 constexpr int SHARE_MAGIC = 0x5ea4ed01;
-inline size_t share_hash(int B) {  // a power of two, twice the sequences at least
-  size_t n = 64;
-  while (n < 2 * size_t(B)) n *= 2;
-  return n;
-}
 inline Share carve_share(void* plan, int B, int rows) {
   Share s;
   char* p = static_cast<char*>(plan);
@@ -79,7 +77,8 @@ inline Share carve_share(void* plan, int B, int rows) {
   s.seqs = reinterpret_cast<ShareSeq*>(take(sizeof(ShareSeq) * size_t(B)));
   s.groups = reinterpret_cast<ShareGroup*>(take(sizeof(ShareGroup) * (size_t(B) / 2 + 1)));
   s.list = reinterpret_cast<int2*>(take(sizeof(int2) * size_t(rows)));
-  s.scratch = reinterpret_cast<int*>(take(sizeof(int) * (8 * size_t(B) + 2 * share_hash(B))));
+  s.found = reinterpret_cast<int4*>(take(sizeof(int4) * ((size_t(B) + SHARE_AHEAD - 1) / SHARE_AHEAD * SHARE_AHEAD)));
+  s.best = reinterpret_cast<unsigned long long*>(take(sizeof(unsigned long long) * size_t(B)));
   s.bytes = size_t(p - static_cast<char*>(plan));
   return s;
 }
