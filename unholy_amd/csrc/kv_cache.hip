@@ -278,33 +278,6 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(const bf16* __restrict__ 
 // ---- pages ------------------------------------------------------------------------------------------------------------
 constexpr int PL_NT = 1024;
 
-constexpr int kMany = 1 << 29;  // sums of pages stop here, past any pool
-__device__ __forceinline__ int add_pages(int a, int b) { return min(a + b, kMany); }
-
-// Exclusive prefix of v (0 .. kMany) over the workgroup's threads; total is their sum (wsum: an int of LDS a wave).
-template <int NT = PL_NT>
-__device__ __forceinline__ int block_scan(int v, int* wsum, int& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x = add_pages(x, y);
-  }
-  int before = __shfl_up(x, 1, 64);
-  if (lane == 0) before = 0;
-  __syncthreads();  // the last call's reads of wsum
-  if (lane == 63) wsum[w] = x;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 64; ++i) {
-    before = add_pages(before, i < w ? wsum[i] : 0);
-    total = add_pages(total, wsum[i]);
-  }
-  return before;
-}
-
 // Workspace of the page calls: a header, the copies to make and int lists.
 struct PagesWs {
   int* n;         // [0] copies, [1] the pages below which a compaction leaves all (live)
@@ -347,7 +320,7 @@ __global__ __launch_bounds__(PL_NT) void kv_reserve_kernel(KvSeqs s, const int32
       }
     }
     int sum;
-    const int before = block_scan(need, wsum, sum);
+    const int before = block_scan<PL_NT>(need, wsum, sum);
     if (b < s.B) {
       w.a[b] = add_pages(total, before);
       w.b[b] = src;
@@ -363,7 +336,7 @@ __global__ __launch_bounds__(PL_NT) void kv_reserve_kernel(KvSeqs s, const int32
       is[j] = p < pages && refs[p] == 0;
       mine += is[j];
     }
-    int sum, at = found + block_scan(mine, wsum, sum);
+    int sum, at = found + block_scan<PL_NT>(mine, wsum, sum);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (is[j]) w.a[s.B + at++] = p0 + tid * 4 + j;
@@ -458,14 +431,14 @@ __global__ __launch_bounds__(PL_NT) void kv_compact_kernel(const int32_t* refs, 
   const int tid = threadIdx.x;
   int mine = 0, live;
   for (int p = tid; p < pages; p += PL_NT) mine += refs[p] > 0;
-  block_scan(mine, wsum, live);
+  block_scan<PL_NT>(mine, wsum, live);
   int nsrc = 0, ndst = 0;
   for (int p0 = 0; p0 < pages; p0 += PL_NT) {
     const int p = p0 + tid;
     const int r = p < pages ? refs[p] : 0;
     const bool src = p < pages && r > 0 && p >= live, dst = p < live && r <= 0;
     int sum;
-    const int at = block_scan(src | dst << 16, wsum, sum);
+    const int at = block_scan<PL_NT>(src | dst << 16, wsum, sum);
     if (src) w.pairs[nsrc + (at & 0xffff)].x = p;
     if (dst) w.pairs[ndst + (at >> 16)].y = p;
     if (p < pages) {
@@ -521,172 +494,6 @@ __global__ __launch_bounds__(64) void kv_free_kernel(KvSeqs s, const int32_t* __
     *e = -1;
   }
   if (lane == 0 && left != len) s.lens[b] = left;
-}
-
-// ---- sequences that begin alike --------------------------------------------------------------------------------------
-// A wave a sequence finds the lowest sequence of its class (the same number, or first page) and how far their tables agree, 256
-// entries at a time; the workgroup that finishes last makes the plan of what all have found: for each class the length that
-// saves the most tiles' reads, then places and lists. Loops over all pairs of sequences go through LDS, up to SH_MOST sequences
-// (through the plan past that).
-constexpr int SH_NT = 256;
-constexpr int SH_MOST = 1024;
-constexpr int SH_AHEAD = SHARE_AHEAD;
-constexpr int SH_KEYS = 2048;  // classes and first positions of sequences, in LDS at a time
-
-// The class of sequence b, -1 if it is in none.
-__device__ __forceinline__ int share_key(const int32_t* group, const KvStep& st, int pages, int page, int b, const Seq& q) {
-  const int n = q.r1 - q.r0, key = group ? group[b] : page_of(st.table, st.max_blocks, pages, b, 0);
-  const int64_t whole = int64_t(min(max(q.first, 0) / page, st.max_blocks)) * page;
-  return n >= 1 && n <= SHARE_ROWS && !too_many(st, q) && whole >= SHARE_TILE && key >= 0 && (!group || key < st.B) ? key : -1;
-}
-
-template <bool LDS>
-__global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restrict__ group, KvStep st, int pages, int page,
-                                                         Share sh) {
-  __shared__ int wsum[SH_NT / 64];
-  __shared__ union {
-    int2 keys[SH_KEYS];
-    struct {
-      int4 found[LDS ? SH_MOST : 1];  // (a multiple of SH_AHEAD, as the plan's)
-      unsigned long long best[LDS ? SH_MOST : 1];
-    } all;
-  } lds;
-  __shared__ int last;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-
-  for (int b0 = blockIdx.x * (SH_NT / 64); b0 < st.B; b0 += gridDim.x * (SH_NT / 64)) {
-    const int b = b0 + wave;
-    Seq q{};
-    int key = -1, rep = -1, first = 0, same = 0;  // rep: the lowest of the class, first: the position of its first row
-    if (b < st.B) {
-      q = seq_of(st, b);
-      key = share_key(group, st, pages, page, b, q);
-    }
-    for (int k0 = 0; k0 < min(b0 + SH_NT / 64, st.B); k0 += SH_KEYS) {
-      __syncthreads();  // the keys' last use
-      for (int i = tid; i < min(SH_KEYS, min(b0 + SH_NT / 64, st.B) - k0); i += SH_NT) {
-        const Seq s = seq_of(st, k0 + i);
-        lds.keys[i] = make_int2(share_key(group, st, pages, page, k0 + i, s), s.first);
-      }
-      __syncthreads();
-      for (int i = 0; key >= 0 && rep < 0 && i < min(SH_KEYS, b + 1 - k0); i += 64) {
-        const uint64_t hit = __ballot(i + lane < min(SH_KEYS, b + 1 - k0) && lds.keys[i + lane].x == key);
-        if (hit) {
-          const int at = i + __ffsll((unsigned long long)hit) - 1;
-          rep = k0 + at;
-          first = lds.keys[at].y;
-        }
-      }
-    }
-    if (rep >= 0) {
-      const int most = min(min(q.first, first) / page, st.max_blocks);
-      const int32_t *x = st.table + size_t(b) * st.max_blocks, *y = st.table + size_t(rep) * st.max_blocks;
-      constexpr int AHEAD = 4;
-      for (bool all = true; all && same < most;) {
-        int u[AHEAD], v[AHEAD];
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-          const int j = min(same + k * 64 + lane, most - 1);
-          u[k] = x[j], v[k] = y[j];
-        }
-        const int from = same;
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-          const bool ok = from + k * 64 + lane < most && u[k] == v[k] && u[k] >= 0 && u[k] < pages;
-          const uint64_t bad = ~__ballot(ok);
-          if (all) same += bad ? __ffsll((unsigned long long)bad) - 1 : 64;
-          all = all && !bad;
-        }
-      }
-    }
-    if (b < st.B && lane < 4) {
-      const int tiles = int(int64_t(same) * page / SHARE_TILE);
-      const int v = lane == 0 ? rep : lane == 1 ? tiles : lane == 2 ? q.r1 - q.r0 : q.first;
-      __hip_atomic_store(&reinterpret_cast<int*>(sh.found + b)[lane], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-  }
-  // (through to memory, as the attention's partial sums go; the last workgroup reads them from there)
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0)
-    last = __hip_atomic_fetch_add(&sh.head->done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-  __syncthreads();
-  if (!last) return;
-
-  // f(i, what was found of sequence i), in order: SH_AHEAD reads on their way at a time
-  const auto for_all = [&](int4* found, auto f) {
-    for (int i0 = 0; i0 < st.B; i0 += SH_AHEAD) {
-      int4 v[SH_AHEAD];
-#pragma unroll
-      for (int k = 0; k < SH_AHEAD; ++k) v[k] = found[i0 + k];
-#pragma unroll
-      for (int k = 0; k < SH_AHEAD; ++k) f(i0 + k, v[k]);
-    }
-  };
-  int4* found = LDS ? lds.all.found : sh.found;  // {lowest of the class, tiles in common with it, rows, position of the first}
-  unsigned long long* best = LDS ? lds.all.best : sh.best;  // by the class's lowest: saved, then tiles (25 bits)
-  for (int b = tid; b < st.B; b += SH_NT) {
-    int v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      v[k] = __hip_atomic_load(&reinterpret_cast<int*>(sh.found + b)[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    found[b] = make_int4(v[0], v[1], v[2], v[3]);
-    best[b] = 0;
-  }
-  if (tid < SH_AHEAD && st.B + tid < (st.B + SH_AHEAD - 1) / SH_AHEAD * SH_AHEAD) found[st.B + tid] = make_int4(-2, 0, 0, 0);
-  __syncthreads();
-  // what each length would save: the tiles of all but one of the sequences that are as long
-  for (int b = tid; b < st.B; b += SH_NT) {
-    const int r = found[b].x, t = found[b].y;
-    if (r < 0 || t == 0) continue;
-    int count = 0;
-    for_all(found, [&](int, const int4& f) { count += int(f.x == r) & int(f.y >= t); });
-    if (count > 1) atomicMax(&best[r], (unsigned long long)min(int64_t(count - 1) * t, int64_t(1) << 38) << 25 | (unsigned long long)t);
-  }
-  __syncthreads();
-  // places: the groups in the order of their lowest sequences, their rows in the order of the slots
-  int groups = 0, list = 0;
-  for (int b0 = 0; b0 < st.B; b0 += SH_NT) {
-    const int b = b0 + tid, r = b < st.B ? found[b].x : -1;
-    const int t = r >= 0 ? int(best[r] & 0x1ffffff) : 0;
-    const bool member = t > 0 && found[b].y >= t;
-    int at = 0, all = 0, lowest = INT32_MAX;
-    if (member)
-      for_all(found, [&](int i, const int4& f) {
-        const bool in = int(f.x == r) & int(f.y >= t);
-        const int n = in ? f.z : 0;
-        all += n;
-        at += i < b ? n : 0;
-        lowest = min(lowest, in ? f.w : INT32_MAX);
-      });
-    const bool head = member && r == b;  // (the lowest of a class is as long as any of it)
-    int sum, many;
-    const int g = groups + block_scan<SH_NT>(head, wsum, many), row0 = list + block_scan<SH_NT>(head ? all : 0, wsum, sum);
-    groups += many;
-    list += sum;
-    if (head) sh.groups[g] = ShareGroup{row0, all, t, b, lowest, {0, 0, 0}};
-    if (b < st.B) sh.seqs[b] = ShareSeq{member ? t : 0, at, row0, g};  // (the last two: the lowest sequence's, for now)
-  }
-  __syncthreads();
-  // (a class's lowest sequence is not written here: all read it)
-  for (int b = tid; b < st.B; b += SH_NT) {
-    ShareSeq s = sh.seqs[b];
-    if (s.tiles == 0) {
-      sh.seqs[b] = ShareSeq{0, 0, 0, 0};
-      continue;
-    }
-    const int4 f = found[b];
-    const ShareSeq head = sh.seqs[f.x];
-    if (f.x != b) sh.seqs[b] = ShareSeq{s.tiles, s.at, head.row0, head.group};
-    const int r0 = seq_of(st, b).r0;
-    for (int i = 0; i < f.z; ++i) sh.list[head.row0 + s.at + i] = make_int2(r0 + i, f.w + i);
-  }
-  if (tid == 0) {
-    ShareHead& h = *sh.head;
-    h.magic = SHARE_MAGIC, h.B = st.B, h.rows = st.rows, h.max_new = st.max_new, h.max_blocks = st.max_blocks, h.page = page;
-    h.groups = groups, h.list = list;
-    __hip_atomic_store(&h.done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // as it was found
-  }
 }
 
 void check_seqs(const char* who, const KvSeqs& s, const int32_t* more, const int32_t* refs, int pages, int page) {
@@ -776,25 +583,6 @@ void kv_append_rope(const bf16* q, int ldq, bf16* qo, int ldqo, int Hq, const bf
   }
   if (!aligned16(wq) || !aligned16(wk)) fail("weights not 16-byte aligned");
   append<true>(who, k, ldk, v, ldv, s, c, AppendTurn{q, qo, wq, wk, ldq, ldqo, Hq, 0, eps, r}, st);
-}
-
-size_t kv_share_plan(int B, int rows) { return B < 0 || rows < 0 ? 0 : carve_share(nullptr, B, rows).bytes; }
-
-void kv_share(const int32_t* group, const KvStep& s, int pages, int page, void* plan, size_t plan_bytes, hipStream_t st) {
-  const auto fail = [](const char* what) { throw std::runtime_error(std::string("kv_share: ") + what); };
-  check_step("kv_share", s);
-  check_pages("kv_share", pages);
-  if (page != 16 && page != 32 && page != 64 && page != 128) fail("page must be 16, 32, 64 or 128");
-  if (s.B > (1 << 24)) fail("B > 2^24");
-  if (!plan) fail("null plan");
-  if (!aligned16(plan)) fail("plan not 16-byte aligned");
-  if (plan_bytes < kv_share_plan(s.B, s.rows)) fail("plan too small");
-  if (s.B == 0 || s.rows == 0 || s.max_new == 0) return;
-  const Share sh = carve_share(plan, s.B, s.rows);
-  const unsigned grid = std::min(cdiv(s.B, SH_NT / 64), 256u);
-  if (s.B <= SH_MOST) kv_share_kernel<true><<<grid, SH_NT, 0, st>>>(group, s, pages, page, sh);
-  else kv_share_kernel<false><<<grid, SH_NT, 0, st>>>(group, s, pages, page, sh);
-  UH_CHECK_LAUNCH();
 }
 
 size_t kv_pages_workspace(int B, int pages) { return B < 0 || pages < 0 ? 0 : carve_pages(nullptr, B, pages).bytes; }

@@ -1,0 +1,601 @@
+// Attention of sequences that begin alike over the 8-bit paged key / value cache: who shares what, and the attention that reads it
+// once (include/unholy/kernels/kv_cache.hpp has the contracts).
+#include "kv_attend_core.hpp"
+
+namespace unholy::kernels {
+
+using namespace uh;
+using namespace kv;
+
+namespace {
+
+// ---- the plan ---------------------------------------------------------------------------------------------------------
+// A wave a sequence finds the lowest sequence of its class (the same number, or first page) and how far their tables agree, 256
+// entries at a time; the workgroup that finishes last makes the plan of what all have found: for each class the length that
+// saves the most tiles' reads, then places and lists. Loops over all pairs of sequences go through LDS, up to SH_MOST sequences
+// (through the plan past that).
+constexpr int SH_NT = 256;
+constexpr int SH_MOST = 1024;
+constexpr int SH_AHEAD = SHARE_AHEAD;
+constexpr int SH_KEYS = 2048;  // classes and first positions of sequences, in LDS at a time
+
+// The class of sequence b, -1 if it is in none.
+__device__ __forceinline__ int share_key(const int32_t* group, const KvStep& st, int pages, int page, int b, const Seq& q) {
+  const int n = q.r1 - q.r0, key = group ? group[b] : page_of(st.table, st.max_blocks, pages, b, 0);
+  const int64_t whole = int64_t(min(max(q.first, 0) / page, st.max_blocks)) * page;
+  return n >= 1 && n <= SHARE_ROWS && !too_many(st, q) && whole >= SHARE_TILE && key >= 0 && (!group || key < st.B) ? key : -1;
+}
+
+template <bool LDS>
+__global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restrict__ group, KvStep st, int pages, int page,
+                                                         Share sh) {
+  __shared__ int wsum[SH_NT / 64];
+  __shared__ union {
+    int2 keys[SH_KEYS];
+    struct {
+      int4 found[LDS ? SH_MOST : 1];  // (a multiple of SH_AHEAD, as the plan's)
+      unsigned long long best[LDS ? SH_MOST : 1];
+    } all;
+  } lds;
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+
+  for (int b0 = blockIdx.x * (SH_NT / 64); b0 < st.B; b0 += gridDim.x * (SH_NT / 64)) {
+    const int b = b0 + wave;
+    Seq q{};
+    int key = -1, rep = -1, first = 0, same = 0;  // rep: the lowest of the class, first: the position of its first row
+    if (b < st.B) {
+      q = seq_of(st, b);
+      key = share_key(group, st, pages, page, b, q);
+    }
+    for (int k0 = 0; k0 < min(b0 + SH_NT / 64, st.B); k0 += SH_KEYS) {
+      __syncthreads();  // the keys' last use
+      for (int i = tid; i < min(SH_KEYS, min(b0 + SH_NT / 64, st.B) - k0); i += SH_NT) {
+        const Seq s = seq_of(st, k0 + i);
+        lds.keys[i] = make_int2(share_key(group, st, pages, page, k0 + i, s), s.first);
+      }
+      __syncthreads();
+      for (int i = 0; key >= 0 && rep < 0 && i < min(SH_KEYS, b + 1 - k0); i += 64) {
+        const uint64_t hit = __ballot(i + lane < min(SH_KEYS, b + 1 - k0) && lds.keys[i + lane].x == key);
+        if (hit) {
+          const int at = i + __ffsll((unsigned long long)hit) - 1;
+          rep = k0 + at;
+          first = lds.keys[at].y;
+        }
+      }
+    }
+    if (rep >= 0) {
+      const int most = min(min(q.first, first) / page, st.max_blocks);
+      const int32_t *x = st.table + size_t(b) * st.max_blocks, *y = st.table + size_t(rep) * st.max_blocks;
+      constexpr int AHEAD = 4;
+      for (bool all = true; all && same < most;) {
+        int u[AHEAD], v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const int j = min(same + k * 64 + lane, most - 1);
+          u[k] = x[j], v[k] = y[j];
+        }
+        const int from = same;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const bool ok = from + k * 64 + lane < most && u[k] == v[k] && u[k] >= 0 && u[k] < pages;
+          const uint64_t bad = ~__ballot(ok);
+          if (all) same += bad ? __ffsll((unsigned long long)bad) - 1 : 64;
+          all = all && !bad;
+        }
+      }
+    }
+    if (b < st.B && lane < 4) {
+      const int tiles = int(int64_t(same) * page / SHARE_TILE);
+      const int v = lane == 0 ? rep : lane == 1 ? tiles : lane == 2 ? q.r1 - q.r0 : q.first;
+      __hip_atomic_store(&reinterpret_cast<int*>(sh.found + b)[lane], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  // (through to memory, as the attention's partial sums go; the last workgroup reads them from there)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0)
+    last = __hip_atomic_fetch_add(&sh.head->done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+
+  // f(i, what was found of sequence i), in order: SH_AHEAD reads on their way at a time
+  const auto for_all = [&](int4* found, auto f) {
+    for (int i0 = 0; i0 < st.B; i0 += SH_AHEAD) {
+      int4 v[SH_AHEAD];
+#pragma unroll
+      for (int k = 0; k < SH_AHEAD; ++k) v[k] = found[i0 + k];
+#pragma unroll
+      for (int k = 0; k < SH_AHEAD; ++k) f(i0 + k, v[k]);
+    }
+  };
+  int4* found = LDS ? lds.all.found : sh.found;  // {lowest of the class, tiles in common with it, rows, position of the first}
+  unsigned long long* best = LDS ? lds.all.best : sh.best;  // by the class's lowest: saved, then tiles (25 bits)
+  for (int b = tid; b < st.B; b += SH_NT) {
+    int v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[k] = __hip_atomic_load(&reinterpret_cast<int*>(sh.found + b)[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    found[b] = make_int4(v[0], v[1], v[2], v[3]);
+    best[b] = 0;
+  }
+  if (tid < SH_AHEAD && st.B + tid < (st.B + SH_AHEAD - 1) / SH_AHEAD * SH_AHEAD) found[st.B + tid] = make_int4(-2, 0, 0, 0);
+  __syncthreads();
+  // what each length would save: the tiles of all but one of the sequences that are as long
+  for (int b = tid; b < st.B; b += SH_NT) {
+    const int r = found[b].x, t = found[b].y;
+    if (r < 0 || t == 0) continue;
+    int count = 0;
+    for_all(found, [&](int, const int4& f) { count += int(f.x == r) & int(f.y >= t); });
+    if (count > 1) atomicMax(&best[r], (unsigned long long)min(int64_t(count - 1) * t, int64_t(1) << 38) << 25 | (unsigned long long)t);
+  }
+  __syncthreads();
+  // places: the groups in the order of their lowest sequences, their rows in the order of the slots
+  int groups = 0, list = 0;
+  for (int b0 = 0; b0 < st.B; b0 += SH_NT) {
+    const int b = b0 + tid, r = b < st.B ? found[b].x : -1;
+    const int t = r >= 0 ? int(best[r] & 0x1ffffff) : 0;
+    const bool member = t > 0 && found[b].y >= t;
+    int at = 0, all = 0, lowest = INT32_MAX;
+    if (member)
+      for_all(found, [&](int i, const int4& f) {
+        const bool in = int(f.x == r) & int(f.y >= t);
+        const int n = in ? f.z : 0;
+        all += n;
+        at += i < b ? n : 0;
+        lowest = min(lowest, in ? f.w : INT32_MAX);
+      });
+    const bool head = member && r == b;  // (the lowest of a class is as long as any of it)
+    int sum, many;
+    const int g = groups + block_scan<SH_NT>(head, wsum, many), row0 = list + block_scan<SH_NT>(head ? all : 0, wsum, sum);
+    groups += many;
+    list += sum;
+    if (head) sh.groups[g] = ShareGroup{row0, all, t, b, lowest, {0, 0, 0}};
+    if (b < st.B) sh.seqs[b] = ShareSeq{member ? t : 0, at, row0, g};  // (the last two: the lowest sequence's, for now)
+  }
+  __syncthreads();
+  // (a class's lowest sequence is not written here: all read it)
+  for (int b = tid; b < st.B; b += SH_NT) {
+    ShareSeq s = sh.seqs[b];
+    if (s.tiles == 0) {
+      sh.seqs[b] = ShareSeq{0, 0, 0, 0};
+      continue;
+    }
+    const int4 f = found[b];
+    const ShareSeq head = sh.seqs[f.x];
+    if (f.x != b) sh.seqs[b] = ShareSeq{s.tiles, s.at, head.row0, head.group};
+    const int r0 = seq_of(st, b).r0;
+    for (int i = 0; i < f.z; ++i) sh.list[head.row0 + s.at + i] = make_int2(r0 + i, f.w + i);
+  }
+  if (tid == 0) {
+    ShareHead& h = *sh.head;
+    h.magic = SHARE_MAGIC, h.B = st.B, h.rows = st.rows, h.max_new = st.max_new, h.max_blocks = st.max_blocks, h.page = page;
+    h.groups = groups, h.list = list;
+    __hip_atomic_store(&h.done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // as it was found
+  }
+}
+
+// ---- the attention -----------------------------------------------------------------------------------------------------
+// Two launches. In the first, some workgroups take the groups' blocks of PR_ROWS rows over the tiles that their sequences have in
+// common (tiled_part: the rows of up to PR_ROWS / heads sequences share each tile's read and conversion), the others every
+// sequence's own tiles (split_segments), side by side: the first are bound by the matrix and vector units, the second by memory and
+// by loads that depend on each other. All leave partial sums, and the second launch joins them by sequence and head.
+
+// How the workgroups are dealt, worked out by each of them from what the device knows.
+struct Deal {
+  uint32_t common;        // workgroups of the groups' blocks; the others are the sequences'
+  uint32_t blocks, share; // blocks times heads; tiles of a part at most
+  bool single;            // whole blocks, `common` of them at a time
+  Split own;
+};
+constexpr uint32_t NONE = 1u << 30;
+// A block's tile, which its workgroup's waves take together, in sequences' tiles, of which each takes its own.
+constexpr float COMMON_TILE = 1.5f;
+
+// Of group i: blocks of rows, and tiles that its rows see.
+struct GroupWork {
+  ShareGroup g;
+  uint32_t blocks, count;
+};
+__device__ __forceinline__ GroupWork group_work(const Attend& a, int i, int n) {
+  GroupWork w{};
+  if (i < a.st.B / 2 + 1) w.g = a.share.groups[i];  // (with what says whether there are so many on its way)
+  if (i < n) {
+    w.blocks = uint32_t(row_groups(w.g.rows * a.group, PR_ROWS));
+    w.count = uint32_t(tiles_of(a, Seq{0, 0, w.g.tiles * TILE, w.g.first}).count);
+  }
+  return w;
+}
+// Of sequence b: segments, and each one's tiles.
+struct SeqWork {
+  Seq q;
+  Tiles t;
+  uint32_t segs;
+  int list;
+  bool over;
+};
+__device__ __forceinline__ SeqWork seq_work(const Attend& a, int b, bool fits) {
+  SeqWork w{};
+  if (b >= a.st.B) return w;
+  const ShareSeq mine = a.share.seqs[b];
+  w.q = seq_of(a.st, b);
+  w.over = too_many(a.st, w.q);
+  if (is_few(a, w.q)) {
+    w.segs = uint32_t(segments_of<true>(a, w.q));
+    w.t = tiles_of(a, w.q, fits ? mine.tiles : 0);
+    w.list = mine.row0 + mine.at;
+  }
+  return w;
+}
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+struct FindLds {
+  uint32_t sums[AT_WAVES][2];
+  int over[AT_WAVES];
+  int found[12];
+};
+
+// The part `at` of the groups' blocks.
+__device__ __forceinline__ bool find_common(const Attend& a, const Deal& deal, int n, GroupWork w, uint32_t at, BlockPart& p, int& sums) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t heads = uint32_t(a.c.heads);
+  uint32_t from = 0;
+  for (int b0 = 0; b0 < n; b0 += 64) {
+    if (n > 64) w = group_work(a, b0 + lane, n);
+    const uint32_t parts = parts_of(w.count, deal.share), wgs = w.blocks * parts * heads, end = from + wave_scan(wgs);
+    const uint64_t hit = __ballot(at < end);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      const uint32_t in = at - lane_of(end - wgs, l), np = lane_of(parts, l);
+      const int row0 = int(lane_of(w.g.row0, l)), block = int(in / heads / np);
+      p.b = int(lane_of(w.g.seq, l));
+      p.h = int(in % heads);
+      p.index = int(in / heads % np);
+      p.parts = int(np);
+      p.row0 = block * PR_ROWS;
+      p.q = Seq{row0, row0 + int(lane_of(w.g.rows, l)), int(lane_of(w.g.tiles, l)) * TILE, int(lane_of(w.g.first, l))};
+      p.t = tiles_of(a, p.q);
+      const int each = p.t.count / p.parts, more = p.t.count % p.parts;
+      p.i0 = p.index * each + min(p.index, more);
+      p.i1 = p.i0 + each + (p.index < more ? 1 : 0);
+      // whole blocks: a head's rows follow each other in the order of the list; else a workgroup has PR_ROWS places of its own
+      sums = deal.single ? (p.h * a.share.head->list + row0) * a.group + p.row0 : int(at) * PR_ROWS;
+      if (threadIdx.x == 0 && p.index == 0)
+        a.common[(size_t(row0) * a.group / PR_ROWS + (b0 + l) + block) * heads + p.h] = Common{sums, p.parts};
+      return true;
+    }
+    from = lane_of(end, 63);
+  }
+  return false;
+}
+
+// The segment that holds unit u of the sequences', a sequence a thread; found through LDS.
+__device__ __forceinline__ bool find_own(const Attend& a, const Deal& deal, bool fits, SeqWork w, uint32_t u, FindLds& lds, Walk& k) {
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  uint32_t from = 0;
+  for (int b0 = 0; b0 < a.st.B; b0 += AT_NT) {
+    if (a.st.B > AT_NT) w = seq_work(a, b0 + tid, fits);
+    const uint32_t each = units_of(deal.own, uint32_t(w.t.count)), n = w.segs * each;
+    uint32_t end = wave_scan(n);
+    __syncthreads();  // the LDS' last use
+    if (lane == 63) lds.sums[wave][0] = end;
+    if (tid == 0) lds.found[0] = -1;
+    __syncthreads();
+    uint32_t all = from;
+#pragma unroll
+    for (int i = 0; i < AT_WAVES; ++i) {
+      end += i < wave ? lds.sums[i][0] : 0;
+      all += lds.sums[i][0];
+    }
+    end += from;
+    if (u < end && u >= end - n) {
+      int* f = lds.found;
+      const uint32_t seg = (u - (end - n)) / each;
+      f[1] = w.q.r0, f[2] = w.q.r1, f[3] = w.q.len, f[4] = w.q.first;
+      f[5] = w.t.sink_tiles, f[6] = w.t.skip, f[7] = w.t.count, f[8] = w.t.from;
+      f[9] = int(seg), f[10] = int(end - n + seg * each), f[11] = w.list;
+      f[0] = b0 + tid;
+    }
+    __syncthreads();
+    const int b = uniform(lds.found[0]);
+    if (b >= 0) {
+      int f[12];
+#pragma unroll
+      for (int i = 1; i < 12; ++i) f[i] = uniform(lds.found[i]);
+      k.b = b;
+      k.q = Seq{f[1], f[2], f[3], f[4]};
+      k.t = Tiles{f[5], f[6], f[7], f[8]};
+      k.h = f[9] % a.c.heads;
+      k.part = f[9] / a.c.heads;
+      k.at = uint32_t(f[10]);
+      k.list = f[11];
+      return true;
+    }
+    from = all;
+  }
+  return false;
+}
+
+template <int D>
+__global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_shared_kernel(Attend a) {
+  __shared__ __align__(1024) union {
+    typename Tiled<D>::Lds tiled;
+    typename Shape<D>::Lds split;
+  } lds;
+  __shared__ FindLds find;
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t heads = uint32_t(a.c.heads);
+  const bool fits = share_fits(a.share.head, a.st, a.c.page);
+  const int n = fits ? a.share.head->groups : 0;
+
+  // all work: the groups' by every wave for itself, a group a lane; the sequences' by all, a sequence a thread
+  GroupWork g{};
+  uint32_t blocks = 0;
+  float common_tiles = 0.0f;
+  for (int b0 = 0; b0 < max(n, 1); b0 += 64) {
+    g = group_work(a, b0 + lane, n);
+    blocks += lane_of(wave_scan(g.blocks), 63) * heads;
+    common_tiles += wave_add(float(g.blocks * heads) * float(g.count));
+  }
+  SeqWork s{};
+  uint32_t tiles = 0, segs = 0;
+  bool over = false;
+  for (int b0 = 0; b0 < a.st.B; b0 += AT_NT) {
+    s = seq_work(a, b0 + tid, fits);
+    tiles += s.segs * (uint32_t(s.t.count) + START);
+    segs += s.segs;
+    over |= s.over;
+  }
+  tiles = lane_of(wave_scan(tiles), 63);
+  segs = lane_of(wave_scan(segs), 63);
+  over = __any(over);
+  if (lane == 0) {
+    find.sums[wave][0] = tiles;
+    find.sums[wave][1] = segs;
+    find.over[wave] = over;
+  }
+  __syncthreads();
+  tiles = segs = 0;
+  over = false;
+#pragma unroll
+  for (int i = 0; i < AT_WAVES; ++i) {
+    tiles += find.sums[i][0];
+    segs += find.sums[i][1];
+    over |= find.over[i] != 0;
+  }
+
+  // workgroups in proportion, some for each
+  Deal deal{};
+  deal.blocks = blocks;
+  deal.share = NONE;
+  if (blocks) {
+    const float part = COMMON_TILE * common_tiles / (COMMON_TILE * common_tiles + float(tiles));
+    const uint32_t most = gridDim.x - gridDim.x / 8, want = min(max(uint32_t(part * float(gridDim.x)), 1u), most);
+    deal.single = blocks >= want;
+    if (deal.single) {
+      const uint32_t rounds = (blocks + most - 1) / most;
+      deal.common = (blocks + rounds - 1) / rounds;
+    } else {
+      const uint32_t sum = uint32_t(common_tiles + 0.5f), least = max(4u, root(0.2f, sum, blocks));
+      if (n <= 64) deal.share = smallest_share(g.blocks * heads, g.count, sum, blocks, want, least);
+      else deal.share = max((sum + want - blocks - 1) / (want - blocks), least);
+      deal.common = 0;
+      for (int b0 = 0; b0 < n; b0 += 64) {
+        if (n > 64) g = group_work(a, b0 + lane, n);
+        deal.common += lane_of(wave_scan(g.blocks * parts_of(g.count, deal.share)), 63) * heads;
+      }
+    }
+  }
+  const uint32_t target = gridDim.x - deal.common;
+  deal.own.whole = segs * 8 <= target;
+  const uint32_t lo = uint32_t(AT_WAVES);
+  deal.own.share = deal.own.whole ? max((tiles - START * segs + target - segs - 1) / (target - segs), lo)
+                                  : max((tiles + target - 1) / target, lo);
+  deal.own.unit = deal.own.whole ? 1 : deal.own.share;
+
+  if (blockIdx.x < deal.common) {
+    for (uint32_t at = blockIdx.x; at < (deal.single ? blocks : deal.common); at += deal.common) {
+      BlockPart bp;
+      int sums;
+      if (!find_common(a, deal, n, g, at, bp, sums)) break;
+      __syncthreads();  // the LDS' last use
+      tiled_part<D, true>(a, lds.tiled, bp, sums, 0);
+    }
+    return;
+  }
+  const uint32_t wg = blockIdx.x - deal.common;
+  if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(wg), int(target));  // (else the join's to do)
+  Walk w;
+  if (find_own(a, deal, fits, s, wg * deal.own.unit, find, w)) split_segments<D, true>(a, lds.split, last, deal.own, w, wg);
+}
+
+// A workgroup per (sequence, FEW of its rows, head): its own parts and its group's, in that order, four channels of a row a
+// thread, the parts dealt to groups of threads.
+constexpr int SJ_FLIGHT = 8;
+template <int D>
+__global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(Attend a) {
+  __shared__ v4f group_o[AT_NT];
+  __shared__ float2 group_ml[AT_NT];
+  const int tid = threadIdx.x, h = int(blockIdx.x % a.c.heads), part = int(blockIdx.x / a.c.heads % a.most_parts);
+  const int b = int(blockIdx.x / a.c.heads / a.most_parts);
+  const ShareSeq mine = a.share.seqs[b];
+  const Common own = a.own[own_at(a, b, part, h)];
+  const Seq q = seq_of(a.st, b);
+  const int row0 = part * FEW, rows = min((q.r1 - q.r0) * a.group - row0, FEW);
+  if (!is_few(a, q) || rows <= 0) return;
+  const bool fits = share_fits(a.share.head, a.st, a.c.page);
+  // the group's sums of these rows: as many parts for each, which begin at rows of one block or of the next
+  int parts = own.parts, upto = 0, begin0 = 0, begin1 = 0;
+  if (fits && tiles_of(a, q, mine.tiles).from) {
+    const int list = mine.at * a.group + row0, block = list / PR_ROWS;
+    const Common* k = a.common + (size_t(mine.row0) * a.group / PR_ROWS + mine.group + block) * a.c.heads + h;
+    parts += k->parts;
+    begin0 = k->row + list % PR_ROWS;
+    upto = (block + 1) * PR_ROWS - list;  // rows in that block
+    begin1 = upto < rows ? k[a.c.heads].row - upto : 0;
+  }
+  if (parts == 1) return;  // written as it was made
+  const int items = rows * (D / 4), groups = min(max(AT_NT / items, 1), AT_WAVES), gi = tid / items;
+  for (int it = gi < groups ? tid - gi * items : items; it < items; it += AT_NT) {
+    const int r = it / (D / 4), d = it % (D / 4) * 4;
+    float m = -INFINITY, sum = 0.0f;
+    v4f acc{0, 0, 0, 0};
+    for (int k0 = gi; k0 < parts; k0 += SJ_FLIGHT * groups) {
+      v4f y[SJ_FLIGHT];
+      float2 x[SJ_FLIGHT];
+#pragma unroll
+      for (int k = 0; k < SJ_FLIGHT; ++k) {
+        const int p = min(k0 + k * groups, parts - 1);
+        const float *ml = a.sml, *o = a.so;
+        size_t at = size_t((r < upto ? begin0 : begin1) + r) + size_t(p - own.parts) * a.c.heads * PR_ROWS;
+        if (p < own.parts) {
+          const bool alone = own.parts == 1;
+          at = alone ? list_row(a, mine.row0 + mine.at, h, row0 + r) : size_t(((own.row + p) * 2 + (p == 0 ? 1 : 0)) * FEW + r);
+          ml = alone ? a.lml : a.pml, o = alone ? a.lo : a.po;
+        }
+        x[k] = *reinterpret_cast<const float2*>(ml + at * 2);
+        y[k] = *reinterpret_cast<const v4f*>(o + at * D + d);
+      }
+      float m1 = m;
+#pragma unroll
+      for (int k = 0; k < SJ_FLIGHT; ++k) m1 = fmaxf(m1, x[k].x);
+      const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m - ref);
+      m = m1;
+      acc *= al;
+      sum *= al;
+#pragma unroll
+      for (int k = 0; k < SJ_FLIGHT; ++k)
+        if (k0 + k * groups < parts) {
+          const float f = __builtin_amdgcn_exp2f(x[k].x - ref);
+          sum += f * x[k].y;
+          acc += f * y[k];
+        }
+    }
+    if (groups == 1) {
+      store_out<D>(a, q.r0 + (row0 + r) / a.group, h * a.group + (row0 + r) % a.group, d, acc, sum, m, d == 0);
+    } else {
+      group_o[tid] = acc;
+      group_ml[tid] = make_float2(m, sum);
+    }
+  }
+  if (groups == 1) return;
+  __syncthreads();
+  if (tid < items) {
+    float m = -INFINITY, sum = 0.0f;
+    v4f acc{0, 0, 0, 0};
+    for (int k = 0; k < groups; ++k) m = fmaxf(m, group_ml[k * items + tid].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    for (int k = 0; k < groups; ++k) {
+      const float2 x = group_ml[k * items + tid];
+      const float f = __builtin_amdgcn_exp2f(x.x - ref);
+      sum += f * x.y;
+      acc += f * group_o[k * items + tid];
+    }
+    const int r = row0 + tid / (D / 4), d = tid % (D / 4) * 4;
+    store_out<D>(a, q.r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
+  }
+}
+
+// Sequences of up to SHARE_ROWS rows, in a group or alone, are split_segments', the others the tiled kernel's.
+Way shared_way(int rows, int max_new, int group) {
+  return {SHARE_ROWS * group, true, std::min(rows, max_new) > SHARE_ROWS};
+}
+// The workspace: counters and blocks, the groups' and the sequences' records, the sequences' sums (those of one part, the others),
+// the groups' (where the tiled kernel's lie: it is done before).
+struct SharedWs {
+  int64_t blocks;     // of the groups, times heads, at most
+  int64_t sum_rows;   // of the groups' sums
+  int64_t list_rows;  // of the groups, times query heads
+  int64_t segments;   // of the sequences
+  int most_parts;
+  size_t common, own, list, split, bytes;  // offsets; all
+};
+SharedWs carve_shared(int rows, int max_new, int B, int Hq, int heads, int dim) {
+  SharedWs w;
+  const int64_t group = Hq / heads, list = std::min<int64_t>(rows, int64_t(SHARE_ROWS) * B);
+  const int64_t most = std::min<int64_t>(std::min(rows, max_new), SHARE_ROWS);
+  w.blocks = (list * group / PR_ROWS + B / 2 + 1) * heads;
+  w.list_rows = list * Hq;
+  w.sum_rows = std::max<int64_t>(int64_t(target_of(dim)) * PR_ROWS, w.list_rows);
+  w.most_parts = int((most * group + FEW - 1) / FEW);
+  w.segments = int64_t(B) * heads * w.most_parts;
+  const auto up = [](size_t n) { return (n + 15) / 16 * 16; };
+  w.common = kHeadBytes;
+  w.own = up(w.common + size_t(w.blocks) * sizeof(Common));
+  const size_t row = (size_t(dim) + 2) * sizeof(float);
+  w.list = up(w.own + size_t(w.segments) * sizeof(Common));
+  w.split = up(w.list + size_t(w.list_rows) * row);
+  w.bytes = w.split + size_t(target_of(dim)) * 2 * FEW * row + size_t(w.sum_rows) * row;
+  return w;
+}
+
+}  // namespace
+
+size_t kv_attend_shared_workspace(int rows, int max_new, int B, int Hq, int heads, int dim) {
+  if (rows < 0 || max_new < 0 || B < 0 || heads < 1 || Hq < heads || dim < 1) return 0;
+  return std::max(carve_shared(rows, max_new, B, Hq, heads, dim).bytes, kv_attend_workspace(rows, max_new, B, Hq, heads, dim));
+}
+
+void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int Hq, float scale, int window, int sinks,
+                      bf16* out, int ldo, float* lse, const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes,
+                      hipStream_t st) {
+  const char* who = "kv_attend_shared";
+  const auto fail = [&](const char* what) { throw std::runtime_error(std::string(who) + ": " + what); };
+  const size_t need = kv_attend_shared_workspace(s.rows, s.max_new, s.B, Hq, c.heads, c.dim);
+  if (!check_attend(who, q, ldq, s, c, Hq, scale, sinks, out, ldo, ws, ws_bytes, need)) return;
+  if (!plan) fail("null plan");
+  if (!aligned16(plan)) fail("plan not 16-byte aligned");
+  if (plan_bytes < kv_share_plan(s.B, s.rows)) fail("plan too small");
+  const Way way = shared_way(s.rows, s.max_new, Hq / c.heads);
+  Attend a = attend_of(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, way, ws);
+  const SharedWs w = carve_shared(s.rows, s.max_new, s.B, Hq, c.heads, c.dim);
+  const int64_t tiles = std::max<int64_t>(cdiv(size_t(s.max_blocks) * c.page, TILE), 1);
+  const int64_t blocks = (cdiv(size_t(s.rows) * a.group, PR_ROWS) + int64_t(s.B)) * c.heads;
+  if (w.segments * 8 > INT32_MAX || blocks > INT32_MAX || w.blocks > INT32_MAX || w.sum_rows > INT32_MAX ||
+      std::max(w.segments, std::min<int64_t>(std::max(blocks, w.blocks), a.target)) * (tiles + START) > INT32_MAX)
+    fail("rows times blocks past 31 bits");
+  a.share = carve_share(const_cast<void*>(plan), s.B, s.rows);
+  a.most_parts = w.most_parts;
+  char* base = static_cast<char*>(ws);
+  a.common = reinterpret_cast<Common*>(base + w.common);
+  a.own = reinterpret_cast<Common*>(base + w.own);
+  a.lo = reinterpret_cast<float*>(base + w.list);
+  a.lml = a.lo + size_t(w.list_rows) * c.dim;
+  a.so = reinterpret_cast<float*>(base + w.split) + size_t(a.target) * 2 * FEW * (c.dim + 2);
+  a.sml = a.so + size_t(w.sum_rows) * c.dim;
+  if (way.tiled) {
+    a.po = a.so;
+    a.pml = a.po + size_t(a.target) * PR_ROWS * c.dim;
+    launch_tiled(a, blocks, st);
+  }
+  a.po = reinterpret_cast<float*>(base + w.split);
+  a.pml = a.po + size_t(a.target) * 2 * FEW * c.dim;
+  by_dim(c.dim, [&]<int D>() { kv_shared_kernel<D><<<a.target, AT_NT, 0, st>>>(a); });
+  by_dim(c.dim, [&]<int D>() { kv_shared_join_kernel<D><<<unsigned(w.segments), AT_NT, 0, st>>>(a); });
+}
+
+size_t kv_share_plan(int B, int rows) { return B < 0 || rows < 0 ? 0 : carve_share(nullptr, B, rows).bytes; }
+
+void kv_share(const int32_t* group, const KvStep& s, int pages, int page, void* plan, size_t plan_bytes, hipStream_t st) {
+  const auto fail = [](const char* what) { throw std::runtime_error(std::string("kv_share: ") + what); };
+  check_step("kv_share", s);
+  check_pages("kv_share", pages);
+  if (page != 16 && page != 32 && page != 64 && page != 128) fail("page must be 16, 32, 64 or 128");
+  if (s.B > (1 << 24)) fail("B > 2^24");
+  if (!plan) fail("null plan");
+  if (!aligned16(plan)) fail("plan not 16-byte aligned");
+  if (plan_bytes < kv_share_plan(s.B, s.rows)) fail("plan too small");
+  if (s.B == 0 || s.rows == 0 || s.max_new == 0) return;
+  const Share sh = carve_share(plan, s.B, s.rows);
+  const unsigned grid = std::min(cdiv(s.B, SH_NT / 64), 256u);
+  if (s.B <= SH_MOST) kv_share_kernel<true><<<grid, SH_NT, 0, st>>>(group, s, pages, page, sh);
+  else kv_share_kernel<false><<<grid, SH_NT, 0, st>>>(group, s, pages, page, sh);
+  UH_CHECK_LAUNCH();
+}
+
+}  // namespace unholy::kernels
