@@ -14,6 +14,15 @@ pytestmark = pytest.mark.gpu
 GUARD = 0xA5
 
 
+def wide(s):
+    """The step with tables so wide that they could name more than what kv_attend takes by itself."""
+    width = int(128e6 if s.D == 256 else 64e6) // (2 * s.B * s.page * s.Hkv * s.D) + 1
+    if s.max_blocks < width:
+        s.table = np.concatenate([s.table, np.full((s.B, width - s.max_blocks), -1, np.int32)], 1)
+        s.max_blocks = width
+    return s
+
+
 def step_of(rng, groups, alone, Hkv, D, page, n=1, order=None, spare_rows=0):
     """A step of groups [(tokens that begin alike, [further tokens of each])] and sequences alone [tokens], n rows each (or a list
     in the order of the sequences), in slots by `order`; and each slot's group (-1: alone)."""
@@ -26,7 +35,7 @@ def step_of(rng, groups, alone, Hkv, D, page, n=1, order=None, spare_rows=0):
     for g, (p, _) in enumerate(groups):
         slots = np.flatnonzero(label == g)
         s.table[slots, :p // page] = s.table[slots[0], :p // page]
-    return s, label
+    return wide(s), label
 
 
 def share_ref(s, group=None, max_new=None):
@@ -195,6 +204,13 @@ def test_more_sequences_than_lanes(groups, each):
     check(s, 2, label, expect=groups)
 
 
+def test_more_sequences_than_the_plan_has_room_for_in_lds():
+    rng = np.random.default_rng(17)
+    s, label = step_of(rng, [(64, [1, 2])] * 500 + [(80, [0, 3, 1])] * 20, [10] * 5, 1, 64, 16, order=rng.permutation(1065))
+    check(s, 1, expect=520)
+    check_plan(Cache(s), plan_of(Cache(s), label)[0], label)
+
+
 def test_a_block_of_a_group_for_every_workgroup():
     """More blocks than the chip has places: none is cut."""
     rng = np.random.default_rng(70)
@@ -319,8 +335,29 @@ def test_the_same_every_time_and_without_lse():
 
 def test_one_sequence():
     rng = np.random.default_rng(12)
-    check(kv_ref.Step(rng, [1], [300], 1, 64, 16), 4, expect=0)
-    check(kv_ref.Step(rng, [20], [300], 1, 64, 16), 4, expect=0)
+    for n in (1, 20):
+        check(kv_ref.Step(rng, [n], [300], 1, 64, 16), 4, expect=0)
+        check(wide(kv_ref.Step(rng, [n], [300], 1, 64, 16)), 4, expect=0)
+
+
+@pytest.mark.parametrize("n", [1, 7])
+def test_narrow_tables(n):
+    """A step that the other kernels take, in the same workspace."""
+    rng = np.random.default_rng(15)
+    s, _ = step_of(rng, [(200, [3, 9])], [40], 2, 64, 16, n=n)
+    narrow = kv_ref.Step.__new__(kv_ref.Step)
+    narrow.__dict__.update(s.__dict__)
+    narrow.max_blocks = 20
+    narrow.table = np.ascontiguousarray(s.table[:, :20])
+    check(narrow, 8, expect=1)
+    c, d = Cache(s), Cache(narrow)
+    q = randn_bf16(rng, (s.rows, 8, 64))
+    need = call("uh_kv_attend_shared_workspace_size", s.rows, n, s.B, 8, 2, 64)
+    ws = dev(np.concatenate([np.zeros(need, np.uint8), np.full(64, GUARD, np.uint8)]))
+    ref, _, tol, _ = kv_ref.attend(s, from_bf16(q).astype(np.float64), 8, 0.1)
+    for x in (c, d, c, d):
+        got = shared(x, q, 8, 0.1, *plan_of(x), ws=ws)[0]
+        assert (np.abs(from_bf16(got) - ref) <= tol).all()
 
 
 def test_captured_steps_replay_with_other_tables():
@@ -333,7 +370,7 @@ def test_captured_steps_replay_with_other_tables():
         s, _ = step_of(rng, groups, alone, 2, 128, 64, n=n)
         s.rows = rows
         steps.append(s)
-    width, pages = max(s.max_blocks for s in steps), max(s.pages for s in steps)
+    width, pages = max(s.max_blocks for s in steps), max(s.pages for s in steps)  # (wide ones)
     for s in steps:
         s.table = np.concatenate([s.table, np.full((B, width - s.max_blocks), -1, np.int32)], 1)
         extra = pages - s.pages
@@ -385,6 +422,7 @@ def test_after_forks():
     s.cu = np.concatenate(([0], np.cumsum(s.n))).astype(np.int32)
     s.rows = int(s.cu[-1])
     shapes = ((p.pages, Hkv, page, D), (p.pages, Hkv, D, page))
+    s = wide(s)
     s.k, s.v = (kv_ref.encode(rng.standard_normal(x) * 64) for x in shapes)
     s.ks, s.vs = (rng.integers(118, 124, (p.pages, Hkv), dtype=np.uint8) for _ in range(2))
     check(s, Hq, [0, 0, 0, 0, 4, 4, 6], expect=2)

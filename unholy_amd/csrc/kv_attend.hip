@@ -75,7 +75,7 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Atten
   bool over;
   const bool some = find_segment(a, sp, w, over);
   if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(blockIdx.x), int(gridDim.x));  // (else the join's to do)
-  if (some) split_segments<D, false>(a, lds, last, sp, w, blockIdx.x);
+  if (some) split_segments<D>(a, lds, last, sp, w, blockIdx.x);
 }
 
 __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p, bool& over) {

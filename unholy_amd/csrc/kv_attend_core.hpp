@@ -318,10 +318,102 @@ __device__ __forceinline__ void store_out(const Attend& a, int row, int hq, int 
   if (first && a.lse) a.lse[size_t(row) * (a.group * a.c.heads) + hq] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
 }
 
-// A workgroup's segments, from w on (of the launch's workgroups, the wg-th). SH (kv_attend_shared): a sequence's rows, up to
-// SHARE_ROWS times the query heads of a head, go FEW at a time; the tiles that its group has in common are left out, and sums that
-// others belong to are left to kv_shared_join_kernel.
-template <int D, bool SH>
+// A tile of a wave's rows: its keys and values in registers (kr, vr, with their scales' bytes) into the rows' sums. pvt: the page of
+// this lane's values; mid: what to do once the keys are used.
+struct FewRow {
+  int pos, pos_lo, pos_hi, len;  // this lane's row's position, all rows' lowest and highest, the sequence's length
+};
+template <int D, class Mid>
+__device__ __forceinline__ void few_tile(const Attend& a, const uint4 (&kr)[4][Shape<D>::KL], uint32_t (&vr)[Shape<D>::DT][4],
+                                         const bf16x8 (&qf)[2 * Shape<D>::KL], int ksb, int vsb, int pvt, int t0, const FewRow& row,
+                                         int g, v4f (&o)[Shape<D>::DT], float& mx, float& l, Mid mid) {
+  using S = Shape<D>;
+  const float ks = e8m0_to_f32(uint8_t(ksb));
+  v4f s[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    s[j] = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int m = 0; m < S::KL; ++m) {
+      s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].x, kr[j][m].y, ks), qf[2 * m], s[j]);
+      s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].z, kr[j][m].w, ks), qf[2 * m + 1], s[j]);
+    }
+  }
+  mid();
+  // what a row does not see: only in the tiles at the ends of what the rows see
+  const bool masked = t0 + TILE - 1 > row.pos_lo || __any(pvt < 0) ||
+                      (a.window > 0 && int64_t(t0) + a.window <= row.pos_hi && t0 + TILE > a.sinks);
+  uint32_t see = 0xffff;
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s[j] *= a.scale2;
+  if (masked) {
+    see = pvt < 0 ? 0 : seen_bits(row.pos, t0 + 16 * g, a.window, a.sinks);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s[k / 4][k % 4] = see >> k & 1 ? s[k / 4][k % 4] : -INFINITY;
+  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k / 4][k % 4]);
+  top = fmaxf(top, __shfl_xor(top, 16, 64));
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  const float m1 = fmaxf(mx, top), ref = m1 == -INFINITY ? 0.0f : m1;
+  if (__any(m1 != mx)) {
+    const float al = __builtin_amdgcn_exp2f(mx - ref);
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) o[d] *= al;
+    l *= al;
+  }
+  mx = m1;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[j][e] = __builtin_amdgcn_exp2f(s[j][e] - ref);
+      l += s[j][e];
+    }
+  bf16x8 p[2];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[hf][e] = __bf16(s[2 * hf + e / 4][e % 4]);
+  if (masked) {  // slots past the last token hold anything: zero
+    const int n = pvt < 0 ? 0 : min(max(row.len - (t0 + 16 * g), 0), 16);
+    const uint32_t all = vsb == NAN_SCALE ? NAN_CODES : 0;  // its codes are NaN, under a scale that is a number then
+    vsb = all ? 127 : vsb;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        vr[d][k] = (vr[d][k] | all) & first_bytes(n - 4 * k);
+        bad |= nan_bytes(vr[d][k]);
+      }
+    if (__builtin_expect(__any(bad != 0), 0)) {
+      // NaN among the values that some row sees, and 0 x NaN is NaN: they are taken out, and a product of 0 / 1 operands
+      // counts for each row and channel the NaN that it sees.
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) {
+        v4f many = mfma_bf16(nan_ones(vr[d][0], vr[d][1]), bit_ones(see), v4f{0, 0, 0, 0});
+        many = mfma_bf16(nan_ones(vr[d][2], vr[d][3]), bit_ones(see >> 8), many);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          vr[d][k] = no_nan(vr[d][k]);
+          if (many[k] > 0.0f) o[d][k] = __builtin_nanf("");
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (one channel tile at a time: registers)
+      }
+    }
+  }
+  const float vs = e8m0_to_f32(uint8_t(vsb));
+#pragma unroll
+  for (int d = 0; d < S::DT; ++d)
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+      o[d] = mfma_bf16(fp8x8_to_bf16(vr[d][2 * hf], vr[d][2 * hf + 1], vs), p[hf], o[d]);
+}
+
+// A workgroup's segments, from w on (of the launch's workgroups, the wg-th).
+template <int D>
 __device__ __forceinline__ void split_segments(Attend a, typename Shape<D>::Lds& lds, int& last, const Split& sp, Walk w,
                                                uint32_t wg) {
   using S = Shape<D>;
@@ -335,7 +427,6 @@ __device__ __forceinline__ void split_segments(Attend a, typename Shape<D>::Lds&
   int ksb, vsb;
   int pos, my_row, my_hq;     // this lane's row (the last one where there are fewer)
   int pos_lo, pos_hi, nrows;  // of all rows
-  int row0 = 0;               // the first of them, from the sequence's first (row, query head) on
   int i, pk, pv, pk1, pv1;
   const auto token = [&](int i) { return w.t.at(i) * TILE; };
   const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
@@ -364,13 +455,9 @@ __device__ __forceinline__ void split_segments(Attend a, typename Shape<D>::Lds&
   };
   const auto begin = [&] {  // a part: its rows, and its first loads on their way
     nrows = (w.q.r1 - w.q.r0) * a.group;
-    if constexpr (SH) {
-      row0 = w.part * FEW;
-      nrows = min(nrows - row0, FEW);
-    }
     i = pt.i0 + wave;
     if (i < pt.i1) lookup(token(i), pk, pv);
-    const int ri = row0 + min(c, nrows - 1);
+    const int ri = min(c, nrows - 1);
     my_row = w.q.r0 + ri / a.group, my_hq = w.h * a.group + ri % a.group;
     pos = w.q.first + ri / a.group;
     pos_lo = w.q.first;
@@ -398,93 +485,14 @@ __device__ __forceinline__ void split_segments(Attend a, typename Shape<D>::Lds&
       const int t0 = token(i);
       const bool more = i + AT_WAVES < pt.i1;
       const int tn = token(more ? i + AT_WAVES : i);
-      const float ks = e8m0_to_f32(uint8_t(ksb));
-      v4f s[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j] = v4f{0, 0, 0, 0};
-#pragma unroll
-        for (int m = 0; m < S::KL; ++m) {
-          s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].x, kr[j][m].y, ks), qf[2 * m], s[j]);
-          s[j] = mfma_bf16(fp8x8_to_bf16(kr[j][m].z, kr[j][m].w, ks), qf[2 * m + 1], s[j]);
-        }
-      }
       const int pvt = pv;
-      if (more) {
-        pk = pk1, pv = pv1;
-        load_k(tn, pk);
-        if (i + 2 * AT_WAVES < pt.i1) lookup(token(i + 2 * AT_WAVES), pk1, pv1);
-      }
-      // what a row does not see: only in the tiles at the ends of what the rows see
-      const bool masked = t0 + TILE - 1 > pos_lo || __any(pvt < 0) ||
-                          (a.window > 0 && int64_t(t0) + a.window <= pos_hi && t0 + TILE > a.sinks);
-      uint32_t see = 0xffff;
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] *= a.scale2;
-      if (masked) {
-        see = pvt < 0 ? 0 : seen_bits(pos, t0 + 16 * g, a.window, a.sinks);
-#pragma unroll
-        for (int k = 0; k < 16; ++k) s[k / 4][k % 4] = see >> k & 1 ? s[k / 4][k % 4] : -INFINITY;
-      }
-#pragma unroll
-      for (int k = 0; k < 16; ++k) top = fmaxf(top, s[k / 4][k % 4]);
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float m1 = fmaxf(mx, top), ref = m1 == -INFINITY ? 0.0f : m1;
-      if (__any(m1 != mx)) {
-        const float al = __builtin_amdgcn_exp2f(mx - ref);
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d) o[d] *= al;
-        l *= al;
-      }
-      mx = m1;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[j][e] = __builtin_amdgcn_exp2f(s[j][e] - ref);
-          l += s[j][e];
+      few_tile<D>(a, kr, vr, qf, ksb, vsb, pvt, t0, FewRow{pos, pos_lo, pos_hi, w.q.len}, g, o, mx, l, [&] {
+        if (more) {
+          pk = pk1, pv = pv1;
+          load_k(tn, pk);
+          if (i + 2 * AT_WAVES < pt.i1) lookup(token(i + 2 * AT_WAVES), pk1, pv1);
         }
-      bf16x8 p[2];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p[hf][e] = __bf16(s[2 * hf + e / 4][e % 4]);
-      if (masked) {  // slots past the last token hold anything: zero
-        const int n = pvt < 0 ? 0 : min(max(w.q.len - (t0 + 16 * g), 0), 16);
-        const uint32_t all = vsb == NAN_SCALE ? NAN_CODES : 0;  // its codes are NaN, under a scale that is a number then
-        vsb = all ? 127 : vsb;
-        uint32_t bad = 0;
-#pragma unroll
-        for (int d = 0; d < S::DT; ++d)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            vr[d][k] = (vr[d][k] | all) & first_bytes(n - 4 * k);
-            bad |= nan_bytes(vr[d][k]);
-          }
-        if (__builtin_expect(__any(bad != 0), 0)) {
-          // NaN among the values that some row sees, and 0 x NaN is NaN: they are taken out, and a product of 0 / 1 operands
-          // counts for each row and channel the NaN that it sees.
-#pragma unroll
-          for (int d = 0; d < S::DT; ++d) {
-            v4f many = mfma_bf16(nan_ones(vr[d][0], vr[d][1]), bit_ones(see), v4f{0, 0, 0, 0});
-            many = mfma_bf16(nan_ones(vr[d][2], vr[d][3]), bit_ones(see >> 8), many);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              vr[d][k] = no_nan(vr[d][k]);
-              if (many[k] > 0.0f) o[d][k] = __builtin_nanf("");
-            }
-            __builtin_amdgcn_sched_barrier(0);  // (one channel tile at a time: registers)
-          }
-        }
-      }
-      const float vs = e8m0_to_f32(uint8_t(vsb));
-#pragma unroll
-      for (int d = 0; d < S::DT; ++d)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-          o[d] = mfma_bf16(fp8x8_to_bf16(vr[d][2 * hf], vr[d][2 * hf + 1], vs), p[hf], o[d]);
+      });
       if (more) load_v(tn, pv);
     }
 
@@ -492,11 +500,8 @@ __device__ __forceinline__ void split_segments(Attend a, typename Shape<D>::Lds&
     // a thread
     const Part done = pt;
     const uint32_t w0 = wg - uint32_t(done.index);
-    const int r0 = w.q.r0, h = w.h, rows = nrows, part0 = SH ? row0 : 0;
-    const bool joined = SH && w.t.from != 0;  // with a group's
-    const int list = SH ? w.list : 0;
-    if (SH && done.index == 0 && tid == 0) a.own[own_at(a, w.b, w.part, h)] = Common{int(w0), done.parts};
-    again = next_segment<SH>(a, sp, w, wg);
+    const int r0 = w.q.r0, h = w.h, rows = nrows;
+    again = next_segment<false>(a, sp, w, wg);
     if (again) {
       pt = part_of(sp, w, w.at, wg);
       begin();
@@ -527,22 +532,15 @@ __device__ __forceinline__ void split_segments(Attend a, typename Shape<D>::Lds&
         sum += f * ml[k].y;
         acc += f * lds.o[k * S::QUADS + at];
       }
-      if (done.parts == 1 && !joined) {
-        store_out<D>(a, r0 + (part0 + r) / a.group, h * a.group + (part0 + r) % a.group, d, acc, sum, m, d == 0);
+      if (done.parts == 1) {
+        store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
       } else {
         const int slot = int(wg * 2 + (done.index == 0 ? 1 : 0)) * FEW + r;
-        if constexpr (SH) {
-          const bool alone = done.parts == 1;  // (a workgroup may begin many of these, but only one that others go on with)
-          const size_t row = alone ? list_row(a, list, h, part0 + r) : size_t(slot);
-          *reinterpret_cast<v4f*>((alone ? a.lo : a.po) + row * D + d) = acc;
-          if (d == 0) *reinterpret_cast<float2*>((alone ? a.lml : a.pml) + row * 2) = make_float2(m, sum);
-        } else {
-          put4(sums_of(a.po), slot * D + d, acc);
-          if (d == 0) put2(sums_of(a.pml), slot * 2, m, sum);
-        }
+        put4(sums_of(a.po), slot * D + d, acc);
+        if (d == 0) put2(sums_of(a.pml), slot * 2, m, sum);
       }
     }
-    if (SH || done.parts == 1) continue;
+    if (done.parts == 1) continue;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
     __syncthreads();
     if (tid == 0)

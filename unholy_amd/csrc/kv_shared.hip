@@ -178,7 +178,7 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
 // ---- the attention -----------------------------------------------------------------------------------------------------
 // Two launches. In the first, some workgroups take the groups' blocks of PR_ROWS rows over the tiles that their sequences have in
 // common (tiled_part: the rows of up to PR_ROWS / heads sequences share each tile's read and conversion), the others every
-// sequence's own tiles (split_segments), side by side: the first are bound by the matrix and vector units, the second by memory and
+// sequence's own tiles (own_segments), side by side: the first are bound by the matrix and vector units, the second by memory and
 // by loads that depend on each other. All leave partial sums, and the second launch joins them by sequence and head.
 
 // How the workgroups are dealt, worked out by each of them from what the device knows.
@@ -190,39 +190,36 @@ struct Deal {
 };
 constexpr uint32_t NONE = 1u << 30;
 // A block's tile, which its workgroup's waves take together, in sequences' tiles, of which each takes its own.
-constexpr float COMMON_TILE = 1.5f;
+constexpr float COMMON_TILE = 6.0f;
 
-// Of group i: blocks of rows, and tiles that its rows see.
+// Of a group: blocks of rows, and tiles that its rows see.
 struct GroupWork {
-  ShareGroup g;
   uint32_t blocks, count;
 };
-__device__ __forceinline__ GroupWork group_work(const Attend& a, int i, int n) {
-  GroupWork w{};
-  if (i < a.st.B / 2 + 1) w.g = a.share.groups[i];  // (with what says whether there are so many on its way)
-  if (i < n) {
-    w.blocks = uint32_t(row_groups(w.g.rows * a.group, PR_ROWS));
-    w.count = uint32_t(tiles_of(a, Seq{0, 0, w.g.tiles * TILE, w.g.first}).count);
+__device__ __forceinline__ GroupWork group_work(const Attend& a, const ShareGroup& g, bool is) {
+  GroupWork w{0, 0};
+  if (is) {
+    w.blocks = uint32_t(row_groups(g.rows * a.group, PR_ROWS));
+    w.count = uint32_t(tiles_of(a, Seq{0, 0, g.tiles * TILE, g.first}).count);
   }
   return w;
 }
+__device__ __forceinline__ ShareGroup group_at(const Attend& a, int i) { return a.share.groups[min(i, a.st.B / 2)]; }
 // Of sequence b: segments, and each one's tiles.
 struct SeqWork {
   Seq q;
   Tiles t;
   uint32_t segs;
   int list;
-  bool over;
 };
-__device__ __forceinline__ SeqWork seq_work(const Attend& a, int b, bool fits) {
+__device__ __forceinline__ SeqWork seq_work(const Attend& a, int b, const ShareSeq& mine, const Seq& q, bool fits, bool& over) {
   SeqWork w{};
   if (b >= a.st.B) return w;
-  const ShareSeq mine = a.share.seqs[b];
-  w.q = seq_of(a.st, b);
-  w.over = too_many(a.st, w.q);
-  if (is_few(a, w.q)) {
-    w.segs = uint32_t(segments_of<true>(a, w.q));
-    w.t = tiles_of(a, w.q, fits ? mine.tiles : 0);
+  w.q = q;
+  over |= too_many(a.st, q);
+  if (is_few(a, q)) {
+    w.segs = uint32_t(segments_of<true>(a, q));
+    w.t = tiles_of(a, q, fits ? mine.tiles : 0);
     w.list = mine.row0 + mine.at;
   }
   return w;
@@ -234,30 +231,33 @@ __device__ __forceinline__ float wave_add(float v) {
 }
 
 struct FindLds {
+  ShareGroup groups[64];  // the first of them
   uint32_t sums[AT_WAVES][2];
   int over[AT_WAVES];
-  int found[12];
+  int found[AT_WAVES][12];
 };
 
 // The part `at` of the groups' blocks.
-__device__ __forceinline__ bool find_common(const Attend& a, const Deal& deal, int n, GroupWork w, uint32_t at, BlockPart& p, int& sums) {
+__device__ __forceinline__ bool find_common(const Attend& a, const Deal& deal, int n, const FindLds& lds, uint32_t at, BlockPart& p,
+                                            int& sums) {
   const int lane = threadIdx.x & 63;
   const uint32_t heads = uint32_t(a.c.heads);
   uint32_t from = 0;
   for (int b0 = 0; b0 < n; b0 += 64) {
-    if (n > 64) w = group_work(a, b0 + lane, n);
+    const ShareGroup g = b0 ? group_at(a, b0 + lane) : lds.groups[lane];
+    const GroupWork w = group_work(a, g, b0 + lane < n);
     const uint32_t parts = parts_of(w.count, deal.share), wgs = w.blocks * parts * heads, end = from + wave_scan(wgs);
     const uint64_t hit = __ballot(at < end);
     if (hit) {
       const int l = __ffsll((unsigned long long)hit) - 1;
       const uint32_t in = at - lane_of(end - wgs, l), np = lane_of(parts, l);
-      const int row0 = int(lane_of(w.g.row0, l)), block = int(in / heads / np);
-      p.b = int(lane_of(w.g.seq, l));
+      const int row0 = int(lane_of(g.row0, l)), block = int(in / heads / np);
+      p.b = int(lane_of(g.seq, l));
       p.h = int(in % heads);
       p.index = int(in / heads % np);
       p.parts = int(np);
       p.row0 = block * PR_ROWS;
-      p.q = Seq{row0, row0 + int(lane_of(w.g.rows, l)), int(lane_of(w.g.tiles, l)) * TILE, int(lane_of(w.g.first, l))};
+      p.q = Seq{row0, row0 + int(lane_of(g.rows, l)), int(lane_of(g.tiles, l)) * TILE, int(lane_of(g.first, l))};
       p.t = tiles_of(a, p.q);
       const int each = p.t.count / p.parts, more = p.t.count % p.parts;
       p.i0 = p.index * each + min(p.index, more);
@@ -273,17 +273,19 @@ __device__ __forceinline__ bool find_common(const Attend& a, const Deal& deal, i
   return false;
 }
 
-// The segment that holds unit u of the sequences', a sequence a thread; found through LDS.
+// The segments that hold the first units of the workgroup's waves, u of the first wave: a sequence a thread, found through LDS.
 __device__ __forceinline__ bool find_own(const Attend& a, const Deal& deal, bool fits, SeqWork w, uint32_t u, FindLds& lds, Walk& k) {
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
+  if (tid < AT_WAVES) lds.found[tid][0] = -1;
   uint32_t from = 0;
   for (int b0 = 0; b0 < a.st.B; b0 += AT_NT) {
-    if (a.st.B > AT_NT) w = seq_work(a, b0 + tid, fits);
+    const int b = b0 + tid;
+    bool over = false;
+    if (a.st.B > AT_NT) w = seq_work(a, b, a.share.seqs[min(b, a.st.B - 1)], seq_of(a.st, min(b, a.st.B - 1)), fits, over);
     const uint32_t each = units_of(deal.own, uint32_t(w.t.count)), n = w.segs * each;
     uint32_t end = wave_scan(n);
     __syncthreads();  // the LDS' last use
     if (lane == 63) lds.sums[wave][0] = end;
-    if (tid == 0) lds.found[0] = -1;
     __syncthreads();
     uint32_t all = from;
 #pragma unroll
@@ -292,64 +294,157 @@ __device__ __forceinline__ bool find_own(const Attend& a, const Deal& deal, bool
       all += lds.sums[i][0];
     }
     end += from;
-    if (u < end && u >= end - n) {
-      int* f = lds.found;
-      const uint32_t seg = (u - (end - n)) / each;
-      f[1] = w.q.r0, f[2] = w.q.r1, f[3] = w.q.len, f[4] = w.q.first;
+#pragma unroll
+    for (int i = 0; i < AT_WAVES; ++i) {
+      const uint32_t ui = u + uint32_t(i) * deal.own.unit;
+      if (ui >= end || ui < end - n) continue;
+      int* f = lds.found[i];
+      const uint32_t seg = (ui - (end - n)) / each;
+      f[0] = b, f[1] = w.q.r0, f[2] = w.q.r1, f[3] = w.q.len, f[4] = w.q.first;
       f[5] = w.t.sink_tiles, f[6] = w.t.skip, f[7] = w.t.count, f[8] = w.t.from;
       f[9] = int(seg), f[10] = int(end - n + seg * each), f[11] = w.list;
-      f[0] = b0 + tid;
-    }
-    __syncthreads();
-    const int b = uniform(lds.found[0]);
-    if (b >= 0) {
-      int f[12];
-#pragma unroll
-      for (int i = 1; i < 12; ++i) f[i] = uniform(lds.found[i]);
-      k.b = b;
-      k.q = Seq{f[1], f[2], f[3], f[4]};
-      k.t = Tiles{f[5], f[6], f[7], f[8]};
-      k.h = f[9] % a.c.heads;
-      k.part = f[9] / a.c.heads;
-      k.at = uint32_t(f[10]);
-      k.list = f[11];
-      return true;
     }
     from = all;
+    if (u + (AT_WAVES - 1) * deal.own.unit < all) break;
   }
-  return false;
+  __syncthreads();
+  int f[12];
+#pragma unroll
+  for (int i = 0; i < 12; ++i) f[i] = uniform(lds.found[wave][i]);
+  k.b = f[0];
+  k.q = Seq{f[1], f[2], f[3], f[4]};
+  k.t = Tiles{f[5], f[6], f[7], f[8]};
+  k.h = f[9] % a.c.heads;
+  k.part = f[9] / a.c.heads;
+  k.at = uint32_t(f[10]);
+  k.list = f[11];
+  return k.b >= 0;
+}
+
+// A wave's segments, from w on (of the launch's waves for them, the wv-th): what a sequence has for itself is mostly a few tiles,
+// which four waves would begin and join for a tile each. A sequence's rows, up to SHARE_ROWS times the query heads of a head, go FEW
+// at a time; the tiles that its group has in common are left out, and sums that others belong to are left to
+// kv_shared_join_kernel. (A second tile on its way all the time: no faster, with 128 channels 4 us slower for its registers.)
+template <int D>
+__device__ __forceinline__ void own_segments(Attend a, const Split& sp, Walk w, uint32_t wv) {
+  using S = Shape<D>;
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int mask = a.c.page - 1, sh = a.page_shift;
+  Part pt = part_of(sp, w, wv * sp.unit, wv);
+  uint4 kr[4][S::KL];
+  uint32_t vr[S::DT][4];
+  int ksb, vsb, pk, pv, pk1, pv1;
+  const auto token = [&](int i) { return w.t.at(i) * TILE; };
+  const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
+    pk = page_of(a.st.table, a.st.max_blocks, a.c.pages, w.b, (t0 + 16 * (c >> 2)) >> sh);
+    pv = page_of(a.st.table, a.st.max_blocks, a.c.pages, w.b, (t0 + 16 * g) >> sh);
+  };
+  const auto load_k = [&](int t0, int pk) {
+    const size_t ph = size_t(max(pk, 0)) * a.c.heads + w.h;
+    const uint8_t* p = a.c.k + ((ph << sh) + ((t0 + 16 * (c >> 2) + (c & 3)) & mask)) * D + 16 * g;
+    ksb = a.c.ks[ph];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int m = 0; m < S::KL; ++m) kr[j][m] = ld16(p + 4 * j * D + 64 * m);
+  };
+  const auto load_v = [&](int t0, int pv) {
+    const size_t ph = size_t(max(pv, 0)) * a.c.heads + w.h;
+    const uint8_t* p = a.c.v + ((ph * D + c) << sh) + ((t0 + 16 * g) & mask);
+    vsb = a.c.vs[ph];
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) {
+      const uint4 x = ld16(p);
+      p += 16 << sh;
+      vr[d][0] = x.x, vr[d][1] = x.y, vr[d][2] = x.z, vr[d][3] = x.w;
+    }
+  };
+  for (bool again = true; again;) {
+    // the part's rows, and its first loads on their way
+    const int row0 = w.part * FEW, rows = min((w.q.r1 - w.q.r0) * a.group - row0, FEW);
+    int i = pt.i0;
+    if (i < pt.i1) lookup(token(i), pk, pv);
+    const int ri = row0 + min(c, rows - 1), r = ri / a.group;
+    const int row = w.q.r0 + r, hq = w.h * a.group + ri - r * a.group;
+    const FewRow fr{w.q.first + r, w.q.first, w.q.first + (w.q.r1 - w.q.r0) - 1, w.q.len};
+    bf16x8 qf[2 * S::KL];
+    const bf16* x = a.q + size_t(row) * a.ldq + size_t(hq) * D + 16 * g;
+#pragma unroll
+    for (int m = 0; m < S::KL; ++m) {
+      qf[2 * m] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m));
+      qf[2 * m + 1] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m + 8));
+    }
+    if (i < pt.i1) {
+      load_k(token(i), pk);
+      load_v(token(i), pv);
+      if (i + 1 < pt.i1) lookup(token(i + 1), pk1, pv1);
+    }
+    v4f o[S::DT];
+    float mx = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) o[d] = v4f{0, 0, 0, 0};
+    for (; i < pt.i1; ++i) {
+      const bool more = i + 1 < pt.i1;
+      const int pvt = pv;
+      few_tile<D>(a, kr, vr, qf, ksb, vsb, pvt, token(i), fr, g, o, mx, l, [&] {
+        if (!more) return;
+        pk = pk1, pv = pv1;
+        load_k(token(i + 1), pk);
+        if (i + 2 < pt.i1) lookup(token(i + 2), pk1, pv1);
+      });
+      if (more) load_v(token(i + 1), pv);
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const bool alone = pt.parts == 1;  // (a wave may begin many of these, but only one that others go on with)
+    if (pt.index == 0 && lane == 0) a.own[own_at(a, w.b, w.part, w.h)] = Common{int(wv), pt.parts};
+    if (c < rows && alone && w.t.from == 0) {
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) store_out<D>(a, row, hq, 16 * d + 4 * g, o[d], l, mx, d == 0 && g == 0);
+    } else if (c < rows) {
+      const size_t slot = alone ? list_row(a, w.list, w.h, row0 + c) : (size_t(wv) * 2 + (pt.index == 0 ? 1 : 0)) * FEW + c;
+      float* to = (alone ? a.lo : a.po) + slot * D + 4 * g;
+#pragma unroll
+      for (int d = 0; d < S::DT; ++d) *reinterpret_cast<v4f*>(to + 16 * d) = o[d];
+      if (g == 0) *reinterpret_cast<float2*>((alone ? a.lml : a.pml) + slot * 2) = make_float2(mx, l);
+    }
+    again = next_segment<true>(a, sp, w, wv);
+    if (again) pt = part_of(sp, w, w.at, wv);
+  }
 }
 
 template <int D>
 __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_shared_kernel(Attend a) {
-  __shared__ __align__(1024) union {
-    typename Tiled<D>::Lds tiled;
-    typename Shape<D>::Lds split;
-  } lds;
+  __shared__ __align__(1024) typename Tiled<D>::Lds lds;
   __shared__ FindLds find;
-  __shared__ int last;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const uint32_t heads = uint32_t(a.c.heads);
+
+  // all work: the groups' by every wave for itself, a group a lane; the sequences' by all, a sequence a thread. (Every load that
+  // depends on no other is on its way before one is waited for.)
+  const int b_in = min(tid, a.st.B - 1);
+  ShareGroup g = group_at(a, lane);
+  const ShareSeq mine = a.share.seqs[b_in];
+  const Seq q = seq_of(a.st, b_in);
   const bool fits = share_fits(a.share.head, a.st, a.c.page);
   const int n = fits ? a.share.head->groups : 0;
-
-  // all work: the groups' by every wave for itself, a group a lane; the sequences' by all, a sequence a thread
-  GroupWork g{};
+  if (tid < 64) find.groups[lane] = g;
   uint32_t blocks = 0;
   float common_tiles = 0.0f;
-  for (int b0 = 0; b0 < max(n, 1); b0 += 64) {
-    g = group_work(a, b0 + lane, n);
-    blocks += lane_of(wave_scan(g.blocks), 63) * heads;
-    common_tiles += wave_add(float(g.blocks * heads) * float(g.count));
+  GroupWork gw{0, 0};
+  for (int b0 = 0; b0 < n; b0 += 64) {
+    if (b0) g = group_at(a, b0 + lane);
+    gw = group_work(a, g, b0 + lane < n);
+    blocks += lane_of(wave_scan(gw.blocks), 63) * heads;
+    common_tiles += wave_add(float(gw.blocks * heads) * float(gw.count));
   }
-  SeqWork s{};
-  uint32_t tiles = 0, segs = 0;
   bool over = false;
-  for (int b0 = 0; b0 < a.st.B; b0 += AT_NT) {
-    s = seq_work(a, b0 + tid, fits);
-    tiles += s.segs * (uint32_t(s.t.count) + START);
-    segs += s.segs;
-    over |= s.over;
+  SeqWork s = seq_work(a, tid, mine, q, fits, over);
+  uint32_t tiles = s.segs * (uint32_t(s.t.count) + START), segs = s.segs;
+  for (int b = AT_NT + tid; b < a.st.B; b += AT_NT) {
+    const SeqWork x = seq_work(a, b, a.share.seqs[b], seq_of(a.st, b), fits, over);
+    tiles += x.segs * (uint32_t(x.t.count) + START);
+    segs += x.segs;
   }
   tiles = lane_of(wave_scan(tiles), 63);
   segs = lane_of(wave_scan(segs), 63);
@@ -375,25 +470,28 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_shared_kernel(Atte
   deal.share = NONE;
   if (blocks) {
     const float part = COMMON_TILE * common_tiles / (COMMON_TILE * common_tiles + float(tiles));
-    const uint32_t most = gridDim.x - gridDim.x / 8, want = min(max(uint32_t(part * float(gridDim.x)), 1u), most);
+    // With up to 128 channels a CU has room for two workgroups. One of each kind there: a block's tile takes 1.6 us, and where some
+    // CUs have two blocks, 2.4 to 2.9, which all wait for (64 sequences behind 8003 tokens: 256 workgroups for blocks 27 us, 320
+    // 30, 384 29, 128 33; 256 behind 32768: 207, 237, 208, 356). Two of the blocks' only where the sequences have next to nothing.
+    const uint32_t most = D <= 128 && part < 0.95f ? gridDim.x / 2 : gridDim.x - gridDim.x / 8;
+    const uint32_t want = min(max(uint32_t(part * float(gridDim.x)), 1u), most);
     deal.single = blocks >= want;
     if (deal.single) {
       const uint32_t rounds = (blocks + most - 1) / most;
       deal.common = (blocks + rounds - 1) / rounds;
     } else {
       const uint32_t sum = uint32_t(common_tiles + 0.5f), least = max(4u, root(0.2f, sum, blocks));
-      if (n <= 64) deal.share = smallest_share(g.blocks * heads, g.count, sum, blocks, want, least);
+      if (n <= 64) deal.share = smallest_share(gw.blocks * heads, gw.count, sum, blocks, want, least);
       else deal.share = max((sum + want - blocks - 1) / (want - blocks), least);
-      deal.common = 0;
       for (int b0 = 0; b0 < n; b0 += 64) {
-        if (n > 64) g = group_work(a, b0 + lane, n);
-        deal.common += lane_of(wave_scan(g.blocks * parts_of(g.count, deal.share)), 63) * heads;
+        if (n > 64) gw = group_work(a, group_at(a, b0 + lane), b0 + lane < n);
+        deal.common += lane_of(wave_scan(gw.blocks * parts_of(gw.count, deal.share)), 63) * heads;
       }
     }
   }
-  const uint32_t target = gridDim.x - deal.common;
+  const uint32_t wgs = gridDim.x - deal.common, target = wgs * AT_WAVES;  // for the sequences; their waves
   deal.own.whole = segs * 8 <= target;
-  const uint32_t lo = uint32_t(AT_WAVES);
+  const uint32_t lo = 2;  // tiles that are worth a wave
   deal.own.share = deal.own.whole ? max((tiles - START * segs + target - segs - 1) / (target - segs), lo)
                                   : max((tiles + target - 1) / target, lo);
   deal.own.unit = deal.own.whole ? 1 : deal.own.share;
@@ -402,16 +500,17 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_shared_kernel(Atte
     for (uint32_t at = blockIdx.x; at < (deal.single ? blocks : deal.common); at += deal.common) {
       BlockPart bp;
       int sums;
-      if (!find_common(a, deal, n, g, at, bp, sums)) break;
+      if (!find_common(a, deal, n, find, at, bp, sums)) break;
       __syncthreads();  // the LDS' last use
-      tiled_part<D, true>(a, lds.tiled, bp, sums, 0);
+      tiled_part<D, true>(a, lds, bp, sums, 0);
     }
     return;
   }
   const uint32_t wg = blockIdx.x - deal.common;
-  if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(wg), int(target));  // (else the join's to do)
+  if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(wg), int(wgs));  // (else the join's to do)
   Walk w;
-  if (find_own(a, deal, fits, s, wg * deal.own.unit, find, w)) split_segments<D, true>(a, lds.split, last, deal.own, w, wg);
+  if (!find_own(a, deal, fits, s, wg * AT_WAVES * deal.own.unit, find, w)) return;
+  own_segments<D>(a, deal.own, w, wg * AT_WAVES + uint32_t(wave));
 }
 
 // A workgroup per (sequence, FEW of its rows, head): its own parts and its group's, in that order, four channels of a row a
@@ -421,14 +520,15 @@ template <int D>
 __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(Attend a) {
   __shared__ v4f group_o[AT_NT];
   __shared__ float2 group_ml[AT_NT];
+  constexpr int ROWS = std::min(AT_NT / (D / 4), FEW);  // of a workgroup: a row's four channels a thread
   const int tid = threadIdx.x, h = int(blockIdx.x % a.c.heads), part = int(blockIdx.x / a.c.heads % a.most_parts);
   const int b = int(blockIdx.x / a.c.heads / a.most_parts);
   const ShareSeq mine = a.share.seqs[b];
   const Common own = a.own[own_at(a, b, part, h)];
   const Seq q = seq_of(a.st, b);
-  const int row0 = part * FEW, rows = min((q.r1 - q.r0) * a.group - row0, FEW);
-  if (!is_few(a, q) || rows <= 0) return;
   const bool fits = share_fits(a.share.head, a.st, a.c.page);
+  const int in0 = int(blockIdx.y) * ROWS, row0 = part * FEW + in0, rows = min((q.r1 - q.r0) * a.group - row0, ROWS);
+  if (!is_few(a, q) || rows <= 0) return;
   // the group's sums of these rows: as many parts for each, which begin at rows of one block or of the next
   int parts = own.parts, upto = 0, begin0 = 0, begin1 = 0;
   if (fits && tiles_of(a, q, mine.tiles).from) {
@@ -440,9 +540,9 @@ __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(Attend a) {
     begin1 = upto < rows ? k[a.c.heads].row - upto : 0;
   }
   if (parts == 1) return;  // written as it was made
-  const int items = rows * (D / 4), groups = min(max(AT_NT / items, 1), AT_WAVES), gi = tid / items;
-  for (int it = gi < groups ? tid - gi * items : items; it < items; it += AT_NT) {
-    const int r = it / (D / 4), d = it % (D / 4) * 4;
+  const int items = rows * (D / 4), groups = min(AT_NT / items, AT_WAVES), gi = tid / items, it = tid - gi * items;
+  const int r = it / (D / 4), d = it % (D / 4) * 4;
+  if (gi < groups) {
     float m = -INFINITY, sum = 0.0f;
     v4f acc{0, 0, 0, 0};
     for (int k0 = gi; k0 < parts; k0 += SJ_FLIGHT * groups) {
@@ -455,7 +555,7 @@ __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(Attend a) {
         size_t at = size_t((r < upto ? begin0 : begin1) + r) + size_t(p - own.parts) * a.c.heads * PR_ROWS;
         if (p < own.parts) {
           const bool alone = own.parts == 1;
-          at = alone ? list_row(a, mine.row0 + mine.at, h, row0 + r) : size_t(((own.row + p) * 2 + (p == 0 ? 1 : 0)) * FEW + r);
+          at = alone ? list_row(a, mine.row0 + mine.at, h, row0 + r) : size_t(((own.row + p) * 2 + (p == 0 ? 1 : 0)) * FEW + in0 + r);
           ml = alone ? a.lml : a.pml, o = alone ? a.lo : a.po;
         }
         x[k] = *reinterpret_cast<const float2*>(ml + at * 2);
@@ -496,12 +596,18 @@ __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(Attend a) {
       sum += f * x.y;
       acc += f * group_o[k * items + tid];
     }
-    const int r = row0 + tid / (D / 4), d = tid % (D / 4) * 4;
-    store_out<D>(a, q.r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
+    store_out<D>(a, q.r0 + (row0 + r) / a.group, h * a.group + (row0 + r) % a.group, d, acc, sum, m, d == 0);
   }
 }
 
-// Sequences of up to SHARE_ROWS rows, in a group or alone, are split_segments', the others the tiled kernel's.
+// Whether a step's tables may name so much that it is worth two launches (16 us at least, 23 with 256 channels; kv_attend's one
+// takes 8 and 12, and where all sequences share one prefix as long overall at 64 MB (16 x 1450 tokens of 8 heads of 128, or twice
+// as many of 64), and at 128 MB with 256 channels). Of what they name the launch knows no more than how wide they are.
+bool worth_sharing(const KvStep& s, const KvCache& c) {
+  const double bytes = 2.0 * s.B * s.max_blocks * c.page * c.heads * c.dim;
+  return s.B > 1 && bytes > (c.dim <= 128 ? 64e6 : 128e6);
+}
+// Sequences of up to SHARE_ROWS rows, in a group or alone, are own_segments', the others the tiled kernel's.
 Way shared_way(int rows, int max_new, int group) {
   return {SHARE_ROWS * group, true, std::min(rows, max_new) > SHARE_ROWS};
 }
@@ -530,7 +636,7 @@ SharedWs carve_shared(int rows, int max_new, int B, int Hq, int heads, int dim) 
   const size_t row = (size_t(dim) + 2) * sizeof(float);
   w.list = up(w.own + size_t(w.segments) * sizeof(Common));
   w.split = up(w.list + size_t(w.list_rows) * row);
-  w.bytes = w.split + size_t(target_of(dim)) * 2 * FEW * row + size_t(w.sum_rows) * row;
+  w.bytes = w.split + size_t(target_of(dim)) * AT_WAVES * 2 * FEW * row + size_t(w.sum_rows) * row;
   return w;
 }
 
@@ -551,6 +657,7 @@ void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c,
   if (!plan) fail("null plan");
   if (!aligned16(plan)) fail("plan not 16-byte aligned");
   if (plan_bytes < kv_share_plan(s.B, s.rows)) fail("plan too small");
+  if (!worth_sharing(s, c)) return kv_attend(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, ws, ws_bytes, st);
   const Way way = shared_way(s.rows, s.max_new, Hq / c.heads);
   Attend a = attend_of(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, way, ws);
   const SharedWs w = carve_shared(s.rows, s.max_new, s.B, Hq, c.heads, c.dim);
@@ -566,7 +673,7 @@ void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c,
   a.own = reinterpret_cast<Common*>(base + w.own);
   a.lo = reinterpret_cast<float*>(base + w.list);
   a.lml = a.lo + size_t(w.list_rows) * c.dim;
-  a.so = reinterpret_cast<float*>(base + w.split) + size_t(a.target) * 2 * FEW * (c.dim + 2);
+  a.so = reinterpret_cast<float*>(base + w.split) + size_t(a.target) * AT_WAVES * 2 * FEW * (c.dim + 2);
   a.sml = a.so + size_t(w.sum_rows) * c.dim;
   if (way.tiled) {
     a.po = a.so;
@@ -574,9 +681,9 @@ void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c,
     launch_tiled(a, blocks, st);
   }
   a.po = reinterpret_cast<float*>(base + w.split);
-  a.pml = a.po + size_t(a.target) * 2 * FEW * c.dim;
+  a.pml = a.po + size_t(a.target) * AT_WAVES * 2 * FEW * c.dim;
   by_dim(c.dim, [&]<int D>() { kv_shared_kernel<D><<<a.target, AT_NT, 0, st>>>(a); });
-  by_dim(c.dim, [&]<int D>() { kv_shared_join_kernel<D><<<unsigned(w.segments), AT_NT, 0, st>>>(a); });
+  by_dim(c.dim, [&]<int D>() { kv_shared_join_kernel<D><<<dim3(unsigned(w.segments), unsigned(FEW * D / 4 / AT_NT)), AT_NT, 0, st>>>(a); });
 }
 
 size_t kv_share_plan(int B, int rows) { return B < 0 || rows < 0 ? 0 : carve_share(nullptr, B, rows).bytes; }
