@@ -71,14 +71,17 @@ __device__ __forceinline__ Slot slot_of(int s, int dim, int first, int rot, bool
   return Slot{u < first ? u : u + rot, w >= dim - rot ? -1 : w < first ? w : w + rot, false};
 }
 
-// The two products of a rotation: (cos, sin) of pos * freq, times mscale. The angle in turns: 64 bits, whole turns cut off, what is
-// left of one (at most a half) rounded to fp32, which is off by 2^-25 turns, 2e-7 radians.
+// The two factors of a rotation: (cos, sin) of pos * freq, times mscale. The angle in turns: 64 bits, whole turns cut off, what is
+// left of one (at most a half) as an fp32 number and its rest r, by which the sine and cosine of the first are turned further
+// (the rest is below 2^-25 turns: its square does not matter).
 __device__ __forceinline__ float2 turn_of(int pos, double freq, float mscale) {
+#pragma clang fp contract(off)
   constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
-  const double t = double(pos) * (freq * kTurn);
+  const double t = double(pos) * (freq * kTurn), part = t - rint(t);
+  const float f = float(part), r = float(part - double(f)) * 6.28318530717958647693f;
   float s, c;
-  sincospif(2.0f * float(t - rint(t)), &s, &c);
-  return make_float2(c * mscale, s * mscale);
+  sincospif(2.0f * f, &s, &c);
+  return make_float2(__builtin_fmaf(-r, s, c) * mscale, __builtin_fmaf(r, c, s) * mscale);
 }
 
 // The slot's V pairs rotated; cs: (cos, sin) of each. v: the two pieces one after the other.
