@@ -3,8 +3,8 @@ reference within the bounds that hold for kv_attend (its products and roundings 
 import numpy as np
 import pytest
 
-from tests import kv_ref
-from tests.helpers import from_bf16, randn_bf16
+from tests import kv_ref, rope_ref
+from tests.helpers import from_bf16, randn_bf16, to_bf16
 from tests.test_gpu_kv import Cache, Pool, attend, dev
 from unholy_amd import call
 from unholy_amd.device import DeviceBuffer, Graph, Stream, synchronize
@@ -427,3 +427,62 @@ def test_after_forks():
     s.ks, s.vs = (rng.integers(118, 124, (p.pages, Hkv), dtype=np.uint8) for _ in range(2))
     check(s, Hq, [0, 0, 0, 0, 4, 4, 6], expect=2)
     check(s, Hq, expect=2)
+
+
+def test_a_serving_loop():
+    """Prompts, forks and decode steps as an engine runs them: pages, norms, rotation and the append in one launch, the plan, the
+    attention. The queries and the new keys against 64 bits, the attention against 64 bits over the cache as it is."""
+    rng = np.random.default_rng(16)
+    page, Hkv, Hq, D, B, rot = 16, 2, 8, 64, 7, 32
+    width = int(64e6) // (2 * B * page * Hkv * D) + 1  # tables of what a long context takes
+    p = Pool(rng, [0] * B, 200, page, width, layers=1, Hkv=Hkv, D=D)
+    p.lazy = True
+    freq = rope_ref.frequencies(rot, 10000.0, 2, 8.0, 1.0, 32.0, 4096.0)
+    f, w = dev(freq), to_bf16(1 + 0.3 * rng.standard_normal((2, D)))
+    dw, heads = [dev(x) for x in w], Hq + 2 * Hkv
+    shapes = ((p.pages, Hkv, page, D), (p.pages, Hkv, D, page), (p.pages, Hkv), (p.pages, Hkv))
+
+    def step(n, groups, group=None):
+        assert p.reserve(n).all()
+        s = kv_ref.Step.__new__(kv_ref.Step)
+        s.n, s.B, s.Hkv, s.D, s.page, s.pages, s.lens, s.table, s.max_blocks = list(n), B, Hkv, D, page, p.pages, p.lens, p.table, width
+        s.cu = np.concatenate(([0], np.cumsum(n))).astype(np.int32)
+        s.rows = int(s.cu[-1])
+        c = Cache.__new__(Cache)
+        c.step, (c.k, c.v, c.ks, c.vs), c.cu, c.lens, c.table = s, p.caches, dev(s.cu), p.d[1], p.d[0]
+        x = randn_bf16(rng, (s.rows, heads, D), 2.0 ** float(rng.integers(-2, 3)))
+        qkv, q = dev(x), dev(np.zeros((s.rows, Hq, D), np.uint16))
+        k = qkv.ptr + 2 * Hq * D
+        call("uh_kv_append_rope", qkv, heads * D, q, Hq * D, Hq, dw[0], k, heads * D, dw[1], 1e-6, k + 2 * Hkv * D, heads * D, c.cu,
+             s.rows, max(n), c.lens, c.table, width, B, f, 0, rot, 0, 1.2, *c.arrays(), p.pages, page, Hkv, D, None)
+        synchronize()
+        s.k, s.v, s.ks, s.vs = (b.download(z, np.uint8) for b, z in zip(p.caches, shapes))
+        p.data = [z.reshape(1, p.pages, -1) for z in (s.k, s.v, s.ks, s.vs)]
+        pos = np.concatenate([s.position(b, 0) + np.arange(s.n[b]) for b in range(B)])
+        got = from_bf16(q.download((s.rows, Hq, D), np.uint16)).astype(np.float64)
+        wide_x, wide_w = from_bf16(x).astype(np.float64), from_bf16(w).astype(np.float64)
+        ref, tol = rope_ref.norm_rope(wide_x[:, :Hq], wide_w[0], 1e-6, pos, freq, 0, rot, False, 1.2)
+        assert (np.abs(got - ref) <= tol).all()
+        ref, tol = rope_ref.norm_rope(wide_x[:, Hq:Hq + Hkv], wide_w[1], 1e-6, pos, freq, 0, rot, False, 1.2)
+        for b in range(B):
+            rows = slice(int(s.cu[b]), int(s.cu[b + 1]))
+            unit = 2.0 ** (s.ks[p.table[b, pos[rows] // page]].astype(np.float64) - 127)[..., None]
+            off = np.abs(s.gather(b)[0][pos[rows]] - ref[rows])  # half a step of e4m3: 2^-4, of subnormal codes 2^-10 of the scale
+            assert (off <= 1.01 * (2.0 ** -4 * np.abs(ref[rows]) + tol[rows] + 2.0 ** -10 * unit)).all()
+        plan = plan_of(c, group)
+        assert len(check_plan(c, plan[0], group)[1]) == groups
+        bits = q.download((s.rows, Hq, D), np.uint16)
+        for window, sinks in ((0, 0), (70, 2)):
+            out, lse = shared(c, bits, Hq, D ** -0.5, *plan, window, sinks)
+            ref, rlse, tol, ltol = kv_ref.attend(s, got, Hq, D ** -0.5, window, sinks)
+            assert (np.abs(from_bf16(out) - ref) <= tol).all() and (np.abs(lse - rlse) <= ltol).all()
+
+    step([150, 0, 0, 0, 90, 0, 20], 0)
+    p.fork([-1, 0, 0, 0, -1, 4, -1])
+    step([1, 1, 3, 1, 1, 1, 1], 2)
+    step([1, 1, 1, 5, 2, 1, 1], 2, [0, 0, 0, 0, 4, 4, 6])
+    p.free([1 << 20, 1 << 20, 0, 152, 1 << 20, 40, 3])
+    p.compact(in_place=True)
+    p.fork([-1, -1, 1, -1, -1, -1, -1])
+    step([1, 1, 1, 1, 1, 1, 1], 1)
+    step([2, 0, 1, 17, 1, 1, 1], 1, [0, 0, 0, 0, -1, -1, -1])

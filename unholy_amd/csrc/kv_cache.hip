@@ -278,6 +278,32 @@ __global__ __launch_bounds__(NT) void kv_append_kernel(const bf16* __restrict__ 
 // ---- pages ------------------------------------------------------------------------------------------------------------
 constexpr int PL_NT = 1024;
 
+constexpr int kMany = 1 << 29;  // sums of pages stop here, past any pool
+__device__ __forceinline__ int add_pages(int a, int b) { return min(a + b, kMany); }
+
+// Exclusive prefix of v (0 .. kMany) over the workgroup's threads; total is their sum (wsum: PL_NT / 64 ints of LDS).
+__device__ __forceinline__ int block_scan(int v, int* wsum, int& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x = add_pages(x, y);
+  }
+  int before = __shfl_up(x, 1, 64);
+  if (lane == 0) before = 0;
+  __syncthreads();  // the last call's reads of wsum
+  if (lane == 63) wsum[w] = x;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < PL_NT / 64; ++i) {
+    before = add_pages(before, i < w ? wsum[i] : 0);
+    total = add_pages(total, wsum[i]);
+  }
+  return before;
+}
+
 // Workspace of the page calls: a header, the copies to make and int lists.
 struct PagesWs {
   int* n;         // [0] copies, [1] the pages below which a compaction leaves all (live)
@@ -320,7 +346,7 @@ __global__ __launch_bounds__(PL_NT) void kv_reserve_kernel(KvSeqs s, const int32
       }
     }
     int sum;
-    const int before = block_scan<PL_NT>(need, wsum, sum);
+    const int before = block_scan(need, wsum, sum);
     if (b < s.B) {
       w.a[b] = add_pages(total, before);
       w.b[b] = src;
@@ -336,7 +362,7 @@ __global__ __launch_bounds__(PL_NT) void kv_reserve_kernel(KvSeqs s, const int32
       is[j] = p < pages && refs[p] == 0;
       mine += is[j];
     }
-    int sum, at = found + block_scan<PL_NT>(mine, wsum, sum);
+    int sum, at = found + block_scan(mine, wsum, sum);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (is[j]) w.a[s.B + at++] = p0 + tid * 4 + j;
@@ -431,14 +457,14 @@ __global__ __launch_bounds__(PL_NT) void kv_compact_kernel(const int32_t* refs, 
   const int tid = threadIdx.x;
   int mine = 0, live;
   for (int p = tid; p < pages; p += PL_NT) mine += refs[p] > 0;
-  block_scan<PL_NT>(mine, wsum, live);
+  block_scan(mine, wsum, live);
   int nsrc = 0, ndst = 0;
   for (int p0 = 0; p0 < pages; p0 += PL_NT) {
     const int p = p0 + tid;
     const int r = p < pages ? refs[p] : 0;
     const bool src = p < pages && r > 0 && p >= live, dst = p < live && r <= 0;
     int sum;
-    const int at = block_scan<PL_NT>(src | dst << 16, wsum, sum);
+    const int at = block_scan(src | dst << 16, wsum, sum);
     if (src) w.pairs[nsrc + (at & 0xffff)].x = p;
     if (dst) w.pairs[ndst + (at >> 16)].y = p;
     if (p < pages) {

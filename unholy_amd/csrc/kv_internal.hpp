@@ -33,33 +33,6 @@ __device__ __forceinline__ int page_of(const int32_t* table, int max_blocks, int
   return p >= 0 && p < pages ? p : -1;
 }
 
-constexpr int kMany = 1 << 29;  // sums of pages stop here, past any pool
-__device__ __forceinline__ int add_pages(int a, int b) { return min(a + b, kMany); }
-
-// Exclusive prefix of v (0 .. kMany) over the workgroup's threads; total is their sum (wsum: an int of LDS a wave).
-template <int NT>
-__device__ __forceinline__ int block_scan(int v, int* wsum, int& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x = add_pages(x, y);
-  }
-  int before = __shfl_up(x, 1, 64);
-  if (lane == 0) before = 0;
-  __syncthreads();  // the last call's reads of wsum
-  if (lane == 63) wsum[w] = x;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 64; ++i) {
-    before = add_pages(before, i < w ? wsum[i] : 0);
-    total = add_pages(total, wsum[i]);
-  }
-  return before;
-}
-
 // What kv_share writes and kv_attend_shared reads (device). Sequences of a group read the first `tiles` tiles of SHARE_TILE tokens,
 // whose pages they have in common, together: all rows of its sequences, in the order of the slots, are the group's list.
 constexpr int SHARE_TILE = 64;
@@ -88,6 +61,7 @@ struct Share {
   int2* list;          // [rows] {row of the step, position}
   int4* found;         // [B, up to a multiple of SHARE_AHEAD] kv_share's own: what it knows of each sequence
   unsigned long long* best;  // [B] the same of each class
+  int2* sums;                // [B]
   size_t bytes;
 };
 constexpr int SHARE_AHEAD = 16;
@@ -106,6 +80,7 @@ inline Share carve_share(void* plan, int B, int rows) {
   s.list = reinterpret_cast<int2*>(take(sizeof(int2) * size_t(rows)));
   s.found = reinterpret_cast<int4*>(take(sizeof(int4) * ((size_t(B) + SHARE_AHEAD - 1) / SHARE_AHEAD * SHARE_AHEAD)));
   s.best = reinterpret_cast<unsigned long long*>(take(sizeof(unsigned long long) * size_t(B)));
+  s.sums = reinterpret_cast<int2*>(take(sizeof(int2) * size_t(B)));
   s.bytes = size_t(p - static_cast<char*>(plan));
   return s;
 }

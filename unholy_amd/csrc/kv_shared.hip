@@ -29,12 +29,13 @@ __device__ __forceinline__ int share_key(const int32_t* group, const KvStep& st,
 template <bool LDS>
 __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restrict__ group, KvStep st, int pages, int page,
                                                          Share sh) {
-  __shared__ int wsum[SH_NT / 64];
+  __shared__ int2 wsum[SH_NT / 64];
   __shared__ union {
     int2 keys[SH_KEYS];
     struct {
       int4 found[LDS ? SH_MOST : 1];  // (a multiple of SH_AHEAD, as the plan's)
       unsigned long long best[LDS ? SH_MOST : 1];
+      int2 sums[LDS ? SH_MOST : 1];
     } all;
   } lds;
   __shared__ int last;
@@ -99,18 +100,19 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
   __syncthreads();
   if (!last) return;
 
-  // f(i, what was found of sequence i), in order: SH_AHEAD reads on their way at a time
-  const auto for_all = [&](int4* found, auto f) {
-    for (int i0 = 0; i0 < st.B; i0 += SH_AHEAD) {
-      int4 v[SH_AHEAD];
+  // f(i, the first two of what was found of sequence i), i < n, in order: SH_AHEAD reads on their way at a time
+  const auto for_all = [&](const int4* found, int n, auto f) {
+    for (int i0 = 0; i0 < n; i0 += SH_AHEAD) {
+      int2 v[SH_AHEAD];
 #pragma unroll
-      for (int k = 0; k < SH_AHEAD; ++k) v[k] = found[i0 + k];
+      for (int k = 0; k < SH_AHEAD; ++k) v[k] = *reinterpret_cast<const int2*>(found + i0 + k);
 #pragma unroll
-      for (int k = 0; k < SH_AHEAD; ++k) f(i0 + k, v[k]);
+      for (int k = 0; k < SH_AHEAD; ++k) f(i0 + k, v[k].x, v[k].y);
     }
   };
   int4* found = LDS ? lds.all.found : sh.found;  // {lowest of the class, tiles in common with it, rows, position of the first}
   unsigned long long* best = LDS ? lds.all.best : sh.best;  // by the class's lowest: saved, then tiles (25 bits)
+  int2* sums = LDS ? lds.all.sums : sh.sums;                // by the same: rows of the group, position of the first of them
   for (int b = tid; b < st.B; b += SH_NT) {
     int v[4];
 #pragma unroll
@@ -118,6 +120,7 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
       v[k] = __hip_atomic_load(&reinterpret_cast<int*>(sh.found + b)[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     found[b] = make_int4(v[0], v[1], v[2], v[3]);
     best[b] = 0;
+    sums[b] = make_int2(0, INT32_MAX);
   }
   if (tid < SH_AHEAD && st.B + tid < (st.B + SH_AHEAD - 1) / SH_AHEAD * SH_AHEAD) found[st.B + tid] = make_int4(-2, 0, 0, 0);
   __syncthreads();
@@ -126,46 +129,57 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
     const int r = found[b].x, t = found[b].y;
     if (r < 0 || t == 0) continue;
     int count = 0;
-    for_all(found, [&](int, const int4& f) { count += int(f.x == r) & int(f.y >= t); });
+    for_all(found, st.B, [&](int, int rep, int tiles) { count += int(rep == r) & int(tiles >= t); });
     if (count > 1) atomicMax(&best[r], (unsigned long long)min(int64_t(count - 1) * t, int64_t(1) << 38) << 25 | (unsigned long long)t);
   }
   __syncthreads();
-  // places: the groups in the order of their lowest sequences, their rows in the order of the slots
-  int groups = 0, list = 0;
-  for (int b0 = 0; b0 < st.B; b0 += SH_NT) {
-    const int b = b0 + tid, r = b < st.B ? found[b].x : -1;
-    const int t = r >= 0 ? int(best[r] & 0x1ffffff) : 0;
-    const bool member = t > 0 && found[b].y >= t;
-    int at = 0, all = 0, lowest = INT32_MAX;
-    if (member)
-      for_all(found, [&](int i, const int4& f) {
-        const bool in = int(f.x == r) & int(f.y >= t);
-        const int n = in ? f.z : 0;
-        all += n;
-        at += i < b ? n : 0;
-        lowest = min(lowest, in ? f.w : INT32_MAX);
-      });
-    const bool head = member && r == b;  // (the lowest of a class is as long as any of it)
-    int sum, many;
-    const int g = groups + block_scan<SH_NT>(head, wsum, many), row0 = list + block_scan<SH_NT>(head ? all : 0, wsum, sum);
-    groups += many;
-    list += sum;
-    if (head) sh.groups[g] = ShareGroup{row0, all, t, b, lowest, {0, 0, 0}};
-    if (b < st.B) sh.seqs[b] = ShareSeq{member ? t : 0, at, row0, g};  // (the last two: the lowest sequence's, for now)
+  // who is in a group: found becomes {lowest of the group or -1, rows, position of the first, first row of the step}
+  for (int b = tid; b < st.B; b += SH_NT) {
+    const int4 f = found[b];
+    const int t = f.x >= 0 ? int(best[f.x] & 0x1ffffff) : 0;
+    const bool member = t > 0 && f.y >= t;
+    if (member) {
+      atomicAdd(&sums[f.x].x, f.z);
+      atomicMin(&sums[f.x].y, f.w);
+    }
+    found[b] = make_int4(member ? f.x : -1, f.z, f.w, seq_of(st, b).r0);
   }
   __syncthreads();
-  // (a class's lowest sequence is not written here: all read it)
+  // the groups in the order of their lowest sequences
+  int groups = 0, list = 0;
+  for (int b0 = 0; b0 < st.B; b0 += SH_NT) {
+    const int b = b0 + tid;
+    const bool head = b < st.B && found[b].x == b;  // (the lowest of a class is as long as any of it)
+    const int rows = head ? sums[b].x : 0;
+    const uint32_t g = wave_scan(head), l = wave_scan(uint32_t(rows));
+    __syncthreads();  // the last round's reads
+    if (lane == 63) wsum[wave] = int2{int(g), int(l)};
+    __syncthreads();
+    int at = groups + int(g) - int(head), row0 = list + int(l) - rows;
+#pragma unroll
+    for (int i = 0; i < SH_NT / 64; ++i) {
+      if (i < wave) at += wsum[i].x, row0 += wsum[i].y;
+      groups += wsum[i].x;
+      list += wsum[i].y;
+    }
+    if (head) {
+      sh.groups[at] = ShareGroup{row0, rows, int(best[b] & 0x1ffffff), b, sums[b].y, {0, 0, 0}};
+      sums[b] = make_int2(row0, at);
+    }
+  }
+  __syncthreads();
+  // the rows of a group in the order of the slots
   for (int b = tid; b < st.B; b += SH_NT) {
-    ShareSeq s = sh.seqs[b];
-    if (s.tiles == 0) {
+    const int4 f = found[b];
+    if (f.x < 0) {
       sh.seqs[b] = ShareSeq{0, 0, 0, 0};
       continue;
     }
-    const int4 f = found[b];
-    const ShareSeq head = sh.seqs[f.x];
-    if (f.x != b) sh.seqs[b] = ShareSeq{s.tiles, s.at, head.row0, head.group};
-    const int r0 = seq_of(st, b).r0;
-    for (int i = 0; i < f.z; ++i) sh.list[head.row0 + s.at + i] = make_int2(r0 + i, f.w + i);
+    int at = 0;
+    for_all(found, b, [&](int i, int rep, int rows) { at += int(rep == f.x) & int(i < b) ? rows : 0; });
+    const int2 to = sums[f.x];
+    sh.seqs[b] = ShareSeq{int(best[f.x] & 0x1ffffff), at, to.x, to.y};
+    for (int i = 0; i < f.y; ++i) sh.list[to.x + at + i] = make_int2(f.w + i, f.z + i);
   }
   if (tid == 0) {
     ShareHead& h = *sh.head;
@@ -183,9 +197,9 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
 
 // How the workgroups are dealt, worked out by each of them from what the device knows.
 struct Deal {
-  uint32_t common;        // workgroups of the groups' blocks; the others are the sequences'
-  uint32_t blocks, share; // blocks times heads; tiles of a part at most
-  bool single;            // whole blocks, `common` of them at a time
+  uint32_t common;  // workgroups of the groups' blocks; those behind them are the sequences'
+  uint32_t share;   // tiles of a part at most
+  bool single;      // whole blocks
   Split own;
 };
 constexpr uint32_t NONE = 1u << 30;
@@ -429,13 +443,14 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_shared_kernel(Atte
   const bool fits = share_fits(a.share.head, a.st, a.c.page);
   const int n = fits ? a.share.head->groups : 0;
   if (tid < 64) find.groups[lane] = g;
-  uint32_t blocks = 0;
+  uint32_t blocks = 0, sum = 0;  // (sum: of the blocks' tiles, where these are fewer than the chip takes; past that it may wrap)
   float common_tiles = 0.0f;
   GroupWork gw{0, 0};
   for (int b0 = 0; b0 < n; b0 += 64) {
     if (b0) g = group_at(a, b0 + lane);
     gw = group_work(a, g, b0 + lane < n);
     blocks += lane_of(wave_scan(gw.blocks), 63) * heads;
+    sum += lane_of(wave_scan(gw.blocks * heads * gw.count), 63);
     common_tiles += wave_add(float(gw.blocks * heads) * float(gw.count));
   }
   bool over = false;
@@ -466,21 +481,20 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_shared_kernel(Atte
 
   // workgroups in proportion, some for each
   Deal deal{};
-  deal.blocks = blocks;
   deal.share = NONE;
+  uint32_t wgs = a.target;  // the sequences'
   if (blocks) {
     const float part = COMMON_TILE * common_tiles / (COMMON_TILE * common_tiles + float(tiles));
     // With up to 128 channels a CU has room for two workgroups. One of each kind there: a block's tile takes 1.6 us, and where some
     // CUs have two blocks, 2.4 to 2.9, which all wait for (64 sequences behind 8003 tokens: 256 workgroups for blocks 27 us, 320
     // 30, 384 29, 128 33; 256 behind 32768: 207, 237, 208, 356). Two of the blocks' only where the sequences have next to nothing.
-    const uint32_t most = D <= 128 && part < 0.95f ? gridDim.x / 2 : gridDim.x - gridDim.x / 8;
-    const uint32_t want = min(max(uint32_t(part * float(gridDim.x)), 1u), most);
+    const uint32_t most = D <= 128 && part < 0.95f ? a.target / 2 : a.target - a.target / 8;
+    const uint32_t want = min(max(uint32_t(part * float(a.target)), 1u), most);
     deal.single = blocks >= want;
-    if (deal.single) {
-      const uint32_t rounds = (blocks + most - 1) / most;
-      deal.common = (blocks + rounds - 1) / rounds;
+    if (deal.single) {  // (where they are more than their share of the chip, one after the other)
+      deal.common = blocks;
     } else {
-      const uint32_t sum = uint32_t(common_tiles + 0.5f), least = max(4u, root(0.2f, sum, blocks));
+      const uint32_t least = max(4u, root(0.2f, sum, blocks));
       if (n <= 64) deal.share = smallest_share(gw.blocks * heads, gw.count, sum, blocks, want, least);
       else deal.share = max((sum + want - blocks - 1) / (want - blocks), least);
       for (int b0 = 0; b0 < n; b0 += 64) {
@@ -488,8 +502,9 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_shared_kernel(Atte
         deal.common += lane_of(wave_scan(gw.blocks * parts_of(gw.count, deal.share)), 63) * heads;
       }
     }
+    wgs = a.target - min(deal.common, most);
   }
-  const uint32_t wgs = gridDim.x - deal.common, target = wgs * AT_WAVES;  // for the sequences; their waves
+  const uint32_t target = wgs * AT_WAVES;  // waves
   deal.own.whole = segs * 8 <= target;
   const uint32_t lo = 2;  // tiles that are worth a wave
   deal.own.share = deal.own.whole ? max((tiles - START * segs + target - segs - 1) / (target - segs), lo)
@@ -497,16 +512,13 @@ __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_shared_kernel(Atte
   deal.own.unit = deal.own.whole ? 1 : deal.own.share;
 
   if (blockIdx.x < deal.common) {
-    for (uint32_t at = blockIdx.x; at < (deal.single ? blocks : deal.common); at += deal.common) {
-      BlockPart bp;
-      int sums;
-      if (!find_common(a, deal, n, find, at, bp, sums)) break;
-      __syncthreads();  // the LDS' last use
-      tiled_part<D, true>(a, lds, bp, sums, 0);
-    }
+    BlockPart bp;
+    int sums;
+    if (find_common(a, deal, n, find, blockIdx.x, bp, sums)) tiled_part<D, true>(a, lds, bp, sums, 0);
     return;
   }
   const uint32_t wg = blockIdx.x - deal.common;
+  if (wg >= wgs) return;
   if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(wg), int(wgs));  // (else the join's to do)
   Walk w;
   if (!find_own(a, deal, fits, s, wg * AT_WAVES * deal.own.unit, find, w)) return;
@@ -682,7 +694,9 @@ void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c,
   }
   a.po = reinterpret_cast<float*>(base + w.split);
   a.pml = a.po + size_t(a.target) * AT_WAVES * 2 * FEW * c.dim;
-  by_dim(c.dim, [&]<int D>() { kv_shared_kernel<D><<<a.target, AT_NT, 0, st>>>(a); });
+  // As many workgroups as the chip has room for, or more where there may be more blocks than half of that.
+  const unsigned grid = unsigned(a.target + std::max<int64_t>(w.blocks - a.target / 2, 0));
+  by_dim(c.dim, [&]<int D>() { kv_shared_kernel<D><<<grid, AT_NT, 0, st>>>(a); });
   by_dim(c.dim, [&]<int D>() { kv_shared_join_kernel<D><<<dim3(unsigned(w.segments), unsigned(FEW * D / 4 / AT_NT)), AT_NT, 0, st>>>(a); });
 }
 
