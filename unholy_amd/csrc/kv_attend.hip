@@ -23,7 +23,7 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w,
       w.q = seq_of(a.st, b);
       rows = w.q.r1 - w.q.r0;
       if (is_few(a, w.q)) {
-        segs = uint32_t(segments_of<false>(a, w.q));
+        segs = uint32_t(segments_of(a, w.q));
         w.t = tiles_of(a, w.q);
       }
     }
@@ -68,14 +68,209 @@ __device__ __forceinline__ bool find_segment(const Attend& a, Split& s, Walk& w,
 
 template <int D>
 __global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_split_kernel(Attend a) {
-  __shared__ __align__(16) typename Shape<D>::Lds lds;
+  using S = Shape<D>;
+  __shared__ __align__(16) typename S::Lds lds;
   __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
+  const uint32_t wg = blockIdx.x;
   Split sp;
   Walk w;
   bool over;
   const bool some = find_segment(a, sp, w, over);
-  if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(blockIdx.x), int(gridDim.x));  // (else the join's to do)
-  if (some) split_segments<D>(a, lds, last, sp, w, blockIdx.x);
+  if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(wg), int(gridDim.x));  // (else the join's to do)
+  if (!some) return;
+  Part pt = part_of(sp, w, wg * sp.unit, wg);
+
+  const int mask = a.c.page - 1, sh = a.page_shift;
+  uint4 kr[4][S::KL];
+  uint32_t vr[S::DT][4];
+  bf16x8 qf[2 * S::KL];
+  int ksb, vsb;
+  int pos, my_row, my_hq;     // this lane's row (the last one where there are fewer)
+  int pos_lo, pos_hi, nrows;  // of all rows
+  int i, pk, pv, pk1, pv1;
+  const auto token = [&](int i) { return w.t.at(i) * TILE; };
+  const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
+    pk = page_of(a.st.table, a.st.max_blocks, a.c.pages, w.b, (t0 + 16 * (c >> 2)) >> sh);
+    pv = page_of(a.st.table, a.st.max_blocks, a.c.pages, w.b, (t0 + 16 * g) >> sh);
+  };
+  const auto load_k = [&](int t0, int pk) {
+    const size_t ph = size_t(max(pk, 0)) * a.c.heads + w.h;
+    const uint8_t* p = a.c.k + ((ph << sh) + ((t0 + 16 * (c >> 2) + (c & 3)) & mask)) * D + 16 * g;
+    ksb = a.c.ks[ph];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int m = 0; m < S::KL; ++m) kr[j][m] = ld16(p + 4 * j * D + 64 * m);
+  };
+  const auto load_v = [&](int t0, int pv) {
+    const size_t ph = size_t(max(pv, 0)) * a.c.heads + w.h;
+    const uint8_t* p = a.c.v + ((ph * D + c) << sh) + ((t0 + 16 * g) & mask);
+    vsb = a.c.vs[ph];
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) {
+      const uint4 x = ld16(p);
+      p += 16 << sh;
+      vr[d][0] = x.x, vr[d][1] = x.y, vr[d][2] = x.z, vr[d][3] = x.w;
+    }
+  };
+  const auto begin = [&] {  // a part: its rows, and its first loads on their way
+    nrows = (w.q.r1 - w.q.r0) * a.group;
+    i = pt.i0 + wave;
+    if (i < pt.i1) lookup(token(i), pk, pv);
+    const int ri = min(c, nrows - 1);
+    my_row = w.q.r0 + ri / a.group, my_hq = w.h * a.group + ri % a.group;
+    pos = w.q.first + ri / a.group;
+    pos_lo = w.q.first;
+    pos_hi = w.q.first + (w.q.r1 - w.q.r0) - 1;
+    const bf16* x = a.q + size_t(my_row) * a.ldq + size_t(my_hq) * D + 16 * g;
+#pragma unroll
+    for (int m = 0; m < S::KL; ++m) {
+      qf[2 * m] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m));
+      qf[2 * m + 1] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m + 8));
+    }
+    if (i < pt.i1) {
+      load_k(token(i), pk);
+      load_v(token(i), pv);
+      if (i + AT_WAVES < pt.i1) lookup(token(i + AT_WAVES), pk1, pv1);
+    }
+  };
+
+  begin();
+  for (bool again = true; again;) {
+    v4f o[S::DT];
+    float mx = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) o[d] = v4f{0, 0, 0, 0};
+    for (; i < pt.i1; i += AT_WAVES) {
+      const int t0 = token(i);
+      const bool more = i + AT_WAVES < pt.i1;
+      const int tn = token(more ? i + AT_WAVES : i);
+      const int pvt = pv;
+      few_tile<D>(a, kr, vr, qf, ksb, vsb, pvt, t0, FewRow{pos, pos_lo, pos_hi, w.q.len}, g, o, mx, l, [&] {
+        if (more) {
+          pk = pk1, pv = pv1;
+          load_k(tn, pk);
+          if (i + 2 * AT_WAVES < pt.i1) lookup(token(i + 2 * AT_WAVES), pk1, pv1);
+        }
+      });
+      if (more) load_v(tn, pv);
+    }
+
+    // the part is summed: the next one's loads go out, then the waves' sums of this one are joined, four channels of a row
+    // a thread
+    const Part done = pt;
+    const uint32_t w0 = wg - uint32_t(done.index);
+    const int r0 = w.q.r0, h = w.h, rows = nrows;
+    again = next_segment(a, sp, w, wg);
+    if (again) {
+      pt = part_of(sp, w, w.at, wg);
+      begin();
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    pipe::lds_barrier();  // the last part's use of the LDS
+#pragma unroll
+    for (int d = 0; d < S::DT; ++d) lds.o[wave * S::QUADS + d * 64 + lane] = o[d];
+    if (g == 0) lds.ml[wave][c] = make_float2(mx, l);
+    pipe::lds_barrier();
+#pragma unroll
+    for (int e = 0; e < S::QUADS; e += AT_NT) {
+      const int at = e + tid, r = at & 15, d = at / 64 * 16 + (at >> 4 & 3) * 4;
+      if (r >= rows) continue;
+      float2 ml[AT_WAVES];  // of the waves: maximum and sum
+      float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < AT_WAVES; ++k) {
+        ml[k] = lds.ml[k][r];
+        m = fmaxf(m, ml[k].x);
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      v4f acc{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < AT_WAVES; ++k) {
+        const float f = __builtin_amdgcn_exp2f(ml[k].x - ref);
+        sum += f * ml[k].y;
+        acc += f * lds.o[k * S::QUADS + at];
+      }
+      if (done.parts == 1) {
+        store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
+      } else {
+        const int slot = int(wg * 2 + (done.index == 0 ? 1 : 0)) * FEW + r;
+        put4(sums_of(a.po), slot * D + d, acc);
+        if (d == 0) put2(sums_of(a.pml), slot * 2, m, sum);
+      }
+    }
+    if (done.parts == 1) continue;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
+    __syncthreads();
+    if (tid == 0)
+      last = __hip_atomic_fetch_add(&a.counters[w0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+             uint32_t(done.parts - 1);
+    __syncthreads();
+    if (!last) continue;
+    if (tid == 0)  // as it was found
+      __hip_atomic_store(&a.counters[w0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // The parts are dealt to `groups` of threads, four channels of a row a thread, and the groups joined in LDS. What takes
+    // time are the rounds of reads, about a microsecond each: as many in flight as the registers hold, but not ten where
+    // there are two (sixteen layers of one token over 4097: 160 us; by a group of all threads, eight at a time, 183).
+    const int items = rows * (D / 4), groups = min(max(AT_NT / items, 1), AT_WAVES), gi = tid / items;
+    for (int it = gi < groups ? tid - gi * items : items; it < items; it += AT_NT) {
+      const int r = it / (D / 4), d = it % (D / 4) * 4;
+      float m = -INFINITY, sum = 0.0f;
+      v4f acc{0, 0, 0, 0};
+      const auto add = [&]<int N>(int k0) {  // parts k0, k0 + groups, ... (N of them)
+        v4f y[N];
+        float2 x[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int p = min(k0 + k * groups, done.parts - 1);
+          const int at = (int(w0 + uint32_t(p)) * 2 + (p == 0 ? 1 : 0)) * FEW + r;
+          x[k] = get2(sums_of(a.pml), at * 2);
+          y[k] = get4(sums_of(a.po), at * D + d);
+        }
+        float m1 = m;
+#pragma unroll
+        for (int k = 0; k < N; ++k) m1 = fmaxf(m1, x[k].x);
+        const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m - ref);
+        m = m1;
+        acc *= al;
+        sum *= al;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (k0 + k * groups < done.parts) {
+            const float f = __builtin_amdgcn_exp2f(x[k].x - ref);
+            sum += f * x[k].y;
+            acc += f * y[k];
+          }
+      };
+      if (done.parts <= 2 * groups) add.template operator()<2>(gi % groups);
+      else
+        for (int k0 = gi % groups; k0 < done.parts; k0 += FLIGHT * groups) add.template operator()<FLIGHT>(k0);
+      if (groups == 1) {
+        store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
+      } else {
+        lds.o[tid] = acc;  // (the waves' sums were read before the counter was)
+        lds.group_ml[tid] = make_float2(m, sum);
+      }
+    }
+    if (groups == 1) continue;
+    pipe::lds_barrier();
+    if (tid < items) {
+      float m = -INFINITY, sum = 0.0f;
+      v4f acc{0, 0, 0, 0};
+      for (int k = 0; k < groups; ++k) m = fmaxf(m, lds.group_ml[k * items + tid].x);
+      const float ref = m == -INFINITY ? 0.0f : m;
+      for (int k = 0; k < groups; ++k) {
+        const float2 x = lds.group_ml[k * items + tid];
+        const float f = __builtin_amdgcn_exp2f(x.x - ref);
+        sum += f * x.y;
+        acc += f * lds.o[k * items + tid];
+      }
+      const int r = tid / (D / 4), d = tid % (D / 4) * 4;
+      store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
+    }
+  }
 }
 
 __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p, bool& over) {
@@ -139,19 +334,20 @@ __device__ __forceinline__ bool find_block(const Attend& a, BlockPart& p, bool& 
   return false;
 }
 
-template <int D>
-__global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tiled_kernel(Attend a) {
-  __shared__ __align__(1024) typename Tiled<D>::Lds lds;
-  BlockPart bp;
-  bool over;
-  const bool some = find_block(a, bp, over);
-  if (threadIdx.x == 0 && blockIdx.x < a.target)
-    a.blocks[blockIdx.x] = some && bp.index == 0
-                               ? Block{bp.parts, int(a.c.heads), bp.row0, min(PR_ROWS, (bp.q.r1 - bp.q.r0) * a.group - bp.row0),
-                                       bp.q.r0, bp.h, over, 0}
-                               : Block{0, 0, 0, 0, 0, 0, over, 0};
-  if (some) tiled_part<D, false>(a, lds, bp, 0, blockIdx.x);
-}
+struct FindBlock {
+  using Call = Attend;
+  template <int D>
+  static __device__ __forceinline__ bool find(const Attend& a, BlockPart& bp, int&) {
+    bool over;
+    const bool some = find_block(a, bp, over);
+    if (threadIdx.x == 0 && blockIdx.x < a.target)
+      a.blocks[blockIdx.x] = some && bp.index == 0
+                                 ? Block{bp.parts, int(a.c.heads), bp.row0, min(PR_ROWS, (bp.q.r1 - bp.q.r0) * a.group - bp.row0),
+                                         bp.q.r0, bp.h, over, 0}
+                                 : Block{0, 0, 0, 0, 0, 0, over, 0};
+    return some;
+  }
+};
 
 // The parts of the tiled kernel's blocks, in order. A thread per row and four channels, JOIN parts at a time: few registers and
 // many threads rather than many parts in flight (eight parts of two quads a thread: 5% more for a step of 256 blocks in two
@@ -258,7 +454,7 @@ Attend attend_of(const bf16* q, int ldq, const KvStep& s, const KvCache& c, int 
 }
 void launch_tiled(const Attend& a, int64_t blocks, hipStream_t st) {
   const unsigned grid = std::max(unsigned(blocks), a.target);
-  by_dim(a.c.dim, [&]<int D>() { kv_tiled_kernel<D><<<grid, AT_NT, 0, st>>>(a); });
+  by_dim(a.c.dim, [&]<int D>() { kv_tiled_kernel<D, FindBlock><<<grid, AT_NT, 0, st>>>(a); });
   const dim3 join(a.target, unsigned(PR_ROWS * a.c.dim / 4 / AT_NT));
   by_dim(a.c.dim, [&]<int D>() { kv_join_kernel<D><<<join, AT_NT, 0, st>>>(a); });
 }

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv_internal.hpp"
 #include "numerics.hpp"
@@ -70,7 +71,9 @@ struct Attend {
   uint32_t* counters;  // of finished parts, by the workgroup of the first; zero between launches (split kernel)
   Block* blocks;       // by the workgroup of the first part (tiled kernel; null where it is not launched)
   float *po, *pml;     // partial sums: values [slot][rows][D]; maximum and weight sum [slot][rows][2]
-  // kv_attend_shared's
+};
+// The same of kv_attend_shared. (A struct of its own: kv_attend's kernels have less to load before their first key.)
+struct AttendShared : Attend {
   Share share;
   Common *common, *own;  // by block of a group and head; by sequence, FEW of its rows and head (the first workgroup of these)
   float *so, *sml;       // the groups' partial sums: values [row][D]; maximum and weight sum [row][2]
@@ -78,7 +81,7 @@ struct Attend {
   int most_parts;        // of FEW rows, of a sequence
 };
 
-__device__ __forceinline__ size_t own_at(const Attend& a, int b, int part, int h) {
+__device__ __forceinline__ size_t own_at(const AttendShared& a, int b, int part, int h) {
   return (size_t(b) * a.most_parts + part) * a.c.heads + h;
 }
 
@@ -179,9 +182,9 @@ __device__ __forceinline__ void clear_rows(const Attend& a, int w, int n) {
 }
 
 // A sequence's segments: its heads, times (kv_attend_shared) the parts of FEW rows that it brings.
-template <bool SH>
-__device__ __forceinline__ int segments_of(const Attend& a, const Seq& q) {
-  return SH ? a.c.heads * row_groups((q.r1 - q.r0) * a.group, FEW) : a.c.heads;
+template <class A>
+__device__ __forceinline__ int segments_of(const A& a, const Seq& q) {
+  return std::is_same_v<A, AttendShared> ? a.c.heads * row_groups((q.r1 - q.r0) * a.group, FEW) : a.c.heads;
 }
 __device__ __forceinline__ bool is_few(const Attend& a, const Seq& q) {
   return q.r1 > q.r0 && (q.r1 - q.r0) * a.group <= a.few && !too_many(a.st, q);
@@ -204,8 +207,9 @@ __device__ __forceinline__ Part part_of(const Split& s, const Walk& w, uint32_t 
   return p;
 }
 // The next segment, if the units of workgroup wg reach it.
-template <bool SH>
-__device__ __forceinline__ bool next_segment(const Attend& a, const Split& s, Walk& w, uint32_t wg) {
+template <class A>
+__device__ __forceinline__ bool next_segment(const A& a, const Split& s, Walk& w, uint32_t wg) {
+  constexpr bool SH = std::is_same_v<A, AttendShared>;
   w.at += units_of(s, uint32_t(w.t.count));
   if (s.whole || w.at >= (wg + 1) * s.unit) return false;
   if (++w.h < a.c.heads) return true;
@@ -412,206 +416,6 @@ __device__ __forceinline__ void few_tile(const Attend& a, const uint4 (&kr)[4][S
       o[d] = mfma_bf16(fp8x8_to_bf16(vr[d][2 * hf], vr[d][2 * hf + 1], vs), p[hf], o[d]);
 }
 
-// A workgroup's segments, from w on (of the launch's workgroups, the wg-th).
-template <int D>
-__device__ __forceinline__ void split_segments(Attend a, typename Shape<D>::Lds& lds, int& last, const Split& sp, Walk w,
-                                               uint32_t wg) {
-  using S = Shape<D>;
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 15, g = lane >> 4;
-  Part pt = part_of(sp, w, wg * sp.unit, wg);
-
-  const int mask = a.c.page - 1, sh = a.page_shift;
-  uint4 kr[4][S::KL];
-  uint32_t vr[S::DT][4];
-  bf16x8 qf[2 * S::KL];
-  int ksb, vsb;
-  int pos, my_row, my_hq;     // this lane's row (the last one where there are fewer)
-  int pos_lo, pos_hi, nrows;  // of all rows
-  int i, pk, pv, pk1, pv1;
-  const auto token = [&](int i) { return w.t.at(i) * TILE; };
-  const auto lookup = [&](int t0, int& pk, int& pv) {  // the pages of this lane's key rows and of its values
-    pk = page_of(a.st.table, a.st.max_blocks, a.c.pages, w.b, (t0 + 16 * (c >> 2)) >> sh);
-    pv = page_of(a.st.table, a.st.max_blocks, a.c.pages, w.b, (t0 + 16 * g) >> sh);
-  };
-  const auto load_k = [&](int t0, int pk) {
-    const size_t ph = size_t(max(pk, 0)) * a.c.heads + w.h;
-    const uint8_t* p = a.c.k + ((ph << sh) + ((t0 + 16 * (c >> 2) + (c & 3)) & mask)) * D + 16 * g;
-    ksb = a.c.ks[ph];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int m = 0; m < S::KL; ++m) kr[j][m] = ld16(p + 4 * j * D + 64 * m);
-  };
-  const auto load_v = [&](int t0, int pv) {
-    const size_t ph = size_t(max(pv, 0)) * a.c.heads + w.h;
-    const uint8_t* p = a.c.v + ((ph * D + c) << sh) + ((t0 + 16 * g) & mask);
-    vsb = a.c.vs[ph];
-#pragma unroll
-    for (int d = 0; d < S::DT; ++d) {
-      const uint4 x = ld16(p);
-      p += 16 << sh;
-      vr[d][0] = x.x, vr[d][1] = x.y, vr[d][2] = x.z, vr[d][3] = x.w;
-    }
-  };
-  const auto begin = [&] {  // a part: its rows, and its first loads on their way
-    nrows = (w.q.r1 - w.q.r0) * a.group;
-    i = pt.i0 + wave;
-    if (i < pt.i1) lookup(token(i), pk, pv);
-    const int ri = min(c, nrows - 1);
-    my_row = w.q.r0 + ri / a.group, my_hq = w.h * a.group + ri % a.group;
-    pos = w.q.first + ri / a.group;
-    pos_lo = w.q.first;
-    pos_hi = w.q.first + (w.q.r1 - w.q.r0) - 1;
-    const bf16* x = a.q + size_t(my_row) * a.ldq + size_t(my_hq) * D + 16 * g;
-#pragma unroll
-    for (int m = 0; m < S::KL; ++m) {
-      qf[2 * m] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m));
-      qf[2 * m + 1] = bf16x8_of(*reinterpret_cast<const uint4*>(x + 64 * m + 8));
-    }
-    if (i < pt.i1) {
-      load_k(token(i), pk);
-      load_v(token(i), pv);
-      if (i + AT_WAVES < pt.i1) lookup(token(i + AT_WAVES), pk1, pv1);
-    }
-  };
-
-  begin();
-  for (bool again = true; again;) {
-    v4f o[S::DT];
-    float mx = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int d = 0; d < S::DT; ++d) o[d] = v4f{0, 0, 0, 0};
-    for (; i < pt.i1; i += AT_WAVES) {
-      const int t0 = token(i);
-      const bool more = i + AT_WAVES < pt.i1;
-      const int tn = token(more ? i + AT_WAVES : i);
-      const int pvt = pv;
-      few_tile<D>(a, kr, vr, qf, ksb, vsb, pvt, t0, FewRow{pos, pos_lo, pos_hi, w.q.len}, g, o, mx, l, [&] {
-        if (more) {
-          pk = pk1, pv = pv1;
-          load_k(tn, pk);
-          if (i + 2 * AT_WAVES < pt.i1) lookup(token(i + 2 * AT_WAVES), pk1, pv1);
-        }
-      });
-      if (more) load_v(tn, pv);
-    }
-
-    // the part is summed: the next one's loads go out, then the waves' sums of this one are joined, four channels of a row
-    // a thread
-    const Part done = pt;
-    const uint32_t w0 = wg - uint32_t(done.index);
-    const int r0 = w.q.r0, h = w.h, rows = nrows;
-    again = next_segment<false>(a, sp, w, wg);
-    if (again) {
-      pt = part_of(sp, w, w.at, wg);
-      begin();
-    }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    pipe::lds_barrier();  // the last part's use of the LDS
-#pragma unroll
-    for (int d = 0; d < S::DT; ++d) lds.o[wave * S::QUADS + d * 64 + lane] = o[d];
-    if (g == 0) lds.ml[wave][c] = make_float2(mx, l);
-    pipe::lds_barrier();
-#pragma unroll
-    for (int e = 0; e < S::QUADS; e += AT_NT) {
-      const int at = e + tid, r = at & 15, d = at / 64 * 16 + (at >> 4 & 3) * 4;
-      if (r >= rows) continue;
-      float2 ml[AT_WAVES];  // of the waves: maximum and sum
-      float m = -INFINITY, sum = 0.0f;
-#pragma unroll
-      for (int k = 0; k < AT_WAVES; ++k) {
-        ml[k] = lds.ml[k][r];
-        m = fmaxf(m, ml[k].x);
-      }
-      const float ref = m == -INFINITY ? 0.0f : m;
-      v4f acc{0, 0, 0, 0};
-#pragma unroll
-      for (int k = 0; k < AT_WAVES; ++k) {
-        const float f = __builtin_amdgcn_exp2f(ml[k].x - ref);
-        sum += f * ml[k].y;
-        acc += f * lds.o[k * S::QUADS + at];
-      }
-      if (done.parts == 1) {
-        store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
-      } else {
-        const int slot = int(wg * 2 + (done.index == 0 ? 1 : 0)) * FEW + r;
-        put4(sums_of(a.po), slot * D + d, acc);
-        if (d == 0) put2(sums_of(a.pml), slot * 2, m, sum);
-      }
-    }
-    if (done.parts == 1) continue;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have left
-    __syncthreads();
-    if (tid == 0)
-      last = __hip_atomic_fetch_add(&a.counters[w0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-             uint32_t(done.parts - 1);
-    __syncthreads();
-    if (!last) continue;
-    if (tid == 0)  // as it was found
-      __hip_atomic_store(&a.counters[w0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // The parts are dealt to `groups` of threads, four channels of a row a thread, and the groups joined in LDS. What takes
-    // time are the rounds of reads, about a microsecond each: as many in flight as the registers hold, but not ten where
-    // there are two (sixteen layers of one token over 4097: 160 us; by a group of all threads, eight at a time, 183).
-    const int items = rows * (D / 4), groups = min(max(AT_NT / items, 1), AT_WAVES), gi = tid / items;
-    for (int it = gi < groups ? tid - gi * items : items; it < items; it += AT_NT) {
-      const int r = it / (D / 4), d = it % (D / 4) * 4;
-      float m = -INFINITY, sum = 0.0f;
-      v4f acc{0, 0, 0, 0};
-      const auto add = [&]<int N>(int k0) {  // parts k0, k0 + groups, ... (N of them)
-        v4f y[N];
-        float2 x[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const int p = min(k0 + k * groups, done.parts - 1);
-          const int at = (int(w0 + uint32_t(p)) * 2 + (p == 0 ? 1 : 0)) * FEW + r;
-          x[k] = get2(sums_of(a.pml), at * 2);
-          y[k] = get4(sums_of(a.po), at * D + d);
-        }
-        float m1 = m;
-#pragma unroll
-        for (int k = 0; k < N; ++k) m1 = fmaxf(m1, x[k].x);
-        const float ref = m1 == -INFINITY ? 0.0f : m1, al = __builtin_amdgcn_exp2f(m - ref);
-        m = m1;
-        acc *= al;
-        sum *= al;
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-          if (k0 + k * groups < done.parts) {
-            const float f = __builtin_amdgcn_exp2f(x[k].x - ref);
-            sum += f * x[k].y;
-            acc += f * y[k];
-          }
-      };
-      if (done.parts <= 2 * groups) add.template operator()<2>(gi % groups);
-      else
-        for (int k0 = gi % groups; k0 < done.parts; k0 += FLIGHT * groups) add.template operator()<FLIGHT>(k0);
-      if (groups == 1) {
-        store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
-      } else {
-        lds.o[tid] = acc;  // (the waves' sums were read before the counter was)
-        lds.group_ml[tid] = make_float2(m, sum);
-      }
-    }
-    if (groups == 1) continue;
-    pipe::lds_barrier();
-    if (tid < items) {
-      float m = -INFINITY, sum = 0.0f;
-      v4f acc{0, 0, 0, 0};
-      for (int k = 0; k < groups; ++k) m = fmaxf(m, lds.group_ml[k * items + tid].x);
-      const float ref = m == -INFINITY ? 0.0f : m;
-      for (int k = 0; k < groups; ++k) {
-        const float2 x = lds.group_ml[k * items + tid];
-        const float f = __builtin_amdgcn_exp2f(x.x - ref);
-        sum += f * x.y;
-        acc += f * lds.o[k * items + tid];
-      }
-      const int r = tid / (D / 4), d = tid % (D / 4) * 4;
-      store_out<D>(a, r0 + r / a.group, h * a.group + r % a.group, d, acc, sum, m, d == 0);
-    }
-  }
-}
-
 // ---- many rows a sequence: prompts ------------------------------------------------------------------------------------
 // Bound by the matrix rate and by the vector work next to it: 8192 rows of 32 heads of 128 take 527 to 562 us, 0.98 to 1.04
 // PFLOP/s (a large bf16 product reaches 1.17 here), the matrix units busy for half of the cycles and the vector units for 72%;
@@ -674,11 +478,17 @@ __device__ __forceinline__ Tiles block_tiles(const Attend& a, const Seq& q, int 
   const int last = min(row0 + PR_ROWS, (q.r1 - q.r0) * a.group) - 1;
   return tiles_of(a, Seq{0, 0, max(min(q.len, q.first + last / a.group + 1), 0), q.first + row0 / a.group});
 }
-// A workgroup's part of a block of rows. COMMON (kv_attend_shared): of a group's list, whose sums are partial ones throughout, in
-// rows from `sums` on; else the partial sums of a block in several parts are the wg-th.
-template <int D, bool COMMON>
-__device__ __forceinline__ void tiled_part(Attend a, typename Tiled<D>::Lds& lds, const BlockPart& bp, int sums, uint32_t wg) {
+// Find names the call (Find::Call, what every workgroup knows) and finds this workgroup's part of a block of rows. COMMON
+// (kv_attend_shared): of a group's list, whose sums are partial ones throughout, in rows from `sums` on. (Written as the kernel
+// itself: the same body as a function that two kernels call is compiled to other registers, and kv_attend 1% slower.)
+template <int D, class Find>
+__global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tiled_kernel(typename Find::Call a) {
+  constexpr bool COMMON = std::is_same_v<typename Find::Call, AttendShared>;
+  BlockPart bp;
+  int sums = 0;
+  if (!Find::template find<D>(a, bp, sums)) return;
   using S = Tiled<D>;
+  __shared__ __align__(1024) typename S::Lds lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), c = lane & 31, h2 = lane >> 5;
   const int b = bp.b, h = bp.h, row0 = bp.row0;
   const Seq q = bp.q;
@@ -956,9 +766,9 @@ __device__ __forceinline__ void tiled_part(Attend a, typename Tiled<D>::Lds& lds
   for (int d = 0; d < S::DT; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      *reinterpret_cast<v4f*>(a.po + (size_t(wg) * (PR_ROWS * D / 4) + ((wave * S::DT + d) * 4 + r) * 64 + lane) * 4) =
+      *reinterpret_cast<v4f*>(a.po + (size_t(blockIdx.x) * (PR_ROWS * D / 4) + ((wave * S::DT + d) * 4 + r) * 64 + lane) * 4) =
           four(d, r);
-  if (h2 == 0) *reinterpret_cast<float2*>(a.pml + (size_t(wg) * PR_ROWS + 32 * wave + c) * 2) = make_float2(ref2, l);
+  if (h2 == 0) *reinterpret_cast<float2*>(a.pml + (size_t(blockIdx.x) * PR_ROWS + 32 * wave + c) * 2) = make_float2(ref2, l);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------

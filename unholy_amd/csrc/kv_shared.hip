@@ -210,7 +210,7 @@ constexpr float COMMON_TILE = 6.0f;
 struct GroupWork {
   uint32_t blocks, count;
 };
-__device__ __forceinline__ GroupWork group_work(const Attend& a, const ShareGroup& g, bool is) {
+__device__ __forceinline__ GroupWork group_work(const AttendShared& a, const ShareGroup& g, bool is) {
   GroupWork w{0, 0};
   if (is) {
     w.blocks = uint32_t(row_groups(g.rows * a.group, PR_ROWS));
@@ -218,7 +218,7 @@ __device__ __forceinline__ GroupWork group_work(const Attend& a, const ShareGrou
   }
   return w;
 }
-__device__ __forceinline__ ShareGroup group_at(const Attend& a, int i) { return a.share.groups[min(i, a.st.B / 2)]; }
+__device__ __forceinline__ ShareGroup group_at(const AttendShared& a, int i) { return a.share.groups[min(i, a.st.B / 2)]; }
 // Of sequence b: segments, and each one's tiles.
 struct SeqWork {
   Seq q;
@@ -226,13 +226,13 @@ struct SeqWork {
   uint32_t segs;
   int list;
 };
-__device__ __forceinline__ SeqWork seq_work(const Attend& a, int b, const ShareSeq& mine, const Seq& q, bool fits, bool& over) {
+__device__ __forceinline__ SeqWork seq_work(const AttendShared& a, int b, const ShareSeq& mine, const Seq& q, bool fits, bool& over) {
   SeqWork w{};
   if (b >= a.st.B) return w;
   w.q = q;
   over |= too_many(a.st, q);
   if (is_few(a, q)) {
-    w.segs = uint32_t(segments_of<true>(a, q));
+    w.segs = uint32_t(segments_of(a, q));
     w.t = tiles_of(a, q, fits ? mine.tiles : 0);
     w.list = mine.row0 + mine.at;
   }
@@ -252,7 +252,7 @@ struct FindLds {
 };
 
 // The part `at` of the groups' blocks.
-__device__ __forceinline__ bool find_common(const Attend& a, const Deal& deal, int n, const FindLds& lds, uint32_t at, BlockPart& p,
+__device__ __forceinline__ bool find_common(const AttendShared& a, const Deal& deal, int n, const FindLds& lds, uint32_t at, BlockPart& p,
                                             int& sums) {
   const int lane = threadIdx.x & 63;
   const uint32_t heads = uint32_t(a.c.heads);
@@ -288,7 +288,7 @@ __device__ __forceinline__ bool find_common(const Attend& a, const Deal& deal, i
 }
 
 // The segments that hold the first units of the workgroup's waves, u of the first wave: a sequence a thread, found through LDS.
-__device__ __forceinline__ bool find_own(const Attend& a, const Deal& deal, bool fits, SeqWork w, uint32_t u, FindLds& lds, Walk& k) {
+__device__ __forceinline__ bool find_own(const AttendShared& a, const Deal& deal, bool fits, SeqWork w, uint32_t u, FindLds& lds, Walk& k) {
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   if (tid < AT_WAVES) lds.found[tid][0] = -1;
   uint32_t from = 0;
@@ -340,7 +340,7 @@ __device__ __forceinline__ bool find_own(const Attend& a, const Deal& deal, bool
 // at a time; the tiles that its group has in common are left out, and sums that others belong to are left to
 // kv_shared_join_kernel. (A second tile on its way all the time: no faster, with 128 channels 4 us slower for its registers.)
 template <int D>
-__device__ __forceinline__ void own_segments(Attend a, const Split& sp, Walk w, uint32_t wv) {
+__device__ __forceinline__ void own_segments(const AttendShared& a, const Split& sp, Walk w, uint32_t wv) {
   using S = Shape<D>;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int mask = a.c.page - 1, sh = a.page_shift;
@@ -422,114 +422,113 @@ __device__ __forceinline__ void own_segments(Attend a, const Split& sp, Walk w, 
       for (int d = 0; d < S::DT; ++d) *reinterpret_cast<v4f*>(to + 16 * d) = o[d];
       if (g == 0) *reinterpret_cast<float2*>((alone ? a.lml : a.pml) + slot * 2) = make_float2(mx, l);
     }
-    again = next_segment<true>(a, sp, w, wv);
+    again = next_segment(a, sp, w, wv);
     if (again) pt = part_of(sp, w, w.at, wv);
   }
 }
 
-template <int D>
-__global__ __launch_bounds__(AT_NT, D <= 128 ? 2 : 1) void kv_shared_kernel(Attend a) {
-  __shared__ __align__(1024) typename Tiled<D>::Lds lds;
-  __shared__ FindLds find;
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const uint32_t heads = uint32_t(a.c.heads);
+// A workgroup's part of a common block for the tiled kernel, or no part: then it goes through own segments.
+struct FindShared {
+  using Call = AttendShared;
+  template <int D>
+  static __device__ __forceinline__ bool find(const AttendShared& a, BlockPart& bp, int& sums) {
+    __shared__ FindLds lds;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const uint32_t heads = uint32_t(a.c.heads);
 
-  // all work: the groups' by every wave for itself, a group a lane; the sequences' by all, a sequence a thread. (Every load that
-  // depends on no other is on its way before one is waited for.)
-  const int b_in = min(tid, a.st.B - 1);
-  ShareGroup g = group_at(a, lane);
-  const ShareSeq mine = a.share.seqs[b_in];
-  const Seq q = seq_of(a.st, b_in);
-  const bool fits = share_fits(a.share.head, a.st, a.c.page);
-  const int n = fits ? a.share.head->groups : 0;
-  if (tid < 64) find.groups[lane] = g;
-  uint32_t blocks = 0, sum = 0;  // (sum: of the blocks' tiles, where these are fewer than the chip takes; past that it may wrap)
-  float common_tiles = 0.0f;
-  GroupWork gw{0, 0};
-  for (int b0 = 0; b0 < n; b0 += 64) {
-    if (b0) g = group_at(a, b0 + lane);
-    gw = group_work(a, g, b0 + lane < n);
-    blocks += lane_of(wave_scan(gw.blocks), 63) * heads;
-    sum += lane_of(wave_scan(gw.blocks * heads * gw.count), 63);
-    common_tiles += wave_add(float(gw.blocks * heads) * float(gw.count));
-  }
-  bool over = false;
-  SeqWork s = seq_work(a, tid, mine, q, fits, over);
-  uint32_t tiles = s.segs * (uint32_t(s.t.count) + START), segs = s.segs;
-  for (int b = AT_NT + tid; b < a.st.B; b += AT_NT) {
-    const SeqWork x = seq_work(a, b, a.share.seqs[b], seq_of(a.st, b), fits, over);
-    tiles += x.segs * (uint32_t(x.t.count) + START);
-    segs += x.segs;
-  }
-  tiles = lane_of(wave_scan(tiles), 63);
-  segs = lane_of(wave_scan(segs), 63);
-  over = __any(over);
-  if (lane == 0) {
-    find.sums[wave][0] = tiles;
-    find.sums[wave][1] = segs;
-    find.over[wave] = over;
-  }
-  __syncthreads();
-  tiles = segs = 0;
-  over = false;
-#pragma unroll
-  for (int i = 0; i < AT_WAVES; ++i) {
-    tiles += find.sums[i][0];
-    segs += find.sums[i][1];
-    over |= find.over[i] != 0;
-  }
-
-  // workgroups in proportion, some for each
-  Deal deal{};
-  deal.share = NONE;
-  uint32_t wgs = a.target;  // the sequences'
-  if (blocks) {
-    const float part = COMMON_TILE * common_tiles / (COMMON_TILE * common_tiles + float(tiles));
-    // With up to 128 channels a CU has room for two workgroups. One of each kind there: a block's tile takes 1.6 us, and where some
-    // CUs have two blocks, 2.4 to 2.9, which all wait for (64 sequences behind 8003 tokens: 256 workgroups for blocks 27 us, 320
-    // 30, 384 29, 128 33; 256 behind 32768: 207, 237, 208, 356). Two of the blocks' only where the sequences have next to nothing.
-    const uint32_t most = D <= 128 && part < 0.95f ? a.target / 2 : a.target - a.target / 8;
-    const uint32_t want = min(max(uint32_t(part * float(a.target)), 1u), most);
-    deal.single = blocks >= want;
-    if (deal.single) {  // (where they are more than their share of the chip, one after the other)
-      deal.common = blocks;
-    } else {
-      const uint32_t least = max(4u, root(0.2f, sum, blocks));
-      if (n <= 64) deal.share = smallest_share(gw.blocks * heads, gw.count, sum, blocks, want, least);
-      else deal.share = max((sum + want - blocks - 1) / (want - blocks), least);
-      for (int b0 = 0; b0 < n; b0 += 64) {
-        if (n > 64) gw = group_work(a, group_at(a, b0 + lane), b0 + lane < n);
-        deal.common += lane_of(wave_scan(gw.blocks * parts_of(gw.count, deal.share)), 63) * heads;
-      }
+    // all work: the groups' by every wave for itself, a group a lane; the sequences' by all, a sequence a thread. (Every load that
+    // depends on no other is on its way before one is waited for.)
+    const int b_in = min(tid, a.st.B - 1);
+    ShareGroup g = group_at(a, lane);
+    const ShareSeq mine = a.share.seqs[b_in];
+    const Seq q = seq_of(a.st, b_in);
+    const bool fits = share_fits(a.share.head, a.st, a.c.page);
+    const int n = fits ? a.share.head->groups : 0;
+    if (tid < 64) lds.groups[lane] = g;
+    uint32_t blocks = 0, sum = 0;  // (sum: of the blocks' tiles, where these are fewer than the chip takes; past that it may wrap)
+    float common_tiles = 0.0f;
+    GroupWork gw{0, 0};
+    for (int b0 = 0; b0 < n; b0 += 64) {
+      if (b0) g = group_at(a, b0 + lane);
+      gw = group_work(a, g, b0 + lane < n);
+      blocks += lane_of(wave_scan(gw.blocks), 63) * heads;
+      sum += lane_of(wave_scan(gw.blocks * heads * gw.count), 63);
+      common_tiles += wave_add(float(gw.blocks * heads) * float(gw.count));
     }
-    wgs = a.target - min(deal.common, most);
-  }
-  const uint32_t target = wgs * AT_WAVES;  // waves
-  deal.own.whole = segs * 8 <= target;
-  const uint32_t lo = 2;  // tiles that are worth a wave
-  deal.own.share = deal.own.whole ? max((tiles - START * segs + target - segs - 1) / (target - segs), lo)
-                                  : max((tiles + target - 1) / target, lo);
-  deal.own.unit = deal.own.whole ? 1 : deal.own.share;
+    bool over = false;
+    SeqWork s = seq_work(a, tid, mine, q, fits, over);
+    uint32_t tiles = s.segs * (uint32_t(s.t.count) + START), segs = s.segs;
+    for (int b = AT_NT + tid; b < a.st.B; b += AT_NT) {
+      const SeqWork x = seq_work(a, b, a.share.seqs[b], seq_of(a.st, b), fits, over);
+      tiles += x.segs * (uint32_t(x.t.count) + START);
+      segs += x.segs;
+    }
+    tiles = lane_of(wave_scan(tiles), 63);
+    segs = lane_of(wave_scan(segs), 63);
+    over = __any(over);
+    if (lane == 0) {
+      lds.sums[wave][0] = tiles;
+      lds.sums[wave][1] = segs;
+      lds.over[wave] = over;
+    }
+    __syncthreads();
+    tiles = segs = 0;
+    over = false;
+#pragma unroll
+    for (int i = 0; i < AT_WAVES; ++i) {
+      tiles += lds.sums[i][0];
+      segs += lds.sums[i][1];
+      over |= lds.over[i] != 0;
+    }
 
-  if (blockIdx.x < deal.common) {
-    BlockPart bp;
-    int sums;
-    if (find_common(a, deal, n, find, blockIdx.x, bp, sums)) tiled_part<D, true>(a, lds, bp, sums, 0);
-    return;
+    // workgroups in proportion, some for each
+    Deal deal{};
+    deal.share = NONE;
+    uint32_t wgs = a.target;  // the sequences'
+    if (blocks) {
+      const float part = COMMON_TILE * common_tiles / (COMMON_TILE * common_tiles + float(tiles));
+      // With up to 128 channels a CU has room for two workgroups. One of each kind there: a block's tile takes 1.6 us, and where some
+      // CUs have two blocks, 2.4 to 2.9, which all wait for (64 sequences behind 8003 tokens: 256 workgroups for blocks 27 us, 320
+      // 30, 384 29, 128 33; 256 behind 32768: 207, 237, 208, 356). Two of the blocks' only where the sequences have next to nothing.
+      const uint32_t most = D <= 128 && part < 0.95f ? a.target / 2 : a.target - a.target / 8;
+      const uint32_t want = min(max(uint32_t(part * float(a.target)), 1u), most);
+      deal.single = blocks >= want;
+      if (deal.single) {  // (where they are more than their share of the chip, one after the other)
+        deal.common = blocks;
+      } else {
+        const uint32_t least = max(4u, root(0.2f, sum, blocks));
+        if (n <= 64) deal.share = smallest_share(gw.blocks * heads, gw.count, sum, blocks, want, least);
+        else deal.share = max((sum + want - blocks - 1) / (want - blocks), least);
+        for (int b0 = 0; b0 < n; b0 += 64) {
+          if (n > 64) gw = group_work(a, group_at(a, b0 + lane), b0 + lane < n);
+          deal.common += lane_of(wave_scan(gw.blocks * parts_of(gw.count, deal.share)), 63) * heads;
+        }
+      }
+      wgs = a.target - min(deal.common, most);
+    }
+    const uint32_t target = wgs * AT_WAVES;  // waves
+    deal.own.whole = segs * 8 <= target;
+    const uint32_t lo = 2;  // tiles that are worth a wave
+    deal.own.share = deal.own.whole ? max((tiles - START * segs + target - segs - 1) / (target - segs), lo)
+                                    : max((tiles + target - 1) / target, lo);
+    deal.own.unit = deal.own.whole ? 1 : deal.own.share;
+
+    if (blockIdx.x < deal.common) return find_common(a, deal, n, lds, blockIdx.x, bp, sums);
+    const uint32_t wg = blockIdx.x - deal.common;
+    if (wg >= wgs) return false;
+    if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(wg), int(wgs));  // (else the join's to do)
+    Walk w;
+    if (!find_own(a, deal, fits, s, wg * AT_WAVES * deal.own.unit, lds, w)) return false;
+    own_segments<D>(a, deal.own, w, wg * AT_WAVES + uint32_t(wave));
+    return false;
   }
-  const uint32_t wg = blockIdx.x - deal.common;
-  if (wg >= wgs) return;
-  if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(wg), int(wgs));  // (else the join's to do)
-  Walk w;
-  if (!find_own(a, deal, fits, s, wg * AT_WAVES * deal.own.unit, find, w)) return;
-  own_segments<D>(a, deal.own, w, wg * AT_WAVES + uint32_t(wave));
-}
+};
 
 // A workgroup per (sequence, FEW of its rows, head): its own parts and its group's, in that order, four channels of a row a
 // thread, the parts dealt to groups of threads.
 constexpr int SJ_FLIGHT = 8;
 template <int D>
-__global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(Attend a) {
+__global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(AttendShared a) {
   __shared__ v4f group_o[AT_NT];
   __shared__ float2 group_ml[AT_NT];
   constexpr int ROWS = std::min(AT_NT / (D / 4), FEW);  // of a workgroup: a row's four channels a thread
@@ -671,7 +670,7 @@ void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c,
   if (plan_bytes < kv_share_plan(s.B, s.rows)) fail("plan too small");
   if (!worth_sharing(s, c)) return kv_attend(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, ws, ws_bytes, st);
   const Way way = shared_way(s.rows, s.max_new, Hq / c.heads);
-  Attend a = attend_of(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, way, ws);
+  AttendShared a{attend_of(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, way, ws)};
   const SharedWs w = carve_shared(s.rows, s.max_new, s.B, Hq, c.heads, c.dim);
   const int64_t tiles = std::max<int64_t>(cdiv(size_t(s.max_blocks) * c.page, TILE), 1);
   const int64_t blocks = (cdiv(size_t(s.rows) * a.group, PR_ROWS) + int64_t(s.B)) * c.heads;
@@ -696,7 +695,7 @@ void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c,
   a.pml = a.po + size_t(a.target) * AT_WAVES * 2 * FEW * c.dim;
   // As many workgroups as the chip has room for, or more where there may be more blocks than half of that.
   const unsigned grid = unsigned(a.target + std::max<int64_t>(w.blocks - a.target / 2, 0));
-  by_dim(c.dim, [&]<int D>() { kv_shared_kernel<D><<<grid, AT_NT, 0, st>>>(a); });
+  by_dim(c.dim, [&]<int D>() { kv_tiled_kernel<D, FindShared><<<grid, AT_NT, 0, st>>>(a); });
   by_dim(c.dim, [&]<int D>() { kv_shared_join_kernel<D><<<dim3(unsigned(w.segments), unsigned(FEW * D / 4 / AT_NT)), AT_NT, 0, st>>>(a); });
 }
 
