@@ -33,10 +33,10 @@ enum class RopeScaling { kNone = 0, kLinear = 1, kTurns = 2, kPairs = 3 };
 void rope_frequencies(double* h_freq, int rot, double base, RopeScaling scaling, double factor, double low, double high,
                       double trained);
 
-// Rows x [rows, heads, dim] (row stride ldx), row r at position pos[r] (any int32; device), into y (row stride ldy). inverse: the
-// transpose, which turns back (and, of a rotation with mscale 1, undoes it): the gradient of x from that of y. dim up to 1024,
-// even or odd. y may be x (with ldy = ldx: then only the rotated part is read and written), otherwise they share no element. The
-// operands need no alignment past their type's: the widest loads that strides and addresses allow are taken.
+// Rows x [rows, heads, dim] (row stride ldx), row r at position pos[r] (any int32; device), into y (row stride ldy). inverse:
+// the transpose, which turns back (and, of a rotation with mscale 1, undoes it): the gradient of x from that of y. dim up to
+// 1024, even or odd. y may be x (with ldy = ldx: then only the rotated part is read and written), otherwise they share no
+// element. The operands need no alignment past their type's: the widest loads that strides and addresses allow are taken.
 void rope(const bf16* x, int ldx, bf16* y, int ldy, const int32_t* pos, int rows, int heads, int dim, const Rope& r,
           bool inverse, hipStream_t st);
 

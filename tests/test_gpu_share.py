@@ -226,6 +226,18 @@ def test_long_common_parts(D, parts):
     check(s, 4, expect=1)
 
 
+@pytest.mark.parametrize("groups,times", [(16, 42), (70, 11)])
+def test_many_tiles_of_64_channels(groups, times):
+    """So many common tiles that every workgroup takes own segments and then a part of a block; and more blocks than workgroups.
+    (The same two pages over and over: a table may name a page as often as it likes.)"""
+    rng = np.random.default_rng(groups)
+    s, _ = step_of(rng, [(128, [int(x) for x in rng.integers(0, 40, 2)]) for _ in range(groups)], [], 8, 64, 64)
+    s.table = np.concatenate([np.tile(s.table[:, :2], times - 1), s.table], 1)
+    s.max_blocks += 2 * (times - 1)
+    s.lens += 128 * (times - 1)
+    check(s, 8, expect=groups)
+
+
 def test_the_plan_takes_what_saves_most():
     """Three begin alike for long, six for a little: of 5 x 2 tiles and 2 x 9 the second; and with numbers that say so, both."""
     rng = np.random.default_rng(3)

@@ -322,8 +322,8 @@ __device__ __forceinline__ void store_out(const Attend& a, int row, int hq, int 
   if (first && a.lse) a.lse[size_t(row) * (a.group * a.c.heads) + hq] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
 }
 
-// A tile of a wave's rows: its keys and values in registers (kr, vr, with their scales' bytes) into the rows' sums. pvt: the page of
-// this lane's values; mid: what to do once the keys are used.
+// A tile of a wave's rows: its keys and values in registers (kr, vr, with their scales' bytes) into the rows' sums. pvt: the
+// page of this lane's values; mid: what to do once the keys are used.
 struct FewRow {
   int pos, pos_lo, pos_hi, len;  // this lane's row's position, all rows' lowest and highest, the sequence's length
 };

@@ -50,7 +50,8 @@ __device__ __forceinline__ uint32_t kv_codes4(float a, float b, float c, float d
 // Pieces of 8 channels x 4 tokens that a thread holds; a workgroup of one wave takes steps of few tokens.
 constexpr int pieces_of(int dim, int page, int nt) { return nt == 64 ? 2 : std::max(1, page * dim / 32 / nt); }
 
-// What kv_append_rope does besides: the queries, and how queries and keys are normalised (no weights: they are not) and rotated.
+// What kv_append_rope does besides: the queries, and how queries and keys are normalised (no weights: they are not) and
+// rotated.
 struct AppendTurn {
   const bf16* q;
   bf16* qo;

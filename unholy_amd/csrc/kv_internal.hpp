@@ -33,8 +33,9 @@ __device__ __forceinline__ int page_of(const int32_t* table, int max_blocks, int
   return p >= 0 && p < pages ? p : -1;
 }
 
-// What kv_share writes and kv_attend_shared reads (device). Sequences of a group read the first `tiles` tiles of SHARE_TILE tokens,
-// whose pages they have in common, together: all rows of its sequences, in the order of the slots, are the group's list.
+// What kv_share writes and kv_attend_shared reads (device). Sequences of a group read the first `tiles` tiles of SHARE_TILE
+// tokens, whose pages they have in common, together: all rows of its sequences, in the order of the slots, are the group's
+// list.
 constexpr int SHARE_TILE = 64;
 constexpr int SHARE_ROWS = 16;  // a sequence that brings more rows is left alone: they fill tiles of rows by themselves
 struct ShareHead {

@@ -1,5 +1,5 @@
-// Attention of sequences that begin alike over the 8-bit paged key / value cache: who shares what, and the attention that reads it
-// once (include/unholy/kernels/kv_cache.hpp has the contracts).
+// Attention of sequences that begin alike over the 8-bit paged key / value cache: who shares what, and the attention that
+// reads it once (include/unholy/kernels/kv_cache.hpp has the contracts).
 #include "kv_attend_core.hpp"
 
 namespace unholy::kernels {
@@ -190,16 +190,18 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
 }
 
 // ---- the attention -----------------------------------------------------------------------------------------------------
-// Two launches. In the first, some workgroups take the groups' blocks of PR_ROWS rows over the tiles that their sequences have in
-// common (tiled_part: the rows of up to PR_ROWS / heads sequences share each tile's read and conversion), the others every
-// sequence's own tiles (own_segments), side by side: the first are bound by the matrix and vector units, the second by memory and
-// by loads that depend on each other. All leave partial sums, and the second launch joins them by sequence and head.
+// Two launches. In the first, some workgroups take the groups' blocks of PR_ROWS rows over the tiles that their sequences have
+// in common (kv_tiled_kernel: the rows of up to PR_ROWS / heads sequences share each tile's read and conversion), the others every
+// sequence's own tiles (own_segments), side by side: the first are bound by the matrix and vector units, the second by memory
+// and by loads that depend on each other. All leave partial sums, and the second launch joins them by sequence and head.
+// (Where the blocks of 64 channels have many tiles, every workgroup takes own segments first and then a part of a block.)
 
 // How the workgroups are dealt, worked out by each of them from what the device knows.
 struct Deal {
   uint32_t common;  // workgroups of the groups' blocks; those behind them are the sequences'
   uint32_t share;   // tiles of a part at most
   bool single;      // whole blocks
+  bool both;        // each workgroup takes own segments and then a part of a block
   Split own;
 };
 constexpr uint32_t NONE = 1u << 30;
@@ -226,7 +228,8 @@ struct SeqWork {
   uint32_t segs;
   int list;
 };
-__device__ __forceinline__ SeqWork seq_work(const AttendShared& a, int b, const ShareSeq& mine, const Seq& q, bool fits, bool& over) {
+__device__ __forceinline__ SeqWork seq_work(const AttendShared& a, int b, const ShareSeq& mine, const Seq& q, bool fits,
+                                            bool& over) {
   SeqWork w{};
   if (b >= a.st.B) return w;
   w.q = q;
@@ -252,8 +255,8 @@ struct FindLds {
 };
 
 // The part `at` of the groups' blocks.
-__device__ __forceinline__ bool find_common(const AttendShared& a, const Deal& deal, int n, const FindLds& lds, uint32_t at, BlockPart& p,
-                                            int& sums) {
+__device__ __forceinline__ bool find_common(const AttendShared& a, const Deal& deal, int n, const FindLds& lds, uint32_t at,
+                                            BlockPart& p, int& sums) {
   const int lane = threadIdx.x & 63;
   const uint32_t heads = uint32_t(a.c.heads);
   uint32_t from = 0;
@@ -288,7 +291,8 @@ __device__ __forceinline__ bool find_common(const AttendShared& a, const Deal& d
 }
 
 // The segments that hold the first units of the workgroup's waves, u of the first wave: a sequence a thread, found through LDS.
-__device__ __forceinline__ bool find_own(const AttendShared& a, const Deal& deal, bool fits, SeqWork w, uint32_t u, FindLds& lds, Walk& k) {
+__device__ __forceinline__ bool find_own(const AttendShared& a, const Deal& deal, bool fits, SeqWork w, uint32_t u, FindLds& lds,
+                                         Walk& k) {
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   if (tid < AT_WAVES) lds.found[tid][0] = -1;
   uint32_t from = 0;
@@ -335,9 +339,9 @@ __device__ __forceinline__ bool find_own(const AttendShared& a, const Deal& deal
   return k.b >= 0;
 }
 
-// A wave's segments, from w on (of the launch's waves for them, the wv-th): what a sequence has for itself is mostly a few tiles,
-// which four waves would begin and join for a tile each. A sequence's rows, up to SHARE_ROWS times the query heads of a head, go FEW
-// at a time; the tiles that its group has in common are left out, and sums that others belong to are left to
+// A wave's segments, from w on (of the launch's waves for them, the wv-th): what a sequence has for itself is mostly a few
+// tiles, which four waves would begin and join for a tile each. A sequence's rows, up to SHARE_ROWS times the query heads of a
+// head, go FEW at a time; the tiles that its group has in common are left out, and sums that others belong to are left to
 // kv_shared_join_kernel. (A second tile on its way all the time: no faster, with 128 channels 4 us slower for its registers.)
 template <int D>
 __device__ __forceinline__ void own_segments(const AttendShared& a, const Split& sp, Walk w, uint32_t wv) {
@@ -436,8 +440,8 @@ struct FindShared {
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const uint32_t heads = uint32_t(a.c.heads);
 
-    // all work: the groups' by every wave for itself, a group a lane; the sequences' by all, a sequence a thread. (Every load that
-    // depends on no other is on its way before one is waited for.)
+    // all work: the groups' by every wave for itself, a group a lane; the sequences' by all, a sequence a thread. (Every load
+    // that depends on no other is on its way before one is waited for.)
     const int b_in = min(tid, a.st.B - 1);
     ShareGroup g = group_at(a, lane);
     const ShareSeq mine = a.share.seqs[b_in];
@@ -445,7 +449,8 @@ struct FindShared {
     const bool fits = share_fits(a.share.head, a.st, a.c.page);
     const int n = fits ? a.share.head->groups : 0;
     if (tid < 64) lds.groups[lane] = g;
-    uint32_t blocks = 0, sum = 0;  // (sum: of the blocks' tiles, where these are fewer than the chip takes; past that it may wrap)
+    // (sum: of the blocks' tiles, where these are fewer than the chip takes; past that it may wrap)
+    uint32_t blocks = 0, sum = 0;
     float common_tiles = 0.0f;
     GroupWork gw{0, 0};
     for (int b0 = 0; b0 < n; b0 += 64) {
@@ -487,11 +492,16 @@ struct FindShared {
     uint32_t wgs = a.target;  // the sequences'
     if (blocks) {
       const float part = COMMON_TILE * common_tiles / (COMMON_TILE * common_tiles + float(tiles));
-      // With up to 128 channels a CU has room for two workgroups. One of each kind there: a block's tile takes 1.6 us, and where some
-      // CUs have two blocks, 2.4 to 2.9, which all wait for (64 sequences behind 8003 tokens: 256 workgroups for blocks 27 us, 320
-      // 30, 384 29, 128 33; 256 behind 32768: 207, 237, 208, 356). Two of the blocks' only where the sequences have next to nothing.
-      const uint32_t most = D <= 128 && part < 0.95f ? a.target / 2 : a.target - a.target / 8;
-      const uint32_t want = min(max(uint32_t(part * float(a.target)), 1u), most);
+      // With up to 128 channels a CU has room for two workgroups. One of each kind there: a block's tile takes 1.6 us, and
+      // where some CUs have two blocks, 2.4 to 2.9, which all wait for (64 sequences behind 8003 tokens: 256 workgroups for
+      // blocks 27 us, 320 30, 384 29, 128 33; 256 behind 32768: 207, 237, 208, 356). Two of the blocks' only where the
+      // sequences have next to nothing. Many tiles of 64 channels: two blocks on every CU, and own segments before them (8
+      // query heads a head, 256 sequences behind 32768 tokens: 272 us / 223; 512 behind 8000: 152 / 141; 64 behind 16000: 44 /
+      // 44; behind 8003: 29.6 / 30.7). With 128 channels a wave alone leaves its unit no more than a tenth: 256 behind 32768
+      // 201 / 225, 128 behind 131,072 327 / 310.
+      deal.both = D == 64 && common_tiles > 16.0f * float(a.target) + 0.5f * float(tiles);
+      const uint32_t most = deal.both ? a.target : D <= 128 && part < 0.95f ? a.target / 2 : a.target - a.target / 8;
+      const uint32_t want = deal.both ? most : min(max(uint32_t(part * float(a.target)), 1u), most);
       deal.single = blocks >= want;
       if (deal.single) {  // (where they are more than their share of the chip, one after the other)
         deal.common = blocks;
@@ -504,7 +514,7 @@ struct FindShared {
           deal.common += lane_of(wave_scan(gw.blocks * parts_of(gw.count, deal.share)), 63) * heads;
         }
       }
-      wgs = a.target - min(deal.common, most);
+      if (!deal.both) wgs = a.target - min(deal.common, most);
     }
     const uint32_t target = wgs * AT_WAVES;  // waves
     deal.own.whole = segs * 8 <= target;
@@ -513,14 +523,15 @@ struct FindShared {
                                     : max((tiles + target - 1) / target, lo);
     deal.own.unit = deal.own.whole ? 1 : deal.own.share;
 
-    if (blockIdx.x < deal.common) return find_common(a, deal, n, lds, blockIdx.x, bp, sums);
-    const uint32_t wg = blockIdx.x - deal.common;
-    if (wg >= wgs) return false;
-    if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(wg), int(wgs));  // (else the join's to do)
-    Walk w;
-    if (!find_own(a, deal, fits, s, wg * AT_WAVES * deal.own.unit, lds, w)) return false;
-    own_segments<D>(a, deal.own, w, wg * AT_WAVES + uint32_t(wave));
-    return false;
+    const bool common = blockIdx.x < deal.common;
+    const uint32_t wg = deal.both || common ? blockIdx.x : blockIdx.x - deal.common;
+    if ((deal.both || !common) && wg < wgs) {
+      if (__builtin_expect(over && !a.blocks, 0)) clear_rows(a, int(wg), int(wgs));  // (else the join's to do)
+      Walk w;
+      if (find_own(a, deal, fits, s, wg * AT_WAVES * deal.own.unit, lds, w))
+        own_segments<D>(a, deal.own, w, wg * AT_WAVES + uint32_t(wave));
+    }
+    return common && find_common(a, deal, n, lds, blockIdx.x, bp, sums);
   }
 };
 
@@ -612,8 +623,8 @@ __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(AttendShared a) {
 }
 
 // Whether a step's tables may name so much that it is worth two launches (16 us at least, 23 with 256 channels; kv_attend's one
-// takes 8 and 12, and where all sequences share one prefix as long overall at 64 MB (16 x 1450 tokens of 8 heads of 128, or twice
-// as many of 64), and at 128 MB with 256 channels). Of what they name the launch knows no more than how wide they are.
+// takes 8 and 12, and where all sequences share one prefix as long overall at 64 MB (16 x 1450 tokens of 8 heads of 128, or
+// twice as many of 64), and at 128 MB with 256 channels). Of what they name the launch knows no more than how wide they are.
 bool worth_sharing(const KvStep& s, const KvCache& c) {
   const double bytes = 2.0 * s.B * s.max_blocks * c.page * c.heads * c.dim;
   return s.B > 1 && bytes > (c.dim <= 128 ? 64e6 : 128e6);
@@ -622,8 +633,8 @@ bool worth_sharing(const KvStep& s, const KvCache& c) {
 Way shared_way(int rows, int max_new, int group) {
   return {SHARE_ROWS * group, true, std::min(rows, max_new) > SHARE_ROWS};
 }
-// The workspace: counters and blocks, the groups' and the sequences' records, the sequences' sums (those of one part, the others),
-// the groups' (where the tiled kernel's lie: it is done before).
+// The workspace: counters and blocks, the groups' and the sequences' records, the sequences' sums (those of one part, the
+// others), the groups' (where the tiled kernel's lie: it is done before).
 struct SharedWs {
   int64_t blocks;     // of the groups, times heads, at most
   int64_t sum_rows;   // of the groups' sums
@@ -696,7 +707,8 @@ void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c,
   // As many workgroups as the chip has room for, or more where there may be more blocks than half of that.
   const unsigned grid = unsigned(a.target + std::max<int64_t>(w.blocks - a.target / 2, 0));
   by_dim(c.dim, [&]<int D>() { kv_tiled_kernel<D, FindShared><<<grid, AT_NT, 0, st>>>(a); });
-  by_dim(c.dim, [&]<int D>() { kv_shared_join_kernel<D><<<dim3(unsigned(w.segments), unsigned(FEW * D / 4 / AT_NT)), AT_NT, 0, st>>>(a); });
+  const dim3 join(unsigned(w.segments), unsigned(FEW * c.dim / 4 / AT_NT));
+  by_dim(c.dim, [&]<int D>() { kv_shared_join_kernel<D><<<join, AT_NT, 0, st>>>(a); });
 }
 
 size_t kv_share_plan(int B, int rows) { return B < 0 || rows < 0 ? 0 : carve_share(nullptr, B, rows).bytes; }

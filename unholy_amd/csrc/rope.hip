@@ -34,12 +34,13 @@ struct Turns {
   bool inverse;
 };
 
-// A workgroup takes the heads [wg_heads y, ..) of wg_rows rows, a head a group of lanes: the rotations of its rows are worked out
-// once, a pair a thread, and kept in LDS, while the first heads are on their way; a lane reads both channels of each of its pairs,
-// so that only the sum of squares crosses lanes, and a head stays in registers between its norm and its rotation.
-// Bound by HBM for many rows: each value is read and written once (8191 rows of 64 + 8 heads of 128 with norms: 62 us, 4.9 TB/s,
-// 4099 rows of 64 heads of 192 without: 43 us, 4.7 TB/s; a large copy reaches 4.8). A few rows take what a launch takes, with one
-// load, one exchange through LDS and one store behind each other: 3.1 us for 7 x 40 heads of 80, 3.6 for 32 x 40 of 128.
+// A workgroup takes the heads [wg_heads y, ..) of wg_rows rows, a head a group of lanes: the rotations of its rows are worked
+// out once, a pair a thread, and kept in LDS, while the first heads are on their way; a lane reads both channels of each of
+// its pairs, so that only the sum of squares crosses lanes, and a head stays in registers between its norm and its rotation.
+// Bound by HBM for many rows: each value is read and written once (8191 rows of 64 + 8 heads of 128 with norms: 62 us, 4.9
+// TB/s, 4099 rows of 64 heads of 192 without: 43 us, 4.7 TB/s; a large copy reaches 4.8). A few rows take what a launch takes,
+// with one load, one exchange through LDS and one store behind each other: 3.1 us for 7 x 40 heads of 80, 3.6 for 32 x 40 of
+// 128.
 template <int V, int N, bool NORM>
 __global__ __launch_bounds__(RT_NT) void turn_kernel(Turns a) {
   extern __shared__ float2 cs[];  // [row][pair]
@@ -159,8 +160,8 @@ void launch(Turns a, bool part, hipStream_t st) {
   const int heads = a.side[0].heads + a.side[1].heads, groups = RT_NT / a.lanes;
   a.wg_rows = std::clamp(groups / heads, 1, a.rows);
   const int chunks = int(cdiv(heads, groups));
-  // As many heads as are done at a time, or where the rows fill the chip all of them, whose rotations are then worked out once (40
-  // heads of 128: 32 rows 3.6 us, all heads a workgroup 4.6; 768 rows 7.9 and 8.1, 1024 10.1 and 9.2, 2048 14.5 and 13.4)
+  // As many heads as are done at a time, or where the rows fill the chip all of them, whose rotations are then worked out once
+  // (40 heads of 128: 32 rows 3.6 us, all heads a workgroup 4.6; 768 rows 7.9 and 8.1, 1024 10.1 and 9.2, 2048 14.5 and 13.4)
   a.wg_heads = a.rows >= 1024 ? heads : int(cdiv(heads, chunks));
   const dim3 grid(cdiv(a.rows, a.wg_rows), cdiv(heads, a.wg_heads));
   const size_t lds = size_t(a.wg_rows) * (a.r.rot / 2) * sizeof(float2);

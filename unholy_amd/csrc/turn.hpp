@@ -66,14 +66,15 @@ __host__ __device__ __forceinline__ int slots_of(int dim, int rot) {
 template <int V>
 __device__ __forceinline__ Slot slot_of(int s, int dim, int first, int rot, bool interleaved) {
   const int turned = rot / (2 * V);
-  if (s < turned) return interleaved ? Slot{first + 2 * V * s, first + 2 * V * s + V, true} : Slot{first + V * s, first + rot / 2 + V * s, true};
+  if (s < turned)
+    return interleaved ? Slot{first + 2 * V * s, first + 2 * V * s + V, true} : Slot{first + V * s, first + rot / 2 + V * s, true};
   const int u = 2 * V * (s - turned), w = u + V;  // of the channels that are not rotated
   return Slot{u < first ? u : u + rot, w >= dim - rot ? -1 : w < first ? w : w + rot, false};
 }
 
-// The two factors of a rotation: (cos, sin) of pos * freq, times mscale. The angle in turns: 64 bits, whole turns cut off, what is
-// left of one (at most a half) as an fp32 number and its rest r, by which the sine and cosine of the first are turned further
-// (the rest is below 2^-25 turns: its square does not matter).
+// The two factors of a rotation: (cos, sin) of pos * freq, times mscale. The angle in turns: 64 bits, whole turns cut off,
+// what is left of one (at most a half) as an fp32 number and its rest r, by which the sine and cosine of the first are turned
+// further (the rest is below 2^-25 turns: its square does not matter).
 __device__ __forceinline__ float2 turn_of(int pos, double freq, float mscale) {
 #pragma clang fp contract(off)
   constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
