@@ -35,7 +35,7 @@ def rope(x, pos, freq, first, rot, interleaved, mscale=1.0, inverse=False):
 
     Bounds: the result is rounded to bf16 (half a step: 2^-8 of it, at least half of the smallest subnormal number's step,
     2^-134). The angle in turns is a product of three numbers in 64 bits (4 roundings: 2^-51 of it at most), its rest of at
-    most a half is rounded to fp32 (2^-26), times 2 pi in radians; sine and cosine are off by four steps of fp32 at most
+    most a half may be rounded to fp32 (2^-26), times 2 pi in radians; sine and cosine are off by four steps of fp32 at most
     (2^-22), times mscale, their products with a and b and the sum another rounding each (3 x 2^-24): together less than
     2^-20 + 2 pi 2^-51 |turns| of mscale (|a| + |b|)."""
     a, b = pairs(x.shape[-1], first, rot, interleaved)

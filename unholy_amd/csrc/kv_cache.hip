@@ -65,7 +65,7 @@ struct AppendTurn {
 template <int D>
 __device__ __forceinline__ void turn_slot(uint4& a, uint4& b, const turn::Slot& s, const bf16* w, const float2* cs, const Rope& r,
                                           float eps) {
-  float v[16];
+  float v[16], scale = 1.0f;
   turn::unpack<8>(a, v);
   turn::unpack<8>(b, v + 8);
   if (w) {
@@ -74,9 +74,11 @@ __device__ __forceinline__ void turn_slot(uint4& a, uint4& b, const turn::Slot& 
     for (int o = D / 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
     turn::unpack<8>(*reinterpret_cast<const uint4*>(w + s.a), ww);
     turn::unpack<8>(*reinterpret_cast<const uint4*>(w + s.b), ww + 8);
-    turn::scale<8>(v, ww, turn::rms_scale(ss, D, eps));
+    turn::weigh<8>(v, ww);
+    scale = turn::rms_scale(ss, D, eps);
   }
   if (s.turned) turn::rotate<8>(v, cs, r.interleaved, false);
+  if (w) turn::scale<8>(v, scale);
   a = turn::pack<8>(v);
   b = turn::pack<8>(v + 8);
 }

@@ -39,7 +39,7 @@ struct Turns {
 // its pairs, so that only the sum of squares crosses lanes, and a head stays in registers between its norm and its rotation.
 // Bound by HBM for many rows: each value is read and written once (8191 rows of 64 + 8 heads of 128 with norms: 62 us, 4.9
 // TB/s, 4099 rows of 64 heads of 192 without: 43 us, 4.7 TB/s; a large copy reaches 4.8). A few rows take what a launch takes,
-// with one load, one exchange through LDS and one store behind each other: 3.1 us for 7 x 40 heads of 80, 3.6 for 32 x 40 of
+// with one load, one exchange through LDS and one store behind each other: 3.0 us for 7 x 40 heads of 80, 3.6 for 32 x 40 of
 // 128.
 template <int V, int N, bool NORM>
 __global__ __launch_bounds__(RT_NT) void turn_kernel(Turns a) {
@@ -108,18 +108,19 @@ __global__ __launch_bounds__(RT_NT) void turn_kernel(Turns a) {
     bool k;
     head_of(v, rr, h, k);
     if (v + groups < vectors) load(v + groups);
+    float scaled = 1.0f;
     if constexpr (NORM) {
       float ss = 0.0f;
 #pragma unroll
       for (int i = 0; i < N; ++i) ss = sum_squares<V>(x[i], ss);
       for (int o = a.lanes / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-      const float r = rms_scale(ss, a.dim, a.eps);
+      scaled = rms_scale(ss, a.dim, a.eps);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         float ww[2 * V];
 #pragma unroll
         for (int j = 0; j < 2 * V; ++j) ww[j] = k ? w[1][i][j] : w[0][i][j];
-        scale<V>(x[i], ww, r);
+        weigh<V>(x[i], ww);
       }
     }
     const Side& s = a.side[k];
@@ -133,6 +134,7 @@ __global__ __launch_bounds__(RT_NT) void turn_kernel(Turns a) {
         for (int j = 0; j < V; ++j) c[j] = cs[rr * pairs + (lane + i * a.lanes) * V + j];
         rotate<V>(x[i], c, a.r.interleaved, a.inverse);
       }
+      if constexpr (NORM) scale<V>(x[i], scaled);
       *reinterpret_cast<raw_t<V>*>(y + at[i].a) = pack<V>(x[i]);
       if (at[i].b >= 0) *reinterpret_cast<raw_t<V>*>(y + at[i].b) = pack<V>(x[i] + V);
     }

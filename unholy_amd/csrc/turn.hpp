@@ -72,17 +72,29 @@ __device__ __forceinline__ Slot slot_of(int s, int dim, int first, int rot, bool
   return Slot{u < first ? u : u + rot, w >= dim - rot ? -1 : w < first ? w : w + rot, false};
 }
 
-// The two factors of a rotation: (cos, sin) of pos * freq, times mscale. The angle in turns: 64 bits, whole turns cut off,
-// what is left of one (at most a half) as an fp32 number and its rest r, by which the sine and cosine of the first are turned
-// further (the rest is below 2^-25 turns: its square does not matter).
+// The two factors of a rotation: (cos, sin) of pos * freq, times mscale, rounded once. In 64 bits, a rotation's factors serve
+// many channels: the angle in turns, whole turns cut off, what is left as some quarters and at most an eighth of a turn, whose
+// sine and cosine are their Taylor series (up to the 11th and 12th power: the next terms are below 2^-37).
 __device__ __forceinline__ float2 turn_of(int pos, double freq, float mscale) {
 #pragma clang fp contract(off)
   constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
-  const double t = double(pos) * (freq * kTurn), part = t - rint(t);
-  const float f = float(part), r = float(part - double(f)) * 6.28318530717958647693f;
-  float s, c;
-  sincospif(2.0f * f, &s, &c);
-  return make_float2(__builtin_fmaf(-r, s, c) * mscale, __builtin_fmaf(r, c, s) * mscale);
+  const double t = double(pos) * (freq * kTurn), part = t - rint(t), quarters = rint(4.0 * part);
+  const double a = (part - 0.25 * quarters) / kTurn, z = a * a;
+  double s = -1.0 / 39916800.0, c = 1.0 / 479001600.0;
+  s = __builtin_fma(s, z, 1.0 / 362880.0);
+  c = __builtin_fma(c, z, -1.0 / 3628800.0);
+  s = __builtin_fma(s, z, -1.0 / 5040.0);
+  c = __builtin_fma(c, z, 1.0 / 40320.0);
+  s = __builtin_fma(s, z, 1.0 / 120.0);
+  c = __builtin_fma(c, z, -1.0 / 720.0);
+  s = __builtin_fma(s, z, -1.0 / 6.0);
+  c = __builtin_fma(c, z, 1.0 / 24.0);
+  s = __builtin_fma(s * z, a, a);
+  c = __builtin_fma(c, z, -0.5);
+  c = __builtin_fma(c, z, 1.0);
+  const int q = int(quarters) & 3;
+  const double x = q & 1 ? -s : c, y = q & 1 ? c : s, m = q & 2 ? -double(mscale) : double(mscale);
+  return make_float2(float(x * m), float(y * m));
 }
 
 // The slot's V pairs rotated; cs: (cos, sin) of each. v: the two pieces one after the other.
@@ -111,11 +123,17 @@ __device__ __forceinline__ float sum_squares(const float (&v)[2 * V], float ss) 
   for (int j = 0; j < 2 * V; ++j) ss = __builtin_fmaf(v[j], v[j], ss);
   return ss;
 }
+// A normalised head is r w x, rotated: the products w x of two bf16 numbers are exact, and r, which all of a head's channels
+// have in common, comes last, so that a channel has a rounding less.
 template <int V>
-__device__ __forceinline__ void scale(float (&v)[2 * V], const float (&w)[2 * V], float r) {
-#pragma clang fp contract(off)
+__device__ __forceinline__ void weigh(float (&v)[2 * V], const float (&w)[2 * V]) {
 #pragma unroll
-  for (int j = 0; j < 2 * V; ++j) v[j] = w[j] * (v[j] * r);
+  for (int j = 0; j < 2 * V; ++j) v[j] *= w[j];
+}
+template <int V>
+__device__ __forceinline__ void scale(float (&v)[2 * V], float r) {
+#pragma unroll
+  for (int j = 0; j < 2 * V; ++j) v[j] *= r;
 }
 
 // Argument checks of every entry that rotates.
