@@ -77,7 +77,7 @@ __device__ __forceinline__ void turn_slot(uint4& a, uint4& b, const turn::Slot& 
     turn::weigh<8>(v, ww);
     scale = turn::rms_scale(ss, D, eps);
   }
-  if (s.turned) turn::rotate<8>(v, cs, r.interleaved, false);
+  if (s.turned) turn::rotate<8>(v, cs, r.interleaved);
   if (w) turn::scale<8>(v, scale);
   a = turn::pack<8>(v);
   b = turn::pack<8>(v + 8);

@@ -95,7 +95,10 @@ __global__ __launch_bounds__(RT_NT) void turn_kernel(Turns a) {
     }
   };
   if (group < vectors) load(group);
-  for (int i = tid; i < rows * pairs; i += RT_NT) cs[i] = turn_of(a.pos[r0 + i / pairs], a.r.freq[i % pairs], a.r.mscale);
+  for (int i = tid; i < rows * pairs; i += RT_NT) {
+    cs[i] = turn_of(a.pos[r0 + i / pairs], a.r.freq[i % pairs], a.r.mscale);
+    if (a.inverse) cs[i].y = -cs[i].y;
+  }
   __syncthreads();
   for (int v = group; v < vectors; v += groups) {  // (the lanes of a head leave together)
     float x[N][2 * V];
@@ -132,7 +135,7 @@ __global__ __launch_bounds__(RT_NT) void turn_kernel(Turns a) {
         float2 c[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) c[j] = cs[rr * pairs + (lane + i * a.lanes) * V + j];
-        rotate<V>(x[i], c, a.r.interleaved, a.inverse);
+        rotate<V>(x[i], c, a.r.interleaved);
       }
       if constexpr (NORM) scale<V>(x[i], scaled);
       *reinterpret_cast<raw_t<V>*>(y + at[i].a) = pack<V>(x[i]);

@@ -45,7 +45,11 @@ __device__ __forceinline__ raw_t<V> pack(const float* v) {
   } else {
     uint32_t w[V / 2];
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) w[i] = uint32_t(f32_to_bf16(v[2 * i])) | uint32_t(f32_to_bf16(v[2 * i + 1])) << 16;
+    for (int i = 0; i < V / 2; ++i) {  // (both in one instruction)
+      typedef float f32x2 __attribute__((ext_vector_type(2)));
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2 * i], v[2 * i + 1]}, bf16x2));
+    }
     raw_t<V> x;
     __builtin_memcpy(&x, w, sizeof(w));
     return x;
@@ -77,9 +81,9 @@ __device__ __forceinline__ Slot slot_of(int s, int dim, int first, int rot, bool
 // sine and cosine are their Taylor series (up to the 11th and 12th power: the next terms are below 2^-37).
 __device__ __forceinline__ float2 turn_of(int pos, double freq, float mscale) {
 #pragma clang fp contract(off)
-  constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
-  const double t = double(pos) * (freq * kTurn), part = t - rint(t), quarters = rint(4.0 * part);
-  const double a = (part - 0.25 * quarters) / kTurn, z = a * a;
+  constexpr double kRadian = 0.15915494309189533577, kTurn = 6.28318530717958647693;  // 1 / (2 pi) turns; in radians
+  const double t = double(pos) * (freq * kRadian), part = t - rint(t), quarters = rint(4.0 * part);
+  const double a = (part - 0.25 * quarters) * kTurn, z = a * a;
   double s = -1.0 / 39916800.0, c = 1.0 / 479001600.0;
   s = __builtin_fma(s, z, 1.0 / 362880.0);
   c = __builtin_fma(c, z, -1.0 / 3628800.0);
@@ -99,16 +103,19 @@ __device__ __forceinline__ float2 turn_of(int pos, double freq, float mscale) {
 
 // The slot's V pairs rotated; cs: (cos, sin) of each. v: the two pieces one after the other.
 template <int V>
-__device__ __forceinline__ void rotate(float (&v)[2 * V], const float2* cs, bool interleaved, bool inverse) {
+__device__ __forceinline__ void rotate(float (&v)[2 * V], const float2* cs, bool interleaved) {
 #pragma clang fp contract(off)  // (each product and sum as written: every kernel that rotates rounds alike)
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float c = cs[j].x, s = inverse ? -cs[j].y : cs[j].y;
-    float& a = interleaved ? v[2 * j] : v[j];
-    float& b = interleaved ? v[2 * j + 1] : v[V + j];
-    const float x = a, y = b;
+  const auto pair = [&](float& a, float& b, int j) {
+    const float c = cs[j].x, s = cs[j].y, x = a, y = b;
     a = __builtin_fmaf(x, c, -(y * s));
     b = __builtin_fmaf(x, s, y * c);
+  };
+  if (interleaved) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) pair(v[2 * j], v[2 * j + 1], j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) pair(v[j], v[V + j], j);
   }
 }
 
