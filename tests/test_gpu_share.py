@@ -226,8 +226,8 @@ def test_long_common_parts(D, parts):
     check(s, 4, expect=1)
 
 
-@pytest.mark.parametrize("groups,times", [(16, 42), (70, 11)])
-def test_many_tiles_of_64_channels(groups, times):
+@pytest.mark.parametrize("groups,times,window", [(16, 42, 0), (70, 11, 0), (16, 42, 5000)])
+def test_many_tiles_of_64_channels(groups, times, window):
     """So many common tiles that every workgroup takes own segments and then a part of a block; and more blocks than workgroups.
     (The same two pages over and over: a table may name a page as often as it likes.)"""
     rng = np.random.default_rng(groups)
@@ -235,7 +235,7 @@ def test_many_tiles_of_64_channels(groups, times):
     s.table = np.concatenate([np.tile(s.table[:, :2], times - 1), s.table], 1)
     s.max_blocks += 2 * (times - 1)
     s.lens += 128 * (times - 1)
-    check(s, 8, expect=groups)
+    check(s, 8, window=window, sinks=window // 1000, expect=groups)
 
 
 def test_the_plan_takes_what_saves_most():
