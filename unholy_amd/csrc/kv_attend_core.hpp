@@ -506,34 +506,25 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
   // (a group's tiles lie before all of its rows)
   const int pos_lo = COMMON ? INT32_MAX : uniform(q.first + min(wrow, nrows - 1) / a.group);
   const int pos_hi = COMMON ? INT32_MAX : uniform(q.first + min(wrow + 31, nrows - 1) / a.group);
-  bf16x8 qf[2 * D / 32];
-  {
-    const bf16* x = a.q + size_t(row) * a.ldq + size_t(hq) * D + 16 * h2;
-#pragma unroll
-    for (int m = 0; m < D / 32; ++m) {
-      const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0;  // scores times |scale|: their largest is the largest weight's
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        uint4 y = *reinterpret_cast<const uint4*>(x + 32 * m + 8 * e);
-        y.x ^= flip, y.y ^= flip, y.z ^= flip, y.w ^= flip;
-        qf[2 * m + e] = bf16x8_of(y);
-      }
-    }
-  }
   const float sc = fmaxf(fabsf(a.scale2), 0x1p-126f);  // (not 0: hidden scores are -inf, and stay so)
 
+  const int n = bp.i1 - bp.i0;
   const auto token = [&](int i) { return tiles.at(bp.i0 + i) * TILE; };
-  const auto meta = [&](int chunk) {  // pages and scales of tiles [16 chunk, 16 chunk + 16)
-    if (tid < PR_META * 4) {
-      const int i = chunk * PR_META + tid / 4;
-      const int pg = i < bp.i1 - bp.i0 ? page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (token(i) + tid % 4 * 16) >> a.page_shift)
-                                     : -1;
+  // pages and scales of tiles [16 chunk, 16 chunk + 16), four groups of tokens a tile and one a lane
+  static_assert(PR_META * 4 == 64);
+  const auto look = [&](int chunk) {
+    const int i = chunk * PR_META + lane / 4;
+    return i < n ? page_of(a.st.table, a.st.max_blocks, a.c.pages, b, (token(i) + lane % 4 * 16) >> a.page_shift) : -1;
+  };
+  const auto meta = [&](int chunk) {
+    if (wave == 0) {
+      const int pg = look(chunk);
       const size_t ph = size_t(max(pg, 0)) * a.c.heads + h;
       const uint64_t none = __ballot(pg < 0);
       if (tid == 0) lds.missing[chunk & 1] = none;
-      lds.page[chunk & 1][tid] = pg;
-      lds.ks[chunk & 1][tid] = e8m0_to_f32(a.c.ks[ph]);
-      lds.vs[chunk & 1][tid] = e8m0_to_f32(a.c.vs[ph]);
+      lds.page[chunk & 1][lane] = pg;
+      lds.ks[chunk & 1][lane] = e8m0_to_f32(a.c.ks[ph]);
+      lds.vs[chunk & 1][lane] = e8m0_to_f32(a.c.vs[ph]);
     }
   };
   const int mask = a.c.page - 1, sh = a.page_shift;
@@ -582,15 +573,34 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
   float ref2 = -INFINITY, l = 0.0f;  // what the weights are relative to (a power of two's exponent); their sum
-  const int n = bp.i1 - bp.i0;
   int next = 0;  // the page of the next tile to fetch, read ahead
   uint64_t missing = 0;
-  if (n > 0) {
-    meta(0);
-    __syncthreads();
-    fetch(0, page_at(0));
+  // The start, with as few loads behind each other as there can be: the pages are looked up while the rows' numbers are on
+  // their way, by every wave for itself (all write the same numbers; a wave reads its own), then rows, scales and the first
+  // two tiles together.
+  bf16x8 qf[2 * D / 32];
+  {
+    const int pg = look(0);
+    const size_t ph = size_t(max(pg, 0)) * a.c.heads + h;
+    const bf16* x = a.q + size_t(row) * a.ldq + size_t(hq) * D + 16 * h2;
+    uint4 y[2 * D / 32];
+#pragma unroll
+    for (int m = 0; m < 2 * D / 32; ++m) y[m] = *reinterpret_cast<const uint4*>(x + 16 * m - 8 * (m & 1));
+    const uint8_t ksb = a.c.ks[ph], vsb = a.c.vs[ph];
+    const uint64_t none = __ballot(pg < 0);
+    lds.page[0][lane] = pg;
+    if (n > 0) fetch(0, page_at(0));
     if (n > 1) fetch(1, page_at(1));
     if (n > 2) next = page_at(2);
+    lds.missing[0] = none;
+    lds.ks[0][lane] = e8m0_to_f32(ksb);
+    lds.vs[0][lane] = e8m0_to_f32(vsb);
+    const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0;  // scores times |scale|: their largest is the largest weight's
+#pragma unroll
+    for (int m = 0; m < 2 * D / 32; ++m) {
+      y[m].x ^= flip, y[m].y ^= flip, y[m].z ^= flip, y[m].w ^= flip;
+      qf[m] = bf16x8_of(y[m]);
+    }
   }
   const int krow = 16 * (c >> 2 & 1) + 4 * (c >> 3) + (c & 3);  // the token that is this lane's row of a half
   const int kat = krow * D + 16 * key_piece<D>(krow, h2), vat = c * 64;
