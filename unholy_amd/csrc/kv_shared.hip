@@ -191,9 +191,9 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
 
 // ---- the attention -----------------------------------------------------------------------------------------------------
 // Two launches. In the first, some workgroups take the groups' blocks of PR_ROWS rows over the tiles that their sequences have
-// in common (kv_tiled_kernel: the rows of up to PR_ROWS / heads sequences share each tile's read and conversion), the others every
-// sequence's own tiles (own_segments), side by side: the first are bound by the matrix and vector units, the second by memory
-// and by loads that depend on each other. All leave partial sums, and the second launch joins them by sequence and head.
+// in common (kv_tiled_kernel: the rows of up to PR_ROWS / heads sequences share each tile's read and conversion), the others
+// every sequence's own tiles (own_segments), side by side: the first are bound by the matrix and vector units, the second by
+// memory and by loads that depend on each other. All leave partial sums, and the second launch joins them by sequence and head.
 // (Where the blocks of 64 channels have many tiles, every workgroup takes own segments first and then a part of a block.)
 
 // How the workgroups are dealt, worked out by each of them from what the device knows.
@@ -536,8 +536,9 @@ struct FindShared {
 };
 
 // A workgroup per (sequence, FEW of its rows, head): its own parts and its group's, in that order, four channels of a row a
-// thread, the parts dealt to groups of threads.
-constexpr int SJ_FLIGHT = 8;
+// thread, the parts dealt to groups of threads, five at a time (64 sequences behind 8003 tokens 6.4, 6.3, 6.1, 6.5, 6.5
+// us with 3, 4, 5, 6 and 10; 256 behind 32768 8.3, 8.4, 8.5, 8.8, 10.9).
+constexpr int SJ_FLIGHT = 5;
 template <int D>
 __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(AttendShared a) {
   __shared__ v4f group_o[AT_NT];
@@ -572,7 +573,10 @@ __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(AttendShared a) {
       float2 x[SJ_FLIGHT];
 #pragma unroll
       for (int k = 0; k < SJ_FLIGHT; ++k) {
-        const int p = min(k0 + k * groups, parts - 1);
+        const int p = k0 + k * groups;
+        x[k] = make_float2(-INFINITY, 0.0f);
+        y[k] = v4f{0, 0, 0, 0};
+        if (p >= parts) continue;
         const float *ml = a.sml, *o = a.so;
         size_t at = size_t((r < upto ? begin0 : begin1) + r) + size_t(p - own.parts) * a.c.heads * PR_ROWS;
         if (p < own.parts) {
@@ -591,12 +595,11 @@ __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(AttendShared a) {
       acc *= al;
       sum *= al;
 #pragma unroll
-      for (int k = 0; k < SJ_FLIGHT; ++k)
-        if (k0 + k * groups < parts) {
-          const float f = __builtin_amdgcn_exp2f(x[k].x - ref);
-          sum += f * x[k].y;
-          acc += f * y[k];
-        }
+      for (int k = 0; k < SJ_FLIGHT; ++k) {
+        const float f = __builtin_amdgcn_exp2f(x[k].x - ref);
+        sum += f * x[k].y;
+        acc += f * y[k];
+      }
     }
     if (groups == 1) {
       store_out<D>(a, q.r0 + (row0 + r) / a.group, h * a.group + (row0 + r) % a.group, d, acc, sum, m, d == 0);
