@@ -243,8 +243,11 @@ struct Deal {
   Split own;
 };
 constexpr uint32_t NONE = 1u << 30;
-// A block's tile, which its workgroup's waves take together, in sequences' tiles, of which each takes its own.
-constexpr float COMMON_TILE = 6.0f;
+// A block's tile, which its workgroup's waves take together, in sequences' tiles, of which each takes its own. (Where that
+// decides: 3 rather than 6 for 4 x 16 sequences of up to 2000 tokens behind 3000, 128 channels: 41 us / 46; 128 of 500 behind
+// 2000: 32 / 37; with 256 channels 8 x 8 of 900 behind 3000: 42 / 57; 128 of 500 behind 2000: 40 / 39. With 2, 2 x 32 of 3000
+// behind 1500 and 256 channels 75 / 51.)
+constexpr float COMMON_TILE = 3.0f;
 
 // Of a group: blocks of rows, and tiles that its rows see.
 struct GroupWork {
@@ -489,13 +492,14 @@ struct FindShared {
     if (tid < 64) lds.groups[lane] = g;
     // (sum: of the blocks' tiles, where these are fewer than the chip takes; past that it may wrap)
     uint32_t blocks = 0, sum = 0;
-    float common_tiles = 0.0f;
+    float common_tiles = 0.0f, rows = 0.0f;  // (rows: of the blocks)
     GroupWork gw{0, 0};
     for (int b0 = 0; b0 < n; b0 += 64) {
       if (b0) g = group_at(a, b0 + lane);
       gw = group_work(a, g, b0 + lane < n);
       blocks += lane_of(wave_scan(gw.blocks), 63) * heads;
       sum += lane_of(wave_scan(gw.blocks * heads * gw.count), 63);
+      rows += wave_add(b0 + lane < n ? float(g.rows * a.group) * float(heads) : 0.0f);
       common_tiles += wave_add(float(gw.blocks * heads) * float(gw.count));
     }
     bool over = false;
@@ -532,13 +536,19 @@ struct FindShared {
       const float part = COMMON_TILE * common_tiles / (COMMON_TILE * common_tiles + float(tiles));
       // With up to 128 channels a CU has room for two workgroups. One of each kind there: a block's tile takes 1.6 us, and
       // where some CUs have two blocks, 2.4 to 2.9, which all wait for (64 sequences behind 8003 tokens: 256 workgroups for
-      // blocks 27 us, 320 30, 384 29, 128 33; 256 behind 32768: 207, 237, 208, 356). Two of the blocks' only where the
-      // sequences have next to nothing. Many tiles of 64 channels: two blocks on every CU, and own segments before them (8
-      // query heads a head, 256 sequences behind 32768 tokens: 272 us / 223; 512 behind 8000: 152 / 141; 64 behind 16000: 44 /
-      // 44; behind 8003: 29.6 / 30.7). With 128 channels a wave alone leaves its unit no more than a tenth: 256 behind 32768
-      // 201 / 225, 128 behind 131,072 327 / 310.
+      // blocks 27 us, 320 30, 384 29, 128 33; 256 behind 32768: 207, 237, 208, 356).
+      // Two of the blocks' where there are tiles enough for as many parts and either the sequences have next to nothing (128
+      // behind 131,072: 375 us / 319; with fewer tiles, 16 behind 16000: 25.7 / 29.8) or the blocks' rows are one wave's of
+      // four, which leaves the others' units free (4 query heads a head, 16 x 4 behind 4000: 50 us / 40, 8 x 8 behind 6000: 43 /
+      // 36; with two waves' rows, 8 query heads: 27 / 28).
+      // Many tiles of 64 channels: two blocks on every CU, and own segments before them (8 query heads a head, 256 sequences
+      // behind 32768 tokens: 272 us / 223; 512 behind 8000: 152 / 141; 64 behind 16000: 44 / 44; behind 8003: 29.6 / 30.7).
+      // With 128 channels a wave alone leaves its unit no more than a tenth: 256 behind 32768 201 / 225.
+      const bool enough = common_tiles > 6.0f * float(a.target);
+      const bool narrow = rows <= 32.0f * float(blocks), little = float(tiles) < 0.32f * common_tiles;
       deal.both = D == 64 && common_tiles > 16.0f * float(a.target) + 0.5f * float(tiles);
-      const uint32_t most = deal.both ? a.target : D <= 128 && part < 0.95f ? a.target / 2 : a.target - a.target / 8;
+      const uint32_t half = a.target / 2, nearly = a.target - a.target / 8;
+      const uint32_t most = deal.both ? a.target : D == 256 || (enough && (narrow || little)) ? nearly : half;
       const uint32_t want = deal.both ? most : min(max(uint32_t(part * float(a.target)), 1u), most);
       deal.single = blocks >= want;
       if (deal.single) {  // (where they are more than their share of the chip, one after the other)
