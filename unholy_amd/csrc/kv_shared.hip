@@ -539,8 +539,8 @@ struct FindShared {
       // blocks 27 us, 320 30, 384 29, 128 33; 256 behind 32768: 207, 237, 208, 356).
       // Two of the blocks' where there are tiles enough for as many parts and either the sequences have next to nothing (128
       // behind 131,072: 375 us / 319; with fewer tiles, 16 behind 16000: 25.7 / 29.8) or the blocks' rows are one wave's of
-      // four, which leaves the others' units free (4 query heads a head, 16 x 4 behind 4000: 50 us / 40, 8 x 8 behind 6000: 43 /
-      // 36; with two waves' rows, 8 query heads: 27 / 28).
+      // four, which leaves the others' units free (4 query heads a head, 16 x 4 behind 4000: 50 us / 40, 8 x 8 behind 6000: 43
+      // / 36; with two waves' rows, 8 query heads: 27 / 28).
       // Many tiles of 64 channels: two blocks on every CU, and own segments before them (8 query heads a head, 256 sequences
       // behind 32768 tokens: 272 us / 223; 512 behind 8000: 152 / 141; 64 behind 16000: 44 / 44; behind 8003: 29.6 / 30.7).
       // With 128 channels a wave alone leaves its unit no more than a tenth: 256 behind 32768 201 / 225.
@@ -673,9 +673,10 @@ __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(AttendShared a) {
   }
 }
 
-// Whether a step's tables may name so much that it is worth two launches (16 us at least, 23 with 256 channels; kv_attend's one
-// takes 8 and 12, and where all sequences share one prefix as long overall at 64 MB (16 x 1450 tokens of 8 heads of 128, or
-// twice as many of 64), and at 128 MB with 256 channels). Of what they name the launch knows no more than how wide they are.
+// Whether a step's tables may name so much that it is worth two launches (13 to 15 us at least, 20 with 256 channels;
+// kv_attend's one takes 8 and 12, and where all sequences share one prefix as long overall near 60 MB (16 x 1450 tokens of 8
+// heads of 128, or twice as many of 64), and at 90 to 140 MB with 256 channels). Of what they name the launch knows no more
+// than how wide they are.
 bool worth_sharing(const KvStep& s, const KvCache& c) {
   const double bytes = 2.0 * s.B * s.max_blocks * c.page * c.heads * c.dim;
   return s.B > 1 && bytes > (c.dim <= 128 ? 64e6 : 128e6);
