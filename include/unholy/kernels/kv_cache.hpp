@@ -86,7 +86,8 @@ void kv_attend(const bf16* q, int ldq, const KvStep& step, const KvCache& cache,
 // table.
 // plan: kv_share_plan bytes, 16-byte aligned, zeroed before the first call that makes one in it. It holds for the step's cu,
 // lens and table as they were when it was made, and stays valid while sequences only grow and none of its pages is changed,
-// moved (kv_compact) or given up.
+// moved (kv_compact) or given up. (One that does not hold for a step of the same sizes makes wrong results, but writes nothing
+// outside of out, lse and the workspace.)
 size_t kv_share_plan(int B, int rows);
 void kv_share(const int32_t* group, const KvStep& step, int pages, int page, void* plan, size_t plan_bytes, hipStream_t st);
 // The operands are kv_attend's; the step's sizes (B, rows, max_new, max_blocks) and the page are those of kv_share's call,

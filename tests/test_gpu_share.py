@@ -333,6 +333,26 @@ def test_a_plan_of_other_sizes_is_not_used():
         assert (np.abs(from_bf16(got) - ref) <= tol).all()
 
 
+@pytest.mark.parametrize("n", [[16, 1, 1, 1, 1, 1], [1, 1, 1, 1, 1, 16], [0, 9, 0, 9, 1, 2]])
+def test_a_plan_of_other_rows_writes_nowhere_else(n):
+    """The plan of a step of one row each and two more: what a step of the same sizes and other rows gets is undefined, but it
+    stays within its arrays, and the next call with a plan of its own is right."""
+    rng = np.random.default_rng(n[0] + 20)
+    s, _ = step_of(rng, [(300, [20, 30, 40, 50, 60, 70])], [], 2, 64, 64, n=[4, 1, 4, 4, 4, 4])
+    t, _ = step_of(rng, [(300, [20, 30, 40, 50, 60, 70])], [], 2, 64, 64, n=n)
+    for x in ("table", "k", "v", "ks", "vs", "lens", "pages", "max_blocks", "rows"):
+        setattr(t, x, getattr(s, x))
+    q = randn_bf16(rng, (s.rows, 16, 64))
+    a, b = Cache(s), Cache(t)
+    plan, need = plan_of(a, most=16)
+    got, _ = shared(b, q, 16, 0.1, plan, need, most=16)
+    assert (got[t.cu[-1]:] == 0x7FC1).all()
+    out, _ = shared(b, q, 16, 0.1, *plan_of(b, most=16), most=16)
+    ref, _, tol, _ = kv_ref.attend(t, from_bf16(q).astype(np.float64), 16, 0.1)
+    err = np.abs(from_bf16(out).astype(np.float64) - ref)[:t.cu[-1]]
+    assert (err <= tol[:t.cu[-1]]).all()
+
+
 def test_the_same_every_time_and_without_lse():
     rng = np.random.default_rng(11)
     s, _ = step_of(rng, [(2000, [3, 700, 100, 0])], [900], 2, 128, 64)

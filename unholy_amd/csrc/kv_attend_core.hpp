@@ -79,10 +79,17 @@ struct AttendShared : Attend {
   float *so, *sml;       // the groups' partial sums: values [row][D]; maximum and weight sum [row][2]
   float *lo, *lml;       // those of a sequence's own tiles that are one part, by (row in the lists, query head), the same way
   int most_parts;        // of FEW rows, of a sequence
+  int lists, sum_rows;   // rows that the lists have room for, and the groups' sums
 };
 
 __device__ __forceinline__ size_t own_at(const AttendShared& a, int b, int part, int h) {
   return (size_t(b) * a.most_parts + part) * a.c.heads + h;
+}
+
+// Where a sequence's rows begin in the groups' lists. (A plan that was made for other rows than the step has, which its caller
+// should not use, gives wrong results, but no place outside of the workspace.)
+__device__ __forceinline__ int list_of(const AttendShared& a, const ShareSeq& s, const Seq& q) {
+  return max(min(s.row0 + s.at, a.lists - (q.r1 - q.r0)), 0);
 }
 
 // Where the sums of a sequence's r-th (row, query head) of head h are, of the sequences in groups.
@@ -224,7 +231,7 @@ __device__ __forceinline__ bool next_segment(const A& a, const Split& s, Walk& w
   if constexpr (SH) {
     const ShareSeq s = a.share.seqs[w.b];
     w.t = tiles_of(a, w.q, share_fits(a.share.head, a.st, a.c.page) ? uniform(s.tiles) : 0);
-    w.list = uniform(s.row0 + s.at);
+    w.list = uniform(list_of(a, s, w.q));
   } else {
     w.t = tiles_of(a, w.q);
   }

@@ -278,7 +278,7 @@ __device__ __forceinline__ SeqWork seq_work(const AttendShared& a, int b, const 
   if (is_few(a, q)) {
     w.segs = uint32_t(segments_of(a, q));
     w.t = tiles_of(a, q, fits ? mine.tiles : 0);
-    w.list = mine.row0 + mine.at;
+    w.list = list_of(a, mine, q);
   }
   return w;
 }
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(AttendShared a) {
   if (fits && tiles_of(a, q, mine.tiles).from) {
     const int list = mine.at * a.group + row0, block = list / PR_ROWS;
     const Common* k = a.common + (size_t(mine.row0) * a.group / PR_ROWS + mine.group + block) * a.c.heads + h;
-    parts += k->parts;
+    parts += min(max(k->parts, 0), int(a.target));  // (see list_of)
     begin0 = k->row + list % PR_ROWS;
     upto = (block + 1) * PR_ROWS - list;  // rows in that block
     begin1 = upto < rows ? k[a.c.heads].row - upto : 0;
@@ -626,10 +626,11 @@ __global__ __launch_bounds__(AT_NT) void kv_shared_join_kernel(AttendShared a) {
         y[k] = v4f{0, 0, 0, 0};
         if (p >= parts) continue;
         const float *ml = a.sml, *o = a.so;
-        size_t at = size_t((r < upto ? begin0 : begin1) + r) + size_t(p - own.parts) * a.c.heads * PR_ROWS;
+        const int64_t slot = int64_t((r < upto ? begin0 : begin1) + r) + int64_t(p - own.parts) * a.c.heads * PR_ROWS;
+        size_t at = size_t(max(min(slot, int64_t(a.sum_rows) - 1), int64_t(0)));
         if (p < own.parts) {
           const bool alone = own.parts == 1;
-          at = alone ? list_row(a, mine.row0 + mine.at, h, row0 + r) : size_t(((own.row + p) * 2 + (p == 0 ? 1 : 0)) * FEW + in0 + r);
+          at = alone ? list_row(a, list_of(a, mine, q), h, row0 + r) : size_t(((own.row + p) * 2 + (p == 0 ? 1 : 0)) * FEW + in0 + r);
           ml = alone ? a.lml : a.pml, o = alone ? a.lo : a.po;
         }
         x[k] = *reinterpret_cast<const float2*>(ml + at * 2);
@@ -742,6 +743,7 @@ void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c,
     fail("rows times blocks past 31 bits");
   a.share = carve_share(const_cast<void*>(plan), s.B, s.rows);
   a.most_parts = w.most_parts;
+  a.lists = int(w.list_rows / Hq), a.sum_rows = int(w.sum_rows);
   char* base = static_cast<char*>(ws);
   a.common = reinterpret_cast<Common*>(base + w.common);
   a.own = reinterpret_cast<Common*>(base + w.own);
