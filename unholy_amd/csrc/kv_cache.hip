@@ -1,6 +1,7 @@
 // The 8-bit paged key / value cache: quantizing a step's tokens into it, and its pages' bookkeeping
 // (include/unholy/kernels/kv_cache.hpp has the layout and the contracts).
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_internal.hpp"
 #include "numerics.hpp"
@@ -60,6 +61,8 @@ struct AppendTurn {
   float eps;
   Rope r;
 };
+
+struct NoTurn {};  // (kv_append's kernels have no more arguments to load than they use)
 
 // Eight channels and their partners of a head, in the workgroup's form (D / 16 lanes a head, all of them here together).
 template <int D>
@@ -121,7 +124,8 @@ __device__ __forceinline__ void turn_queries(const KvStep& st, const AppendTurn&
 // TURN: kv_append_rope's, whose grid has further layers of workgroups for the queries.
 template <int D, int PAGE, int NT, bool TURN>
 __global__ __launch_bounds__(NT) void kv_append_kernel(const bf16* __restrict__ kx, int ldk, const bf16* __restrict__ vx,
-                                                       int ldv, KvStep st, KvCache c, int nblk, AppendTurn t) {
+                                                       int ldv, KvStep st, KvCache c, int nblk,
+                                                       std::conditional_t<TURN, AppendTurn, NoTurn> t) {
   constexpr int CH = D / 8, Q = pieces_of(D, PAGE, NT);
   __shared__ float red[NT / 64];
   if constexpr (TURN)
@@ -546,7 +550,7 @@ void check_ws(const char* who, const void* ws, size_t bytes, size_t need) {
 // The launch of kv_append, and with t of kv_append_rope.
 template <bool TURN>
 static void append(const char* who, const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& s, const KvCache& c,
-                   AppendTurn t, hipStream_t st) {
+                   std::conditional_t<TURN, AppendTurn, NoTurn> t, hipStream_t st) {
   const auto fail = [&](const char* what) { throw std::runtime_error(std::string(who) + ": " + what); };
   if (!k || !v) fail("null operand");
   if (int64_t(ldk) < int64_t(c.heads) * c.dim || int64_t(ldv) < int64_t(c.heads) * c.dim || ldk % 8 || ldv % 8)
@@ -589,7 +593,7 @@ void kv_append(const bf16* k, int ldk, const bf16* v, int ldv, const KvStep& s, 
   check_cache("kv_append", c);
   check_step("kv_append", s);
   if (s.B == 0 || s.rows == 0 || s.max_new == 0 || s.max_blocks == 0) return;
-  append<false>("kv_append", k, ldk, v, ldv, s, c, AppendTurn{}, st);
+  append<false>("kv_append", k, ldk, v, ldv, s, c, NoTurn{}, st);
 }
 
 void kv_append_rope(const bf16* q, int ldq, bf16* qo, int ldqo, int Hq, const bf16* wq, const bf16* k, int ldk, const bf16* wk,
