@@ -85,9 +85,10 @@ void kv_attend(const bf16* q, int ldq, const KvStep& step, const KvCache& cache,
 // and as long as saves the most; the others are alone. Wrong numbers cost time, never results: what is shared is read off the
 // table.
 // plan: kv_share_plan bytes, 16-byte aligned, zeroed before the first call that makes one in it. It holds for the step's cu,
-// lens and table as they were when it was made, and stays valid while sequences only grow and none of its pages is changed,
-// moved (kv_compact) or given up. (One that does not hold for a step of the same sizes makes wrong results, but writes nothing
-// outside of out, lse and the workspace.)
+// lens and table as they were when it was made, and stays valid, under a window too, for steps of the same cu while sequences
+// only grow and none of its pages is changed, moved (kv_compact) or given up. (Under a window, common tiles that no row sees any
+// more are read until the next plan.) One that does not hold for a step of the same sizes makes wrong results, but writes
+// nothing outside of out, lse and the workspace.
 size_t kv_share_plan(int B, int rows);
 void kv_share(const int32_t* group, const KvStep& step, int pages, int page, void* plan, size_t plan_bytes, hipStream_t st);
 // The operands are kv_attend's; the step's sizes (B, rows, max_new, max_blocks) and the page are those of kv_share's call,

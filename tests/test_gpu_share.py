@@ -353,6 +353,42 @@ def test_a_plan_of_other_rows_writes_nowhere_else(n):
     assert (err <= tol[:t.cu[-1]]).all()
 
 
+def grown(s, q, Hq, by, window, sinks):
+    """The attention of a step by the plan of a step before, when its sequences were `by` tokens shorter."""
+    lens = s.lens.copy()
+    s.lens = (lens - np.asarray(by)).astype(np.int32)
+    c = Cache(s)
+    plan, need = plan_of(c)
+    _, groups = check_plan(c, plan)
+    s.lens = lens
+    c.lens.upload(lens)
+    got, lse = shared(c, q, Hq, 0.1, plan, need, window, sinks)
+    ref, rlse, tol, ltol = kv_ref.attend(s, from_bf16(q).astype(np.float64), Hq, 0.1, window, sinks)
+    assert (np.abs(from_bf16(got) - ref) <= tol).all() and (np.abs(lse - rlse) <= ltol).all()
+    return groups
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (100, 0), (170, 3), (250, 70), (420, 0), (2 ** 31 - 1, 0)])
+@pytest.mark.parametrize("by", [0, 1, 3, 64, 130, [1, 0, 5, 200, 2, 70, 0]])
+@pytest.mark.parametrize("D,page,Hq,n", [(64, 16, 4, 1), (128, 64, 16, 3), (256, 32, 2, 1)])
+def test_a_plan_kept_while_sequences_grow(window, sinks, by, D, page, Hq, n):
+    """The plan of an earlier step of the same rows: what a window hides moves on with the lengths. Windows that end in what the
+    sequences share, in what they have for themselves, and that leave nothing of either."""
+    rng = np.random.default_rng(window % 1000 + D)
+    s, _ = step_of(rng, [(330, [200, 240, 290, 400]), (128, [202, 205])], [450], 2, D, page, n=n)
+    assert len(grown(s, randn_bf16(rng, (s.rows, Hq, D)), Hq, by, window, sinks)) == 2
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [700, 2000])
+def test_a_long_plan_kept_while_sequences_grow(D, window):
+    """Blocks that are cut into parts, the first of which no row sees any more."""
+    rng = np.random.default_rng(window + D)
+    s, _ = step_of(rng, [(3000, [600, 800, 500])], [1500], 1, D, 64)
+    for by in (5, 300, [1, 500, 0, 64]):
+        assert len(grown(s, randn_bf16(rng, (s.rows, 4, D)), 4, by, window, 2)) == 1
+
+
 def test_the_same_every_time_and_without_lse():
     rng = np.random.default_rng(11)
     s, _ = step_of(rng, [(2000, [3, 700, 100, 0])], [900], 2, 128, 64)

@@ -508,9 +508,15 @@ __global__ __launch_bounds__(AT_NT, D == 64 ? 3 : D == 128 ? 2 : 1) void kv_tile
   const int hq = h * a.group + ri % a.group;
   if constexpr (COMMON) {
     const int2 listed = a.share.list[row];
-    row = listed.x, pos = listed.y;
+    row = listed.x;
+    // A group's tiles lie before all of its rows: where a row is matters to a window only, and that moves on with the lengths
+    // of this step, not those of the plan's.
+    pos = 1 << 30;
+    if (a.window > 0) {
+      const Seq s = seq_of(a.st, listed.y);
+      pos = s.first + row - s.r0;
+    }
   }
-  // (a group's tiles lie before all of its rows)
   const int pos_lo = COMMON ? INT32_MAX : uniform(q.first + min(wrow, nrows - 1) / a.group);
   const int pos_hi = COMMON ? INT32_MAX : uniform(q.first + min(wrow + 31, nrows - 1) / a.group);
   const float sc = fmaxf(fabsf(a.scale2), 0x1p-126f);  // (not 0: hidden scores are -inf, and stay so)

@@ -52,14 +52,14 @@ struct ShareSeq {
 struct ShareGroup {
   int row0, rows, tiles;
   int seq;    // whose table is read
-  int first;  // the lowest position of its rows
+  int first;  // the lowest position of its rows when the plan was made: no row has a lower one while sequences grow
   int pad[3];
 };
 struct Share {
   ShareHead* head;
   ShareSeq* seqs;      // [B]
   ShareGroup* groups;  // [B / 2 + 1]
-  int2* list;          // [rows] {row of the step, position}
+  int2* list;          // [rows] {row of the step, its sequence}
   int4* found;         // [B, up to a multiple of SHARE_AHEAD] kv_share's own: what it knows of each sequence
   unsigned long long* best;  // [B] the same of each class
   int2* sums;                // [B]

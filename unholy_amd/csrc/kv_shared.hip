@@ -217,7 +217,7 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
     }
     const int2 to = sums[f.x];
     sh.seqs[b] = ShareSeq{int(best[f.x] & 0x1ffffff), at, to.x, to.y};
-    for (int i = 0; i < f.y; ++i) sh.list[to.x + at + i] = make_int2(f.w + i, f.z + i);
+    for (int i = 0; i < f.y; ++i) sh.list[to.x + at + i] = make_int2(f.w + i, b);
   }
   if (tid == 0) {
     ShareHead& h = *sh.head;
