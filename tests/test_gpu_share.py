@@ -389,6 +389,28 @@ def test_a_long_plan_kept_while_sequences_grow(D, window):
         assert len(grown(s, randn_bf16(rng, (s.rows, 4, D)), 4, by, window, 2)) == 1
 
 
+@pytest.mark.parametrize("B", [40, 1100])
+def test_a_cu_that_does_not_ascend_writes_nowhere_else(B):
+    """Every other sequence names the same 16 rows: more than the plan's list has room for. Nobody is in a group then, and plan, rows
+    and workspace end where they end. The next plan in the same place is right."""
+    rng = np.random.default_rng(B)
+    s, _ = step_of(rng, [(128, [int(x) for x in rng.integers(0, 30, B)])], [], 1, 64, 64)
+    t = kv_ref.Step.__new__(kv_ref.Step)
+    t.__dict__.update(s.__dict__, rows=16, lens=s.lens + 15)
+    t.cu = (np.arange(B + 1) % 2 * 16).astype(np.int32)
+    bad = Cache(t)
+    plan, need = plan_of(bad, most=16)
+    got = plan.download(16 + 4 * B, np.int32)
+    assert got[6:8].tolist() == [0, 0] and (got[16:].reshape(B, 4)[:, 0] == 0).all()
+    shared(bad, randn_bf16(rng, (16, 2, 64)), 2, 0.1, plan, need, most=16)
+    t.cu = np.minimum(np.arange(B + 1), 16).astype(np.int32)
+    t.n = np.diff(t.cu).tolist()
+    bad.cu.upload(t.cu)
+    call("uh_kv_share", None, bad.cu, 16, 16, bad.lens, bad.table, t.max_blocks, B, t.pages, 64, plan, need, None)
+    synchronize()
+    check_plan(bad, plan, most=16)
+
+
 def test_the_same_every_time_and_without_lse():
     rng = np.random.default_rng(11)
     s, _ = step_of(rng, [(2000, [3, 700, 100, 0])], [900], 2, 128, 64)

@@ -195,11 +195,14 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
       sums[b] = make_int2(row0, at);
     }
   }
+  // (A cu that does not ascend names rows more than once: where that is more than the list has room for, nobody is in a group.)
+  const bool fits = list <= st.rows;
+  if (!fits) groups = list = 0;
   __syncthreads();
   // the rows of a group in the order of the slots
   for (int b = tid; b < st.B; b += SH_NT) {
     const int4 f = found[b];
-    if (f.x < 0) {
+    if (f.x < 0 || !fits) {
       sh.seqs[b] = ShareSeq{0, 0, 0, 0};
       continue;
     }
