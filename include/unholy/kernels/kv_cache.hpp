@@ -82,8 +82,8 @@ void kv_attend(const bf16* q, int ldq, const KvStep& step, const KvCache& cache,
 // group [B] (device, may be null): sequences with the same number, in [0, B), may be taken together, others (-1) are alone;
 // null: those with the same first page. Of such sequences those that bring 1 to 16 rows and have the same pages as the lowest
 // of them for long enough (in whole pages before any new row, and in multiples of 64 tokens) become a group, as many of them
-// and as long as saves the most; the others are alone. Wrong numbers cost time, never results: what is shared is read off the
-// table.
+// and as long as saves the most; the others are alone, and so are all past the first 4096. Wrong numbers cost time, never
+// results: what is shared is read off the table.
 // plan: kv_share_plan bytes, 16-byte aligned, zeroed before the first call that makes one in it. It holds for the step's cu,
 // lens and table as they were when it was made, and stays valid, under a window too, for steps of the same cu while sequences
 // only grow and none of its pages is changed, moved (kv_compact) or given up. (Under a window, common tiles that no row sees any

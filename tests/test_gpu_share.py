@@ -7,7 +7,7 @@ from tests import kv_ref, rope_ref
 from tests.helpers import from_bf16, randn_bf16, to_bf16
 from tests.test_gpu_kv import Cache, Pool, attend, dev
 from unholy_amd import call
-from unholy_amd.device import DeviceBuffer, Graph, Stream, synchronize
+from unholy_amd.device import DeviceBuffer, Event, Graph, Stream, synchronize
 
 pytestmark = pytest.mark.gpu
 
@@ -209,6 +209,53 @@ def test_more_sequences_than_the_plan_has_room_for_in_lds():
     s, label = step_of(rng, [(64, [1, 2])] * 500 + [(80, [0, 3, 1])] * 20, [10] * 5, 1, 64, 16, order=rng.permutation(1065))
     check(s, 1, expect=520)
     check_plan(Cache(s), plan_of(Cache(s), label)[0], label)
+
+
+def test_more_sequences_than_the_plan_compares():
+    """Of pairs that begin alike those among the first 4096 sequences are groups, the others alone; the attention of all."""
+    rng = np.random.default_rng(19)
+    B, page, Hkv, D = 4500, 64, 1, 64
+    s = kv_ref.Step.__new__(kv_ref.Step)
+    s.n, s.B, s.Hkv, s.D, s.page, s.rows, s.max_blocks = [1] * B, B, Hkv, D, page, B, 2
+    s.cu, s.lens = np.arange(B + 1, dtype=np.int32), rng.integers(65, 100, B).astype(np.int32)
+    s.pages = B // 2 + B
+    order = rng.permutation(s.pages).astype(np.int32)
+    s.table = np.stack([order[np.arange(B) // 2], order[B // 2 + np.arange(B)]], 1)
+    s.k, s.v = (kv_ref.encode(rng.standard_normal(x) * 64) for x in ((s.pages, Hkv, page, D), (s.pages, Hkv, D, page)))
+    s.ks, s.vs = (rng.integers(118, 124, (s.pages, Hkv), dtype=np.uint8) for _ in range(2))
+    s = wide(s)
+    c = Cache(s)
+    plan, need = plan_of(c)
+    got = plan.download(16 + 4 * B, np.int32)
+    assert got[6:8].tolist() == [2048, 4096]
+    assert (got[16:].reshape(B, 4)[:, 0] == (np.arange(B) < 4096)).all()
+    q = randn_bf16(rng, (B, 2, D))
+    out, lse = shared(c, q, 2, 0.1, plan, need)
+    ref, rlse, tol, ltol = kv_ref.attend(s, from_bf16(q).astype(np.float64), 2, 0.1)
+    assert (np.abs(from_bf16(out) - ref) <= tol).all() and (np.abs(lse - rlse) <= ltol).all()
+
+
+def test_the_time_of_a_plan_does_not_grow_with_the_square_of_its_sequences():
+    """A million of them, among which all pairs would be compared for minutes."""
+    B, page = 1 << 20, 64
+    cu, lens = dev(np.arange(B + 1, dtype=np.int32)), dev(np.full(B, 70, np.int32))
+    table = dev(np.stack([np.arange(B, dtype=np.int32) // 2, np.full(B, -1, np.int32)], 1))
+    need = call("uh_kv_share_plan_size", B, B)
+    plan = dev(np.concatenate([np.zeros(need, np.uint8), np.full(64, GUARD, np.uint8)]))
+    st, times = Stream(), []
+    for _ in range(2):
+        a, b = Event(), Event()
+        a.record(st)
+        call("uh_kv_share", None, cu, B, 1, lens, table, 2, B, B, page, plan, need, st.handle)
+        b.record(st)
+        st.synchronize()
+        times.append(a.elapsed_ms(b))
+    got = plan.download(need + 64, np.uint8)
+    assert (got[need:] == GUARD).all()
+    got = got[:64 + 16 * B].view(np.int32)
+    assert got[6:8].tolist() == [2048, 4096] and (got[16:].reshape(B, 4)[:, 0] == (np.arange(B) < 4096)).all()
+    print(f"{times} ms")
+    assert min(times) < 100.0
 
 
 def test_a_block_of_a_group_for_every_workgroup():

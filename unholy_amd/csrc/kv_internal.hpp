@@ -38,6 +38,8 @@ __device__ __forceinline__ int page_of(const int32_t* table, int max_blocks, int
 // list.
 constexpr int SHARE_TILE = 64;
 constexpr int SHARE_ROWS = 16;  // a sequence that brings more rows is left alone: they fill tiles of rows by themselves
+constexpr int SHARE_SEQS = 4096;  // sequences past these are alone: the plan compares all pairs
+__host__ __device__ inline int share_seqs(int B) { return B < SHARE_SEQS ? B : SHARE_SEQS; }
 struct ShareHead {
   int magic, B, rows, max_new, max_blocks, page;
   int groups, list;  // their number, rows in the list
@@ -58,11 +60,11 @@ struct ShareGroup {
 struct Share {
   ShareHead* head;
   ShareSeq* seqs;      // [B]
-  ShareGroup* groups;  // [B / 2 + 1]
+  ShareGroup* groups;  // [n / 2 + 1], n the sequences that may be in groups
   int2* list;          // [rows] {row of the step, its sequence}
-  int4* found;         // [B, up to a multiple of SHARE_AHEAD] kv_share's own: what it knows of each sequence
-  unsigned long long* best;  // [B] the same of each class
-  int2* sums;                // [B]
+  int4* found;         // [n, up to a multiple of SHARE_AHEAD] kv_share's own: what it knows of each sequence
+  unsigned long long* best;  // [n] the same of each class
+  int2* sums;                // [n]
   size_t bytes;
 };
 constexpr int SHARE_AHEAD = 16;
@@ -70,6 +72,7 @@ constexpr int SHARE_MAGIC = 0x5ea4ed01;
 inline Share carve_share(void* plan, int B, int rows) {
   Share s;
   char* p = static_cast<char*>(plan);
+  const size_t n = size_t(share_seqs(B));
   const auto take = [&](size_t bytes) {
     char* at = p;
     p += (bytes + 15) / 16 * 16;
@@ -77,11 +80,11 @@ inline Share carve_share(void* plan, int B, int rows) {
   };
   s.head = reinterpret_cast<ShareHead*>(take(sizeof(ShareHead)));
   s.seqs = reinterpret_cast<ShareSeq*>(take(sizeof(ShareSeq) * size_t(B)));
-  s.groups = reinterpret_cast<ShareGroup*>(take(sizeof(ShareGroup) * (size_t(B) / 2 + 1)));
+  s.groups = reinterpret_cast<ShareGroup*>(take(sizeof(ShareGroup) * (n / 2 + 1)));
   s.list = reinterpret_cast<int2*>(take(sizeof(int2) * size_t(rows)));
-  s.found = reinterpret_cast<int4*>(take(sizeof(int4) * ((size_t(B) + SHARE_AHEAD - 1) / SHARE_AHEAD * SHARE_AHEAD)));
-  s.best = reinterpret_cast<unsigned long long*>(take(sizeof(unsigned long long) * size_t(B)));
-  s.sums = reinterpret_cast<int2*>(take(sizeof(int2) * size_t(B)));
+  s.found = reinterpret_cast<int4*>(take(sizeof(int4) * ((n + SHARE_AHEAD - 1) / SHARE_AHEAD * SHARE_AHEAD)));
+  s.best = reinterpret_cast<unsigned long long*>(take(sizeof(unsigned long long) * n));
+  s.sums = reinterpret_cast<int2*>(take(sizeof(int2) * n));
   s.bytes = size_t(p - static_cast<char*>(plan));
   return s;
 }

@@ -13,7 +13,8 @@ namespace {
 // A wave a sequence finds the lowest sequence of its class (the same number, or first page) and how far their tables agree, 256
 // entries at a time; the workgroup that finishes last makes the plan of what all have found: for each class the length that
 // saves the most tiles' reads, then places and lists. Loops over all pairs of sequences go through LDS, up to SH_MOST sequences
-// (through the plan past that).
+// (through the plan past that). They take time with the square of how many there are (256 14 us, 1024 84, 2048 0.8 ms, 4096 2.9,
+// and 8192 would take 11): sequences past the first SHARE_SEQS are in no group, and cost the plan a store each.
 constexpr int SH_NT = 256;
 constexpr int SH_MOST = 1024;
 constexpr int SH_AHEAD = SHARE_AHEAD;
@@ -42,18 +43,20 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
   } lds;
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int B = share_seqs(st.B);  // sequences that may be in a group
 
-  for (int b0 = blockIdx.x * (SH_NT / 64); b0 < st.B; b0 += gridDim.x * (SH_NT / 64)) {
+  for (int64_t b = int64_t(B) + blockIdx.x * SH_NT + tid; b < st.B; b += gridDim.x * SH_NT) sh.seqs[b] = ShareSeq{0, 0, 0, 0};
+  for (int b0 = blockIdx.x * (SH_NT / 64); b0 < B; b0 += gridDim.x * (SH_NT / 64)) {
     const int b = b0 + wave;
     Seq q{};
     int key = -1, rep = -1, first = 0, same = 0;  // rep: the lowest of the class, first: the position of its first row
-    if (b < st.B) {
+    if (b < B) {
       q = seq_of(st, b);
       key = share_key(group, st, pages, page, b, q);
     }
-    for (int k0 = 0; k0 < min(b0 + SH_NT / 64, st.B); k0 += SH_KEYS) {
+    for (int k0 = 0; k0 < min(b0 + SH_NT / 64, B); k0 += SH_KEYS) {
       __syncthreads();  // the keys' last use
-      for (int i = tid; i < min(SH_KEYS, min(b0 + SH_NT / 64, st.B) - k0); i += SH_NT) {
+      for (int i = tid; i < min(SH_KEYS, min(b0 + SH_NT / 64, B) - k0); i += SH_NT) {
         const Seq s = seq_of(st, k0 + i);
         lds.keys[i] = make_int2(share_key(group, st, pages, page, k0 + i, s), s.first);
       }
@@ -88,7 +91,7 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
         }
       }
     }
-    if (b < st.B && lane < 4) {
+    if (b < B && lane < 4) {
       const int tiles = int(int64_t(same) * page / SHARE_TILE);
       const int v = lane == 0 ? rep : lane == 1 ? tiles : lane == 2 ? q.r1 - q.r0 : q.first;
       __hip_atomic_store(&reinterpret_cast<int*>(sh.found + b)[lane], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -128,7 +131,7 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
   int4* found = LDS ? lds.all.found : sh.found;  // {lowest of the class, tiles in common with it, rows, position of the first}
   unsigned long long* best = LDS ? lds.all.best : sh.best;  // by the class's lowest: saved, then tiles (25 bits)
   int2* sums = LDS ? lds.all.sums : sh.sums;                // by the same: rows of the group, position of the first of them
-  for (int b = tid; b < st.B; b += SH_NT) {
+  for (int b = tid; b < B; b += SH_NT) {
     int v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -141,27 +144,27 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
     best[b] = 0;
     sums[b] = make_int2(0, INT32_MAX);
   }
-  if (tid < SH_AHEAD && st.B + tid < (st.B + SH_AHEAD - 1) / SH_AHEAD * SH_AHEAD) {
-    found[st.B + tid] = make_int4(-2, 0, 0, 0);
-    if constexpr (LDS) lds.all.key[st.B + tid] = none;
+  if (tid < SH_AHEAD && B + tid < (B + SH_AHEAD - 1) / SH_AHEAD * SH_AHEAD) {
+    found[B + tid] = make_int4(-2, 0, 0, 0);
+    if constexpr (LDS) lds.all.key[B + tid] = none;
   }
   __syncthreads();
   // what each length would save: the tiles of all but one of the sequences that are as long
-  for (int b = tid; b < st.B; b += SH_NT) {
+  for (int b = tid; b < B; b += SH_NT) {
     const int r = found[b].x, t = found[b].y;
     if (r < 0 || t == 0) continue;
     int count = 0;
     if constexpr (LDS) {
       const uint32_t from = uint32_t(r) << 21 | uint32_t(t);
-      for_keys(0, st.B, [&](int, uint32_t key) { count += int(key - from <= uint32_t(LONG - t)); });
+      for_keys(0, B, [&](int, uint32_t key) { count += int(key - from <= uint32_t(LONG - t)); });
     } else {
-      for_all(found, st.B, [&](int, int rep, int tiles) { count += int(rep == r) & int(tiles >= t); });
+      for_all(found, B, [&](int, int rep, int tiles) { count += int(rep == r) & int(tiles >= t); });
     }
     if (count > 1) atomicMax(&best[r], (unsigned long long)min(int64_t(count - 1) * t, int64_t(1) << 38) << 25 | (unsigned long long)t);
   }
   __syncthreads();
   // who is in a group: found becomes {lowest of the group or -1, rows, position of the first, first row of the step}
-  for (int b = tid; b < st.B; b += SH_NT) {
+  for (int b = tid; b < B; b += SH_NT) {
     const int4 f = found[b];
     const int t = f.x >= 0 ? int(best[f.x] & 0x1ffffff) : 0;
     const bool member = t > 0 && f.y >= t;
@@ -175,9 +178,9 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
   __syncthreads();
   // the groups in the order of their lowest sequences
   int groups = 0, list = 0;
-  for (int b0 = 0; b0 < st.B; b0 += SH_NT) {
+  for (int b0 = 0; b0 < B; b0 += SH_NT) {
     const int b = b0 + tid;
-    const bool head = b < st.B && found[b].x == b;  // (the lowest of a class is as long as any of it)
+    const bool head = b < B && found[b].x == b;  // (the lowest of a class is as long as any of it)
     const int rows = head ? sums[b].x : 0;
     const uint32_t g = wave_scan(head), l = wave_scan(uint32_t(rows));
     __syncthreads();  // the last round's reads
@@ -200,7 +203,7 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
   if (!fits) groups = list = 0;
   __syncthreads();
   // the rows of a group in the order of the slots
-  for (int b = tid; b < st.B; b += SH_NT) {
+  for (int b = tid; b < B; b += SH_NT) {
     const int4 f = found[b];
     if (f.x < 0 || !fits) {
       sh.seqs[b] = ShareSeq{0, 0, 0, 0};
@@ -264,7 +267,7 @@ __device__ __forceinline__ GroupWork group_work(const AttendShared& a, const Sha
   }
   return w;
 }
-__device__ __forceinline__ ShareGroup group_at(const AttendShared& a, int i) { return a.share.groups[min(i, a.st.B / 2)]; }
+__device__ __forceinline__ ShareGroup group_at(const AttendShared& a, int i) { return a.share.groups[min(i, share_seqs(a.st.B) / 2)]; }
 // Of sequence b: segments, and each one's tiles.
 struct SeqWork {
   Seq q;
@@ -703,7 +706,7 @@ SharedWs carve_shared(int rows, int max_new, int B, int Hq, int heads, int dim) 
   SharedWs w;
   const int64_t group = Hq / heads, list = std::min<int64_t>(rows, int64_t(SHARE_ROWS) * B);
   const int64_t most = std::min<int64_t>(std::min(rows, max_new), SHARE_ROWS);
-  w.blocks = (list * group / PR_ROWS + B / 2 + 1) * heads;
+  w.blocks = (list * group / PR_ROWS + share_seqs(B) / 2 + 1) * heads;
   w.list_rows = list * Hq;
   w.sum_rows = std::max<int64_t>(int64_t(target_of(dim)) * PR_ROWS, w.list_rows);
   w.most_parts = int((most * group + FEW - 1) / FEW);
