@@ -285,6 +285,33 @@ def test_many_tiles_of_64_channels(groups, times, window):
     check(s, 8, window=window, sinks=window // 1000, expect=groups)
 
 
+@pytest.mark.parametrize("D,Hq,Hkv,groups,each,times,alone,window", [
+    (128, 8, 8, 4, 2, 50, [20] * 40, 0), (128, 8, 8, 4, 2, 60, [20] * 40, 6600), (128, 4, 4, 2, 2, 200, [2000], 0),
+    (128, 48, 8, 8, 6, 26, [], 0), (128, 8, 8, 60, 2, 4, [9] * 20, 0), (64, 8, 8, 16, 2, 16, [30] * 40, 0),
+    (64, 8, 8, 16, 2, 30, [700], 2000), (64, 40, 8, 16, 7, 16, [], 0)])
+def test_blocks_on_most_of_the_chip(D, Hq, Hkv, groups, each, times, alone, window):
+    """So many common tiles, of few rows each or beside little else, that blocks take seven of eight workgroups: cut into parts, or
+    (the fifth) whole; the sequences' own tiles share the rest, segment after segment or (the third) one in parts. (The same two
+    pages over and over, as above.)"""
+    rng = np.random.default_rng(groups * times + D)
+    s, _ = step_of(rng, [(128, [int(x) for x in rng.integers(0, 40, each)]) for _ in range(groups)], [], Hkv, D, 64)
+    blocks, tiles = groups * Hkv * -(-each * Hq // Hkv // 128), 2 * times  # of which some leave the window
+    assert 6 * 512 < blocks * (min(tiles, window // 64) if window else tiles) and (D == 128 or blocks * tiles < 16 * 512)
+    t, _ = step_of(rng, [], alone, Hkv, D, 64) if alone else (None, None)
+    s.table = np.concatenate([np.tile(s.table[:, :2], times - 1), s.table], 1)
+    s.lens += 128 * (times - 1)
+    s.ctx = [x + 128 * (times - 1) for x in s.ctx]
+    if alone:  # behind the others
+        width = max(s.table.shape[1], t.table.shape[1])
+        at = np.where(t.table >= 0, t.table + s.pages, -1)
+        s.table = np.concatenate([np.pad(x, ((0, 0), (0, width - x.shape[1])), constant_values=-1) for x in (s.table, at)])
+        s.k, s.v, s.ks, s.vs = (np.concatenate(x) for x in ((s.k, t.k), (s.v, t.v), (s.ks, t.ks), (s.vs, t.vs)))
+        s.pages, s.n, s.ctx, s.lens = s.pages + t.pages, s.n + t.n, s.ctx + t.ctx, np.concatenate([s.lens, t.lens])
+        s.B, s.rows, s.cu = len(s.n), s.rows + t.rows, np.arange(len(s.n) + 1, dtype=np.int32)
+    s.max_blocks = s.table.shape[1]
+    check(s, Hq, window=window, sinks=window // 1000, expect=groups)
+
+
 def test_the_plan_takes_what_saves_most():
     """Three begin alike for long, six for a little: of 5 x 2 tiles and 2 x 9 the second; and with numbers that say so, both."""
     rng = np.random.default_rng(3)
