@@ -60,9 +60,9 @@ struct ShareGroup {
 struct Share {
   ShareHead* head;
   ShareSeq* seqs;      // [B]
-  ShareGroup* groups;  // [n / 2 + 1], n the sequences that may be in groups
+  ShareGroup* groups;  // [B / 2 + 1]
   int2* list;          // [rows] {row of the step, its sequence}
-  int4* found;         // [n, up to a multiple of SHARE_AHEAD] kv_share's own: what it knows of each sequence
+  int4* found;         // [n = share_seqs(B), up to a multiple of SHARE_AHEAD] kv_share's own: what it knows of each sequence
   unsigned long long* best;  // [n] the same of each class
   int2* sums;                // [n]
   size_t bytes;
@@ -80,7 +80,7 @@ inline Share carve_share(void* plan, int B, int rows) {
   };
   s.head = reinterpret_cast<ShareHead*>(take(sizeof(ShareHead)));
   s.seqs = reinterpret_cast<ShareSeq*>(take(sizeof(ShareSeq) * size_t(B)));
-  s.groups = reinterpret_cast<ShareGroup*>(take(sizeof(ShareGroup) * (n / 2 + 1)));
+  s.groups = reinterpret_cast<ShareGroup*>(take(sizeof(ShareGroup) * (size_t(B) / 2 + 1)));
   s.list = reinterpret_cast<int2*>(take(sizeof(int2) * size_t(rows)));
   s.found = reinterpret_cast<int4*>(take(sizeof(int4) * ((n + SHARE_AHEAD - 1) / SHARE_AHEAD * SHARE_AHEAD)));
   s.best = reinterpret_cast<unsigned long long*>(take(sizeof(unsigned long long) * n));

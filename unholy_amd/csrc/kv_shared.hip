@@ -43,9 +43,10 @@ __global__ __launch_bounds__(SH_NT) void kv_share_kernel(const int32_t* __restri
   } lds;
   __shared__ int last;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int B = share_seqs(st.B);  // sequences that may be in a group
+  const int B = LDS ? st.B : share_seqs(st.B);  // sequences that may be in a group
 
-  for (int64_t b = int64_t(B) + blockIdx.x * SH_NT + tid; b < st.B; b += gridDim.x * SH_NT) sh.seqs[b] = ShareSeq{0, 0, 0, 0};
+  if constexpr (!LDS)
+    for (int b = B + int(blockIdx.x) * SH_NT + tid; b < st.B; b += int(gridDim.x) * SH_NT) sh.seqs[b] = ShareSeq{0, 0, 0, 0};
   for (int b0 = blockIdx.x * (SH_NT / 64); b0 < B; b0 += gridDim.x * (SH_NT / 64)) {
     const int b = b0 + wave;
     Seq q{};
@@ -267,7 +268,7 @@ __device__ __forceinline__ GroupWork group_work(const AttendShared& a, const Sha
   }
   return w;
 }
-__device__ __forceinline__ ShareGroup group_at(const AttendShared& a, int i) { return a.share.groups[min(i, share_seqs(a.st.B) / 2)]; }
+__device__ __forceinline__ ShareGroup group_at(const AttendShared& a, int i) { return a.share.groups[min(i, a.st.B / 2)]; }
 // Of sequence b: segments, and each one's tiles.
 struct SeqWork {
   Seq q;
