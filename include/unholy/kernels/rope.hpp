@@ -13,9 +13,10 @@ using bf16 = uint16_t;
 // How heads are rotated: channels [first, first + rot) of a head, in pairs (2i, 2i + 1) of that part (interleaved) or
 // (i, i + rot / 2) (halves), pair i by the angle position * freq[i]:
 //   (a, b) -> mscale (a cos - b sin, a sin + b cos).
-// freq [rot / 2] (device, 8-byte aligned; null where rot is 0): radians a position. Angles are taken in 64 bits, turns cut off
-// before they are rounded to 32, so that far positions are as exact as near ones. rot even; rot 0: nothing is rotated. The
-// other channels are left as they are.
+// freq [rot / 2] (device, 8-byte aligned; null where rot is 0): radians a position. An angle's turns are cut off and its sine and
+// cosine taken in 64 bits, these rounded once to 32 (with mscale), and what a far angle's product has past 64 bits counts: far
+// positions are as exact as near ones (any position; |angles| below 2^40). rot even; rot 0: nothing is rotated. The other
+// channels are left as they are.
 struct Rope {
   const double* freq;
   int first, rot;

@@ -1,5 +1,7 @@
 """Rotary positions, the norms before them and both into the paged cache, on the GPU against plain numpy (tests/rope_ref.py),
 within bounds that count the roundings; what is one launch against the calls that it stands for, bit for bit."""
+from fractions import Fraction
+
 import numpy as np
 import pytest
 
@@ -110,6 +112,43 @@ def test_far_positions_are_as_exact_as_near_ones():
     rope(Rows(len(pos), 2, 128, data=x), y, dev(pos), df, t)
     ref, tol = rope_ref.rope(from_bf16(x).astype(np.float64), pos, f, 0, 128, False)
     near(y.down(), ref, tol, "far")
+
+
+def exact_turn(pos, freq):
+    """Cosine and sine of pos * freq, whole turns cut off in rational numbers (pi to 50 digits)."""
+    turn = 2 * Fraction(314159265358979323846264338327950288419716939937511, 10 ** 50)
+    angle = [float((p * Fraction(f)) % turn) for p in pos.tolist() for f in freq.tolist()]
+    angle = np.array(angle).reshape(len(pos), len(freq))
+    return np.cos(angle), np.sin(angle)
+
+
+@pytest.mark.parametrize("far", [1000, 1 << 24, 1 << 28, 2 ** 31 - 1])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_the_error_of_an_angle_does_not_grow_with_the_position(far, interleaved):
+    """Pairs that a rotation turns almost onto an axis: a cos - b sin is next to nothing, and shows by how much the factors are
+    off. Bounds: each factor is rounded once (2^-25, its sine or cosine and angle another eighth of that), the product b sin
+    is (2^-24 of it), the sum is (2^-24), and the result to bf16 (2^-8)."""
+    rng = np.random.default_rng(far % 1000)
+    rot, rows = 32, 400
+    freq = rope_ref.frequencies(rot, 5.0)
+    pos = rng.integers(far // 2, far + 1, rows).astype(np.int32)
+    pos[::3] *= -1
+    c, s = exact_turn(pos, freq)
+    a, b = s[:, None], c[:, None]  # (a cos - b sin = 0, before a and b are bf16)
+    x = np.stack([a, b], -1).reshape(rows, 1, rot) if interleaved else np.concatenate([a, b], -1)
+    x = to_bf16(x.astype(np.float32))
+    t = (0, rot, int(interleaved), 1.0)
+    y = Rows(rows, 1, rot)
+    rope(Rows(rows, 1, rot, data=x), y, dev(pos), dev(freq), t)
+    ia, ib = rope_ref.pairs(rot, 0, rot, interleaved)
+    wide, got = from_bf16(x).astype(np.float64)[:, 0], from_bf16(y.down()).astype(np.float64)[:, 0]
+    for sign, u, v, out in ((-1, c, s, ia), (1, s, c, ib)):
+        ref = wide[:, ia] * u + sign * wide[:, ib] * v
+        tol = (np.abs(wide[:, ia]) + np.abs(wide[:, ib])) * 2.0 ** -25 * 1.125 + 2.0 ** -24 * (np.abs(wide[:, ib] * v) + np.abs(ref))
+        tol += 2.0 ** -8 * np.abs(ref)
+        err = np.abs(got[:, out] - ref)
+        print(f"far {far} worst error {np.max(err / tol):.3f} of bound")
+        assert (err <= tol).all()
 
 
 def test_turning_back_undoes_it():

@@ -77,13 +77,19 @@ __device__ __forceinline__ Slot slot_of(int s, int dim, int first, int rot, bool
 }
 
 // The two factors of a rotation: (cos, sin) of pos * freq, times mscale, rounded once. In 64 bits, a rotation's factors serve
-// many channels: the angle in turns, whole turns cut off, what is left as some quarters and at most an eighth of a turn, whose
-// sine and cosine are their Taylor series (up to the 11th and 12th power: the next terms are below 2^-37).
+// many channels: the angle in quarters of a turn, of which whole ones are cut off, and at most an eighth of a turn is left,
+// whose sine and cosine are their Taylor series (up to the 11th and 12th power: the next terms are below 2^-37). Far positions
+// lose nothing: quarters a position are two numbers, of which the first has 21 bits and its product with a position (32 bits) is
+// exact, and the second is below 2^-20 of it and holds what 2 / pi and freq's product have past 64 bits (an angle is off by
+// 2^-72 of it, and by 2^-52 of what is left; one rounded product for the angle is off by 2^-52 of it: 2^-21 at position 2^31).
 __device__ __forceinline__ float2 turn_of(int pos, double freq, float mscale) {
 #pragma clang fp contract(off)
-  constexpr double kRadian = 0.15915494309189533577, kTurn = 6.28318530717958647693;  // 1 / (2 pi) turns; in radians
-  const double t = double(pos) * (freq * kRadian), part = t - rint(t), quarters = rint(4.0 * part);
-  const double a = (part - 0.25 * quarters) * kTurn, z = a * a;
+  constexpr double kQuarters = 0.63661977236758134308, kQuartersRest = -3.9357353350364972e-17;  // 2 / pi: 64 bits, the rest
+  constexpr double kQuarter = 1.57079632679489661923;  // in radians
+  const double p = double(pos), each = freq * kQuarters, past = __builtin_fma(freq, kQuartersRest, __builtin_fma(freq, kQuarters, -each));
+  const double hi = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, each) & 0xffffffff00000000u), lo = (each - hi) + past;
+  const double much = p * hi, quarters = rint(__builtin_fma(p, lo, much));
+  const double a = __builtin_fma(p, lo, much - quarters) * kQuarter, z = a * a;
   double s = -1.0 / 39916800.0, c = 1.0 / 479001600.0;
   s = __builtin_fma(s, z, 1.0 / 362880.0);
   c = __builtin_fma(c, z, -1.0 / 3628800.0);
@@ -96,7 +102,7 @@ __device__ __forceinline__ float2 turn_of(int pos, double freq, float mscale) {
   s = __builtin_fma(s * z, a, a);
   c = __builtin_fma(c, z, -0.5);
   c = __builtin_fma(c, z, 1.0);
-  const int q = int(quarters) & 3;
+  const int q = int(__builtin_bit_cast(uint64_t, quarters + 0x1.8p52)) & 3;  // (the sum's last bits are a whole number's)
   const double x = q & 1 ? -s : c, y = q & 1 ? c : s, m = q & 2 ? -double(mscale) : double(mscale);
   return make_float2(float(x * m), float(y * m));
 }
