@@ -350,6 +350,13 @@ def test_append_rope_rows_that_are_left_alone():
     check_append(t, 4, 0, 64)
 
 
+@pytest.mark.parametrize("rows,n,max_new,Hq", [(66000, 1, 1, 2), (140000, 2, 3, 1), (20000, 1, 1, 64), (66000, 70, 70, 2)])
+def test_append_rope_with_far_more_rows_than_sequences_have(rows, n, max_new, Hq):
+    """Row arrays of a large batch for a sequence of it."""
+    rng = np.random.default_rng(rows)
+    check_append(kv_ref.Step(rng, [n], [5], 1, 64, 16, spare_rows=rows), Hq, 0, 64, max_new=max_new)
+
+
 @pytest.mark.parametrize("B", [65, 200])
 def test_append_rope_of_many_sequences(B):
     rng = np.random.default_rng(B)

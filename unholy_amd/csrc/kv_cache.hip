@@ -557,23 +557,25 @@ static void append(const char* who, const bf16* k, int ldk, const bf16* v, int l
     fail("ldk / ldv >= heads * dim, % 8");
   if (!aligned16(k) || !aligned16(v)) fail("rows not 16-byte aligned");
   const int64_t most = std::min(s.max_new, s.rows);  // (up to 2^31 - 1)
-  const int reach = int(std::min<int64_t>((most - 1 + c.page - 1) / c.page + 1, s.max_blocks));
-  const int nblk = std::max(reach, 1);  // blocks that they can reach (none: the queries' workgroups are laid out by it all the same)
-  if (int64_t(s.B) * nblk > INT32_MAX) fail("B * blocks past 31 bits");
-  dim3 grid(unsigned(s.B) * unsigned(nblk), unsigned(c.heads), 2);
   // A wave holds 128 pieces of 8 channels x 4 tokens: enough for `most` tokens, wherever they begin, or a workgroup of four
   // (64 sequences of one token in eight layers: 50 us by waves, 59 by workgroups)
   const bool few = ((most + 2) / 4 + 1) * (c.dim / 8) <= 64 * pieces_of(c.dim, c.page, 64);
+  int64_t nblk = std::min<int64_t>((most - 1 + c.page - 1) / c.page + 1, s.max_blocks), queries = 0;  // blocks that they can reach
   if constexpr (TURN) {
     const int heads = (few ? 64 : 256) / (c.dim / 16);  // of a workgroup at a time
     t.row_wgs = few ? int(cdiv(t.Hq, heads)) : 1;
-    const size_t layer = size_t(grid.x) * grid.y, wgs = t.Hq ? size_t(s.rows) * t.row_wgs : 0;
-    if ((wgs + layer - 1) / layer > 65533) fail("rows past what a launch takes");
-    grid.z += unsigned((wgs + layer - 1) / layer);
+    queries = t.Hq ? int64_t(s.rows) * t.row_wgs : 0;
+    // (more blocks, which hold nothing, where the queries' workgroups would be too many layers)
+    const int64_t layer = int64_t(s.B) * c.heads, layers = 65533;
+    nblk = std::max({nblk, (queries + layers * layer - 1) / (layers * layer), int64_t(1)});
   }
+  if (s.B * nblk > INT32_MAX) fail("B * blocks past 31 bits");
+  dim3 grid(unsigned(s.B * nblk), unsigned(c.heads), 2);
+  const int64_t layer = int64_t(grid.x) * grid.y;
+  grid.z += unsigned((queries + layer - 1) / layer);
   const auto go = [&]<int D, int PAGE>() {
-    if (few) kv_append_kernel<D, PAGE, 64, TURN><<<grid, 64, 0, st>>>(k, ldk, v, ldv, s, c, nblk, t);
-    else kv_append_kernel<D, PAGE, 256, TURN><<<grid, 256, 0, st>>>(k, ldk, v, ldv, s, c, nblk, t);
+    if (few) kv_append_kernel<D, PAGE, 64, TURN><<<grid, 64, 0, st>>>(k, ldk, v, ldv, s, c, int(nblk), t);
+    else kv_append_kernel<D, PAGE, 256, TURN><<<grid, 256, 0, st>>>(k, ldk, v, ldv, s, c, int(nblk), t);
   };
   const auto by_page = [&]<int D>() {
     switch (c.page) {
