@@ -93,8 +93,8 @@ size_t kv_share_plan(int B, int rows);
 void kv_share(const int32_t* group, const KvStep& step, int pages, int page, void* plan, size_t plan_bytes, hipStream_t st);
 // The operands are kv_attend's; the step's sizes (B, rows, max_new, max_blocks) and the page are those of kv_share's call,
 // earlier on the same stream or finished: a plan of others is not used. Steps whose tables (B * max_blocks entries) can name
-// no more than 64 MB of keys and values, 128 with dim 256, are kv_attend's without further ado: it is faster there. ws as
-// kv_attend's (its own size; a workspace may serve both calls).
+// no more than 64 MB of keys and values, 128 with dim 256, are kv_attend's without further ado (it is faster there), and so are
+// those too large for the shared form's 31-bit counts. ws as kv_attend's (its own size; a workspace may serve both calls).
 size_t kv_attend_shared_workspace(int rows, int max_new, int B, int Hq, int heads, int dim);
 void kv_attend_shared(const bf16* q, int ldq, const KvStep& step, const KvCache& cache, int Hq, float scale, int window,
                       int sinks, bf16* out, int ldo, float* lse, const void* plan, size_t plan_bytes, void* ws,

@@ -504,6 +504,25 @@ def test_one_sequence():
         check(wide(kv_ref.Step(rng, [n], [300], 1, 64, 16)), 4, expect=0)
 
 
+def test_tables_too_wide_for_the_shared_form():
+    """A launch sized for 16 rows of each of 2048 sequences, over tables of a million tokens: more segments times tiles than 31 bits
+    count. It is kv_attend's, which counts them by sequences."""
+    rng = np.random.default_rng(21)
+    B, page, Hkv, Hq, D = 2048, 128, 8, 64, 64
+    s = kv_ref.Step.__new__(kv_ref.Step)
+    s.n, s.B, s.Hkv, s.D, s.page, s.rows, s.max_blocks, s.pages = [1] * B, B, Hkv, D, page, B, 8192, 40
+    s.cu, s.lens = np.arange(B + 1, dtype=np.int32), rng.integers(100, 300, B).astype(np.int32)
+    s.table = np.full((B, s.max_blocks), -1, np.int32)
+    s.table[:, :3] = rng.integers(0, s.pages, (B, 3))
+    s.k, s.v = (kv_ref.encode(rng.standard_normal(x) * 64) for x in ((s.pages, Hkv, page, D), (s.pages, Hkv, D, page)))
+    s.ks, s.vs = (rng.integers(118, 124, (s.pages, Hkv), dtype=np.uint8) for _ in range(2))
+    c, q = Cache(s), randn_bf16(rng, (B, Hq, D))
+    plan, need = plan_of(c, most=16)
+    got, lse = shared(c, q, Hq, 0.1, plan, need, most=16)
+    want, wlse = attend(c, q, Hq, 0.1, max_new=16)
+    assert np.array_equal(got, want) and np.array_equal(lse, wlse)
+
+
 @pytest.mark.parametrize("n", [1, 7])
 def test_narrow_tables(n):
     """A step that the other kernels take, in the same workspace."""

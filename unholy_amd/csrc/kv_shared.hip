@@ -739,15 +739,17 @@ void kv_attend_shared(const bf16* q, int ldq, const KvStep& s, const KvCache& c,
   if (!plan) fail("null plan");
   if (!aligned16(plan)) fail("plan not 16-byte aligned");
   if (plan_bytes < kv_share_plan(s.B, s.rows)) fail("plan too small");
-  if (!worth_sharing(s, c)) return kv_attend(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, ws, ws_bytes, st);
   const Way way = shared_way(s.rows, s.max_new, Hq / c.heads);
   AttendShared a{attend_of(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, way, ws)};
   const SharedWs w = carve_shared(s.rows, s.max_new, s.B, Hq, c.heads, c.dim);
   const int64_t tiles = std::max<int64_t>(cdiv(size_t(s.max_blocks) * c.page, TILE), 1);
   const int64_t blocks = (cdiv(size_t(s.rows) * a.group, PR_ROWS) + int64_t(s.B)) * c.heads;
-  if (w.segments * 8 > INT32_MAX || blocks > INT32_MAX || w.blocks > INT32_MAX || w.sum_rows > INT32_MAX ||
-      std::max(w.segments, std::min<int64_t>(std::max(blocks, w.blocks), a.target)) * (tiles + START) > INT32_MAX)
-    fail("rows times blocks past 31 bits");
+  // (kv_attend counts fewer segments, and refuses what is too much for it)
+  const bool too_large =
+      w.segments * 8 > INT32_MAX || blocks > INT32_MAX || w.blocks > INT32_MAX || w.sum_rows > INT32_MAX ||
+      std::max(w.segments, std::min<int64_t>(std::max(blocks, w.blocks), a.target)) * (tiles + START) > INT32_MAX;
+  if (too_large || !worth_sharing(s, c))
+    return kv_attend(q, ldq, s, c, Hq, scale, window, sinks, out, ldo, lse, ws, ws_bytes, st);
   a.share = carve_share(const_cast<void*>(plan), s.B, s.rows);
   a.most_parts = w.most_parts;
   a.lists = int(w.list_rows / Hq), a.sum_rows = int(w.sum_rows);
