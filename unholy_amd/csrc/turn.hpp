@@ -86,8 +86,9 @@ __device__ __forceinline__ float2 turn_of(int pos, double freq, float mscale) {
 #pragma clang fp contract(off)
   constexpr double kQuarters = 0.63661977236758134308, kQuartersRest = -3.9357353350364972e-17;  // 2 / pi: 64 bits, the rest
   constexpr double kQuarter = 1.57079632679489661923;  // in radians
-  const double p = double(pos), each = freq * kQuarters, past = __builtin_fma(freq, kQuartersRest, __builtin_fma(freq, kQuarters, -each));
-  const double hi = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, each) & 0xffffffff00000000u), lo = (each - hi) + past;
+  const double p = double(pos);
+  const double hi = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, freq * kQuarters) & 0xffffffff00000000u);
+  const double lo = __builtin_fma(freq, kQuartersRest, __builtin_fma(freq, kQuarters, -hi));
   const double much = p * hi, quarters = rint(__builtin_fma(p, lo, much));
   const double a = __builtin_fma(p, lo, much - quarters) * kQuarter, z = a * a;
   double s = -1.0 / 39916800.0, c = 1.0 / 479001600.0;
