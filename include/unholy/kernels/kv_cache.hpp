@@ -77,13 +77,18 @@ void kv_attend(const bf16* q, int ldq, const KvStep& step, const KvCache& cache,
 // ---- sequences that begin alike ---------------------------------------------------------------------------------------
 // Sequences whose tables begin with the same pages (forks, requests behind the same instructions) need those pages' tokens
 // read and multiplied once for all of their rows. kv_share finds out which on the device, once for the layers of a step, and
-// kv_attend_shared is kv_attend with that plan: the same results but for the order of its sums.
+// kv_attend_shared is kv_attend with that plan: the same results but for the order of sums and how far they are off. The common
+// tokens go the way of kv_attend's prompts, whose weights are rounded to bf16 (for the product with the values only) relative to
+// a maximum that lags by up to 2^8, so that the largest is rounded too: outputs are off by 2.0e-3 to 2.3e-3 of their norm, those
+// of kv_attend's single tokens by 1.8e-3, and their rounding to bf16 alone is 1.65e-3.
 //
 // group [B] (device, may be null): sequences with the same number, in [0, B), may be taken together, others (-1) are alone;
 // null: those with the same first page. Of such sequences those that bring 1 to 16 rows and have the same pages as the lowest
 // of them for long enough (in whole pages before any new row, and in multiples of 64 tokens) become a group, as many of them
-// and as long as saves the most; the others are alone, and so are all past the first 4096. Wrong numbers cost time, never
-// results: what is shared is read off the table.
+// and as long as saves the most; the others are alone, and so are all past the first 4096. A number has one group at most, and
+// its lowest sequence decides with what the others are compared: where numbers are known, sequences of one prefix that others
+// share only the beginning of should have their own. Wrong numbers cost time, never results: what is shared is read off the
+// table.
 // plan: kv_share_plan bytes, 16-byte aligned, zeroed before the first call that makes one in it. It holds for the step's cu,
 // lens and table as they were when it was made, and stays valid, under a window too, for steps of the same cu while sequences
 // only grow and none of its pages is changed, moved (kv_compact) or given up. (Under a window, common tiles that no row sees any
@@ -94,7 +99,9 @@ void kv_share(const int32_t* group, const KvStep& step, int pages, int page, voi
 // The operands are kv_attend's; the step's sizes (B, rows, max_new, max_blocks) and the page are those of kv_share's call,
 // earlier on the same stream or finished: a plan of others is not used. Steps whose tables (B * max_blocks entries) can name
 // no more than 64 MB of keys and values, 128 with dim 256, are kv_attend's without further ado (it is faster there), and so are
-// those too large for the shared form's 31-bit counts. ws as kv_attend's (its own size; a workspace may serve both calls).
+// those too large for the shared form's 31-bit counts. That goes by how wide the tables are, which is all that the launch knows:
+// short sequences in wide tables, and sequences that share little, are faster by kv_attend. ws as kv_attend's (its own size; a
+// workspace may serve both calls).
 size_t kv_attend_shared_workspace(int rows, int max_new, int B, int Hq, int heads, int dim);
 void kv_attend_shared(const bf16* q, int ldq, const KvStep& step, const KvCache& cache, int Hq, float scale, int window,
                       int sinks, bf16* out, int ldo, float* lse, const void* plan, size_t plan_bytes, void* ws,

@@ -43,8 +43,9 @@ void rope(const bf16* x, int ldx, bf16* y, int ldy, const int32_t* pos, int rows
 
 // Queries q [rows, Hq, dim] and keys k [rows, Hkv, dim], each head x divided by the root of (its mean square + eps) and times
 // the weight of each channel, wq and wk [dim], then rotated as above, into qo and ko, in one launch. Sums and the rotation in
-// fp32, one rounding to bf16 at the end (a head whose squares pass fp32, channels past 10^18, has no finite norm). Row strides
-// at least heads * dim; Hq or Hkv 0: no such operand. Aliasing as in rope.
+// fp32, one rounding to bf16 at the end (a head whose squares pass fp32, channels past 10^18, has no finite norm, and a channel
+// whose product with its weight does no finite value; a head of zeros with eps 0 is 0 / 0). Row strides at least heads * dim; Hq
+// or Hkv 0: no such operand. Aliasing as in rope.
 void qk_norm_rope(const bf16* q, int ldq, bf16* qo, int ldqo, int Hq, const bf16* wq, const bf16* k, int ldk, bf16* ko,
                   int ldko, int Hkv, const bf16* wk, float eps, const int32_t* pos, int rows, int dim, const Rope& r,
                   hipStream_t st);

@@ -412,7 +412,7 @@ int uh_kv_attend(const uint16_t* q, int ldq, const int32_t* cu, int rows, int ma
                  uint16_t* out, int ldo, float* lse, void* ws, size_t ws_bytes, void* stream);
 /* Sequences whose tables begin with the same pages: uh_kv_share finds them on the device, once for the layers of a step, and
  * uh_kv_attend_shared is uh_kv_attend with that plan, which reads those pages once for all rows of a group (the same results but
- * for the order of sums). group int32 [B] (may be NULL: those with the same first page): sequences with the same number in
+ * for the order of sums and their roundings, those of prompts). group int32 [B] (may be NULL: those with the same first page): sequences with the same number in
  * [0, B) may be taken together, -1: alone (as are all past the first 4096). plan: uh_kv_share_plan_size bytes, 16-byte aligned,
  * zeroed before its first call. ws: uh_kv_attend_shared_workspace_size bytes, as uh_kv_attend's. */
 size_t uh_kv_share_plan_size(int B, int rows);
