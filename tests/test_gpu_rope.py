@@ -310,6 +310,41 @@ def test_append_rope_of_a_part(first, rot, Hq, Hkv):
     check_append(s, Hq, first, rot, pad=8)
 
 
+@pytest.mark.parametrize("n,ctx", [([1, 1, 1], [0, 63, 200]), ([90, 1, 20], [0, 7, 33])])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("wq,wk", [(True, True), (True, False), (False, True)])
+def test_append_rope_in_place(n, ctx, interleaved, wq, wk):
+    """Queries rotated where they stand in the projection's rows, beside keys and values that stay; norms of one of the two."""
+    rng = np.random.default_rng(sum(n))
+    s = kv_ref.Step(rng, n, ctx, 2, 128, 64, spare_rows=2)
+    f, df, t = turn(128, 32, 64, interleaved, 1.1)
+    w = [dev(to_bf16(1 + 0.3 * rng.standard_normal(128))) if x else None for x in (wq, wk)]
+    x = randn_bf16(rng, (s.rows, 9, 128))
+    a, qo, b, c, d = Rows(s.rows, 9, 128, 8, data=x), Rows(s.rows, 5, 128), Rows(s.rows, 9, 128, 8, data=x), Cache(s), Cache(s)
+    append_rope(c, a, qo, 5, *w, df, t)
+    append_rope(d, b, b, 5, *w, df, t)
+    synchronize()
+    used, got = int(s.cu[-1]), b.down()
+    assert np.array_equal(got[:used, :5], qo.down()[:used])
+    assert np.array_equal(got[used:], x[used:]) and np.array_equal(got[:, 5:], x[:, 5:]) and np.array_equal(a.down(), x)
+    for u, v in zip(c.down(), d.down()):
+        assert np.array_equal(u, v)
+    pos = positions(s)
+    for heads, weight in ((slice(0, 5), w[0]), (slice(5, 7), w[1])):  # each as its own call does it
+        one = Rows(s.rows, heads.stop - heads.start, 128, data=x[:, heads])
+        if weight is None:
+            rope(one, one, dev(pos), df, t)
+        else:
+            none = Rows(s.rows, 0, 128)
+            norm_rope(one, none, one, none, weight, None, 1e-6, dev(pos), df, t)
+        if heads.start == 0:
+            assert np.array_equal(one.down()[:used], got[:used, :5])
+        else:
+            run_append(e := Cache(s), one.down(), x[:, 7:])
+            for u, v in zip(c.down(), e.down()):
+                assert np.array_equal(u, v)
+
+
 def test_append_rope_against_64_bits():
     """Keys in the cache: the rounding to bf16 (2^-8 and what rope_ref counts), and half a step of e4m3 (2^-4, of subnormal
     codes 2^-10 of the scale)."""

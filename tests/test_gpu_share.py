@@ -163,6 +163,16 @@ def test_drafts(n, Hq, Hkv, D, page):
     check(s, Hq, expect=1, pad=8)
 
 
+@pytest.mark.parametrize("n", [1, 3, 16])
+@pytest.mark.parametrize("Hq,Hkv", [(17, 1), (40, 2), (130, 1)])
+def test_more_query_heads_than_an_operand_has_rows(n, Hq, Hkv):
+    """Parts of 16 rows and blocks of 128 that end inside a token's heads; beside a sequence alone."""
+    rng = np.random.default_rng(n + Hq)
+    s, _ = step_of(rng, [(200, [3, 90, 0]), (64, [1, 40])], [150], Hkv, 64, 32, n=n)
+    check(s, Hq, expect=2)
+    check(s, Hq, window=120, sinks=3, expect=2)
+
+
 @pytest.mark.parametrize("n", [[1, 16, 17, 3, 1, 40], [5, 0, 1, 2, 0, 1], [200, 1, 1, 1, 1, 1], [17, 300, 20, 18, 30, 19]])
 def test_steps_of_many_kinds(n):
     """Sequences with more than 16 rows, or none, among the others: they are in no group."""
@@ -495,6 +505,26 @@ def test_the_same_every_time_and_without_lse():
         again, l2 = shared(c, q, 8, 0.1, plan, need)
         assert np.array_equal(first, again) and np.array_equal(lse, l2)
     assert np.array_equal(first, shared(c, q, 8, 0.1, plan, need, lse=False)[0])
+
+
+def test_two_streams_read_one_plan():
+    """Layers on two streams at once, a workspace each, behind one plan."""
+    rng = np.random.default_rng(22)
+    s, _ = step_of(rng, [(1500, [3, 200, 100, 0])], [900], 2, 128, 64)
+    c, st = Cache(s), (Stream(), Stream())
+    plan, need_plan = plan_of(c)
+    q = [randn_bf16(rng, (s.rows, 8, 128)) for _ in st]
+    want = [shared(c, x, 8, 0.1, plan, need_plan)[0] for x in q]
+    need = call("uh_kv_attend_shared_workspace_size", s.rows, 1, s.B, 8, 2, 128)
+    dq, ws, out = [dev(x) for x in q], [dev(np.zeros(need, np.uint8)) for _ in st], [DeviceBuffer(q[0].nbytes) for _ in st]
+    synchronize()
+    for _ in range(20):
+        for t, x, w, o in zip(st, dq, ws, out):
+            call("uh_kv_attend_shared", x, 8 * 128, c.cu, s.rows, 1, c.lens, c.table, s.max_blocks, s.B, *c.arrays(), s.pages, s.page, 8,
+                 2, 128, 0.1, 0, 0, o, 8 * 128, None, plan, need_plan, w, need, t.handle)
+    for t, o, x in zip(st, out, want):
+        t.synchronize()
+        assert np.array_equal(o.download(x.shape, np.uint16), x)
 
 
 def test_one_sequence():
